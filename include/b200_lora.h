@@ -446,6 +446,61 @@ int lora_b200_decode_attention(void* out, const float* planes, int32_t n_planes,
                                int32_t block_size, const int32_t* context_lens, const int64_t* slot_mapping, float scale,
                                void* stream);
 
+/*
+ * A paged key-value cache as the calls below take it: block b of a sequence's table holds its positions [b * block_size, (b + 1)
+ * * block_size); the row of (block, position in block, kv head) starts at block * k_block + position * k_token + head * k_head
+ * elements of k (v likewise) and has head_dim adjacent elements. Strides are multiples of 8 elements, k and v 16-byte aligned.
+ * Counterpart in the reference: the k_cache / v_cache of Attention (nanovllm_voxcpm/layers/attention.py:52-68).
+ */
+typedef struct {
+  void *k, *v;
+  int32_t num_blocks, block_size;
+  int64_t k_block, k_token, k_head, v_block, v_token, v_head;
+} lora_b200_paged_cache;
+
+/*
+ * RMS norm of every q and k head of the packed rows qkv [T, (num_heads + 2 num_kv_heads) * head_dim] over its head_dim elements,
+ * times q_weight / k_weight [head_dim], rotation as lora_b200_glue_rope_kv_store (positions, cos_table and sin_table all null:
+ * none), everything in fp32 and rounded once; k and v rows to cache slot slot_mapping[t] = block * block_size + position in block
+ * (slots outside the cache, -1 among them: nowhere). q_out [T, num_heads, head_dim] with row stride q_out_ld: q goes there and
+ * qkv stays as it is; null: q and k are replaced in qkv. cache null: nothing is stored (q_out is then null too). head_dim a
+ * multiple of 16 up to 256; slots of one call are distinct. bf16, fp16.
+ */
+int lora_b200_glue_qk_norm_rope_kv_store(void* qkv, int64_t qkv_ld, int32_t T, int32_t num_heads, int32_t num_kv_heads,
+                                         int32_t head_dim, const void* q_weight, const void* k_weight, float eps,
+                                         const int64_t* positions, const void* cos_table, const void* sin_table,
+                                         int32_t table_dim, int32_t table_dtype, int32_t max_position, void* q_out,
+                                         int64_t q_out_ld, const lora_b200_paged_cache* cache, const int32_t* slot_mapping,
+                                         int32_t dtype, void* stream);
+
+/*
+ * Attention over a paged cache: out[t, h] = softmax over the keys j that token t sees of scale * q[t, h] . k_j, times v_j; token t
+ * at position p sees j <= p, with window > 0 only the last `window` of them (itself among them) and the first `sinks`.
+ *  q, out        [T, num_heads, head_dim], token and head strides in elements (multiples of 8; q and out 16-byte aligned)
+ *  lse           float [T, num_heads]: log of the sum of exp(scale * q . k); -inf without a key (the output is then zero). Or null
+ *  block_tables  int32 [n_seqs, table_width], row stride table_ld; an entry outside the cache: its keys are left out (a window's
+ *                caller may have given the block back), as are keys behind the table. Entries of blocks without a seen key are not used
+ *  context_lens  int32 [n_seqs]: tokens of the sequence, the new ones included (< 0: none)
+ * decode:  T = n_seqs, token t is the last of its sequence.
+ * prefill: the tokens [cu_seqlens[i], cu_seqlens[i + 1]) of q are the last ones of sequence i (cu_seqlens ascending); rows of out
+ *          (and lse) outside [cu_seqlens[0], cu_seqlens[n_seqs]) are left as they are.
+ * head_dim 64 or 128, scale > 0, bf16 and fp16. workspace: device memory of lora_b200_paged_workspace_bytes, 16-byte aligned, of
+ * this call alone until it has run. Counterpart in the reference: flash_attn_with_kvcache and flash_attn_varlen_func with a block
+ * table in Attention.forward (nanovllm_voxcpm/layers/attention.py:70-79); it has no window.
+ */
+size_t lora_b200_paged_workspace_bytes(int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t prefill);
+int lora_b200_paged_decode_attention(void* out, int64_t out_token, int64_t out_head, float* lse, const void* q, int64_t q_token,
+                                     int64_t q_head, int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                     const lora_b200_paged_cache* cache, const int32_t* block_tables, int64_t table_ld,
+                                     int32_t table_width, const int32_t* context_lens, float scale, int32_t window,
+                                     int32_t sinks, int32_t dtype, void* workspace, size_t workspace_bytes, void* stream);
+int lora_b200_paged_prefill_attention(void* out, int64_t out_token, int64_t out_head, float* lse, const void* q, int64_t q_token,
+                                      int64_t q_head, int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                      const lora_b200_paged_cache* cache, const int32_t* block_tables, int64_t table_ld,
+                                      int32_t table_width, const int32_t* context_lens, const int32_t* cu_seqlens,
+                                      int32_t n_seqs, float scale, int32_t window, int32_t sinks, int32_t dtype,
+                                      void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -29,6 +29,14 @@ E_INVAL, E_UNSUPPORTED, E_CUDA, E_WORKSPACE = -1, -2, -3, -4
 
 _DTYPES = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, torch.float32: DT_F32}
 
+
+class PagedCache(ctypes.Structure):
+    """``lora_b200_paged_cache``"""
+
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("num_blocks", c_int32), ("block_size", c_int32), ("k_block", c_int64),
+                ("k_token", c_int64), ("k_head", c_int64), ("v_block", c_int64), ("v_token", c_int64), ("v_head", c_int64)]
+
+
 #: every symbol declared in include/b200_lora.h, with (restype, argtypes)
 _SIGNATURES = {
     "lora_b200_version": (c_int32, []),
@@ -123,6 +131,21 @@ _SIGNATURES = {
         c_int32,
         [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32,
          c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_float, c_void_p],
+    ),
+    "lora_b200_glue_qk_norm_rope_kv_store": (
+        c_int32, [c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p,
+                  c_int32, c_int32, c_int32, c_void_p, c_int64, POINTER(PagedCache), c_void_p, c_int32, c_void_p],
+    ),
+    "lora_b200_paged_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32]),
+    "lora_b200_paged_decode_attention": (
+        c_int32,
+        [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, POINTER(PagedCache),
+         c_void_p, c_int64, c_int32, c_void_p, c_float, c_int32, c_int32, c_int32, c_void_p, c_size_t, c_void_p],
+    ),
+    "lora_b200_paged_prefill_attention": (
+        c_int32,
+        [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, POINTER(PagedCache),
+         c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_int32, c_float, c_int32, c_int32, c_int32, c_void_p, c_size_t, c_void_p],
     ),
     "lora_b200_tp_allreduce": (
         c_int32, [c_void_p, c_void_p, c_int32, POINTER(c_void_p), c_int32, c_int32, c_int32, c_void_p],

@@ -14,6 +14,8 @@
 #include "grouped_tc.cuh"
 #include "decode_step.cuh"
 #include "prefill_attention.cuh"
+#include "head_norm.cuh"
+#include "paged_attention.cuh"
 
 using namespace b200lora;
 
@@ -332,6 +334,84 @@ int lora_b200_prefill_attention(void* out, int64_t out_ld, const void* qkv, int6
   a.qkv = static_cast<const __nv_bfloat16*>(qkv); a.ld = qkv_ld; a.out = static_cast<__nv_bfloat16*>(out); a.out_ld = out_ld;
   a.cu_seqlens = cu_seqlens; a.Hq = num_heads; a.Hk = num_kv_heads; a.T = T; a.scale = scale;
   return prefill_attention_launch(a, head_dim, n_seqs, max_seqlen, static_cast<cudaStream_t>(stream));
+}
+
+int lora_b200_glue_qk_norm_rope_kv_store(void* qkv, int64_t qkv_ld, int32_t T, int32_t num_heads, int32_t num_kv_heads,
+                                         int32_t head_dim, const void* q_weight, const void* k_weight, float eps,
+                                         const int64_t* positions, const void* cos_table, const void* sin_table,
+                                         int32_t table_dim, int32_t table_dtype, int32_t max_position, void* q_out,
+                                         int64_t q_out_ld, const lora_b200_paged_cache* cache, const int32_t* slot_mapping,
+                                         int32_t dtype, void* stream) {
+  HeadNormParams p = {};
+  p.r.qkv = qkv; p.r.qkv_ld = qkv_ld; p.r.T = T; p.r.Hq = num_heads; p.r.Hk = num_kv_heads; p.r.D = head_dim;
+  p.r.positions = positions; p.r.cos = cos_table; p.r.sin = sin_table;
+  p.r.table_dim = table_dim; p.r.table_dtype = table_dtype; p.r.max_pos = max_position; p.r.slot_mapping = slot_mapping;
+  p.r.apply_rope = (cos_table != nullptr || sin_table != nullptr || positions != nullptr) ? 1 : 0;
+  p.q_weight = q_weight; p.k_weight = k_weight; p.eps = eps; p.q_out = q_out; p.q_out_ld = q_out_ld;
+  if (cache != nullptr) {
+    if (cache->k == nullptr) return fail(B200_LORA_EINVAL, "qk_norm_rope_kv_store: a cache is null");
+    p.cache = *cache;
+  }
+  return head_norm_launch(p, dtype, static_cast<cudaStream_t>(stream));
+}
+
+size_t lora_b200_paged_workspace_bytes(int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t prefill) {
+  (void)T; (void)prefill;
+  if (num_kv_heads < 1 || num_heads < num_kv_heads || head_dim < 1) return 0;
+  return paged_workspace_bytes(num_heads, num_kv_heads, head_dim);
+}
+
+// What decode and prefill have in common; cu_seqlens null: decode
+static int paged_attention_checked(const char* what, void* out, int64_t out_token, int64_t out_head, float* lse, const void* q, int64_t q_token,
+                                   int64_t q_head, int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                   const lora_b200_paged_cache* cache, const int32_t* block_tables, int64_t table_ld,
+                                   int32_t table_width, const int32_t* context_lens, const int32_t* cu_seqlens, int32_t n_seqs,
+                                   bool prefill, float scale, int32_t window, int32_t sinks, int32_t dtype, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  if (T < 0 || n_seqs < 0 || table_width < 0 || window < 0 || sinks < 0)
+    return fail(B200_LORA_EINVAL, "%s: T=%d, %d sequences, %d table entries, window %d, sinks %d", what, T, n_seqs, table_width, window, sinks);
+  if (num_kv_heads < 1 || num_heads < 1 || num_heads % num_kv_heads != 0)
+    return fail(B200_LORA_EINVAL, "%s: %d heads over %d kv heads", what, num_heads, num_kv_heads);
+  if (!(scale > 0.f) || scale > 3.0e38f) return fail(B200_LORA_EINVAL, "%s: scale must be positive and finite", what);
+  if (dtype != B200_LORA_BF16 && dtype != B200_LORA_F16) return fail(B200_LORA_EUNSUPPORTED, "%s: bf16 and fp16 only", what);
+  if (head_dim != 64 && head_dim != 128) return fail(B200_LORA_EUNSUPPORTED, "%s: head_dim %d (64 and 128 only)", what, head_dim);
+  if (T == 0 || n_seqs == 0) return B200_LORA_OK;
+  if (!out || !q || !cache || (!block_tables && table_width > 0) || !context_lens || (prefill && !cu_seqlens)) return fail(B200_LORA_EINVAL, "%s: null pointer", what);
+  int rc = paged_cache_check(*cache, what);
+  if (rc != B200_LORA_OK) return rc;
+  if (!aligned16(q) || !aligned16(out) || q_token % 8 || q_head % 8 || out_token % 8 || out_head % 8)
+    return fail(B200_LORA_EUNSUPPORTED, "%s: rows of q and out must start on 16-byte boundaries", what);
+  if (!aligned16(workspace)) return fail(B200_LORA_EUNSUPPORTED, "%s: the workspace must be 16-byte aligned", what);
+  if (workspace == nullptr || workspace_bytes < lora_b200_paged_workspace_bytes(T, num_heads, num_kv_heads, head_dim, prefill))
+    return fail(B200_LORA_EWORKSPACE, "%s: %zu bytes of workspace, needs %zu", what, workspace == nullptr ? (size_t)0 : workspace_bytes,
+                lora_b200_paged_workspace_bytes(T, num_heads, num_kv_heads, head_dim, prefill));
+  PagedArgs a = {};
+  a.q = q; a.q_token = q_token; a.q_head = q_head; a.out = out; a.out_token = out_token; a.out_head = out_head; a.lse = lse;
+  a.cache = *cache; a.tables = block_tables; a.table_ld = table_ld; a.table_width = table_width; a.context_lens = context_lens;
+  a.cu_seqlens = cu_seqlens; a.n_req = n_seqs; a.T = T; a.Hq = num_heads; a.Hk = num_kv_heads; a.window = window; a.sinks = sinks;
+  a.sc = scale * 1.4426950408889634f;
+  return paged_decode_launch(a, head_dim, dtype, workspace, static_cast<cudaStream_t>(stream));
+}
+
+int lora_b200_paged_decode_attention(void* out, int64_t out_token, int64_t out_head, float* lse, const void* q, int64_t q_token,
+                                     int64_t q_head, int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                     const lora_b200_paged_cache* cache, const int32_t* block_tables, int64_t table_ld,
+                                     int32_t table_width, const int32_t* context_lens, float scale, int32_t window,
+                                     int32_t sinks, int32_t dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  return paged_attention_checked("paged_decode_attention", out, out_token, out_head, lse, q, q_token, q_head, T, num_heads, num_kv_heads,
+                                 head_dim, cache, block_tables, table_ld, table_width, context_lens, nullptr, T, false, scale, window, sinks,
+                                 dtype, workspace, workspace_bytes, stream);
+}
+
+int lora_b200_paged_prefill_attention(void* out, int64_t out_token, int64_t out_head, float* lse, const void* q, int64_t q_token,
+                                      int64_t q_head, int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                      const lora_b200_paged_cache* cache, const int32_t* block_tables, int64_t table_ld,
+                                      int32_t table_width, const int32_t* context_lens, const int32_t* cu_seqlens,
+                                      int32_t n_seqs, float scale, int32_t window, int32_t sinks, int32_t dtype,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
+  return paged_attention_checked("paged_prefill_attention", out, out_token, out_head, lse, q, q_token, q_head, T, num_heads, num_kv_heads,
+                                 head_dim, cache, block_tables, table_ld, table_width, context_lens, cu_seqlens, n_seqs, true, scale, window,
+                                 sinks, dtype, workspace, workspace_bytes, stream);
 }
 
 size_t lora_b200_tp_exchange_bytes(int32_t tp, int32_t capacity) { return tp_exchange_bytes(tp, capacity); }

@@ -40,6 +40,10 @@ decltype(&lora_b200_glue_rope_kv_store) p_rope = nullptr;
 decltype(&lora_b200_shrink_buckets) p_shrink = nullptr;
 decltype(&lora_b200_expand_buckets) p_expand = nullptr;
 decltype(&lora_b200_prefill_attention) p_attention = nullptr;
+decltype(&lora_b200_glue_qk_norm_rope_kv_store) p_head_norm = nullptr;
+decltype(&lora_b200_paged_workspace_bytes) p_paged_bytes = nullptr;
+decltype(&lora_b200_paged_decode_attention) p_paged_decode = nullptr;
+decltype(&lora_b200_paged_prefill_attention) p_paged_prefill = nullptr;
 PyObject* scratch_for = nullptr;  // lora.scratch_for(device, bytes)
 PyObject *s_weight, *s_lora_a, *s_tts, *s_sorted, *s_ids, *s_counts, *s_offsets, *s_num_active;
 
@@ -517,6 +521,129 @@ PyObject* rope_kv_store(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// A cache [blocks, block size, kv heads, head dim] with adjacent elements in a row; false = not handled
+bool read_cache(PyObject* ko, PyObject* vo, at::ScalarType dt, int64_t hk, int64_t d, int dev, lora_b200_paged_cache* c) {
+  const at::Tensor *k = tensor_of(ko), *v = tensor_of(vo);
+  if (k == nullptr || v == nullptr || !on(*k, dev) || !on(*v, dev) || k->scalar_type() != dt || v->scalar_type() != dt || k->dim() != 4 ||
+      k->sizes() != v->sizes() || k->stride(3) != 1 || v->stride(3) != 1 || (hk >= 0 && k->size(2) != hk) || k->size(3) != d ||
+      k->size(0) < 1 || k->size(1) < 1 || k->size(0) > INT32_MAX || k->size(1) > INT32_MAX)
+    return false;
+  *c = {k->data_ptr(), v->data_ptr(), (int32_t)k->size(0), (int32_t)k->size(1), k->stride(0), k->stride(1), k->stride(2),
+        v->stride(0), v->stride(1), v->stride(2)};
+  return true;
+}
+
+// qk_norm_rope_kv_store(qkv, heads, kv_heads, head_dim, q_weight, k_weight, eps, positions, cos, sin, k_cache, v_cache, slot_mapping,
+// q_out | None) -> (status, q, k | None, v), or None; the form with rotation and caches
+PyObject* qk_norm_rope_kv_store(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 14) { PyErr_SetString(PyExc_TypeError, "qk_norm_rope_kv_store takes 14 arguments"); return nullptr; }
+  const at::Tensor *qkv = tensor_of(args[0]), *qw = tensor_of(args[4]), *kw = tensor_of(args[5]), *pos = tensor_of(args[7]),
+                   *cos = tensor_of(args[8]), *sin = tensor_of(args[9]), *slots = tensor_of(args[12]);
+  if (!qkv || !qw || !kw || !pos || !cos || !sin || !slots || !qkv->is_cuda() || qkv->dim() != 2 || qkv->stride(1) != 1) return not_handled();
+  const int dev = qkv->get_device();
+  if (dev != c10::cuda::current_device()) return not_handled();
+  const at::ScalarType dt = qkv->scalar_type();
+  const int code = dtype_code(dt), table = dtype_code(cos->scalar_type());
+  const int64_t hq = PyLong_AsLongLong(args[1]), hk = PyLong_AsLongLong(args[2]), d = PyLong_AsLongLong(args[3]);
+  const double eps = PyFloat_AsDouble(args[6]);
+  if (PyErr_Occurred()) { PyErr_Clear(); return not_handled(); }
+  const int64_t T = qkv->size(0), ld = qkv->stride(0);
+  if (code < 0 || table < 0 || T > INT32_MAX || hq < 0 || hk < 1 || d < 1 || hq > 65536 || hk > 65536 || d > 65536 ||
+      qkv->size(1) != (hq + 2 * hk) * d)
+    return not_handled();
+  for (const at::Tensor* t : {qw, kw, pos, cos, sin, slots})
+    if (!on(*t, dev) || !t->is_contiguous()) return not_handled();
+  if (qw->scalar_type() != dt || kw->scalar_type() != dt || qw->numel() != d || kw->numel() != d || pos->scalar_type() != at::kLong ||
+      pos->numel() != T || cos->dim() != 2 || cos->sizes() != sin->sizes() || sin->scalar_type() != cos->scalar_type() ||
+      cos->size(0) > INT32_MAX || slots->scalar_type() != at::kInt || slots->numel() != T)
+    return not_handled();
+  lora_b200_paged_cache cache;
+  if (!read_cache(args[10], args[11], dt, hk, d, dev, &cache)) return not_handled();
+  const at::Tensor* out = nullptr;
+  if (args[13] != Py_None) {
+    out = tensor_of(args[13]);
+    if (out == nullptr || !on(*out, dev) || out->scalar_type() != dt || out->dim() != 3 || out->size(0) != T || out->size(1) != hq ||
+        out->size(2) != d || out->stride(2) != 1 || (hq > 1 && out->stride(1) != d))
+      return not_handled();
+  }
+  const int rc = p_head_norm(qkv->data_ptr(), ld, (int)T, (int)hq, (int)hk, (int)d, qw->data_ptr(), kw->data_ptr(), (float)eps,
+                             static_cast<const int64_t*>(pos->data_ptr()), cos->data_ptr(), sin->data_ptr(), (int)cos->size(1), table,
+                             (int)cos->size(0), out ? out->data_ptr() : nullptr, out ? (T > 1 ? out->stride(0) : hq * d) : 0, &cache,
+                             static_cast<const int32_t*>(slots->data_ptr()), code, c10::cuda::getCurrentCUDAStream(dev).stream());
+  const int64_t off = qkv->storage_offset();
+  auto view = [&](int64_t heads, int64_t first) {
+    return THPVariable_Wrap(qkv->as_strided({T, heads, d}, {ld, d, 1}, off + first));
+  };
+  if (out != nullptr) return Py_BuildValue("(iOON)", rc, args[13], Py_None, view(hk, (hq + hk) * d));
+  return Py_BuildValue("(iNNN)", rc, view(hq, 0), view(hk, hq * d), view(hk, (hq + hk) * d));
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_attention(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens | None, scale, window, sinks, out | None, lse?)
+// -> (status, out, lse | None), or None
+PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 11) { PyErr_SetString(PyExc_TypeError, "paged_attention takes 11 arguments"); return nullptr; }
+  const at::Tensor *q = tensor_of(args[0]), *tables = tensor_of(args[3]), *ctx = tensor_of(args[4]), *cu = nullptr;
+  if (!q || !tables || !ctx || !q->is_cuda() || q->dim() != 3 || q->stride(2) != 1) return not_handled();
+  const int dev = q->get_device();
+  const at::ScalarType dt = q->scalar_type();
+  const int code = dtype_code(dt);
+  const int64_t T = q->size(0), hq = q->size(1), d = q->size(2);
+  if (code < 0 || dev != c10::cuda::current_device() || T > INT32_MAX || hq < 1 || hq > 65536 || d > 65536) return not_handled();
+  lora_b200_paged_cache cache;
+  if (!read_cache(args[1], args[2], dt, -1, d, dev, &cache)) return not_handled();
+  const int64_t hk = tensor_of(args[1])->size(2);
+  if (hk < 1 || hk > 65536) return not_handled();
+  for (const at::Tensor* t : {tables, ctx})
+    if (!on(*t, dev) || t->scalar_type() != at::kInt) return not_handled();
+  const int64_t n = ctx->numel();
+  if (ctx->dim() != 1 || !ctx->is_contiguous() || tables->dim() != 2 || tables->size(0) != n || tables->size(1) > INT32_MAX || n > INT32_MAX ||
+      (tables->size(1) > 1 && tables->stride(1) != 1))
+    return not_handled();
+  if (args[5] != Py_None) {
+    cu = tensor_of(args[5]);
+    if (cu == nullptr || !on(*cu, dev) || cu->scalar_type() != at::kInt || cu->dim() != 1 || !cu->is_contiguous() || cu->numel() != n + 1)
+      return not_handled();
+  } else if (n != T) {
+    return not_handled();
+  }
+  const double scale = PyFloat_AsDouble(args[6]);
+  const int64_t window = PyLong_AsLongLong(args[7]), sinks = PyLong_AsLongLong(args[8]);
+  if (PyErr_Occurred()) { PyErr_Clear(); return not_handled(); }
+  if (window < 0 || sinks < 0 || window > INT32_MAX || sinks > INT32_MAX || (sinks > 0 && window == 0)) return not_handled();
+  at::Tensor fresh, lse;
+  const at::Tensor* out = &fresh;
+  if (args[9] == Py_None) {
+    fresh = at::empty({T, hq, d}, q->options());
+  } else {
+    out = tensor_of(args[9]);
+    if (out == nullptr || !on(*out, dev) || out->scalar_type() != dt || out->sizes() != q->sizes() || out->stride(2) != 1) return not_handled();
+  }
+  if (args[10] == Py_True) lse = at::empty({T, hq}, q->options().dtype(at::kFloat));
+  const size_t need = p_paged_bytes((int)T, (int)hq, (int)hk, (int)d, cu ? 1 : 0);
+  const at::Tensor ws = at::empty({(int64_t)need}, q->options().dtype(at::kByte));
+  void* stream = c10::cuda::getCurrentCUDAStream(dev).stream();
+  float* lse_ptr = lse.defined() ? static_cast<float*>(lse.data_ptr()) : nullptr;
+  int rc;
+  if (cu != nullptr)
+    rc = p_paged_prefill(out->data_ptr(), out->stride(0), out->stride(1), lse_ptr, q->data_ptr(), q->stride(0), q->stride(1), (int)T, (int)hq,
+                         (int)hk, (int)d, &cache, static_cast<const int32_t*>(tables->data_ptr()), tables->stride(0), (int)tables->size(1),
+                         static_cast<const int32_t*>(ctx->data_ptr()), static_cast<const int32_t*>(cu->data_ptr()), (int)n, (float)scale,
+                         (int)window, (int)sinks, code, ws.data_ptr(), need, stream);
+  else
+    rc = p_paged_decode(out->data_ptr(), out->stride(0), out->stride(1), lse_ptr, q->data_ptr(), q->stride(0), q->stride(1), (int)T, (int)hq,
+                        (int)hk, (int)d, &cache, static_cast<const int32_t*>(tables->data_ptr()), tables->stride(0), (int)tables->size(1),
+                        static_cast<const int32_t*>(ctx->data_ptr()), (float)scale, (int)window, (int)sinks, code, ws.data_ptr(), need, stream);
+  PyObject* lse_out = Py_None;
+  if (lse.defined()) lse_out = THPVariable_Wrap(lse);
+  else Py_INCREF(Py_None);
+  if (args[9] != Py_None) return Py_BuildValue("(iON)", rc, args[9], lse_out);
+  return Py_BuildValue("(iNN)", rc, THPVariable_Wrap(fresh), lse_out);
+  END_HANDLE_TH_ERRORS
+}
+
 // One projection of a decoder layer: (parameters dict of the module, lora_B names | None, widths, columns, rank buffer).
 // lora_A is one parameter, stacked [slices, S, r, in] or a single [S, r, in].
 struct Projection {
@@ -855,6 +982,10 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   B200_BIND(p_expand, lora_b200_expand_buckets)
   B200_BIND(p_attention, lora_b200_prefill_attention)
   B200_BIND(p_rope, lora_b200_glue_rope_kv_store)
+  B200_BIND(p_head_norm, lora_b200_glue_qk_norm_rope_kv_store)
+  B200_BIND(p_paged_bytes, lora_b200_paged_workspace_bytes)
+  B200_BIND(p_paged_decode, lora_b200_paged_decode_attention)
+  B200_BIND(p_paged_prefill, lora_b200_paged_prefill_attention)
 #undef B200_BIND
   Py_INCREF(args[1]);
   Py_XDECREF(scratch_for);
@@ -864,7 +995,7 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 #define B200_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {B200_METHOD(add), B200_METHOD(shrink), B200_METHOD(expand), B200_METHOD(linear), B200_METHOD(add_rms_norm), B200_METHOD(silu_mul),
-                         B200_METHOD(rope_kv_store), B200_METHOD(prefill_layers), B200_METHOD(bucket_lists), B200_METHOD(pack_lists), B200_METHOD(bind), {nullptr, nullptr, 0, nullptr}};
+                         B200_METHOD(rope_kv_store), B200_METHOD(qk_norm_rope_kv_store), B200_METHOD(paged_attention), B200_METHOD(prefill_layers), B200_METHOD(bucket_lists), B200_METHOD(pack_lists), B200_METHOD(bind), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "b200lora_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -1,11 +1,14 @@
 """Decoder-layer glue around the projections as single launches: residual add + RMSNorm, RoPE + KV-cache
 store, SiLU * up. Host mirror of the reference's modules for these steps
 (``nanovllm_voxcpm/layers/layernorm.py``, ``layers/activation.py``, ``layers/attention.py:10-49``,
-``models/voxcpm2/model.py:81-94``); the kernels are ``csrc/glue.cuh`` behind ``lora_b200_glue_*``.
+``models/voxcpm2/model.py:81-94``), and the form of the middle one with norms of the heads; the kernels are ``csrc/glue.cuh`` and
+``csrc/head_norm.cuh`` behind ``lora_b200_glue_*``.
 CUDA tensors only, bf16 / fp16; there is no fallback path.
 """
 
 from __future__ import annotations
+
+import ctypes
 
 import torch
 import torch.nn as nn
@@ -149,6 +152,86 @@ def rope_kv_store(qkv: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim
             N.current_stream(qkv.device)))
     q, k, v = qkv2.split([q_size, kv_size, kv_size], dim=-1)
     return (q.view(T, num_heads, head_dim), k.view(T, num_kv_heads, head_dim), v.view(T, num_kv_heads, head_dim))
+
+
+def paged_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype: torch.dtype, kv_heads: int | None, head_dim: int) -> N.PagedCache:
+    """The caches ``[blocks, block_size, kv_heads, head_dim]`` (any strides with adjacent elements in a head) as the library takes
+    them."""
+    shape = k_cache.shape
+    if k_cache.dim() != 4 or v_cache.shape != shape or shape[3] != head_dim or (kv_heads is not None and shape[2] != kv_heads) or \
+            min(shape) < 1:
+        raise ValueError(f"the caches must be [blocks, block_size, kv_heads, head_dim] tensors of one shape, got {tuple(shape)} and "
+                         f"{tuple(v_cache.shape)}")
+    if k_cache.dtype != dtype or v_cache.dtype != dtype:
+        raise ValueError(f"the caches must be {dtype}, as the rows are")
+    if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
+        raise ValueError("the elements of a cache row must be adjacent")
+    return N.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), shape[0], shape[1], *k_cache.stride()[:3], *v_cache.stride()[:3])
+
+
+def qk_norm_rope_kv_store(qkv: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, q_weight: torch.Tensor,
+                          k_weight: torch.Tensor, eps: float, *, positions: torch.Tensor | None = None,
+                          cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, k_cache: torch.Tensor | None = None,
+                          v_cache: torch.Tensor | None = None, slot_mapping: torch.Tensor | None = None,
+                          q_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor]:
+    """``rope_kv_store`` with an RMS norm of every query and key head (``q_weight`` / ``k_weight`` ``[head_dim]``) ahead of the
+    rotation; fp32 throughout, rounded once. The caches are ``[blocks, block_size, kv_heads, head_dim]`` and may be strided (one
+    tensor that holds k and v of a block, heads ahead of positions); ``slot_mapping`` int32 holds block * block_size + position in
+    the block, each at most once; slots outside the cache (-1) are skipped.
+
+    Returns the ``q, k, v`` views of ``qkv``, q and k replaced IN PLACE; or, with ``q_out [T, num_heads, head_dim]``, leaves
+    ``qkv`` as it is and returns ``q_out, None, v``: k is in the cache only."""
+    if k_cache is not None:
+        got = N.native().qk_norm_rope_kv_store(qkv, num_heads, num_kv_heads, head_dim, q_weight, k_weight, eps, positions, cos, sin,
+                                               k_cache, v_cache, slot_mapping, q_out)
+        if got is not None:
+            N.check(got[0])
+            return got[1], got[2], got[3]
+    N.require_cuda(qkv, q_weight, k_weight, positions, cos, sin, k_cache, v_cache, slot_mapping, q_out)
+    qkv2 = _rows(qkv, "qkv")
+    T = qkv2.size(0)
+    q_size, kv_size = num_heads * head_dim, num_kv_heads * head_dim
+    if min(num_heads, num_kv_heads, head_dim) < 0 or qkv2.size(1) != q_size + 2 * kv_size:
+        raise ValueError("qkv rows must hold q | k | v")
+    for w in (q_weight, k_weight):
+        if w.dtype != qkv.dtype or w.numel() != head_dim or not w.is_contiguous():
+            raise ValueError("the norm weights must be contiguous [head_dim] vectors of the dtype of qkv")
+    rope = positions is not None or cos is not None or sin is not None
+    table_dim = table_dtype = max_pos = 0
+    if rope:
+        if positions is None or cos is None or sin is None:
+            raise ValueError("rotation needs positions, cos and sin")
+        if positions.dtype != torch.int64 or positions.numel() != T or not positions.is_contiguous():
+            raise ValueError("positions must be a contiguous int64 tensor with one entry per row")
+        if cos.shape != sin.shape or cos.dim() != 2 or cos.dtype != sin.dtype or not (cos.is_contiguous() and sin.is_contiguous()):
+            raise ValueError("cos and sin must be contiguous [max_position, dim] tables of one dtype")
+        max_pos, table_dim = cos.shape
+        table_dtype = N.dtype_code(cos.dtype)
+    if (k_cache is None) != (v_cache is None):
+        raise ValueError("k_cache and v_cache come together")
+    cache = None
+    if k_cache is not None:
+        if slot_mapping is None or slot_mapping.dtype != torch.int32 or slot_mapping.numel() != T or not slot_mapping.is_contiguous():
+            raise ValueError("slot_mapping must be a contiguous int32 tensor with one entry per row")
+        cache = paged_cache(k_cache, v_cache, qkv.dtype, num_kv_heads, head_dim)
+    if q_out is not None:
+        if cache is None:
+            raise ValueError("with q_out, k goes to the cache only: it needs one")
+        if q_out.shape != (T, num_heads, head_dim) or q_out.dtype != qkv.dtype or q_out.stride(2) != 1 or \
+                (num_heads > 1 and q_out.stride(1) != head_dim):
+            raise ValueError("q_out must be [T, num_heads, head_dim] of the dtype of qkv, with a token's heads side by side")
+    devices = {t.device for t in (qkv, q_weight, k_weight, positions, cos, sin, k_cache, v_cache, slot_mapping, q_out) if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f"tensors on several devices: {sorted(map(str, devices))}")
+    with N.on_device(qkv.device):
+        N.check(N.lib().lora_b200_glue_qk_norm_rope_kv_store(
+            qkv2.data_ptr(), qkv2.stride(0), T, num_heads, num_kv_heads, head_dim, q_weight.data_ptr(), k_weight.data_ptr(), float(eps),
+            N.ptr(positions), N.ptr(cos), N.ptr(sin), table_dim, table_dtype, max_pos, N.ptr(q_out),
+            0 if q_out is None else q_out.stride(0) if T > 1 else q_size, None if cache is None else ctypes.byref(cache),
+            N.ptr(slot_mapping) if cache is not None else None, N.dtype_code(qkv.dtype), N.current_stream(qkv.device)))
+    q, k, v = qkv2.split([q_size, kv_size, kv_size], dim=-1)
+    v = v.view(T, num_kv_heads, head_dim)
+    return (q.view(T, num_heads, head_dim), k.view(T, num_kv_heads, head_dim), v) if q_out is None else (q_out, None, v)
 
 
 def store_kvcache(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
