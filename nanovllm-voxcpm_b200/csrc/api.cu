@@ -16,6 +16,7 @@
 #include "prefill_attention.cuh"
 #include "head_norm.cuh"
 #include "paged_attention.cuh"
+#include "paged_prefill.cuh"
 
 using namespace b200lora;
 
@@ -390,6 +391,7 @@ static int paged_attention_checked(const char* what, void* out, int64_t out_toke
   a.cache = *cache; a.tables = block_tables; a.table_ld = table_ld; a.table_width = table_width; a.context_lens = context_lens;
   a.cu_seqlens = cu_seqlens; a.n_req = n_seqs; a.T = T; a.Hq = num_heads; a.Hk = num_kv_heads; a.window = window; a.sinks = sinks;
   a.sc = scale * 1.4426950408889634f;
+  if (prefill) return paged_prefill_launch(a, head_dim, dtype, workspace, static_cast<cudaStream_t>(stream));
   return paged_decode_launch(a, head_dim, dtype, workspace, static_cast<cudaStream_t>(stream));
 }
 

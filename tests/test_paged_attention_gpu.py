@@ -145,6 +145,12 @@ def test_prefill_pages_and_windows(page, window, sinks):
     PP.check(p, *_prefill(p, return_lse=True), f"pages of {page}, window {window}, {sinks} sinks")
 
 
+@pytest.mark.parametrize("page", [1, 7, 12, 100])
+def test_prefill_pages_that_the_tile_kernel_does_not_take(page):
+    p = PP.make(8, 2, 64, page, [130, 61], [30, 61], window=40, sinks=3, seed=page, poison=True)
+    PP.check(p, *_prefill(p, return_lse=True), f"pages of {page}")
+
+
 def test_prefill_tokens_ahead_of_their_context():
     """More new tokens than the context holds: the first ones have no position, see nothing and give zeros."""
     p = PP.make(8, 2, 64, 16, [5], [9], seed=4)
