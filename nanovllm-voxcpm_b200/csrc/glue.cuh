@@ -35,7 +35,21 @@ struct Vec8 {
   uint4 raw;
   __device__ __forceinline__ float get(int i) const { return to_float<T>(reinterpret_cast<const T*>(&raw)[i]); }
   __device__ __forceinline__ void set(int i, float v) { reinterpret_cast<T*>(&raw)[i] = from_float<T>(v); }
+  __device__ __forceinline__ float2 pair(int i) const;  // values 2 i and 2 i + 1
+  __device__ __forceinline__ void set_pair(int i, float2 v);
 };
+
+template <>
+__device__ __forceinline__ float2 Vec8<__nv_bfloat16>::pair(int i) const {
+  const uint32_t v = reinterpret_cast<const uint32_t*>(&raw)[i];
+  return make_float2(bf16_lo(v), bf16_hi(v));
+}
+template <>
+__device__ __forceinline__ float2 Vec8<__half>::pair(int i) const { return unpack_f16x2(reinterpret_cast<const uint32_t*>(&raw)[i]); }
+template <>
+__device__ __forceinline__ void Vec8<__nv_bfloat16>::set_pair(int i, float2 v) { reinterpret_cast<uint32_t*>(&raw)[i] = pack_bf16x2(v.x, v.y); }
+template <>
+__device__ __forceinline__ void Vec8<__half>::set_pair(int i, float2 v) { reinterpret_cast<uint32_t*>(&raw)[i] = pack_f16x2(v.x, v.y); }
 
 // One warp per row. `residual` may be null (plain rms_norm of x); `hidden_out` may be null or alias
 // `residual` / `x`. norm_of_rounded_sum = 1: the norm sees the sum rounded to T (hidden = residual + x,

@@ -17,87 +17,230 @@ struct HeadNormParams {
   lora_b200_paged_cache cache;
 };
 
-// `lanes` threads (a power of two) keep a head: each 8 columns of the first half and the 8 opposite ones. They take `per_group`
-// heads of one token in turn, with the angles in registers.
-template <typename T>
-__global__ void __launch_bounds__(kRopeThreads) head_norm_kernel(const HeadNormParams p, int lanes, int per_group) {
-  glue_enter();
-  const int half = p.r.D >> 1, heads = p.r.Hq + 2 * p.r.Hk, groups = (heads + per_group - 1) / per_group;
-  const int64_t unit = ((int64_t)blockIdx.x * kRopeThreads + threadIdx.x) / lanes;
-  const int64_t tok64 = unit / groups;
-  const int tok = (int)min(tok64, (int64_t)p.r.T - 1), j = 8 * (threadIdx.x & (lanes - 1));
-  const int head0 = (int)(unit - tok64 * groups) * per_group;
-  const bool live = tok64 < p.r.T && j < half;  // (the others take part in the sums of their warp)
-  T* const row = static_cast<T*>(p.r.qkv) + (int64_t)tok * p.r.qkv_ld + j;
+// Two fp32 operations in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)), "l"(reinterpret_cast<const uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+  return d;
+}
 
-  float c1[8], s1[8], c2[8], s2[8];
-  if (p.r.apply_rope && live) {
-    int64_t pos = p.r.positions[tok];
-    pos = pos < 0 ? 0 : (pos >= p.r.max_pos ? p.r.max_pos - 1 : pos);
-    const int64_t tb = pos * p.r.table_dim + j;
-    const int hi_off = p.r.table_dim == p.r.D ? half : 0;
-    table_load8(p.r.cos, p.r.table_dtype, tb, c1);
-    table_load8(p.r.sin, p.r.table_dtype, tb, s1);
-    table_load8(p.r.cos, p.r.table_dtype, tb + hi_off, c2);
-    table_load8(p.r.sin, p.r.table_dtype, tb + hi_off, s2);
-  } else {
+// Weights and rotation of a thread's columns as one: lo' = rstd (a1 lo + b1 hi), hi' = rstd (a2 lo + b2 hi)
+struct HeadTurn {
+  float2 a1[4], b1[4], a2[4], b2[4];
+  // at `tb` of the tables: the angles of the first of the thread's columns; w1, w2: its weights in the two halves
+  template <typename T>
+  __device__ __forceinline__ void load(const RopeKvParams& r, const Vec8<T>& w1, const Vec8<T>& w2, const void* cos, const void* sin, int64_t tb) {
+    const int half = r.D >> 1;
+    float c[8], s[8];
+    if (r.apply_rope) {
+      table_load8(cos, r.table_dtype, tb, c);
+      table_load8(sin, r.table_dtype, tb, s);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) { c1[e] = c2[e] = 1.f; s1[e] = s2[e] = 0.f; }
+      for (int e = 0; e < 8; ++e) { c[e] = 1.f; s[e] = 0.f; }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      a1[e] = mul2(w1.pair(e), make_float2(c[2 * e], c[2 * e + 1]));
+      b1[e] = mul2(w2.pair(e), make_float2(-s[2 * e], -s[2 * e + 1]));
+    }
+    if (r.apply_rope && r.table_dim == r.D) {  // (the second half has angles of its own)
+      table_load8(cos, r.table_dtype, tb + half, c);
+      table_load8(sin, r.table_dtype, tb + half, s);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      a2[e] = mul2(w1.pair(e), make_float2(s[2 * e], s[2 * e + 1]));
+      b2[e] = mul2(w2.pair(e), make_float2(c[2 * e], c[2 * e + 1]));
+    }
   }
-  int64_t at_k = -1, at_v = -1;
-  if (p.cache.k != nullptr) {
-    const int slot = p.r.slot_mapping[tok];
-    if (slot >= 0 && slot < (int64_t)p.cache.num_blocks * p.cache.block_size) {
-      const int blk = slot / p.cache.block_size, in_block = slot - blk * p.cache.block_size;
-      at_k = blk * p.cache.k_block + in_block * p.cache.k_token + j;
-      at_v = blk * p.cache.v_block + in_block * p.cache.v_token + j;
+  template <typename T>
+  __device__ __forceinline__ void apply(Vec8<T>& lo, Vec8<T>& hi, float rstd) const {
+    const float2 r2 = make_float2(rstd, rstd);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 a = lo.pair(e), b = hi.pair(e);
+      lo.set_pair(e, mul2(r2, fma2(b, b1[e], mul2(a, a1[e]))));
+      hi.set_pair(e, mul2(r2, fma2(b, b2[e], mul2(a, a2[e]))));
     }
   }
-  for (int i = 0; i < per_group; ++i) {
-    const int head = head0 + i, kv = head - p.r.Hq, v = kv - p.r.Hk;  // kv < 0: a q head; v < 0: a q or k head
-    const bool here = live && head < heads;
-    Vec8<T> lo, hi;
-    lo.raw = hi.raw = make_uint4(0, 0, 0, 0);
-    if (here) {
-      lo.raw = *reinterpret_cast<const uint4*>(row + (int64_t)head * p.r.D);
-      hi.raw = *reinterpret_cast<const uint4*>(row + (int64_t)head * p.r.D + half);
-    }
-    float x[2][8], ss = 0.f;
+};
+
+template <typename T>
+__device__ __forceinline__ Vec8<T> load8(const T* at) {
+  Vec8<T> v;
+  v.raw = *reinterpret_cast<const uint4*>(at);
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* at, const Vec8<T>& v) { *reinterpret_cast<uint4*>(at) = v.raw; }
+
+// Sum of the squares of a head over its 1 << lane_shift lanes; every lane of the warp calls it
+template <typename T>
+__device__ __forceinline__ float head_squares(const Vec8<T>& lo, const Vec8<T>& hi, int lane_shift) {
+  float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[0][e] = lo.get(e);
-      x[1][e] = hi.get(e);
-      ss += x[0][e] * x[0][e] + x[1][e] * x[1][e];
-    }
-    for (int o = lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (!here) continue;
-    if (v < 0) {
-      const float rstd = rsqrtf(ss / (float)p.r.D + p.eps);
-      const T* w = static_cast<const T*>(kv < 0 ? p.q_weight : p.k_weight) + j;
-      Vec8<T> w1, w2;
-      w1.raw = *reinterpret_cast<const uint4*>(w);
-      w2.raw = *reinterpret_cast<const uint4*>(w + half);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float a = x[0][e] * rstd * w1.get(e), b = x[1][e] * rstd * w2.get(e);
-        lo.set(e, a * c1[e] - b * s1[e]);
-        hi.set(e, b * c2[e] + a * s2[e]);
-      }
-    }
-    T* dst = nullptr;
-    if (kv < 0 && p.q_out != nullptr) dst = static_cast<T*>(p.q_out) + (int64_t)tok * p.q_out_ld + (int64_t)head * p.r.D + j;
-    else if (v < 0 && p.q_out == nullptr) dst = row + (int64_t)head * p.r.D;
-    if (dst != nullptr) {
-      *reinterpret_cast<uint4*>(dst) = lo.raw;
-      *reinterpret_cast<uint4*>(dst + half) = hi.raw;
-    }
-    if (kv >= 0 && at_k >= 0) {
-      T* c = v < 0 ? static_cast<T*>(p.cache.k) + at_k + kv * p.cache.k_head : static_cast<T*>(p.cache.v) + at_v + v * p.cache.v_head;
-      *reinterpret_cast<uint4*>(c) = lo.raw;
-      *reinterpret_cast<uint4*>(c + half) = hi.raw;
-    }
+  for (int e = 0; e < 4; ++e) {
+    const float2 a = lo.pair(e), b = hi.pair(e);
+    sum = fma2(b, b, fma2(a, a, sum));
+  }
+  float ss = sum.x + sum.y;
+  for (int o = (1 << lane_shift) >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  return ss;
+}
+
+__device__ __forceinline__ int64_t table_row(const RopeKvParams& r, int tok) {
+  const int64_t pos = r.positions[tok];
+  return (pos < 0 ? 0 : (pos >= r.max_pos ? r.max_pos - 1 : pos)) * r.table_dim;
+}
+
+// Where a token's k and v go: element offsets, -1: nowhere
+__device__ __forceinline__ void cache_rows(const HeadNormParams& p, int tok, int64_t* at_k, int64_t* at_v) {
+  *at_k = *at_v = -1;
+  if (p.cache.k == nullptr) return;
+  const int slot = p.r.slot_mapping[tok];
+  if (slot < 0 || slot >= (int64_t)p.cache.num_blocks * p.cache.block_size) return;
+  const int blk = slot / p.cache.block_size, in_block = slot - blk * p.cache.block_size;
+  *at_k = blk * p.cache.k_block + in_block * p.cache.k_token;
+  *at_v = blk * p.cache.v_block + in_block * p.cache.v_token;
+}
+
+// Results of columns j.. and D/2 + j.. of a head to where they belong
+template <typename T>
+__device__ __forceinline__ void store_head(const HeadNormParams& p, int tok, int head, int j, int64_t at_k, int64_t at_v, const Vec8<T>& lo, const Vec8<T>& hi) {
+  const int half = p.r.D >> 1, kv = head - p.r.Hq, v = kv - p.r.Hk;
+  T* dst = nullptr;
+  if (kv < 0 && p.q_out != nullptr) dst = static_cast<T*>(p.q_out) + (int64_t)tok * p.q_out_ld + (int64_t)head * p.r.D + j;
+  else if (v < 0 && p.q_out == nullptr) dst = static_cast<T*>(p.r.qkv) + (int64_t)tok * p.r.qkv_ld + (int64_t)head * p.r.D + j;
+  if (dst != nullptr) {
+    store8(dst, lo);
+    store8(dst + half, hi);
+  }
+  if (kv >= 0 && at_k >= 0) {
+    T* c = v < 0 ? static_cast<T*>(p.cache.k) + at_k + kv * p.cache.k_head + j : static_cast<T*>(p.cache.v) + at_v + v * p.cache.v_head + j;
+    store8(c, lo);
+    store8(c + half, hi);
   }
 }
+
+// Few tokens: 1 << lane_shift threads keep a head, each 8 columns of the first half and the 8 opposite ones.
+template <typename T>
+__global__ void __launch_bounds__(kRopeThreads) head_norm_kernel(const HeadNormParams p, int lane_shift) {
+  glue_enter();
+  const int half = p.r.D >> 1, heads = p.r.Hq + 2 * p.r.Hk;
+  const uint32_t unit = blockIdx.x * (kRopeThreads >> lane_shift) + (threadIdx.x >> lane_shift), tok_u = unit / (uint32_t)heads;
+  const int tok = (int)min(tok_u, (uint32_t)p.r.T - 1), j = 8 * (threadIdx.x & ((1 << lane_shift) - 1)), head = (int)(unit - tok_u * heads);
+  const bool live = tok_u < (uint32_t)p.r.T && j < half;  // (the others take part in the sums of their warp)
+  Vec8<T> lo, hi;
+  lo.raw = hi.raw = make_uint4(0, 0, 0, 0);
+  if (live) {
+    const T* src = static_cast<const T*>(p.r.qkv) + (int64_t)tok * p.r.qkv_ld + (int64_t)head * p.r.D + j;
+    lo = load8(src);
+    hi = load8(src + half);
+  }
+  const float ss = head_squares(lo, hi, lane_shift);
+  if (!live) return;
+  if (head < p.r.Hq + p.r.Hk) {
+    HeadTurn turn;
+    const T* w = static_cast<const T*>(head < p.r.Hq ? p.q_weight : p.k_weight) + j;
+    turn.load(p.r, load8(w), load8(w + half), p.r.cos, p.r.sin, p.r.apply_rope ? table_row(p.r, tok) + j : 0);
+    turn.apply(lo, hi, rsqrtf(ss / (float)p.r.D + p.eps));
+  }
+  int64_t at_k, at_v;
+  cache_rows(p, tok, &at_k, &at_v);
+  store_head(p, tok, head, j, at_k, at_v, lo, hi);
+}
+
+// Many tokens: the rows of `tokens` tokens and their table rows come by bulk copies into one of two stages while the other is
+// worked on, two CTAs on an SM; a thread keeps the angles and weights of its columns for all heads of its token that it takes.
+struct HeadRing { int tokens, row_bytes, table_bytes, stage_bytes; };
+
+template <typename T>
+__global__ void __launch_bounds__(kRopeThreads, 2) head_norm_ring_kernel(const HeadNormParams p, const HeadRing ring, int lane_shift) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ __align__(8) uint64_t full[2];
+  __shared__ volatile int abort_flag;
+  const int tid = threadIdx.x, half = p.r.D >> 1, heads = p.r.Hq + 2 * p.r.Hk;
+  if (tid == 0) {
+    mbar_init(smem_u32(&full[0]), 1);
+    mbar_init(smem_u32(&full[1]), 1);
+    abort_flag = 0;
+    mbar_fence_init();
+  }
+  __syncthreads();
+  glue_enter();
+  const int n_groups = (p.r.T + ring.tokens - 1) / ring.tokens;
+  const int one = ring.row_bytes + 2 * ring.table_bytes;  // bytes of a token
+  auto load = [&](int group, int st) {  // the first warp
+    const int t0 = group * ring.tokens, n = min(ring.tokens, p.r.T - t0);
+    const uint32_t bar = smem_u32(&full[st]), base = smem_u32(smem) + st * ring.stage_bytes;
+    if (tid == 0) mbar_arrive_expect_tx(bar, (uint32_t)(n * one));
+    __syncwarp();
+    for (int i = tid; i < n; i += 32) {
+      const uint32_t dst = base + i * one;
+      bulk_g2s(dst, static_cast<const char*>(p.r.qkv) + 2 * (int64_t)(t0 + i) * p.r.qkv_ld, ring.row_bytes, bar);
+      if (p.r.apply_rope) {
+        const int64_t at = table_row(p.r, t0 + i) * (p.r.table_dtype == B200_LORA_F32 ? 4 : 2);
+        bulk_g2s(dst + ring.row_bytes, static_cast<const char*>(p.r.cos) + at, ring.table_bytes, bar);
+        bulk_g2s(dst + ring.row_bytes + ring.table_bytes, static_cast<const char*>(p.r.sin) + at, ring.table_bytes, bar);
+      }
+    }
+  };
+  if (tid < 32)
+    for (int k = 0; k < 2; ++k)
+      if ((int)blockIdx.x + k * (int)gridDim.x < n_groups) load(blockIdx.x + k * gridDim.x, k);
+  const int sub = tid >> lane_shift, j = 8 * (tid & ((1 << lane_shift) - 1));
+  const int per_token = (kRopeThreads >> lane_shift) / ring.tokens;  // subgroups of a token
+  const int tok_in = sub / per_token, first = sub - tok_in * per_token;
+  for (int k = 0, group = blockIdx.x; group < n_groups; ++k, group += gridDim.x) {
+    const int st = k & 1, tok = group * ring.tokens + tok_in;
+    const bool live = tok < p.r.T && j < half;
+    int64_t at_k = -1, at_v = -1;
+    if (live) cache_rows(p, tok, &at_k, &at_v);
+    if (!mbar_wait_bounded(smem_u32(&full[st]), (uint32_t)((k >> 1) & 1), &abort_flag)) break;
+    const uint8_t* at = smem + st * ring.stage_bytes + tok_in * one;
+    const T* row = reinterpret_cast<const T*>(at) + j;
+    HeadTurn turn;
+    int kind = -1;  // of the weights in `turn`: 0 q, 1 k
+    for (int h = first; h - first < heads; h += per_token) {  // (all subgroups go round equally often: their lanes sum together)
+      const bool here = live && h < heads;
+      Vec8<T> lo, hi;
+      lo.raw = hi.raw = make_uint4(0, 0, 0, 0);
+      if (here) {
+        lo = load8(row + h * p.r.D);
+        hi = load8(row + h * p.r.D + half);
+      }
+      const float ss = head_squares(lo, hi, lane_shift);
+      if (!here) continue;
+      if (h < p.r.Hq + p.r.Hk) {
+        const int want = h < p.r.Hq ? 0 : 1;
+        if (kind != want) {
+          const T* w = static_cast<const T*>(want == 0 ? p.q_weight : p.k_weight) + j;
+          turn.load(p.r, load8(w), load8(w + half), at + ring.row_bytes, at + ring.row_bytes + ring.table_bytes, j);
+        }
+        kind = want;
+        turn.apply(lo, hi, rsqrtf(ss / (float)p.r.D + p.eps));
+      }
+      store_head(p, tok, h, j, at_k, at_v, lo, hi);
+    }
+    __syncthreads();
+    if (tid < 32 && group + 2 * (int)gridDim.x < n_groups) load(group + 2 * gridDim.x, st);
+  }
+  if (tid == 0 && abort_flag != 0) atomicOr(&g_b200_status, kStatusWaitGaveUp);
+}
+
+constexpr int kHeadStage = 52 << 10;  // bytes of a stage at most: two of them and two CTAs on an SM
+// Rows of a call, in bytes, from which the copies pay: us, a thread per piece / stages, heads 16 / 2 of 64: 1024 tokens (2.6 MB) 3.6 /
+// 4.9, 2048 7.3 / 7.4, 4096 11.0 / 9.2, 8192 20 / 15.5; 32 / 8 of 128: 256 tokens (3.1 MB) 3.5 / 5.6, 512 7.0 / 7.1, 1024 12.6 / 8.9,
+// 8192 81 / 44.
+constexpr int64_t kHeadRingBytes = 5 << 20;
 
 inline int paged_cache_check(const lora_b200_paged_cache& c, const char* what) {
   if (c.k == nullptr || c.v == nullptr) return fail(B200_LORA_EINVAL, "%s: a cache is null", what);
@@ -133,14 +276,33 @@ inline int head_norm_launch(const HeadNormParams& p, int dtype, cudaStream_t str
     if (rc != B200_LORA_OK) return rc;
     if (r.slot_mapping == nullptr) return fail(B200_LORA_EINVAL, "qk_norm_rope_kv_store: a cache needs slot_mapping");
   }
-  int lanes = 1;
-  while (lanes * 16 < r.D) lanes *= 2;
-  const int heads = r.Hq + 2 * r.Hk, per_group = 1;
-  const int64_t blocks = ((int64_t)r.T * ceil_div_i(heads, per_group) * lanes + kRopeThreads - 1) / kRopeThreads;
-  if (blocks > INT32_MAX) return fail(B200_LORA_EUNSUPPORTED, "qk_norm_rope_kv_store: %d rows of %d heads", r.T, heads);
-  if (dtype == B200_LORA_BF16)
-    return launch_dependent(head_norm_kernel<__nv_bfloat16>, "head_norm_kernel", dim3((unsigned)blocks), kRopeThreads, 0, stream, p, lanes, per_group);
-  return launch_dependent(head_norm_kernel<__half>, "head_norm_kernel", dim3((unsigned)blocks), kRopeThreads, 0, stream, p, lanes, per_group);
+  int lane_shift = 0;
+  while ((16 << lane_shift) < r.D) ++lane_shift;
+  const int heads = r.Hq + 2 * r.Hk;
+  HeadRing ring;
+  ring.row_bytes = (int)std::min<int64_t>(2 * width, 1 << 20);
+  ring.table_bytes = r.apply_rope ? r.table_dim * (r.table_dtype == B200_LORA_F32 ? 4 : 2) : 0;
+  const int one = ring.row_bytes + 2 * ring.table_bytes;
+  ring.tokens = 1;
+  while (2 * ring.tokens * one <= kHeadStage && 2 * ring.tokens <= (kRopeThreads >> lane_shift) && ceil_div_i(r.T, 2 * ring.tokens) >= 2 * 148) ring.tokens *= 2;
+  ring.stage_bytes = ring.tokens * one;
+  if (2 * width * r.T >= kHeadRingBytes && one <= kHeadStage) {
+    const int smem = 2 * ring.stage_bytes, grid = std::min(2 * 148, ceil_div_i(r.T, ring.tokens));
+#define B200_HEAD_RING(TT)                                                                                                                           \
+  {                                                                                                                                                  \
+    const cudaError_t e = cudaFuncSetAttribute(head_norm_ring_kernel<TT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kHeadStage);              \
+    if (e != cudaSuccess) return fail(B200_LORA_ECUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));                                          \
+    return launch_dependent(head_norm_ring_kernel<TT>, "head_norm_ring_kernel", dim3((unsigned)grid), kRopeThreads, (size_t)smem, stream, p, ring, lane_shift); \
+  }
+    if (dtype == B200_LORA_BF16) B200_HEAD_RING(__nv_bfloat16)
+    B200_HEAD_RING(__half)
+#undef B200_HEAD_RING
+  }
+  const int64_t units = (int64_t)r.T * heads;
+  if (units > INT32_MAX) return fail(B200_LORA_EUNSUPPORTED, "qk_norm_rope_kv_store: %d rows of %d heads", r.T, heads);
+  const dim3 blocks((unsigned)(((units << lane_shift) + kRopeThreads - 1) / kRopeThreads));
+  if (dtype == B200_LORA_BF16) return launch_dependent(head_norm_kernel<__nv_bfloat16>, "head_norm_kernel", blocks, kRopeThreads, 0, stream, p, lane_shift);
+  return launch_dependent(head_norm_kernel<__half>, "head_norm_kernel", blocks, kRopeThreads, 0, stream, p, lane_shift);
 }
 
 }  // namespace b200lora
