@@ -17,20 +17,6 @@ struct HeadNormParams {
   lora_b200_paged_cache cache;
 };
 
-// Two fp32 operations in one instruction
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(reinterpret_cast<uint64_t&>(d))
-      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)), "l"(reinterpret_cast<const uint64_t&>(c)));
-  return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(d)) : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
-  return d;
-}
-
 // Weights and rotation of a thread's columns as one: lo' = rstd (a1 lo + b1 hi), hi' = rstd (a2 lo + b2 hi)
 struct HeadTurn {
   float2 a1[4], b1[4], a2[4], b2[4];

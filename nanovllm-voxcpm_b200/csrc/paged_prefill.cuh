@@ -16,16 +16,22 @@
 namespace b200lora {
 
 constexpr int kPpRows = 128, kPpKeys = 128;       // of a tile
-// Two softmax warpgroups; a third with the loading warp and the MMA warp, which leaves its registers to them: the launch has 168 a
-// thread, 384 * 168 = 64512, and 2 * 208 + 88 = 3 * 168.
-constexpr int kPpThreads = 384, kPpSoftmaxRegs = 208, kPpOtherRegs = 88;
+#ifndef B200_POLY
+#define B200_POLY 16
+#endif
+constexpr int kPpPolyEvery = B200_POLY;
 constexpr int kPpPanel = kPpKeys * 128;           // bytes of 128 rows of 64 columns
+// One softmax warpgroup per tile; one more with the loading warp and the MMA warp, which leaves its registers to them. Two tiles: 168
+// registers a thread at launch, 384 * 168 = 64512, and 2 * 208 + 88 = 3 * 168; one tile, two CTAs on an SM: 128, and 208 + 48 = 2 * 128.
+__host__ __device__ constexpr int pp_threads(int tiles) { return 128 * (tiles + 1); }
+constexpr int kPpSoftmaxRegs = 208;
+__host__ __device__ constexpr int pp_other_regs(int tiles) { return tiles == 2 ? 88 : 48; }
 template <int D>
-__host__ __device__ constexpr int pp_stages() { return D == 64 ? 3 : 2; }
+__host__ __device__ constexpr int pp_stages(int tiles) { return (D == 64 ? 1 : 0) + tiles; }
 template <int D>
 __host__ __device__ constexpr int pp_tile() { return kPpKeys * D * 2; }
 template <int D>
-__host__ __device__ constexpr int pp_smem() { return (2 * pp_stages<D>() + 2) * pp_tile<D>() + 1024; }
+__host__ __device__ constexpr int pp_smem(int tiles) { return (2 * pp_stages<D>(tiles) + tiles) * pp_tile<D>() + 1024; }
 
 struct PpMaps { CUtensorMap q, k, v; };
 struct PpArgs {
@@ -78,14 +84,35 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// (NaN where one of them is)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^x for x <= 8 or so on the FMA units: x = n + f with n whole and f in [-0.5, 0.5] (adding and subtracting 1.5 * 2^23 rounds to n), 2^f
+// by a polynomial with constant term 1, least in its largest relative error (1.7e-7 in fp32; weighted least squares until the
+// extrema are even), n added to the exponent. From -127 down exactly 0.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  constexpr float kRound = 12582912.f;
+  x = make_float2(fmaxf(x.x, -127.f), fmaxf(x.y, -127.f));
+  const float2 t = add2(x, make_float2(kRound, kRound)), f = fma2(add2(t, make_float2(-kRound, -kRound)), make_float2(-1.f, -1.f), x);
+  float2 y = fma2(f, make_float2(0x1.5bba14p-10f, 0x1.5bba14p-10f), make_float2(0x1.3cea88p-7f, 0x1.3cea88p-7f));
+  y = fma2(f, y, make_float2(0x1.c6b752p-5f, 0x1.c6b752p-5f));
+  y = fma2(f, y, make_float2(0x1.ebf9bcp-3f, 0x1.ebf9bcp-3f));
+  y = fma2(f, y, make_float2(0x1.62e42ap-1f, 0x1.62e42ap-1f));
+  y = fma2(f, y, make_float2(1.f, 1.f));
+  return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23)), __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23)));
+}
 // bits [0, n) of a word, n of any sign and size
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
 
-template <int D, bool kF16>
-__global__ void __launch_bounds__(kPpThreads, 1) paged_prefill_kernel(const __grid_constant__ PpMaps maps, const __grid_constant__ PpArgs a) {
+template <int D, bool kF16, int kTiles>
+__global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_kernel(const __grid_constant__ PpMaps maps, const __grid_constant__ PpArgs a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  constexpr int kSt = pp_stages<D>(), kTile = pp_tile<D>(), kPanels = D / 64;
-  enum { Q_FULL, S_READY, P_READY = S_READY + 2, O_DONE = P_READY + 2, K_FULL = O_DONE + 2, K_FREE = K_FULL + kSt, V_FULL = K_FREE + kSt,
+  constexpr int kSt = pp_stages<D>(kTiles), kTile = pp_tile<D>(), kPanels = D / 64;
+  constexpr int kLoader = 4 * kTiles, kIssuer = kLoader + 1, kTmem = 256 * kTiles, kO = kTiles * kPpKeys;  // warps; columns: all, the first of O
+  enum { Q_FULL, S_READY, P_READY = S_READY + 2, O_DONE = P_READY + 4, K_FULL = O_DONE + 2, K_FREE = K_FULL + kSt, V_FULL = K_FREE + kSt,
          V_FREE = V_FULL + kSt, N_BARS = V_FREE + kSt };
   __shared__ __align__(8) uint64_t bars[N_BARS];
   __shared__ uint32_t s_tmem, s_boxes[4];
@@ -97,11 +124,11 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prefill_kernel(const __gr
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
 
   if (tid == 0) {
-    for (int i = 0; i < N_BARS; ++i) mbar_init(bar(i), i == P_READY || i == P_READY + 1 ? kPpRows : 1);
+    for (int i = 0; i < N_BARS; ++i) mbar_init(bar(i), i >= P_READY && i < O_DONE ? kPpRows : 1);
     abort_flag = 0;
     mbar_fence_init();
   }
-  if (warp == 9) tmem_alloc(smem_u32(&s_tmem), 512);
+  if (warp == kIssuer) tmem_alloc(smem_u32(&s_tmem), kTmem);
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
@@ -110,7 +137,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prefill_kernel(const __gr
 
   // ---- which tokens: the blocks of the sequences in order, the last ones first (their contexts are the longest)
   const int blk = a.n_blocks - 1 - (int)blockIdx.x / a.head_tiles, head0 = ((int)blockIdx.x % a.head_tiles) << a.h_shift;
-  const int per_tile = kPpRows >> a.h_shift, span = 2 * per_tile;
+  const int per_tile = kPpRows >> a.h_shift, span = kTiles * per_tile;
   int req = -1, begin = 0, len = 0, q0 = 0;
   for (int base = 0, run = 0; base < p.n_req && req < 0; base += 32) {
     const int i = base + lane;
@@ -147,11 +174,11 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prefill_kernel(const __gr
     const int n_tiles = key_end <= 0 || n_here == 0 ? 0 : sink_tiles + max(0, (key_end + kPpKeys - 1) / kPpKeys - first_tile);
     auto key0_of = [&](int i) { return (i < sink_tiles ? i : i - sink_tiles + first_tile) * kPpKeys; };
 
-    if (warp < 8) {  // ------------------------------------------------------------------- softmax
+    if (warp < kLoader) {  // ------------------------------------------------------------------- softmax
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPpSoftmaxRegs));
       const int t = warp >> 2, row = (warp & 3) * 32 + lane, tok = t * per_tile + (row >> a.h_shift), head = head0 + (row & ((1 << a.h_shift) - 1));
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-      const uint32_t s_at = tmem + t * kPpKeys + lanes, o_at = tmem + 2 * kPpKeys + t * D + lanes;
+      const uint32_t s_at = tmem + t * kPpKeys + lanes, o_at = tmem + kO + t * D + lanes;
       const int pos = pos0 + tok;
       const int lo = p.window > 0 ? max(pos, 0) - (p.window - 1) : 0;
       const int tile_lo = pos0 + t * per_tile, tile_hi = tile_lo + per_tile - 1;  // positions of the tile
@@ -164,32 +191,39 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prefill_kernel(const __gr
         tc_fence_after_sync();
         uint32_t s[4][32];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_at + 32 * c, s[c]);
+        for (int c = 0; c < 2; ++c) tmem_ld_32x32(s_at + 32 * c, s[c]);
         const uint32_t boxes = s_boxes[i & 3];
-        tmem_ld_wait();
-        if (key0 + kPpKeys - 1 > tile_lo || (p.window > 0 && key0 < max(tile_hi, 0) - (p.window - 1) && key0 + kPpKeys > p.sinks) || boxes != all_boxes) {
+        const bool masked = key0 + kPpKeys - 1 > tile_lo || (p.window > 0 && key0 < max(tile_hi, 0) - (p.window - 1) && key0 + kPpKeys > p.sinks) || boxes != all_boxes;
+        float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int at = key0 + 32 * c;
-            uint32_t seen = bits_below(pos + 1 - at) & (~bits_below(lo - at) | bits_below(p.sinks - at));
-            uint32_t there = 0;  // (a copy has 8 rows or more)
+        for (int half = 0; half < 2; ++half) {
+          tmem_ld_wait();
+          if (half == 0) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) there |= (boxes >> ((32 * c + 8 * g) >> box_shift)) & 1u ? 0xffu << (8 * g) : 0u;
-            seen &= there;
-            asm volatile("" : "+r"(seen));  // (one word at a time: 128 tests at once cost 350 bytes of spills)
+            for (int c = 2; c < 4; ++c) tmem_ld_32x32(s_at + 32 * c, s[c]);
+          }
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (!((seen >> j) & 1u)) s[c][j] = 0xff800000u;  // -inf
+          for (int c = 2 * half; c < 2 * half + 2; ++c) {
+            if (masked) {
+              const int at = key0 + 32 * c;
+              uint32_t seen = bits_below(pos + 1 - at) & (~bits_below(lo - at) | bits_below(p.sinks - at));
+              uint32_t there = 0;  // (a copy has 8 rows or more)
+#pragma unroll
+              for (int g = 0; g < 4; ++g) there |= (boxes >> ((32 * c + 8 * g) >> box_shift)) & 1u ? 0xffu << (8 * g) : 0u;
+              seen &= there;
+              asm volatile("" : "+r"(seen));  // (one word at a time: 128 tests at once cost 350 bytes of spills)
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (!((seen >> j) & 1u)) s[c][j] = 0xff800000u;  // -inf
+            }
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) top4[j / 2 % 4] = max3(top4[j / 2 % 4], __uint_as_float(s[c][j]), __uint_as_float(s[c][j + 1]));
           }
         }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) mx = fmaxf(mx, fmaxf(__uint_as_float(s[c][j]), __uint_as_float(s[c][j + 1])));
+        const float mx = max3(max3(top4[0], top4[1], top4[2]), top4[3], top4[3]);
         // The maximum moves only where it would grow by more than 2^8: until then probabilities stay below that, and O as it is.
         const float top = mx * p.sc;
-        const bool grows = top > m + 8.f;
+        const bool grows = !(top <= m + 8.f);  // (a NaN among the scores makes the maximum and with it the whole row NaN)
         if (__any_sync(0xffffffffu, grows)) {
           const float f = grows ? ex2(m - top) : 1.f;
           if (grows) m = top;
@@ -206,23 +240,27 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prefill_kernel(const __gr
             }
           }
         }
-        const float base = m == -INFINITY ? 0.f : -m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const float base = m == -INFINITY ? 0.f : fmaf(m, 0.f, -m);  // (an infinite score: NaN, as inf - inf)
+        const float2 scale2 = make_float2(p.sc, p.sc), base2 = make_float2(base, base);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t packed[16];
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
-            const float x = ex2(fmaf(__uint_as_float(s[c][j]), p.sc, base)), y = ex2(fmaf(__uint_as_float(s[c][j + 1]), p.sc, base));
-            sum[j / 2 % 4] += x + y;
-            packed[j / 2] = pack_16x2<kF16>(x, y);  // (rounded to the type of V; the sum is that of the unrounded ones)
+            const float2 x = fma2(make_float2(__uint_as_float(s[c][j]), __uint_as_float(s[c][j + 1])), scale2, base2);
+            const float2 y = j % kPpPolyEvery == kPpPolyEvery - 2 ? exp2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
+            sum[j / 2 % 2] = add2(sum[j / 2 % 2], y);
+            packed[j / 2] = pack_16x2<kF16>(y.x, y.y);  // (rounded to the type of V; the sum is that of the unrounded ones)
           }
           tmem_st_32x16(s_at + 16 * c, packed);
+          if (c & 1) {  // half of P: its products may begin
+            tmem_st_wait();
+            tc_fence_before_sync();
+            mbar_arrive(bar(P_READY + 2 * t + (c >> 1)));
+          }
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_st_wait();
-        tc_fence_before_sync();
-        mbar_arrive(bar(P_READY + t));
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }
       const bool live = tok < n_here;
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // (no visible key: zeros; NaN stays)
@@ -257,15 +295,15 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prefill_kernel(const __gr
       if (live && p.lse != nullptr) p.lse[token * p.Hq + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
       tc_fence_before_sync();
     } else {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPpOtherRegs));
-      if (warp == 8) {  // ------------------------------------------------------------------ loads
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(pp_other_regs(kTiles)));
+      if (warp == kLoader) {  // ------------------------------------------------------------------ loads
         const uint32_t leader = elect_one();
         const int kvh = head0 / (p.Hq / p.Hk);
         const int32_t* table = p.tables + req * p.table_ld;
         if (n_tiles > 0) {
           if (leader) {
-            mbar_arrive_expect_tx(bar(Q_FULL), 2 * kTile);
-            for (int t = 0; t < 2; ++t)
+            mbar_arrive_expect_tx(bar(Q_FULL), kTiles * kTile);
+            for (int t = 0; t < kTiles; ++t)
               for (int c = 0; c < kPanels; ++c)
                 tma_load_3d_at(q_u32 + t * kTile + c * kPpPanel, &maps.q, 64 * c, head0, begin + q0 + t * per_tile, bar(Q_FULL));
           }
@@ -298,7 +336,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prefill_kernel(const __gr
             }
           }
         }
-      } else if (warp == 9) {  // ---------------------------------------------------------- products
+      } else if (warp == kIssuer) {  // ---------------------------------------------------------- products
         const uint32_t leader = elect_one();
         const uint32_t type = kF16 ? 0u : (1u << 7) | (1u << 10);
         const uint32_t idesc_s = (1u << 4) | type | ((uint32_t)(kPpKeys >> 3) << 17) | ((uint32_t)(kPpRows >> 4) << 24);
@@ -317,8 +355,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prefill_kernel(const __gr
         if (n_tiles > 0) {
           pp_wait(bar(Q_FULL), 0, &abort_flag);
           pp_wait(bar(K_FULL), 0, &abort_flag);
-          scores(0, 0);
-          scores(1, 0);
+          for (int t = 0; t < kTiles; ++t) scores(t, 0);
           umma_commit_elected(bar(K_FREE), leader);
           for (int i = 0; i < n_tiles; ++i) {
             const int st = i % kSt, next = (i + 1) % kSt;
@@ -334,13 +371,16 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prefill_kernel(const __gr
               fence_proxy_async_smem();
               __syncwarp();
             }
-            for (int t = 0; t < 2; ++t) {
-              pp_wait(bar(P_READY + t), (uint32_t)(i & 1), &abort_flag);
-              tc_fence_after_sync();
-  #pragma unroll
-              for (int k = 0; k < kPpKeys / 16; ++k)
-                umma_ts_elected(tmem + 2 * kPpKeys + t * D, tmem + t * kPpKeys + 8 * k, lo_v(v_u32 + st * kTile + k * 2048), hi_k, idesc_o,
+            for (int t = 0; t < kTiles; ++t) {
+#pragma unroll
+              for (int k = 0; k < kPpKeys / 16; ++k) {
+                if (k % 4 == 0) {
+                  pp_wait(bar(P_READY + 2 * t + k / 4), (uint32_t)(i & 1), &abort_flag);
+                  tc_fence_after_sync();
+                }
+                umma_ts_elected(tmem + kO + t * D, tmem + t * kPpKeys + 8 * k, lo_v(v_u32 + st * kTile + k * 2048), hi_k, idesc_o,
                                 i > 0 || k > 0, leader);
+              }
               if (i + 1 < n_tiles) {
                 // (behind P V of this tile in the same thread: P has been read when S is written over it)
                 if (t == 0) pp_wait(bar(K_FULL + next), (uint32_t)(((i + 1) / kSt) & 1), &abort_flag);
@@ -358,9 +398,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_prefill_kernel(const __gr
       }
     }
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kIssuer) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, kTmem);
   }
   if (tid == 0 && abort_flag != 0) atomicOr(&g_b200_status, kStatusWaitGaveUp);
 }
@@ -388,7 +428,7 @@ inline bool pp_cache_map(CUtensorMap* out, const lora_b200_paged_cache& c, bool 
 }
 
 // Whether the tensor-core kernel takes a call: copies of 8 cache rows or more that lie in one block, and strides that its maps take.
-inline bool paged_prefill_plan(const PagedArgs& p, int D, bool f16, PpMaps* maps, PpArgs* a) {
+inline bool paged_prefill_plan(const PagedArgs& p, int D, bool f16, int tiles, PpMaps* maps, PpArgs* a) {
   if (p.cache.block_size % 8 != 0) return false;
   a->p = p;
   a->box = 8;
@@ -398,7 +438,7 @@ inline bool paged_prefill_plan(const PagedArgs& p, int D, bool f16, PpMaps* maps
   while (a->h_shift < 4 && group % (2 << a->h_shift) == 0) ++a->h_shift;
   a->head_tiles = p.Hq >> a->h_shift;
   const int per_tile = kPpRows >> a->h_shift;
-  const int64_t blocks = (int64_t)p.T / (2 * per_tile) + p.n_req;
+  const int64_t blocks = (int64_t)p.T / (tiles * per_tile) + p.n_req;
   if (blocks * a->head_tiles > INT32_MAX) return false;
   a->n_blocks = (int)blocks;
   const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)p.Hq, (cuuint64_t)p.T};
@@ -409,21 +449,26 @@ inline bool paged_prefill_plan(const PagedArgs& p, int D, bool f16, PpMaps* maps
          pp_cache_map(&maps->v, p.cache, true, p.Hk, D, a->box, f16, &a->v_heads_inner);
 }
 
-template <int D, bool kF16>
+template <int D, bool kF16, int kTiles>
 inline int paged_prefill_launch_t(const PpMaps& maps, const PpArgs& a, cudaStream_t stream) {
-  const cudaError_t e = cudaFuncSetAttribute(paged_prefill_kernel<D, kF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, pp_smem<D>());
+  const auto kernel = paged_prefill_kernel<D, kF16, kTiles>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, pp_smem<D>(kTiles));
   if (e != cudaSuccess) return fail(B200_LORA_ECUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-  return launch_dependent(paged_prefill_kernel<D, kF16>, "paged_prefill_kernel", dim3((unsigned)(a.n_blocks * a.head_tiles)), kPpThreads, pp_smem<D>(), stream,
-                          maps, a);
+  return launch_dependent(kernel, "paged_prefill_kernel", dim3((unsigned)(a.n_blocks * a.head_tiles)), pp_threads(kTiles), pp_smem<D>(kTiles), stream, maps, a);
 }
 
+#ifndef B200_TILES64
+#define B200_TILES64 1
+#define B200_TILES128 2
+#endif
 inline int paged_prefill_launch(const PagedArgs& p, int D, int dtype, void* workspace, cudaStream_t stream) {
   PpMaps maps;
   PpArgs a = {};
   const bool f16 = dtype == B200_LORA_F16;
-  if (!paged_prefill_plan(p, D, f16, &maps, &a)) return paged_decode_launch(p, D, dtype, workspace, stream);
-  if (D == 64) return f16 ? paged_prefill_launch_t<64, true>(maps, a, stream) : paged_prefill_launch_t<64, false>(maps, a, stream);
-  return f16 ? paged_prefill_launch_t<128, true>(maps, a, stream) : paged_prefill_launch_t<128, false>(maps, a, stream);
+  const int tiles = D == 64 ? B200_TILES64 : B200_TILES128;
+  if (!paged_prefill_plan(p, D, f16, tiles, &maps, &a)) return paged_decode_launch(p, D, dtype, workspace, stream);
+  if (D == 64) return f16 ? paged_prefill_launch_t<64, true, B200_TILES64>(maps, a, stream) : paged_prefill_launch_t<64, false, B200_TILES64>(maps, a, stream);
+  return f16 ? paged_prefill_launch_t<128, true, B200_TILES128>(maps, a, stream) : paged_prefill_launch_t<128, false, B200_TILES128>(maps, a, stream);
 }
 
 }  // namespace b200lora
