@@ -356,10 +356,15 @@ int lora_b200_glue_qk_norm_rope_kv_store(void* qkv, int64_t qkv_ld, int32_t T, i
   return head_norm_launch(p, dtype, static_cast<cudaStream_t>(stream));
 }
 
-size_t lora_b200_paged_workspace_bytes(int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t prefill) {
-  (void)T; (void)prefill;
+size_t lora_b200_paged_decode_workspace_bytes(int32_t num_heads, int32_t num_kv_heads, int32_t head_dim) {
   if (num_kv_heads < 1 || num_heads < num_kv_heads || head_dim < 1) return 0;
   return paged_workspace_bytes(num_heads, num_kv_heads, head_dim);
+}
+
+size_t lora_b200_paged_prefill_workspace_bytes(int32_t T, int32_t n_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                               int32_t table_width, int32_t block_size, int32_t window) {
+  if (num_kv_heads < 1 || num_heads < num_kv_heads || head_dim < 1) return 0;
+  return paged_prefill_workspace_bytes(T, n_seqs, num_heads, num_kv_heads, head_dim, (int64_t)table_width * block_size, window);
 }
 
 // What decode and prefill have in common; cu_seqlens null: decode
@@ -383,9 +388,10 @@ static int paged_attention_checked(const char* what, void* out, int64_t out_toke
   if (!aligned16(q) || !aligned16(out) || q_token % 8 || q_head % 8 || out_token % 8 || out_head % 8)
     return fail(B200_LORA_EUNSUPPORTED, "%s: rows of q and out must start on 16-byte boundaries", what);
   if (!aligned16(workspace)) return fail(B200_LORA_EUNSUPPORTED, "%s: the workspace must be 16-byte aligned", what);
-  if (workspace == nullptr || workspace_bytes < lora_b200_paged_workspace_bytes(T, num_heads, num_kv_heads, head_dim, prefill))
-    return fail(B200_LORA_EWORKSPACE, "%s: %zu bytes of workspace, needs %zu", what, workspace == nullptr ? (size_t)0 : workspace_bytes,
-                lora_b200_paged_workspace_bytes(T, num_heads, num_kv_heads, head_dim, prefill));
+  const size_t need = prefill ? lora_b200_paged_prefill_workspace_bytes(T, n_seqs, num_heads, num_kv_heads, head_dim, table_width, cache->block_size, window)
+                              : lora_b200_paged_decode_workspace_bytes(num_heads, num_kv_heads, head_dim);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(B200_LORA_EWORKSPACE, "%s: %zu bytes of workspace, needs %zu", what, workspace == nullptr ? (size_t)0 : workspace_bytes, need);
   PagedArgs a = {};
   a.q = q; a.q_token = q_token; a.q_head = q_head; a.out = out; a.out_token = out_token; a.out_head = out_head; a.lse = lse;
   a.cache = *cache; a.tables = block_tables; a.table_ld = table_ld; a.table_width = table_width; a.context_lens = context_lens;

@@ -41,7 +41,8 @@ decltype(&lora_b200_shrink_buckets) p_shrink = nullptr;
 decltype(&lora_b200_expand_buckets) p_expand = nullptr;
 decltype(&lora_b200_prefill_attention) p_attention = nullptr;
 decltype(&lora_b200_glue_qk_norm_rope_kv_store) p_head_norm = nullptr;
-decltype(&lora_b200_paged_workspace_bytes) p_paged_bytes = nullptr;
+decltype(&lora_b200_paged_decode_workspace_bytes) p_decode_bytes = nullptr;
+decltype(&lora_b200_paged_prefill_workspace_bytes) p_prefill_bytes = nullptr;
 decltype(&lora_b200_paged_decode_attention) p_paged_decode = nullptr;
 decltype(&lora_b200_paged_prefill_attention) p_paged_prefill = nullptr;
 PyObject* scratch_for = nullptr;  // lora.scratch_for(device, bytes)
@@ -622,7 +623,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (out == nullptr || !on(*out, dev) || out->scalar_type() != dt || out->sizes() != q->sizes() || out->stride(2) != 1) return not_handled();
   }
   if (args[10] == Py_True) lse = at::empty({T, hq}, q->options().dtype(at::kFloat));
-  const size_t need = p_paged_bytes((int)T, (int)hq, (int)hk, (int)d, cu ? 1 : 0);
+  const size_t need = cu == nullptr ? p_decode_bytes((int)hq, (int)hk, (int)d)
+                                    : p_prefill_bytes((int)T, (int)n, (int)hq, (int)hk, (int)d, (int)tables->size(1), cache.block_size, (int)window);
   const at::Tensor ws = at::empty({(int64_t)need}, q->options().dtype(at::kByte));
   void* stream = c10::cuda::getCurrentCUDAStream(dev).stream();
   float* lse_ptr = lse.defined() ? static_cast<float*>(lse.data_ptr()) : nullptr;
@@ -983,7 +985,8 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   B200_BIND(p_attention, lora_b200_prefill_attention)
   B200_BIND(p_rope, lora_b200_glue_rope_kv_store)
   B200_BIND(p_head_norm, lora_b200_glue_qk_norm_rope_kv_store)
-  B200_BIND(p_paged_bytes, lora_b200_paged_workspace_bytes)
+  B200_BIND(p_decode_bytes, lora_b200_paged_decode_workspace_bytes)
+  B200_BIND(p_prefill_bytes, lora_b200_paged_prefill_workspace_bytes)
   B200_BIND(p_paged_decode, lora_b200_paged_decode_attention)
   B200_BIND(p_paged_prefill, lora_b200_paged_prefill_attention)
 #undef B200_BIND

@@ -16,10 +16,7 @@
 namespace b200lora {
 
 constexpr int kPpRows = 128, kPpKeys = 128;       // of a tile
-#ifndef B200_POLY
-#define B200_POLY 16
-#endif
-constexpr int kPpPolyEvery = B200_POLY;
+constexpr int kPpOutPitch = 80;      // bytes of 32 columns of a row in shared memory, and 16 to spread the banks
 constexpr int kPpPanel = kPpKeys * 128;           // bytes of 128 rows of 64 columns
 // One softmax warpgroup per tile; one more with the loading warp and the MMA warp, which leaves its registers to them. Two tiles: 168
 // registers a thread at launch, 384 * 168 = 64512, and 2 * 208 + 88 = 3 * 168; one tile, two CTAs on an SM: 128, and 208 + 48 = 2 * 128.
@@ -31,7 +28,15 @@ __host__ __device__ constexpr int pp_stages(int tiles) { return (D == 64 ? 1 : 0
 template <int D>
 __host__ __device__ constexpr int pp_tile() { return kPpKeys * D * 2; }
 template <int D>
-__host__ __device__ constexpr int pp_smem(int tiles) { return (2 * pp_stages<D>(tiles) + tiles) * pp_tile<D>() + 1024; }
+__host__ __device__ constexpr int pp_smem(int tiles) { return (2 * pp_stages<D>(tiles) + tiles) * pp_tile<D>() + tiles * kPpRows * kPpOutPitch + 1024; }
+
+// Items that do not fill a wave of CTAs may be cut into parts along the keys, joined by a second launch: us, whole / cut, 16 / 2 heads,
+// 16 tokens behind 8192 keys (heads of 128) 112 / 29, behind 65536 844 / 56, 500 behind 3000 (64) 42 / 25; 32 / 8 of 128, 4096 behind
+// 12288 (3.5 waves of items of even length) 905 / 868. Not where every item is short, nor whole prompts of more than half a
+// wave: their last items are their shortest (8192 tokens 223 / 239).
+constexpr int kPpSplitTiles = 8;     // tiles of an item, at least
+constexpr int kPpSplitWaves = 6;     // waves of CTAs at most
+constexpr int kPpShare = 2, kPpParts = 32;  // tiles of a part at least, parts at most (the join reads them one after another)
 
 struct PpMaps { CUtensorMap q, k, v; };
 struct PpArgs {
@@ -39,6 +44,7 @@ struct PpArgs {
   int h_shift, head_tiles;   // heads of a tile = 1 << h_shift; tiles over all heads
   int n_blocks;              // blocks of tokens that the launch has CTAs for
   int box;                   // cache rows of a copy: 8 .. 128, a power of two that divides the block size
+  float* parts; void* joins;  // split: partial results and what there is to join
   int k_heads_inner, v_heads_inner;  // order of the map's middle dimensions: (head, position) or (position, head)
 };
 
@@ -90,41 +96,130 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// 2^x for x <= 8 or so on the FMA units: x = n + f with n whole and f in [-0.5, 0.5] (adding and subtracting 1.5 * 2^23 rounds to n), 2^f
-// by a polynomial with constant term 1, least in its largest relative error (1.7e-7 in fp32; weighted least squares until the
-// extrema are even), n added to the exponent. From -127 down exactly 0.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-  constexpr float kRound = 12582912.f;
-  x = make_float2(fmaxf(x.x, -127.f), fmaxf(x.y, -127.f));
-  const float2 t = add2(x, make_float2(kRound, kRound)), f = fma2(add2(t, make_float2(-kRound, -kRound)), make_float2(-1.f, -1.f), x);
-  float2 y = fma2(f, make_float2(0x1.5bba14p-10f, 0x1.5bba14p-10f), make_float2(0x1.3cea88p-7f, 0x1.3cea88p-7f));
-  y = fma2(f, y, make_float2(0x1.c6b752p-5f, 0x1.c6b752p-5f));
-  y = fma2(f, y, make_float2(0x1.ebf9bcp-3f, 0x1.ebf9bcp-3f));
-  y = fma2(f, y, make_float2(0x1.62e42ap-1f, 0x1.62e42ap-1f));
-  y = fma2(f, y, make_float2(1.f, 1.f));
-  return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23)), __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23)));
-}
 // bits [0, n) of a word, n of any sign and size
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
 
-template <int D, bool kF16, int kTiles>
+// A piece of work: tiles [i0, i1) of the keys that a block of tokens sees, for one set of heads.
+struct PpPiece {
+  int head0, begin, q0, n_here;                // first head; first row of the sequence; first token and tokens of the block
+  int req, pos0, held, key_end, lo_first, sink_end;  // position of the first token; keys that a row sees: [0, sink_end), [lo_first, key_end)
+  int first_tile, sink_tiles, i0, i1;
+  int parts;                                   // 0: no more pieces; 1: the whole item; else the item is in that many parts
+  __device__ __forceinline__ int key0(int i) const { return (i < sink_tiles ? i : i - sink_tiles + first_tile) * kPpKeys; }
+};
+
+// New rows of request i, and its first one; a range that leaves the rows of q counts as none
+__device__ __forceinline__ int pp_rows(const PagedArgs& p, int i, int* begin) {
+  *begin = p.cu_seqlens[i];
+  const int e = p.cu_seqlens[i + 1];
+  return *begin >= 0 && e <= p.T && e > *begin ? e - *begin : 0;
+}
+// Sum of the lanes up to this one
+__device__ __forceinline__ int warp_upto(int v) {
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int u = __shfl_up_sync(0xffffffffu, v, d);
+    if ((int)(threadIdx.x & 31) >= d) v += u;
+  }
+  return v;
+}
+
+// 32 requests, one per lane: new rows, the first of them, context; blocks of the requests up to this one
+struct PpLane { int begin, len, ctx, mine, upto; };
+__device__ __forceinline__ PpLane pp_lane(const PpArgs& a, int span, int i) {
+  PpLane q = {0, 0, 0, 0, 0};
+  if (i < a.p.n_req) {
+    q.ctx = max(a.p.context_lens[i], 0);
+    q.len = pp_rows(a.p, i, &q.begin);
+  }
+  q.mine = (q.len + span - 1) / span;
+  q.upto = warp_upto(q.mine);
+  return q;
+}
+__device__ __forceinline__ int pp_items(const PpArgs& a, int span, const PpLane& lanes0) {
+  int blocks = __shfl_sync(0xffffffffu, lanes0.upto, 31);
+  for (int base = 32; base < a.p.n_req; base += 32) blocks += __shfl_sync(0xffffffffu, pp_lane(a, span, base + (threadIdx.x & 31)).upto, 31);
+  return min(blocks, a.n_blocks) * a.head_tiles;  // (overlapping ranges could have more)
+}
+
+// Item `item` of the n_items, longest contexts first as far as one warp can tell (up to 32 requests: blocks by the position that
+// they end at; more: the last block of the last sequence first), the sets of heads of a block one after another. A whole warp calls
+// it, with the first 32 requests in hand.
+__device__ __forceinline__ void pp_find(const PpArgs& a, int span, int item, int n_items, const PpLane& lanes0, PpPiece* w) {
+  const PagedArgs& p = a.p;
+  const int lane = threadIdx.x & 31, back = item / a.head_tiles;
+  w->head0 = (item - back * a.head_tiles) << a.h_shift;
+  PpLane q = lanes0;
+  int base = 0, who, block;
+  if (p.n_req <= 32) {
+    const int from = max(q.ctx - q.len, 0) / span, to = from + q.mine;  // levels of the request: its blocks, counted from position 0
+    auto at_or_above = [&](int level) { return (int)__reduce_add_sync(0xffffffffu, (unsigned)max(0, to - max(level, from))); };
+    int level = 0, above = (int)__reduce_max_sync(0xffffffffu, (unsigned)to);
+    while (above - level > 1) {  // the highest level with more than `back` blocks at or above it
+      const int mid = (level + above) >> 1;
+      if (at_or_above(mid) > back) level = mid;
+      else above = mid;
+    }
+    const bool has = from <= level && level < to;
+    const int nth = back - at_or_above(level + 1);
+    const uint32_t mask = __ballot_sync(0xffffffffu, has);
+    who = max(0, __ffs(__ballot_sync(0xffffffffu, has && __popc(mask & ((1u << lane) - 1u)) == nth)) - 1);
+    block = level - __shfl_sync(0xffffffffu, from, who);
+  } else {
+    const int blk = n_items / a.head_tiles - 1 - back;
+    for (int run = 0;; base += 32, q = pp_lane(a, span, base + lane)) {
+      const uint32_t hit = __ballot_sync(0xffffffffu, run + q.upto > blk);
+      if (hit != 0) {
+        who = __ffs(hit) - 1;
+        block = blk - run - __shfl_sync(0xffffffffu, q.upto - q.mine, who);
+        break;
+      }
+      run += __shfl_sync(0xffffffffu, q.upto, 31);
+    }
+  }
+  const int len = __shfl_sync(0xffffffffu, q.len, who);
+  w->req = base + who;
+  w->begin = __shfl_sync(0xffffffffu, q.begin, who);
+  w->q0 = block * span;
+  w->n_here = min(span, len - w->q0);
+  w->pos0 = __shfl_sync(0xffffffffu, q.ctx, who) - len + w->q0;
+  w->held = (int)min((int64_t)min(w->pos0 + w->n_here, INT32_MAX - 255), (int64_t)p.table_width * p.cache.block_size);
+  w->key_end = w->held;
+  w->lo_first = p.window > 0 ? max(0, max(w->pos0, 0) - (p.window - 1)) : 0;
+  w->sink_end = max(0, min(min(p.sinks, w->lo_first), w->key_end));
+  w->first_tile = w->lo_first / kPpKeys;
+  w->sink_tiles = min((w->sink_end + kPpKeys - 1) / kPpKeys, w->first_tile);
+  w->i0 = 0;
+  w->i1 = w->key_end <= 0 ? 0 : w->sink_tiles + max(0, (w->key_end + kPpKeys - 1) / kPpKeys - w->first_tile);
+  w->parts = 1;
+}
+
+// The part of an item that CTA c leaves for the join (slot c): numerators [row / 128][column / 4][row % 128] of four columns, then
+// maximum and sum of every row.
+template <int D>
+__host__ __device__ constexpr int pp_slot_floats(int tiles) { return tiles * kPpRows * (D + 2); }
+// Of the item whose parts the CTAs c, c + stride, ... (`parts` of them) hold; parts < 2: none
+struct PpJoin { int head0, token0, n_here, parts, stride, pad[3]; };
+
+template <int D, bool kF16, int kTiles, bool kSplit>
 __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_kernel(const __grid_constant__ PpMaps maps, const __grid_constant__ PpArgs a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   constexpr int kSt = pp_stages<D>(kTiles), kTile = pp_tile<D>(), kPanels = D / 64;
   constexpr int kLoader = 4 * kTiles, kIssuer = kLoader + 1, kTmem = 256 * kTiles, kO = kTiles * kPpKeys;  // warps; columns: all, the first of O
-  enum { Q_FULL, S_READY, P_READY = S_READY + 2, O_DONE = P_READY + 4, K_FULL = O_DONE + 2, K_FREE = K_FULL + kSt, V_FULL = K_FREE + kSt,
-         V_FREE = V_FULL + kSt, N_BARS = V_FREE + kSt };
+  enum { Q_FULL, Q_FREE, S_READY, P_READY = S_READY + 2, O_DONE = P_READY + 4, K_FULL = O_DONE + 2, K_FREE = K_FULL + kSt, V_FULL = K_FREE + kSt,
+         V_FREE = V_FULL + kSt, PIECE = V_FREE + kSt, TAKEN = PIECE + 2, N_BARS = TAKEN + 2 };
   __shared__ __align__(8) uint64_t bars[N_BARS];
   __shared__ uint32_t s_tmem, s_boxes[4];
+  __shared__ PpPiece s_piece[2];
   __shared__ volatile int abort_flag;
   const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
   const PagedArgs& p = a.p;
   // (V first: what a wrong stride of its descriptor could reach stays inside the allocation)
-  const uint32_t v_u32 = (smem_u32(smem_raw) + 1023u) & ~1023u, k_u32 = v_u32 + kSt * kTile, q_u32 = k_u32 + kSt * kTile;
+  const uint32_t raw = smem_u32(smem_raw), v_u32 = (raw + 1023u) & ~1023u, k_u32 = v_u32 + kSt * kTile, q_u32 = k_u32 + kSt * kTile, out_u32 = q_u32 + kTiles * kTile;
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
 
   if (tid == 0) {
-    for (int i = 0; i < N_BARS; ++i) mbar_init(bar(i), i >= P_READY && i < O_DONE ? kPpRows : 1);
+    for (int i = 0; i < N_BARS; ++i) mbar_init(bar(i), i >= P_READY && i < O_DONE ? kPpRows : i >= TAKEN ? 4 * kTiles + 1 : 1);
     abort_flag = 0;
     mbar_fence_init();
   }
@@ -134,65 +229,39 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
   tc_fence_after_sync();
   glue_enter();  // (dependents may start: every CTA of this launch holds its tensor memory by then)
   const uint32_t tmem = s_tmem;
-
-  // ---- which tokens: the blocks of the sequences in order, the last ones first (their contexts are the longest)
-  const int blk = a.n_blocks - 1 - (int)blockIdx.x / a.head_tiles, head0 = ((int)blockIdx.x % a.head_tiles) << a.h_shift;
   const int per_tile = kPpRows >> a.h_shift, span = kTiles * per_tile;
-  int req = -1, begin = 0, len = 0, q0 = 0;
-  for (int base = 0, run = 0; base < p.n_req && req < 0; base += 32) {
-    const int i = base + lane;
-    int b = 0, n = 0;
-    if (i < p.n_req) {
-      b = p.cu_seqlens[i];
-      const int e = p.cu_seqlens[i + 1];
-      n = b >= 0 && e <= p.T && e > b ? e - b : 0;
-    }
-    int upto = (n + span - 1) / span;
-    const int mine = upto;
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const int v = __shfl_up_sync(0xffffffffu, upto, d);
-      if (lane >= d) upto += v;
-    }
-    const uint32_t hit = __ballot_sync(0xffffffffu, run + upto > blk);
-    if (hit != 0) {
-      const int who = __ffs(hit) - 1;
-      req = base + who;
-      begin = __shfl_sync(0xffffffffu, b, who);
-      len = __shfl_sync(0xffffffffu, n, who);
-      q0 = (blk - run - __shfl_sync(0xffffffffu, upto - mine, who)) * span;
-    }
-    run += __shfl_sync(0xffffffffu, upto, 31);
-  }
-    const int n_here = req < 0 ? 0 : min(span, len - q0);                             // tokens of this CTA
-    const int ctx = req < 0 ? 0 : max(p.context_lens[req], 0), pos0 = ctx - len + q0;  // position of the first
-    const int held = (int)min((int64_t)min(ctx, INT32_MAX - 255), (int64_t)p.table_width * p.cache.block_size);
-    const int key_end = min(pos0 + n_here, held);                                     // keys that any row sees: [0, sink_end) and
-    const int lo_first = p.window > 0 ? max(0, max(pos0, 0) - (p.window - 1)) : 0;    // [lo_first, key_end)
-    const int sink_end = max(0, min(min(p.sinks, lo_first), key_end));
-    const int first_tile = lo_first / kPpKeys, sink_tiles = min((sink_end + kPpKeys - 1) / kPpKeys, first_tile);
-    const int n_tiles = key_end <= 0 || n_here == 0 ? 0 : sink_tiles + max(0, (key_end + kPpKeys - 1) / kPpKeys - first_tile);
-    auto key0_of = [&](int i) { return (i < sink_tiles ? i : i - sink_tiles + first_tile) * kPpKeys; };
 
-    if (warp < kLoader) {  // ------------------------------------------------------------------- softmax
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPpSoftmaxRegs));
-      const int t = warp >> 2, row = (warp & 3) * 32 + lane, tok = t * per_tile + (row >> a.h_shift), head = head0 + (row & ((1 << a.h_shift) - 1));
-      const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-      const uint32_t s_at = tmem + t * kPpKeys + lanes, o_at = tmem + kO + t * D + lanes;
-      const int pos = pos0 + tok;
+  // Pieces come from the loading warp through two places in shared memory.
+  auto take = [&](int k, PpPiece* w) {
+    pp_wait(bar(PIECE + (k & 1)), (uint32_t)(k >> 1) & 1, &abort_flag);
+    *w = s_piece[k & 1];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(TAKEN + (k & 1)));
+    return w->parts > 0 && abort_flag == 0;
+  };
+  if (warp < kLoader) {  // ------------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPpSoftmaxRegs));
+    const int t = warp >> 2, row = (warp & 3) * 32 + lane, tok = t * per_tile + (row >> a.h_shift);
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + t * kPpKeys + lanes, o_at = tmem + kO + t * D + lanes;
+    const uint32_t all_boxes = bits_below(kPpKeys / a.box);
+    const int box_shift = 31 - __clz(a.box);
+    const uint32_t stage = out_u32 + warp * (32 * kPpOutPitch);  // 32 columns of the warp's rows on their way out
+    uint32_t n = 0, pieces = 0;  // tiles and pieces with tiles so far: phases of the barriers
+    PpPiece w;
+    for (int k = 0; take(k, &w); ++k) {
+      const int pos = w.pos0 + tok;
       const int lo = p.window > 0 ? max(pos, 0) - (p.window - 1) : 0;
-      const int tile_lo = pos0 + t * per_tile, tile_hi = tile_lo + per_tile - 1;  // positions of the tile
-      const uint32_t all_boxes = bits_below(kPpKeys / a.box);
-      const int box_shift = 31 - __clz(a.box);
+      const int tile_lo = w.pos0 + t * per_tile, tile_hi = tile_lo + per_tile - 1;  // positions of the tile
       float m = -INFINITY, l = 0.f;  // maximum that the probabilities refer to, in units of log2; their sum
-      for (int i = 0; i < n_tiles; ++i) {
-        const int key0 = key0_of(i);
-        pp_wait(bar(S_READY + t), (uint32_t)(i & 1), &abort_flag);
+      for (int i = w.i0; i < w.i1; ++i, ++n) {
+        const int key0 = w.key0(i);
+        pp_wait(bar(S_READY + t), n & 1, &abort_flag);
         tc_fence_after_sync();
         uint32_t s[4][32];
 #pragma unroll
         for (int c = 0; c < 2; ++c) tmem_ld_32x32(s_at + 32 * c, s[c]);
-        const uint32_t boxes = s_boxes[i & 3];
+        const uint32_t boxes = s_boxes[n & 3];
         const bool masked = key0 + kPpKeys - 1 > tile_lo || (p.window > 0 && key0 < max(tile_hi, 0) - (p.window - 1) && key0 + kPpKeys > p.sinks) || boxes != all_boxes;
         float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -228,7 +297,7 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
           const float f = grows ? ex2(m - top) : 1.f;
           if (grows) m = top;
           l *= f;
-          if (i > 0) {  // (S of this tile came behind P V of the one before: O is complete)
+          if (i > w.i0) {  // (S of this tile came behind P V of the one before: O is complete)
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) {
               uint32_t o[16];
@@ -249,7 +318,7 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
             const float2 x = fma2(make_float2(__uint_as_float(s[c][j]), __uint_as_float(s[c][j + 1])), scale2, base2);
-            const float2 y = j % kPpPolyEvery == kPpPolyEvery - 2 ? exp2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
+            const float2 y = make_float2(ex2(x.x), ex2(x.y));
             sum[j / 2 % 2] = add2(sum[j / 2 % 2], y);
             packed[j / 2] = pack_16x2<kF16>(y.x, y.y);  // (rounded to the type of V; the sum is that of the unrounded ones)
           }
@@ -262,25 +331,33 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
         }
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }
-      const bool live = tok < n_here;
+      const bool live = tok < w.n_here, any = w.i1 > w.i0, whole = !kSplit || w.parts == 1;
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // (no visible key: zeros; NaN stays)
-      const int64_t token = begin + q0 + tok;
-      char* dst = static_cast<char*>(p.out) + 2 * (token * p.out_token + head * p.out_head);
-      if (n_tiles > 0) {
-        pp_wait(bar(O_DONE + t), 0, &abort_flag);
+      const int64_t token0 = (int64_t)w.begin + w.q0;
+      if (any) {
+        pp_wait(bar(O_DONE + t), pieces & 1, &abort_flag);
+        ++pieces;
         tc_fence_after_sync();
       }
+      if (whole) {
+        // Through shared memory, so that four lanes write 64 adjacent bytes of a row. (A row's pieces straight from its thread: 32
+        // half-used sectors a store, 3200 cycles for a tile of 128 columns.)
+        char* dst[4];
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        if (n_tiles > 0) {
-          tmem_ld_32x32(o_at + 32 * c, o);
-          tmem_ld_wait();
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = 0;
+        for (int r = 0; r < 4; ++r) {
+          const int of = (warp & 3) * 32 + 8 * r + (lane >> 2), its = t * per_tile + (of >> a.h_shift);
+          dst[r] = its < w.n_here ? static_cast<char*>(p.out) + 2 * ((token0 + its) * p.out_token + (w.head0 + (of & ((1 << a.h_shift) - 1))) * p.out_head) + 16 * (lane & 3) : nullptr;
         }
-        if (live) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          if (any) {
+            tmem_ld_32x32(o_at + 32 * c, o);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = 0;
+          }
 #pragma unroll
           for (int j = 0; j < 32; j += 8) {
             uint4 v;
@@ -288,121 +365,238 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
             v.y = pack_16x2<kF16>(__uint_as_float(o[j + 2]) * inv, __uint_as_float(o[j + 3]) * inv);
             v.z = pack_16x2<kF16>(__uint_as_float(o[j + 4]) * inv, __uint_as_float(o[j + 5]) * inv);
             v.w = pack_16x2<kF16>(__uint_as_float(o[j + 6]) * inv, __uint_as_float(o[j + 7]) * inv);
-            stg128(dst + 2 * (32 * c + j), v);
+            sts128(stage + lane * kPpOutPitch + 2 * j, v);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (dst[r] != nullptr) stg128(dst[r] + 64 * c, lds128(stage + (8 * r + (lane >> 2)) * kPpOutPitch + 16 * (lane & 3)));
+          __syncwarp();
+        }
+        if (live && p.lse != nullptr) p.lse[(token0 + tok) * p.Hq + w.head0 + (row & ((1 << a.h_shift) - 1))] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+      } else {
+        float* const part = a.parts + (int64_t)blockIdx.x * pp_slot_floats<D>(kTiles);
+        float4* const at = reinterpret_cast<float4*>(part) + t * (D / 4) * kPpRows + row;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld_32x32(o_at + 32 * c, o);
+          tmem_ld_wait();
+          if (live) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) stg128(at + (8 * c + j / 4) * kPpRows, make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]));
+          }
+        }
+        if (live) reinterpret_cast<float2*>(part + kTiles * kPpRows * D)[t * kPpRows + row] = make_float2(m, l);
+      }
+      tc_fence_before_sync();
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(pp_other_regs(kTiles)));
+    if (warp == kLoader) {  // ------------------------------------------------------------------ loads
+      const uint32_t leader = elect_one();
+      const int n_boxes = kPpKeys / a.box;
+      uint32_t n = 0, pieces = 0;
+      const PpLane lanes0 = pp_lane(a, span, lane);
+      const int n_items = pp_items(a, span, lanes0), G = gridDim.x, waves = n_items / G, rest = n_items - waves * G;
+      // Split: the items that do not fill a wave are cut into parts, CTA i + s * rest has part s of item i.
+      const int most = kSplit && rest > 0 ? G / rest : 1;
+      if (kSplit && leader) static_cast<PpJoin*>(a.joins)[blockIdx.x].parts = 0;
+      PpPiece w;
+      bool more_pieces = true;
+      for (int k = 0; more_pieces; ++k) {
+        w.parts = 0;
+        // (every other wave backwards: contexts get shorter from item to item)
+        const int c = k & 1 ? G - 1 - (int)blockIdx.x : (int)blockIdx.x;
+        if (k < waves) {
+          pp_find(a, span, k * G + c, n_items, lanes0, &w);
+        } else if (k == waves && most >= 2) {
+          const int i = blockIdx.x % rest, s = blockIdx.x / rest;
+          if (s < most) {
+            pp_find(a, span, k * G + i, n_items, lanes0, &w);
+            const int tiles = w.i1;
+            w.parts = max(1, min(min(most, kPpParts), tiles / kPpShare));
+            if (s >= w.parts) w.parts = 0;
+            if (w.parts > 1) {
+              w.i0 = (int)((int64_t)tiles * s / w.parts);
+              w.i1 = (int)((int64_t)tiles * (s + 1) / w.parts);
+              if (s == 0 && leader) static_cast<PpJoin*>(a.joins)[i] = {w.head0, w.begin + w.q0, w.n_here, w.parts, rest, {0, 0, 0}};
+            }
+          }
+        } else if (k == waves && c < rest) {
+          pp_find(a, span, k * G + c, n_items, lanes0, &w);
+        }
+        more_pieces = w.parts > 0;
+        if (k >= 2) pp_wait(bar(TAKEN + (k & 1)), (uint32_t)((k >> 1) - 1) & 1, &abort_flag);
+        if (abort_flag != 0) { w.parts = 0; more_pieces = false; }
+        if (leader) {
+          s_piece[k & 1] = w;
+          mbar_arrive(bar(PIECE + (k & 1)));
+        }
+        if (!more_pieces || w.i1 <= w.i0) continue;
+        const int kvh = w.head0 / (p.Hq / p.Hk);
+        const int32_t* table = p.tables + w.req * p.table_ld;
+        for (int i = w.i0; i < w.i1; ++i, ++n) {
+          const int st = n % kSt, key = w.key0(i) + lane * a.box;
+          int block = -1, in_block = 0;
+          if (lane < n_boxes && key < w.held) {
+            const int page = key / p.cache.block_size;
+            block = table[page];
+            in_block = key - page * p.cache.block_size;
+          }
+          if (i == w.i0) {
+            if (pieces > 0) pp_wait(bar(Q_FREE), (pieces - 1) & 1, &abort_flag);
+            ++pieces;
+            if (leader) {
+              mbar_arrive_expect_tx(bar(Q_FULL), kTiles * kTile);
+              for (int t = 0; t < kTiles; ++t)
+                for (int c = 0; c < kPanels; ++c)
+                  tma_load_3d_at(q_u32 + t * kTile + c * kPpPanel, &maps.q, 64 * c, w.head0, w.begin + w.q0 + t * per_tile, bar(Q_FULL));
+            }
+          }
+          const bool there = (unsigned)block < (unsigned)p.cache.num_blocks;
+          if (!there) { block = p.cache.num_blocks; in_block = 0; }  // outside the map: zeros
+          const uint32_t boxes = __ballot_sync(0xffffffffu, there);
+          for (int which = 0; which < 2; ++which) {
+            const uint32_t full = bar((which ? V_FULL : K_FULL) + st);
+            if (n >= kSt) pp_wait(bar((which ? V_FREE : K_FREE) + st), (n / kSt - 1) & 1, &abort_flag);
+            if (leader) {
+              if (which == 0) s_boxes[n & 3] = boxes;  // (read up to kSt tiles later: fewer than four)
+              mbar_arrive_expect_tx(full, kTile);
+            }
+            __syncwarp();
+            if (lane < n_boxes) {
+              const uint32_t dst = (which ? v_u32 : k_u32) + st * kTile + lane * a.box * 128;
+              const bool inner = which ? a.v_heads_inner : a.k_heads_inner;
+              for (int c = 0; c < kPanels; ++c)
+                tma_load_4d(dst + c * kPpPanel, which ? &maps.v : &maps.k, 64 * c, inner ? kvh : in_block, inner ? in_block : kvh, block, full);
+            }
           }
         }
       }
-      if (live && p.lse != nullptr) p.lse[token * p.Hq + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-      tc_fence_before_sync();
-    } else {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(pp_other_regs(kTiles)));
-      if (warp == kLoader) {  // ------------------------------------------------------------------ loads
-        const uint32_t leader = elect_one();
-        const int kvh = head0 / (p.Hq / p.Hk);
-        const int32_t* table = p.tables + req * p.table_ld;
-        if (n_tiles > 0) {
-          if (leader) {
-            mbar_arrive_expect_tx(bar(Q_FULL), kTiles * kTile);
-            for (int t = 0; t < kTiles; ++t)
-              for (int c = 0; c < kPanels; ++c)
-                tma_load_3d_at(q_u32 + t * kTile + c * kPpPanel, &maps.q, 64 * c, head0, begin + q0 + t * per_tile, bar(Q_FULL));
-          }
-          const int n_boxes = kPpKeys / a.box;
-          for (int i = 0; i < n_tiles; ++i) {
-            const int st = i % kSt, key = key0_of(i) + lane * a.box;
-            int block = -1, in_block = 0;
-            if (lane < n_boxes && key < held) {
-              const int page = key / p.cache.block_size;
-              block = table[page];
-              in_block = key - page * p.cache.block_size;
-            }
-            const bool there = (unsigned)block < (unsigned)p.cache.num_blocks;
-            if (!there) { block = p.cache.num_blocks; in_block = 0; }  // outside the map: zeros
-            const uint32_t boxes = __ballot_sync(0xffffffffu, there);
-            for (int which = 0; which < 2; ++which) {
-              const uint32_t full = bar((which ? V_FULL : K_FULL) + st);
-              if (i >= kSt) pp_wait(bar((which ? V_FREE : K_FREE) + st), (uint32_t)((i / kSt - 1) & 1), &abort_flag);
-              if (leader) {
-                if (which == 0) s_boxes[i & 3] = boxes;  // (read up to kSt tiles later: fewer than four)
-                mbar_arrive_expect_tx(full, kTile);
-              }
-              __syncwarp();
-              if (lane < n_boxes) {
-                const uint32_t dst = (which ? v_u32 : k_u32) + st * kTile + lane * a.box * 128;
-                const bool inner = which ? a.v_heads_inner : a.k_heads_inner;
-                for (int c = 0; c < kPanels; ++c)
-                  tma_load_4d(dst + c * kPpPanel, which ? &maps.v : &maps.k, 64 * c, inner ? kvh : in_block, inner ? in_block : kvh, block, full);
-              }
-            }
-          }
-        }
-      } else if (warp == kIssuer) {  // ---------------------------------------------------------- products
-        const uint32_t leader = elect_one();
-        const uint32_t type = kF16 ? 0u : (1u << 7) | (1u << 10);
-        const uint32_t idesc_s = (1u << 4) | type | ((uint32_t)(kPpKeys >> 3) << 17) | ((uint32_t)(kPpRows >> 4) << 24);
-        const uint32_t idesc_o = (1u << 4) | type | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kPpRows >> 4) << 24);  // V: keys are its rows
-        const uint32_t hi_k = (uint32_t)(umma_smem_desc(0, 128) >> 32);
-        auto lo_k = [](uint32_t addr) { return ((addr & 0x3FFFF) >> 4) | (1u << 16); };
-        auto lo_v = [](uint32_t addr) { return ((addr & 0x3FFFF) >> 4) | ((uint32_t)(kPpPanel >> 4) << 16); };  // 64-column panels
-        auto scores = [&](int t, int st) {
-  #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t at = (k >> 2) * kPpPanel + (k & 3) * 32;
-            umma_elected(tmem + t * kPpKeys, lo_k(q_u32 + t * kTile + at), lo_k(k_u32 + st * kTile + at), hi_k, idesc_s, k > 0, leader);
-          }
-          umma_commit_elected(bar(S_READY + t), leader);
-        };
-        if (n_tiles > 0) {
-          pp_wait(bar(Q_FULL), 0, &abort_flag);
-          pp_wait(bar(K_FULL), 0, &abort_flag);
-          for (int t = 0; t < kTiles; ++t) scores(t, 0);
-          umma_commit_elected(bar(K_FREE), leader);
-          for (int i = 0; i < n_tiles; ++i) {
-            const int st = i % kSt, next = (i + 1) % kSt;
-            pp_wait(bar(V_FULL + st), (uint32_t)((i / kSt) & 1), &abort_flag);
-            // Rows of V that no token of this CTA sees may hold anything (a block's stale rows): they become zero, as 0 * V must.
-            const int key0 = key0_of(i);
-            if (!(key0 + kPpKeys <= sink_end || (key0 >= lo_first && key0 + kPpKeys <= key_end))) {
-              for (int x = lane; x < kPpKeys * kPanels * 8; x += 32) {
-                const int row = x / (kPanels * 8), key = key0 + row, c = x % (kPanels * 8);
-                if (!(key < sink_end || (key >= lo_first && key < key_end)))
-                  sts128(v_u32 + st * kTile + (c >> 3) * kPpPanel + row * 128 + (c & 7) * 16, make_uint4(0, 0, 0, 0));
-              }
-              fence_proxy_async_smem();
-              __syncwarp();
-            }
-            for (int t = 0; t < kTiles; ++t) {
+    } else if (warp == kIssuer) {  // ---------------------------------------------------------- products
+      const uint32_t leader = elect_one();
+      const uint32_t type = kF16 ? 0u : (1u << 7) | (1u << 10);
+      const uint32_t idesc_s = (1u << 4) | type | ((uint32_t)(kPpKeys >> 3) << 17) | ((uint32_t)(kPpRows >> 4) << 24);
+      const uint32_t idesc_o = (1u << 4) | type | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kPpRows >> 4) << 24);  // V: keys are its rows
+      const uint32_t hi_k = (uint32_t)(umma_smem_desc(0, 128) >> 32);
+      auto lo_k = [](uint32_t addr) { return ((addr & 0x3FFFF) >> 4) | (1u << 16); };
+      auto lo_v = [](uint32_t addr) { return ((addr & 0x3FFFF) >> 4) | ((uint32_t)(kPpPanel >> 4) << 16); };  // 64-column panels
+      auto scores = [&](int t, int st) {
 #pragma unroll
-              for (int k = 0; k < kPpKeys / 16; ++k) {
-                if (k % 4 == 0) {
-                  pp_wait(bar(P_READY + 2 * t + k / 4), (uint32_t)(i & 1), &abort_flag);
-                  tc_fence_after_sync();
-                }
-                umma_ts_elected(tmem + kO + t * D, tmem + t * kPpKeys + 8 * k, lo_v(v_u32 + st * kTile + k * 2048), hi_k, idesc_o,
-                                i > 0 || k > 0, leader);
-              }
-              if (i + 1 < n_tiles) {
-                // (behind P V of this tile in the same thread: P has been read when S is written over it)
-                if (t == 0) pp_wait(bar(K_FULL + next), (uint32_t)(((i + 1) / kSt) & 1), &abort_flag);
-                scores(t, next);
-              } else {
-                umma_commit_elected(bar(O_DONE + t), leader);
-              }
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t at = (k >> 2) * kPpPanel + (k & 3) * 32;
+          umma_elected(tmem + t * kPpKeys, lo_k(q_u32 + t * kTile + at), lo_k(k_u32 + st * kTile + at), hi_k, idesc_s, k > 0, leader);
+        }
+        umma_commit_elected(bar(S_READY + t), leader);
+      };
+      uint32_t n = 0, pieces = 0;
+      PpPiece w;
+      for (int k = 0; take(k, &w); ++k) {
+        if (w.i1 <= w.i0) continue;
+        pp_wait(bar(Q_FULL), pieces & 1, &abort_flag);
+        ++pieces;
+        pp_wait(bar(K_FULL + n % kSt), (n / kSt) & 1, &abort_flag);
+        for (int t = 0; t < kTiles; ++t) scores(t, n % kSt);
+        umma_commit_elected(bar(K_FREE + n % kSt), leader);
+        if (w.i1 == w.i0 + 1) umma_commit_elected(bar(Q_FREE), leader);
+        for (int i = w.i0; i < w.i1; ++i, ++n) {
+          const int st = n % kSt, next = (n + 1) % kSt;
+          const bool more = i + 1 < w.i1;
+          pp_wait(bar(V_FULL + st), (n / kSt) & 1, &abort_flag);
+          // Rows of V that no token of this CTA sees may hold anything (a block's stale rows): they become zero, as 0 * V must.
+          const int key0 = w.key0(i);
+          if (!(key0 + kPpKeys <= w.sink_end || (key0 >= w.lo_first && key0 + kPpKeys <= w.key_end))) {
+            for (int x = lane; x < kPpKeys * kPanels * 8; x += 32) {
+              const int row = x / (kPanels * 8), key = key0 + row, c = x % (kPanels * 8);
+              if (!(key < w.sink_end || (key >= w.lo_first && key < w.key_end)))
+                sts128(v_u32 + st * kTile + (c >> 3) * kPpPanel + row * 128 + (c & 7) * 16, make_uint4(0, 0, 0, 0));
             }
-            if (i + 1 < n_tiles) {
-              umma_commit_elected(bar(V_FREE + st), leader);
-              umma_commit_elected(bar(K_FREE + next), leader);
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          for (int t = 0; t < kTiles; ++t) {
+#pragma unroll
+            for (int k = 0; k < kPpKeys / 16; ++k) {
+              if (k % 4 == 0) {
+                pp_wait(bar(P_READY + 2 * t + k / 4), n & 1, &abort_flag);
+                tc_fence_after_sync();
+              }
+              umma_ts_elected(tmem + kO + t * D, tmem + t * kPpKeys + 8 * k, lo_v(v_u32 + st * kTile + k * 2048), hi_k, idesc_o,
+                              i > w.i0 || k > 0, leader);
+            }
+            if (more) {
+              // (behind P V of this tile in the same thread: P has been read when S is written over it)
+              if (t == 0) pp_wait(bar(K_FULL + next), ((n + 1) / kSt) & 1, &abort_flag);
+              scores(t, next);
+            } else {
+              umma_commit_elected(bar(O_DONE + t), leader);
             }
           }
+          umma_commit_elected(bar(V_FREE + st), leader);
+          if (more) umma_commit_elected(bar(K_FREE + next), leader);
+          if (i + 2 == w.i1) umma_commit_elected(bar(Q_FREE), leader);
         }
+      }
+      // the last commits must have arrived before this CTA's shared memory is given up
+      if (n > 0) {
+        pp_wait(bar(V_FREE + (n - 1) % kSt), ((n - 1) / kSt) & 1, &abort_flag);
+        pp_wait(bar(Q_FREE), (pieces - 1) & 1, &abort_flag);
       }
     }
+  }
   __syncthreads();
   if (warp == kIssuer) {
     tc_fence_after_sync();
     tmem_dealloc(tmem, kTmem);
   }
   if (tid == 0 && abort_flag != 0) atomicOr(&g_b200_status, kStatusWaitGaveUp);
+}
+
+// Joins the parts of the item that CTA blockIdx.x has the first part of. A thread per row of the item, 16 columns (blockIdx.y): eight
+// parts' worth of them are under way at a time.
+template <int D, bool kF16, int kTiles>
+__global__ void __launch_bounds__(kTiles * kPpRows) paged_prefill_join_kernel(const __grid_constant__ PpArgs a) {
+  glue_enter();
+  const PpJoin j = static_cast<const PpJoin*>(a.joins)[blockIdx.x];
+  if (j.parts < 2) return;
+  const PagedArgs& p = a.p;
+  const int t = threadIdx.x / kPpRows, row = threadIdx.x % kPpRows, tok = t * (kPpRows >> a.h_shift) + (row >> a.h_shift);
+  if (tok >= j.n_here) return;
+  const int head = j.head0 + (row & ((1 << a.h_shift) - 1)), c0 = 4 * blockIdx.y;
+  const float* const first = a.parts + (int64_t)blockIdx.x * pp_slot_floats<D>(kTiles);
+  const int64_t step = (int64_t)j.stride * pp_slot_floats<D>(kTiles);
+  auto stats = [&](int k) { return reinterpret_cast<const float2*>(first + k * step + kTiles * kPpRows * D)[t * kPpRows + row]; };
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < j.parts; ++k) top = fmaxf(top, stats(k).x);
+  float4 o[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int k = 0; k < j.parts; ++k) {
+    const float2 ml = stats(k);
+    const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);  // (a row of NaN has NaN for its maximum)
+    sum += f * ml.y;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float4 v = reinterpret_cast<const float4*>(first + k * step)[(t * (D / 4) + c0 + c) * kPpRows + row];
+      o[c] = make_float4(o[c].x + f * v.x, o[c].y + f * v.y, o[c].z + f * v.z, o[c].w + f * v.w);
+    }
+  }
+  const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+  const int64_t token = (int64_t)j.token0 + tok;
+  char* const dst = static_cast<char*>(p.out) + 2 * (token * p.out_token + head * p.out_head + 4 * c0);
+#pragma unroll
+  for (int c = 0; c < 4; c += 2) {
+    uint4 v;
+    v.x = pack_16x2<kF16>(o[c].x * inv, o[c].y * inv);
+    v.y = pack_16x2<kF16>(o[c].z * inv, o[c].w * inv);
+    v.z = pack_16x2<kF16>(o[c + 1].x * inv, o[c + 1].y * inv);
+    v.w = pack_16x2<kF16>(o[c + 1].z * inv, o[c + 1].w * inv);
+    stg128(dst + 8 * c, v);
+  }
+  if (c0 == 0 && p.lse != nullptr) p.lse[token * p.Hq + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
 // ------------------------------------------------------------------ host
@@ -427,15 +621,20 @@ inline bool pp_cache_map(CUtensorMap* out, const lora_b200_paged_cache& c, bool 
   return head >= 0 && token >= 0 && block >= 0 && pp_map(out, v ? c.v : c.k, f16, 4, dims, strides, b);
 }
 
+// Heads of a tile, as a power of two: they divide a group
+inline int pp_h_shift(int group) {
+  int s = 0;
+  while (s < 4 && group % (2 << s) == 0) ++s;
+  return s;
+}
+
 // Whether the tensor-core kernel takes a call: copies of 8 cache rows or more that lie in one block, and strides that its maps take.
 inline bool paged_prefill_plan(const PagedArgs& p, int D, bool f16, int tiles, PpMaps* maps, PpArgs* a) {
   if (p.cache.block_size % 8 != 0) return false;
   a->p = p;
   a->box = 8;
   while (a->box < kPpKeys && p.cache.block_size % (2 * a->box) == 0) a->box *= 2;
-  const int group = p.Hq / p.Hk;
-  a->h_shift = 0;
-  while (a->h_shift < 4 && group % (2 << a->h_shift) == 0) ++a->h_shift;
+  a->h_shift = pp_h_shift(p.Hq / p.Hk);
   a->head_tiles = p.Hq >> a->h_shift;
   const int per_tile = kPpRows >> a->h_shift;
   const int64_t blocks = (int64_t)p.T / (tiles * per_tile) + p.n_req;
@@ -449,26 +648,51 @@ inline bool paged_prefill_plan(const PagedArgs& p, int D, bool f16, int tiles, P
          pp_cache_map(&maps->v, p.cache, true, p.Hk, D, a->box, f16, &a->v_heads_inner);
 }
 
-template <int D, bool kF16, int kTiles>
-inline int paged_prefill_launch_t(const PpMaps& maps, const PpArgs& a, cudaStream_t stream) {
-  const auto kernel = paged_prefill_kernel<D, kF16, kTiles>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, pp_smem<D>(kTiles));
-  if (e != cudaSuccess) return fail(B200_LORA_ECUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-  return launch_dependent(kernel, "paged_prefill_kernel", dim3((unsigned)(a.n_blocks * a.head_tiles)), pp_threads(kTiles), pp_smem<D>(kTiles), stream, maps, a);
+// Whether a launch cuts the items that do not fill a wave of CTAs into parts, as told by what the host knows: items at most, and
+// tiles of an item at most.
+inline bool pp_splits(int T, int n_req, int Hq, int h_shift, int tiles, int64_t max_context, int window) {
+  const int span = tiles * (kPpRows >> h_shift);
+  const int64_t items = ((int64_t)T / span + n_req) * (Hq >> h_shift);
+  const int64_t keys = window > 0 ? std::min<int64_t>(max_context, (int64_t)window + span) : max_context;
+  const int wave = 148 * (3 - tiles);
+  return keys / kPpKeys >= kPpSplitTiles && (2 * items <= wave || (items <= kPpSplitWaves * wave && keys >= 2 * (int64_t)T));
+}
+constexpr int pp_tiles(int D) { return D == 64 ? 1 : 2; }
+inline size_t pp_split_bytes(int D) {
+  const int tiles = pp_tiles(D), ctas = 148 * (3 - tiles);
+  return (size_t)ctas * tiles * kPpRows * (D + 2) * 4 + ctas * sizeof(PpJoin);
+}
+inline size_t paged_prefill_workspace_bytes(int T, int n_req, int Hq, int Hk, int D, int64_t max_context, int window) {
+  const size_t tokens = paged_workspace_bytes(Hq, Hk, D);
+  return pp_splits(T, n_req, Hq, pp_h_shift(Hq / Hk), pp_tiles(D), max_context, window) ? std::max(tokens, pp_split_bytes(D)) : tokens;
 }
 
-#ifndef B200_TILES64
-#define B200_TILES64 1
-#define B200_TILES128 2
-#endif
+template <int D, bool kF16, bool kSplit>
+inline int paged_prefill_launch_t(const PpMaps& maps, const PpArgs& a, cudaStream_t stream) {
+  constexpr int kTiles = pp_tiles(D), kCtas = 148 * (3 - kTiles);
+  const auto kernel = paged_prefill_kernel<D, kF16, kTiles, kSplit>;
+  constexpr int smem = pp_smem<D>(kTiles);
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return fail(B200_LORA_ECUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  const int ctas = kSplit ? kCtas : (int)std::min<int64_t>(kCtas, (int64_t)a.n_blocks * a.head_tiles);
+  const int rc = launch_dependent(kernel, "paged_prefill_kernel", dim3((unsigned)ctas), pp_threads(kTiles), (size_t)smem, stream, maps, a);
+  if (rc != B200_LORA_OK || !kSplit) return rc;
+  return launch_dependent(paged_prefill_join_kernel<D, kF16, kTiles>, "paged_prefill_join_kernel", dim3((unsigned)ctas, D / 16), kTiles * kPpRows, 0, stream, a);
+}
+
 inline int paged_prefill_launch(const PagedArgs& p, int D, int dtype, void* workspace, cudaStream_t stream) {
   PpMaps maps;
   PpArgs a = {};
   const bool f16 = dtype == B200_LORA_F16;
-  const int tiles = D == 64 ? B200_TILES64 : B200_TILES128;
-  if (!paged_prefill_plan(p, D, f16, tiles, &maps, &a)) return paged_decode_launch(p, D, dtype, workspace, stream);
-  if (D == 64) return f16 ? paged_prefill_launch_t<64, true, B200_TILES64>(maps, a, stream) : paged_prefill_launch_t<64, false, B200_TILES64>(maps, a, stream);
-  return f16 ? paged_prefill_launch_t<128, true, B200_TILES128>(maps, a, stream) : paged_prefill_launch_t<128, false, B200_TILES128>(maps, a, stream);
+  if (!paged_prefill_plan(p, D, f16, pp_tiles(D), &maps, &a)) return paged_decode_launch(p, D, dtype, workspace, stream);
+  if (pp_splits(p.T, p.n_req, p.Hq, a.h_shift, pp_tiles(D), (int64_t)p.table_width * p.cache.block_size, p.window)) {
+    a.parts = static_cast<float*>(workspace);
+    a.joins = static_cast<char*>(workspace) + pp_split_bytes(D) - 148 * (3 - pp_tiles(D)) * sizeof(PpJoin);
+    if (D == 64) return f16 ? paged_prefill_launch_t<64, true, true>(maps, a, stream) : paged_prefill_launch_t<64, false, true>(maps, a, stream);
+    return f16 ? paged_prefill_launch_t<128, true, true>(maps, a, stream) : paged_prefill_launch_t<128, false, true>(maps, a, stream);
+  }
+  if (D == 64) return f16 ? paged_prefill_launch_t<64, true, false>(maps, a, stream) : paged_prefill_launch_t<64, false, false>(maps, a, stream);
+  return f16 ? paged_prefill_launch_t<128, true, false>(maps, a, stream) : paged_prefill_launch_t<128, false, false>(maps, a, stream);
 }
 
 }  // namespace b200lora

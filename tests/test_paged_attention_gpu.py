@@ -159,6 +159,23 @@ def test_prefill_tokens_ahead_of_their_context():
     assert bool((out[:4] == 0).all()) and bool((lse[:4] == -float("inf")).all())
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,contexts,window,sinks", [([16], [6000], 0, 0), ([3, 1, 70], [4000, 9000, 3500], 0, 0), ([600], [4200], 0, 0),
+                                                       ([40, 0, 5], [50, 7000, 4000], 3500, 200), ([1], [20000], 0, 0), ([9], [5], 0, 0)])
+def test_prefill_shares_of_long_contexts(new, contexts, window, sinks, dim):
+    """Few tokens behind long contexts: the keys of a block are shared out over the CTAs and joined; run to run the same."""
+    p = PP.make(16, 2, dim, 64, contexts, new, window=window, sinks=sinks, seed=dim + len(new), poison=True, behind=2)
+    pad = max(0, 4096 // 64 - p["args"][3].size(1))  # (the table's width is what tells how long contexts may be)
+    args = list(p["args"])
+    args[3] = torch.nn.functional.pad(args[3], (0, pad), value=-1)
+    out = torch.full_like(args[0], 7.0)
+    got, lse = A.paged_prefill_attention(*args, scale=p["scale"], window=window, sinks=sinks, out=out, return_lse=True)
+    PP.check(p, got, lse, f"{new} {contexts}")
+    assert bool((out[sum(new):] == 7).all())
+    again, lse2 = A.paged_prefill_attention(*args, scale=p["scale"], window=window, sinks=sinks, return_lse=True)
+    assert torch.equal(again[:sum(new)], got[:sum(new)]) and torch.equal(lse2[:sum(new)], lse[:sum(new)])
+
+
 def test_prefill_rows_around_the_sequences():
     """cu_seqlens that begin behind row 0: rows ahead of the first and behind the last sequence stay as they are."""
     p = PP.make(8, 2, 128, 16, [40, 90], [40, 20], seed=8)
