@@ -66,15 +66,17 @@ __host__ __device__ constexpr int paged_block_keys() { return D == 64 ? 32 : 16;
 template <int D>
 __host__ __device__ constexpr int paged_stage_bytes() { return 2 * paged_block_keys<D>() * (D * 2 + 16); }
 template <int D, int NT>
-__host__ __device__ constexpr int paged_smem() {
-  const int ring = kPagedWarps * kPagedStages * paged_stage_bytes<D>(), merge = kPagedWarps * 8 * NT * (D + 2) * 4;
-  return 8 * NT * (D * 2 + 16) + (ring > merge ? ring : merge);
-}
+__host__ __device__ constexpr int paged_smem() { return 2 * 8 * NT * (D * 2 + 16) + kPagedWarps * kPagedStages * paged_stage_bytes<D>(); }
 
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // Joined or single result of a head's two columns
@@ -86,127 +88,203 @@ __device__ __forceinline__ void store_result(const PagedArgs& a, int row, int he
   if (a.lse != nullptr && d == 0) a.lse[(int64_t)row * a.Hq + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
-// A CTA takes a contiguous share of the (row, kv head and chunk, block of keys) sequence. Its warps take the blocks of an item
-// in turn, each through a ring of its own; the keys are the rows of the matrix instruction (S^T = K Q^T, then O^T = V^T P^T), so
-// that eight heads fill it.
-template <int D, int NT, bool kF16>
-__global__ void __launch_bounds__(kPagedThreads, NT == 1 ? 2 : 1) paged_decode_kernel(const PagedArgs a) {
-  extern __shared__ __align__(1024) uint8_t smem[];
+// Blocks [u0, u1) of the keys of one (row, kv head, chunk of its q heads)
+struct PagedPiece {
+  int row, kvh, head0, n_heads, u0, u1, n_units;  // n_units: of the whole item; row < 0: none
+  RowKeys keys;
+};
+
+// Walks the pieces of a CTA: whole items in turn, or an equal share of the blocks of all items.
+template <int kKeys>
+struct PagedWalk {
+  long long at, end, row_at;  // share: units; first unit of `row`
+  int row, step;              // step > 0: whole items `at`, at + step, ...
+  static __device__ __forceinline__ int units(const RowKeys& r) { return r.n_keys < 0 ? 0 : max(1, (r.n_keys + kKeys - 1) / kKeys); }
+  __device__ __forceinline__ PagedPiece next(const PagedArgs& a) {
+    const int per_row = a.Hk * a.chunks, group = a.Hq / a.Hk;
+    PagedPiece w;
+    w.row = -1;
+    int item = 0;
+    while (at < end) {
+      if (step > 0) {
+        row = (int)(at / per_row);
+        item = (int)(at - (long long)row * per_row);
+        at += step;
+        w.keys = row_keys(a, row);
+        w.n_units = units(w.keys);
+        if (w.n_units == 0) continue;
+        w.u0 = 0;
+        w.u1 = w.n_units;
+      } else {
+        w.keys = row_keys(a, row);
+        w.n_units = units(w.keys);
+        if (at >= row_at + (long long)w.n_units * per_row) {
+          row_at += (long long)w.n_units * per_row;
+          ++row;
+          continue;
+        }
+        const unsigned in_row = (unsigned)(at - row_at);
+        item = (int)(in_row / (unsigned)w.n_units);
+        w.u0 = (int)(in_row - (unsigned)item * (unsigned)w.n_units);
+        w.u1 = (int)min((long long)w.n_units, w.u0 + (end - at));
+        at += w.u1 - w.u0;
+      }
+      w.row = row;
+      w.kvh = item / a.chunks;
+      const int chunk = item - w.kvh * a.chunks;
+      w.head0 = w.kvh * group + chunk * a.heads;
+      w.n_heads = min(a.heads, group - chunk * a.heads);
+      return w;
+    }
+    return w;
+  }
+};
+
+// The warps of a CTA take the blocks of an item in turn, each through a ring of its own; the keys are the rows of the matrix
+// instruction (S^T = K Q^T, then O^T = V^T P^T), so that eight heads fill it. What the next piece needs first (its lengths, table
+// entries, queries, two blocks) is asked for ahead of the end of this one.
+template <int D, int NT, bool kF16, bool kShare>
+__global__ void __launch_bounds__(kPagedThreads, 2) paged_decode_kernel(const PagedArgs a) {
+  extern __shared__ __align__(16) uint8_t paged_smem_raw[];  // (a name of its own: 1024-byte alignment would cost heads of 64 the second CTA)
+  uint8_t* const smem = paged_smem_raw;
   constexpr int kPitch = D * 2 + 16, kKeys = paged_block_keys<D>(), kStage = paged_stage_bytes<D>(), kPieces = D / 8;
   constexpr int kMT = kKeys / 16, kPerLoad = 32 / kPieces;  // rows of a load instruction
+  constexpr int kQ = 8 * NT * kPitch, kQEach = (8 * NT * kPieces + kPagedThreads - 1) / kPagedThreads;
+  static_assert(8 * NT * (D + 2) * 4 <= kStage, "a warp's result lies in one stage");
   __shared__ int s_row;
-  __shared__ long long s_at, s_scan[kPagedThreads], s_total;
+  __shared__ long long s_at, s_sum[kPagedWarps];
   __shared__ uint32_t s_live[kPagedWarps][kPagedStages];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int per_row = a.Hk * a.chunks, group = a.Hq / a.Hk;
+  const int per_row = a.Hk * a.chunks;
+  using Walk = PagedWalk<kKeys>;
   glue_enter();
 
-  auto units_of = [&](int row) {
-    const RowKeys r = row_keys(a, row);
-    return r.n_keys < 0 ? 0 : max(1, (r.n_keys + kKeys - 1) / kKeys);
-  };
-  // ---- where this CTA's share begins
-  const int rows_each = (a.T + kPagedThreads - 1) / kPagedThreads;
-  {
+  Walk walk;
+  long long total = 0;
+  int G = gridDim.x;
+  if (!kShare) {
+    walk.step = gridDim.x;
+    walk.at = blockIdx.x;
+    walk.end = (long long)a.T * per_row;
+  } else {
+    // where this CTA's share begins: sums over the rows, a thread a run of them
+    const int rows_each = (a.T + kPagedThreads - 1) / kPagedThreads;
     long long sum = 0;
-    for (int i = 0, row = tid * rows_each; i < rows_each && row < a.T; ++i, ++row) sum += units_of(row);
-    s_scan[tid] = sum;
-    __syncthreads();
-    if (tid == 0) {
-      long long run = 0;
-      for (int i = 0; i < kPagedThreads; ++i) { const long long v = s_scan[i]; s_scan[i] = run; run += v; }
-      s_total = run * per_row;
+    for (int i = 0, row = tid * rows_each; i < rows_each && row < a.T; ++i, ++row) sum += Walk::units(row_keys(a, row));
+    long long upto = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const long long v = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += v;
     }
+    if (lane == 31) s_sum[warp] = upto;
     __syncthreads();
-  }
-  const long long total = s_total;
-  const int G = (int)max(1ll, min((long long)gridDim.x, total / kPagedWarps));  // shares of a block for every warp, or more
-  if (tid == 0) a.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
-  if ((int)blockIdx.x >= G || total == 0) return;
-  const long long begin = total * blockIdx.x / G, end = total * (blockIdx.x + 1) / G;
-  {
-    const long long from = s_scan[tid] * per_row, to = tid + 1 < kPagedThreads ? s_scan[tid + 1] * per_row : total;
-    if (from <= begin && begin < to) {
+    long long ahead = 0;
+#pragma unroll
+    for (int w = 0; w < kPagedWarps; ++w) {
+      if (w < warp) ahead += s_sum[w];
+      total += s_sum[w];
+    }
+    total *= per_row;
+    G = (int)max(1ll, min((long long)gridDim.x, total / kPagedWarps));  // shares of a block for every warp, or more
+    if (tid == 0) a.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if ((int)blockIdx.x >= G || total == 0) return;
+    walk.step = 0;
+    walk.at = total * blockIdx.x / G;
+    walk.end = total * (blockIdx.x + 1) / G;
+    const long long to = (ahead + upto) * per_row, from = to - sum * per_row;
+    if (from <= walk.at && walk.at < to) {
       long long at = from;
       int row = tid * rows_each;
       for (;; ++row) {
-        const long long n = (long long)units_of(row) * per_row;
-        if (begin < at + n) break;
+        const long long n = (long long)Walk::units(row_keys(a, row)) * per_row;
+        if (walk.at < at + n) break;
         at += n;
       }
       s_row = row;
       s_at = at;
     }
     __syncthreads();
+    walk.row = s_row;
+    walk.row_at = s_at;
   }
-  int row = s_row;
-  long long row_at = s_at;  // first unit of the row
 
-  const uint32_t q_u32 = smem_u32(smem), ring = q_u32 + 8 * NT * kPitch + (uint32_t)(warp * kPagedStages * kStage);
+  const uint32_t q_u32 = smem_u32(smem), ring_at = 2 * kQ + warp * kPagedStages * kStage, ring = q_u32 + ring_at;
   const char *k_base = static_cast<const char*>(a.cache.k), *v_base = static_cast<const char*>(a.cache.v);
-  bool first_piece = true;
-  for (long long at = begin; at < end;) {
-    const RowKeys keys = row_keys(a, row);
-    const int n_units = keys.n_keys < 0 ? 0 : max(1, (keys.n_keys + kKeys - 1) / kKeys);
-    if (at >= row_at + (long long)n_units * per_row) {
-      row_at += (long long)n_units * per_row;
-      ++row;
-      continue;
-    }
-    const int item = (int)((at - row_at) / n_units), u0 = (int)((at - row_at) - (long long)item * n_units);
-    const int u1 = (int)min((long long)n_units, u0 + (end - at));
-    const int kvh = item / a.chunks, chunk = item - kvh * a.chunks;
-    const int head0 = kvh * group + chunk * a.heads, n_heads = min(a.heads, group - chunk * a.heads);
-    const int32_t* table = a.tables + keys.req * a.table_ld;
-
-    // this warp's blocks: u0 + warp, u0 + warp + 4, ...
-    auto load = [&](int u, int stage) {
-      if (u < u1) {
-        const int i = u * kKeys + lane;
-        int64_t kr = 0, vr = 0;
-        bool live = false;
-        if (lane < kKeys && i < keys.n_keys) {
-          const int key = keys.key(i), page = key / a.cache.block_size, in_page = key - page * a.cache.block_size;
-          const int blk = table[page];
-          live = (unsigned)blk < (unsigned)a.cache.num_blocks;  // (an entry outside the cache: its keys are left out)
-          if (live) {
-            kr = 2 * (blk * a.cache.k_block + in_page * a.cache.k_token + kvh * a.cache.k_head);
-            vr = 2 * (blk * a.cache.v_block + in_page * a.cache.v_token + kvh * a.cache.v_head);
-          }
-        }
-        const uint32_t mask = __ballot_sync(0xffffffffu, live);
-        if (lane == 0) s_live[warp][stage] = mask;
-        const int p = lane % kPieces;
-#pragma unroll
-        for (int j = 0; j < kKeys / kPerLoad; ++j) {
-          const int r = j * kPerLoad + lane / kPieces;
-          const int64_t ks = __shfl_sync(0xffffffffu, kr, r), vs = __shfl_sync(0xffffffffu, vr, r);
-          const uint32_t bytes = (mask >> r) & 1u ? 16u : 0u;  // (rows that are not seen are zero: 0 * V must be 0)
-          const uint32_t dst = ring + (uint32_t)(stage * kStage + r * kPitch + p * 16);
-          cp_async_16(dst, k_base + ks + p * 16, bytes);
-          cp_async_16(dst + kKeys * kPitch, v_base + vs + p * 16, bytes);
-        }
+  // The block of the cache that holds the lane's key of block u, -1: none. (One block ahead of its use: a look-up takes as long as
+  // the rows themselves.)
+  auto entry = [&](const PagedPiece& w, int u) {
+    const int i = u * kKeys + lane;
+    if (w.row < 0 || u >= w.u1 || lane >= kKeys || i >= w.keys.n_keys) return -1;
+    return a.tables[w.keys.req * a.table_ld + w.keys.key(i) / a.cache.block_size];
+  };
+  auto load = [&](const PagedPiece& w, int u, int blk, int stage) {
+    if (w.row >= 0 && u < w.u1) {
+      const bool live = (unsigned)blk < (unsigned)a.cache.num_blocks;  // (an entry outside the cache: its keys are left out)
+      int64_t kr = 0, vr = 0;
+      if (live) {
+        const int in_block = w.keys.key(u * kKeys + lane) % a.cache.block_size;
+        kr = 2 * (blk * a.cache.k_block + in_block * a.cache.k_token + w.kvh * a.cache.k_head);
+        vr = 2 * (blk * a.cache.v_block + in_block * a.cache.v_token + w.kvh * a.cache.v_head);
       }
-      cp_async_commit();
-    };
+      const uint32_t mask = __ballot_sync(0xffffffffu, live);
+      if (lane == 0) s_live[warp][stage] = mask;
+      const int p = lane % kPieces;
 #pragma unroll
-    for (int s = 0; s < kPagedStages - 1; ++s) load(u0 + warp + s * kPagedWarps, s);
-
-    // q of the chunk's heads; unused rows are zero
-    for (int i = tid; i < 8 * NT * kPieces; i += kPagedThreads) {
-      const int h = i / kPieces, p = i - h * kPieces;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (h < n_heads) v = *reinterpret_cast<const uint4*>(static_cast<const char*>(a.q) + 2 * (row * a.q_token + (head0 + h) * a.q_head + p * 8));
-      sts128(q_u32 + (uint32_t)(h * kPitch + p * 16), v);
+      for (int j = 0; j < kKeys / kPerLoad; ++j) {
+        const int r = j * kPerLoad + lane / kPieces;
+        const int64_t ks = __shfl_sync(0xffffffffu, kr, r), vs = __shfl_sync(0xffffffffu, vr, r);
+        const uint32_t bytes = (mask >> r) & 1u ? 16u : 0u;  // (rows that are not seen are zero: 0 * V must be 0)
+        const uint32_t dst = ring + (uint32_t)(stage * kStage + r * kPitch + p * 16);
+        cp_async_16(dst, k_base + ks + p * 16, bytes);
+        cp_async_16(dst + kKeys * kPitch, v_base + vs + p * 16, bytes);
+      }
     }
-    __syncthreads();
+    cp_async_commit();
+  };
+  auto after = [](int stage, int n) { return stage + n >= kPagedStages ? stage + n - kPagedStages : stage + n; };
+  // a thread's pieces of q of the piece's heads; unused rows are zero
+  uint4 q_piece[kQEach];
+  auto load_q = [&](const PagedPiece& w) {
+#pragma unroll
+    for (int e = 0; e < kQEach; ++e) {
+      const int i = tid + e * kPagedThreads, h = i / kPieces, p = i - h * kPieces;
+      q_piece[e] = make_uint4(0, 0, 0, 0);
+      if (w.row >= 0 && h < w.n_heads)
+        q_piece[e] = *reinterpret_cast<const uint4*>(static_cast<const char*>(a.q) + 2 * (w.row * a.q_token + (w.head0 + h) * a.q_head + p * 8));
+    }
+  };
+  auto put_q = [&](int buf) {
+#pragma unroll
+    for (int e = 0; e < kQEach; ++e) {
+      const int i = tid + e * kPagedThreads, h = i / kPieces, p = i - h * kPieces;
+      if (h < 8 * NT) sts128(q_u32 + (uint32_t)(buf * kQ + h * kPitch + p * 16), q_piece[e]);
+    }
+  };
+
+  PagedPiece w = walk.next(a);
+  int stage = 0, buf = 0;
+  bool first_piece = true;
+  {
+    const int e0 = entry(w, w.u0 + warp), e1 = entry(w, w.u0 + warp + kPagedWarps);
+    load_q(w);
+    load(w, w.u0 + warp, e0, 0);
+    load(w, w.u0 + warp + kPagedWarps, e1, 1);
+    put_q(0);
+  }
+  while (w.row >= 0) {
+    int e = entry(w, w.u0 + warp + 2 * kPagedWarps);
+    const PagedPiece following = walk.next(a);
+    const int e0 = entry(following, following.u0 + warp), e1 = entry(following, following.u0 + warp + kPagedWarps);
+    load_q(following);
+    __syncthreads();  // q is there; the stages that held results may be filled again
     uint32_t qf[NT][D / 16][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int k = 0; k < D / 32; ++k) {
         uint32_t r[4];
-        ldsm_x4(q_u32 + (uint32_t)((8 * n + (lane & 7)) * kPitch + (lane >> 3) * 16 + 64 * k), r);
+        ldsm_x4(q_u32 + (uint32_t)(buf * kQ + (8 * n + (lane & 7)) * kPitch + (lane >> 3) * 16 + 64 * k), r);
         qf[n][2 * k][0] = r[0]; qf[n][2 * k][1] = r[1];
         qf[n][2 * k + 1][0] = r[2]; qf[n][2 * k + 1][1] = r[3];
       }
@@ -218,9 +296,9 @@ __global__ void __launch_bounds__(kPagedThreads, NT == 1 ? 2 : 1) paged_decode_k
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) o[n][d][0] = o[n][d][1] = o[n][d][2] = o[n][d][3] = 0.f;
     }
-    int stage = 0;
-    for (int u = u0 + warp; u < u1; u += kPagedWarps) {
-      load(u + (kPagedStages - 1) * kPagedWarps, stage == 0 ? kPagedStages - 1 : stage - 1);
+    for (int u = w.u0 + warp; u < w.u1; u += kPagedWarps) {
+      load(w, u + 2 * kPagedWarps, e, after(stage, 2));
+      e = entry(w, u + 3 * kPagedWarps);
       cp_async_wait_group<kPagedStages - 1>();
       __syncwarp();
       const uint32_t ks = ring + (uint32_t)(stage * kStage), vs = ks + kKeys * kPitch, live = s_live[warp][stage];
@@ -244,10 +322,10 @@ __global__ void __launch_bounds__(kPagedThreads, NT == 1 ? 2 : 1) paged_decode_k
 #pragma unroll
         for (int i = 0; i < kMT; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const bool seen = (live >> (16 * i + g + 8 * (e >> 1))) & 1u;
-            s[n][i][e] = seen ? s[n][i][e] * a.sc : -INFINITY;
-            grows |= s[n][i][e] > m[n][e & 1] + 8.f;
+          for (int x = 0; x < 4; ++x) {
+            const bool seen = (live >> (16 * i + g + 8 * (x >> 1))) & 1u;
+            s[n][i][x] = seen ? s[n][i][x] * a.sc : -INFINITY;
+            grows |= s[n][i][x] > m[n][x & 1] + 8.f;
           }
       if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
@@ -260,7 +338,7 @@ __global__ void __launch_bounds__(kPagedThreads, NT == 1 ? 2 : 1) paged_decode_k
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            const float f = mx == -INFINITY ? 1.f : exp2f(m[n][c] - mx);
+            const float f = mx == -INFINITY ? 1.f : ex2(m[n][c] - mx);
             m[n][c] = mx;
             l[n][c] *= f;
 #pragma unroll
@@ -273,10 +351,10 @@ __global__ void __launch_bounds__(kPagedThreads, NT == 1 ? 2 : 1) paged_decode_k
 #pragma unroll
         for (int i = 0; i < kMT; ++i) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float top = m[n][e & 1];
-            s[n][i][e] = exp2f(s[n][i][e] - (top == -INFINITY ? 0.f : top));
-            l[n][e & 1] += s[n][i][e];
+          for (int x = 0; x < 4; ++x) {
+            const float top = m[n][x & 1];
+            s[n][i][x] = ex2(s[n][i][x] - (top == -INFINITY ? 0.f : top));
+            l[n][x & 1] += s[n][i][x];
           }
           // (probabilities are rounded to the type of V for the matrix product; their sum is that of the unrounded ones)
           pf[n][i][0] = transpose_8x8(pack_16x2<kF16>(s[n][i][0], s[n][i][1]));
@@ -292,9 +370,11 @@ __global__ void __launch_bounds__(kPagedThreads, NT == 1 ? 2 : 1) paged_decode_k
           for (int n = 0; n < NT; ++n) mma_16816<kF16>(o[n][d], vf[0], vf[1], vf[2], vf[3], pf[n][i][0], pf[n][i][1]);
         }
       __syncwarp();  // every lane has read the stage
-      stage = stage + 1 == kPagedStages ? 0 : stage + 1;
+      stage = after(stage, 1);
     }
-    cp_async_wait_group<0>();
+    load(following, following.u0 + warp, e0, stage);
+    load(following, following.u0 + warp + kPagedWarps, e1, after(stage, 1));
+    put_q(buf ^ 1);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -303,38 +383,42 @@ __global__ void __launch_bounds__(kPagedThreads, NT == 1 ? 2 : 1) paged_decode_k
         l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 8);
         l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 16);
       }
-    __syncthreads();  // every warp is done with its ring
-    float* acc = reinterpret_cast<float*>(smem + 8 * NT * kPitch);
-    float* ml = acc + kPagedWarps * 8 * NT * D;
+    // the warps' results, each in the third stage of its ring, where nothing is under way
+    __shared__ int s_third[kPagedWarps];
+    float* const mine = reinterpret_cast<float*>(smem + ring_at + after(stage, 2) * kStage);
+    if (lane == 0) s_third[warp] = after(stage, 2);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int h = 8 * n + 2 * t + c;
-        float* dst = acc + (warp * 8 * NT + h) * D + g;
+        float* dst = mine + h * D + g;
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) { dst[16 * d] = o[n][d][c]; dst[16 * d + 8] = o[n][d][c + 2]; }
-        if (g == 0) { ml[(warp * 8 * NT + h) * 2] = m[n][c]; ml[(warp * 8 * NT + h) * 2 + 1] = l[n][c]; }
+        if (g == 0) { mine[8 * NT * D + 2 * h] = m[n][c]; mine[8 * NT * D + 2 * h + 1] = l[n][c]; }
       }
     __syncthreads();
-    const bool whole = u0 == 0 && u1 == n_units;
+    const float* part[kPagedWarps];
+#pragma unroll
+    for (int k = 0; k < kPagedWarps; ++k) part[k] = reinterpret_cast<const float*>(smem + 2 * kQ + (k * kPagedStages + s_third[k]) * kStage);
+    const bool whole = !kShare || (w.u0 == 0 && w.u1 == w.n_units);
     const int slot = 2 * blockIdx.x + (first_piece ? 0 : 1);
-    for (int i = tid; i < n_heads * (D / 2); i += kPagedThreads) {
+    for (int i = tid; i < w.n_heads * (D / 2); i += kPagedThreads) {
       const int h = i / (D / 2), d = 2 * (i - h * (D / 2));
       float top = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kPagedWarps; ++w) top = fmaxf(top, ml[(w * 8 * NT + h) * 2]);
+      for (int k = 0; k < kPagedWarps; ++k) top = fmaxf(top, part[k][8 * NT * D + 2 * h]);
       float sum = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-      for (int w = 0; w < kPagedWarps; ++w) {
-        const float mw = ml[(w * 8 * NT + h) * 2], f = mw == -INFINITY ? 0.f : exp2f(mw - top);
-        const float2 v = *reinterpret_cast<const float2*>(acc + (w * 8 * NT + h) * D + d);
-        sum += f * ml[(w * 8 * NT + h) * 2 + 1];
+      for (int k = 0; k < kPagedWarps; ++k) {
+        const float2 ml = *reinterpret_cast<const float2*>(part[k] + 8 * NT * D + 2 * h), v = *reinterpret_cast<const float2*>(part[k] + h * D + d);
+        const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+        sum += f * ml.y;
         x += f * v.x;
         y += f * v.y;
       }
       if (whole) {
-        store_result<kF16>(a, row, head0 + h, d, x, y, top, sum);
+        store_result<kF16>(a, w.row, w.head0 + h, d, x, y, top, sum);
       } else {
         const int64_t at_slot = (int64_t)slot * a.heads + h;
         *reinterpret_cast<float2*>(a.part_o + at_slot * D + d) = make_float2(x, y);
@@ -342,43 +426,58 @@ __global__ void __launch_bounds__(kPagedThreads, NT == 1 ? 2 : 1) paged_decode_k
       }
     }
     // the CTA that begins an item and does not end it says who ends it: the last one whose share begins before the item's end
-    if (u0 == 0 && !whole && tid == 0) {
-      const long long item_end = row_at + (long long)(item + 1) * n_units;
+    if (kShare && w.u0 == 0 && !whole && tid == 0) {
+      const long long item_end = total * (blockIdx.x + 1) / G + (w.n_units - w.u1);  // (its last piece)
       int last = (int)min((long long)G - 1, (item_end * G - 1) / total);
       while (last + 1 < G && total * (last + 1) / G < item_end) ++last;  // (the shares' bounds are rounded down)
       while (total * last / G >= item_end) --last;
-      a.joins[blockIdx.x] = make_int4(row, item, slot, last);
+      a.joins[blockIdx.x] = make_int4(w.row, w.head0, slot, last);
     }
-    __syncthreads();  // the ring may be filled again
-    at += u1 - u0;
     first_piece = false;
+    buf ^= 1;
+    w = following;
   }
+  cp_async_wait_group<0>();
 }
 
-// Joins the parts of an item that begins in CTA blockIdx.x: its own, then the first one of every CTA up to the last.
+// Joins the parts of the item that begins in CTA blockIdx.x: its own, then the first one of every CTA up to the last; one of its
+// heads (blockIdx.y). D / 4 threads keep four columns each; groups of them take the parts in turn.
 template <int D, bool kF16>
 __global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const PagedArgs a) {
+  constexpr int kLanes = D / 4, kGroups = kPagedThreads / kLanes;
+  __shared__ float4 s_o[kGroups][kLanes];
+  __shared__ float2 s_ml[kGroups];
   glue_enter();
   const int4 j = a.joins[blockIdx.x];
-  if (j.x < 0) return;
-  const int group = a.Hq / a.Hk, kvh = j.y / a.chunks, chunk = j.y - kvh * a.chunks;
-  const int head0 = kvh * group + chunk * a.heads, n_heads = min(a.heads, group - chunk * a.heads);
-  const int parts = j.w - (int)blockIdx.x + 1;
-  auto slot_of = [&](int i) { return (int64_t)(i == 0 ? j.z : 2 * ((int)blockIdx.x + i)) * a.heads; };
-  for (int i = threadIdx.x; i < n_heads * (D / 2); i += kPagedThreads) {
-    const int h = i / (D / 2), d = 2 * (i - h * (D / 2));
-    float top = -INFINITY, sum = 0.f, x = 0.f, y = 0.f;
-    for (int k = 0; k < parts; ++k) {
-      const int64_t at = slot_of(k) + h;
-      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2), v = *reinterpret_cast<const float2*>(a.part_o + at * D + d);
-      const float up = fmaxf(top, ml.x), f0 = top == -INFINITY ? 0.f : exp2f(top - up), f1 = ml.x == -INFINITY ? 0.f : exp2f(ml.x - up);
-      x = f0 * x + f1 * v.x;
-      y = f0 * y + f1 * v.y;
-      sum = f0 * sum + f1 * ml.y;
-      top = up;
-    }
-    store_result<kF16>(a, j.x, head0 + h, d, x, y, top, sum);
+  const int group = a.Hq / a.Hk, in_group = j.y % group, n_heads = min(a.heads, group - in_group);
+  if (j.x < 0 || (int)blockIdx.y >= n_heads) return;
+  const int parts = j.w - (int)blockIdx.x + 1, c = threadIdx.x % kLanes, mine = threadIdx.x / kLanes;
+  auto slot_of = [&](int k) { return (int64_t)(k == 0 ? j.z : 2 * ((int)blockIdx.x + k)) * a.heads + blockIdx.y; };
+  auto stats = [&](int k) { return *reinterpret_cast<const float2*>(a.part_ml + slot_of(k) * 2); };
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < parts; ++k) top = fmaxf(top, stats(k).x);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int k = mine; k < parts; k += kGroups) {
+    const float2 ml = stats(k);
+    const float4 v = *reinterpret_cast<const float4*>(a.part_o + slot_of(k) * D + 4 * c);
+    const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+    sum += f * ml.y;
+    o = make_float4(o.x + f * v.x, o.y + f * v.y, o.z + f * v.z, o.w + f * v.w);
   }
+  s_o[mine][c] = o;
+  if (c == 0) s_ml[mine].y = sum;
+  __syncthreads();
+  if (mine != 0) return;
+  for (int k = 1; k < kGroups; ++k) {
+    const float4 v = s_o[k][c];
+    sum += s_ml[k].y;
+    o = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+  }
+  store_result<kF16>(a, j.x, j.y + blockIdx.y, 4 * c, o.x, o.y, top, sum);
+  const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+  *reinterpret_cast<uint32_t*>(static_cast<char*>(a.out) + 2 * (j.x * a.out_token + (j.y + (int)blockIdx.y) * a.out_head + 4 * c + 2)) = pack_16x2<kF16>(o.z * inv, o.w * inv);
 }
 
 inline size_t paged_parts_bytes(int heads, int D) { return (size_t)2 * kPagedCtas * heads * D * 4; }
@@ -387,13 +486,28 @@ inline size_t paged_workspace_bytes(int Hq, int Hk, int D) {
   return paged_parts_bytes(heads, D) + (size_t)2 * kPagedCtas * heads * 8 + kPagedCtas * sizeof(int4);
 }
 
-template <int D, int NT, bool kF16>
-inline int paged_decode_launch_t(const PagedArgs& a, cudaStream_t stream) {
-  const cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<D, NT, kF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, paged_smem<D, NT>());
+#ifndef B200_WHOLE
+#define B200_WHOLE 32
+#endif
+template <int D, int NT, bool kF16, bool kShare>
+inline int paged_decode_launch_t(const PagedArgs& a, int ctas, cudaStream_t stream) {
+  const auto kernel = paged_decode_kernel<D, NT, kF16, kShare>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, paged_smem<D, NT>());
   if (e != cudaSuccess) return fail(B200_LORA_ECUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-  const int rc = launch_dependent(paged_decode_kernel<D, NT, kF16>, "paged_decode_kernel", dim3(kPagedCtas), kPagedThreads, paged_smem<D, NT>(), stream, a);
-  if (rc != B200_LORA_OK) return rc;
-  return launch_dependent(paged_join_kernel<D, kF16>, "paged_join_kernel", dim3(kPagedCtas), kPagedThreads, 0, stream, a);
+  const int rc = launch_dependent(kernel, "paged_decode_kernel", dim3((unsigned)ctas), kPagedThreads, paged_smem<D, NT>(), stream, a);
+  if (rc != B200_LORA_OK || !kShare) return rc;
+  return launch_dependent(paged_join_kernel<D, kF16>, "paged_join_kernel", dim3((unsigned)ctas, (unsigned)a.heads), kPagedThreads, 0, stream, a);
+}
+
+// Items of a few blocks at most, as the table's width and the window tell: each by one CTA, and nothing to join
+template <int D, int NT, bool kF16>
+inline int paged_decode_launch_by(const PagedArgs& a, cudaStream_t stream) {
+  int64_t keys = (int64_t)a.table_width * a.cache.block_size;
+  if (a.window > 0) keys = std::min<int64_t>(keys, (int64_t)a.window + a.sinks);
+  const int64_t units = (keys + paged_block_keys<D>() - 1) / paged_block_keys<D>(), items = (int64_t)a.T * a.Hk * a.chunks;
+  if (units <= B200_WHOLE || (units <= 2 * B200_WHOLE && items >= kPagedCtas))
+    return paged_decode_launch_t<D, NT, kF16, false>(a, (int)std::min<int64_t>(kPagedCtas, items), stream);
+  return paged_decode_launch_t<D, NT, kF16, true>(a, kPagedCtas, stream);
 }
 
 inline int paged_decode_launch(PagedArgs a, int D, int dtype, void* workspace, cudaStream_t stream) {
@@ -406,11 +520,11 @@ inline int paged_decode_launch(PagedArgs a, int D, int dtype, void* workspace, c
   a.joins = reinterpret_cast<int4*>(ws + paged_parts_bytes(a.heads, D) + (size_t)2 * kPagedCtas * a.heads * 8);
   const bool f16 = dtype == B200_LORA_F16, wide = a.heads > 8;
   if (D == 64) {
-    if (wide) return f16 ? paged_decode_launch_t<64, 2, true>(a, stream) : paged_decode_launch_t<64, 2, false>(a, stream);
-    return f16 ? paged_decode_launch_t<64, 1, true>(a, stream) : paged_decode_launch_t<64, 1, false>(a, stream);
+    if (wide) return f16 ? paged_decode_launch_by<64, 2, true>(a, stream) : paged_decode_launch_by<64, 2, false>(a, stream);
+    return f16 ? paged_decode_launch_by<64, 1, true>(a, stream) : paged_decode_launch_by<64, 1, false>(a, stream);
   }
-  if (wide) return f16 ? paged_decode_launch_t<128, 2, true>(a, stream) : paged_decode_launch_t<128, 2, false>(a, stream);
-  return f16 ? paged_decode_launch_t<128, 1, true>(a, stream) : paged_decode_launch_t<128, 1, false>(a, stream);
+  if (wide) return f16 ? paged_decode_launch_by<128, 2, true>(a, stream) : paged_decode_launch_by<128, 2, false>(a, stream);
+  return f16 ? paged_decode_launch_by<128, 1, true>(a, stream) : paged_decode_launch_by<128, 1, false>(a, stream);
 }
 
 }  // namespace b200lora

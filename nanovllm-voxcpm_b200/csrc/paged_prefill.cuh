@@ -85,11 +85,6 @@ __device__ __forceinline__ void pp_wait(uint32_t bar, uint32_t parity, volatile 
   }
   *abort_flag = 1;
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // (NaN where one of them is)
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
