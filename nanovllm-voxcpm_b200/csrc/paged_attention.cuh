@@ -98,7 +98,8 @@ struct PagedPiece {
 template <int kKeys>
 struct PagedWalk {
   long long at, end, row_at;  // share: units; first unit of `row`
-  int row, step;              // step > 0: whole items `at`, at + step, ...
+  int row, step;              // step > 0: items `at`, at + step, ..., of each the rank-th of `ranks` parts
+  int rank, ranks;
   static __device__ __forceinline__ int units(const RowKeys& r) { return r.n_keys < 0 ? 0 : max(1, (r.n_keys + kKeys - 1) / kKeys); }
   __device__ __forceinline__ PagedPiece next(const PagedArgs& a) {
     const int per_row = a.Hk * a.chunks, group = a.Hq / a.Hk;
@@ -113,8 +114,8 @@ struct PagedWalk {
         w.keys = row_keys(a, row);
         w.n_units = units(w.keys);
         if (w.n_units == 0) continue;
-        w.u0 = 0;
-        w.u1 = w.n_units;
+        w.u0 = (int)((int64_t)w.n_units * rank / ranks);
+        w.u1 = (int)((int64_t)w.n_units * (rank + 1) / ranks);
       } else {
         w.keys = row_keys(a, row);
         w.n_units = units(w.keys);
@@ -143,7 +144,10 @@ struct PagedWalk {
 // The warps of a CTA take the blocks of an item in turn, each through a ring of its own; the keys are the rows of the matrix
 // instruction (S^T = K Q^T, then O^T = V^T P^T), so that eight heads fill it. What the next piece needs first (its lengths, table
 // entries, queries, two blocks) is asked for ahead of the end of this one.
-template <int D, int NT, bool kF16, bool kShare>
+// kWay: whose the items are
+constexpr int kWhole = 0, kShares = 1, kClusters = 2;  // one CTA's each; of a share of all blocks; a cluster's each, joined in its shared memory
+
+template <int D, int NT, bool kF16, int kWay>
 __global__ void __launch_bounds__(kPagedThreads, 2) paged_decode_kernel(const PagedArgs a) {
   extern __shared__ __align__(16) uint8_t paged_smem_raw[];  // (a name of its own: 1024-byte alignment would cost heads of 64 the second CTA)
   uint8_t* const smem = paged_smem_raw;
@@ -157,14 +161,22 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_decode_kernel(const Pa
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int per_row = a.Hk * a.chunks;
   using Walk = PagedWalk<kKeys>;
+  constexpr bool kShare = kWay == kShares;
+  uint32_t rank = 0, ranks = 1;
+  if (kWay == kClusters) {
+    rank = cluster_ctarank();
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+  }
   glue_enter();
 
   Walk walk;
   long long total = 0;
   int G = gridDim.x;
   if (!kShare) {
-    walk.step = gridDim.x;
-    walk.at = blockIdx.x;
+    walk.step = (int)(gridDim.x / ranks);
+    walk.at = blockIdx.x / ranks;
+    walk.rank = (int)rank;
+    walk.ranks = (int)ranks;
     walk.end = (long long)a.T * per_row;
   } else {
     // where this CTA's share begins: sums over the rows, a thread a run of them
@@ -277,7 +289,12 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_decode_kernel(const Pa
     const PagedPiece following = walk.next(a);
     const int e0 = entry(following, following.u0 + warp), e1 = entry(following, following.u0 + warp + kPagedWarps);
     load_q(following);
-    __syncthreads();  // q is there; the stages that held results may be filled again
+    if (kWay == kClusters) {
+      cluster_arrive();
+      cluster_wait();
+    } else {
+      __syncthreads();  // q is there; the stages that held results may be filled again
+    }
     uint32_t qf[NT][D / 16][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -401,6 +418,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_decode_kernel(const Pa
     const float* part[kPagedWarps];
 #pragma unroll
     for (int k = 0; k < kPagedWarps; ++k) part[k] = reinterpret_cast<const float*>(smem + 2 * kQ + (k * kPagedStages + s_third[k]) * kStage);
+    __shared__ float2 s_ml[8 * NT];
     const bool whole = !kShare || (w.u0 == 0 && w.u1 == w.n_units);
     const int slot = 2 * blockIdx.x + (first_piece ? 0 : 1);
     for (int i = tid; i < w.n_heads * (D / 2); i += kPagedThreads) {
@@ -417,12 +435,46 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_decode_kernel(const Pa
         x += f * v.x;
         y += f * v.y;
       }
-      if (whole) {
+      if (kWay == kClusters) {  // (in place: no other thread reads or writes these two columns)
+        *reinterpret_cast<float2*>(const_cast<float*>(part[0]) + h * D + d) = make_float2(x, y);
+        if (d == 0) s_ml[h] = make_float2(top, sum);
+      } else if (whole) {
         store_result<kF16>(a, w.row, w.head0 + h, d, x, y, top, sum);
       } else {
         const int64_t at_slot = (int64_t)slot * a.heads + h;
         *reinterpret_cast<float2*>(a.part_o + at_slot * D + d) = make_float2(x, y);
         if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at_slot * 2) = make_float2(top, sum);
+      }
+    }
+    if (kWay == kClusters) {
+      // the cluster's parts: every CTA joins some of the columns
+      cluster_arrive();
+      cluster_wait();
+      const int all = w.n_heads * (D / 2);
+      for (int i = (int)((int64_t)all * rank / ranks) + tid, to = (int)((int64_t)all * (rank + 1) / ranks); i < to; i += kPagedThreads) {
+        const int h = i / (D / 2), d = 2 * (i - h * (D / 2));
+        float2 ml[8], v[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          ml[c] = make_float2(-INFINITY, 0.f);
+          v[c] = make_float2(0.f, 0.f);
+          if (c < (int)ranks) {
+            ml[c] = ld_cluster_f32x2(mapa_shared(smem_u32(&s_ml[h]), c));
+            const uint32_t third = ld_cluster_u32(mapa_shared(smem_u32(&s_third[0]), c));
+            v[c] = ld_cluster_f32x2(mapa_shared(q_u32 + 2 * kQ + third * kStage + 4 * (h * D + d), c));
+          }
+        }
+        float top = -INFINITY, sum = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) top = fmaxf(top, ml[c].x);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const float f = ml[c].x == -INFINITY ? 0.f : ex2(ml[c].x - top);
+          sum += f * ml[c].y;
+          x += f * v[c].x;
+          y += f * v[c].y;
+        }
+        store_result<kF16>(a, w.row, w.head0 + h, d, x, y, top, sum);
       }
     }
     // the CTA that begins an item and does not end it says who ends it: the last one whose share begins before the item's end
@@ -438,6 +490,10 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_decode_kernel(const Pa
     w = following;
   }
   cp_async_wait_group<0>();
+  if (kWay == kClusters) {  // (no CTA leaves while another reads its part)
+    cluster_arrive();
+    cluster_wait();
+  }
 }
 
 // Joins the parts of the item that begins in CTA blockIdx.x: its own, then the first one of every CTA up to the last; one of its
@@ -486,28 +542,52 @@ inline size_t paged_workspace_bytes(int Hq, int Hk, int D) {
   return paged_parts_bytes(heads, D) + (size_t)2 * kPagedCtas * heads * 8 + kPagedCtas * sizeof(int4);
 }
 
-#ifndef B200_WHOLE
-#define B200_WHOLE 32
-#endif
-template <int D, int NT, bool kF16, bool kShare>
-inline int paged_decode_launch_t(const PagedArgs& a, int ctas, cudaStream_t stream) {
-  const auto kernel = paged_decode_kernel<D, NT, kF16, kShare>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, paged_smem<D, NT>());
+template <int D, int NT, bool kF16, int kWay>
+inline int paged_decode_launch_t(const PagedArgs& a, int ctas, int cluster, cudaStream_t stream) {
+  const auto kernel = paged_decode_kernel<D, NT, kF16, kWay>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, paged_smem<D, NT>());
   if (e != cudaSuccess) return fail(B200_LORA_ECUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-  const int rc = launch_dependent(kernel, "paged_decode_kernel", dim3((unsigned)ctas), kPagedThreads, paged_smem<D, NT>(), stream, a);
-  if (rc != B200_LORA_OK || !kShare) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kPagedThreads);
+  cfg.dynamicSmemBytes = paged_smem<D, NT>();
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = bgmv_options().pdl ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, kernel, a);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(B200_LORA_ECUDA, "paged_decode_kernel launch: %s", cudaGetErrorString(e));
+  }
+  if (kWay != kShares) return B200_LORA_OK;
   return launch_dependent(paged_join_kernel<D, kF16>, "paged_join_kernel", dim3((unsigned)ctas, (unsigned)a.heads), kPagedThreads, 0, stream, a);
 }
 
-// Items of a few blocks at most, as the table's width and the window tell: each by one CTA, and nothing to join
+// How the items (row, kv head, chunk) meet the CTAs, by what the host knows: their number, and the blocks of keys of one at most
+// (the table's width, the window). us, one CTA an item / clusters of 2, 4, 8 / equal shares:
+//   16 / 2 heads of 64: one request of 700 tokens (2 items, 22 blocks) 8.0 / 7.7, 6.7, 6.1 / 10.9; of 8000 48 / 28, 18, 12.4 / 15.9;
+//   of 32000 208 / 110, 62, 34 / 21; 64 of 1000 (128 items, 32 blocks) 11.9 / 12.7, 17, 34 / 16.7; 64 of 8000 64 / 51, 53, 81 / 53
+//   16 / 2 of 128: 16 of 4000 (32, 250) 56 / 34, 22, 18.7 / 23; 64 of 2000 (128, 125) 33 / 30, 33, 58 / 34; 128 of a window of 1024
+//   (256, 65) 28 / 35, 56, 95 / 35; 32 / 8 of 128: 8 of 300 (64, 19) 7.8 / 8.5, 8.5, 12.9 / 13.1; 8 of 2000 30 / 21, 18.3, 23 / 22;
+//   ragged, 48 of 500 to 8192 (384, 512) 204 / 171, 187, 258 / 140; 16 of 100 to 16000 (128, 1000) 208 / 134, 142, 137 / 110
 template <int D, int NT, bool kF16>
 inline int paged_decode_launch_by(const PagedArgs& a, cudaStream_t stream) {
   int64_t keys = (int64_t)a.table_width * a.cache.block_size;
   if (a.window > 0) keys = std::min<int64_t>(keys, (int64_t)a.window + a.sinks);
   const int64_t units = (keys + paged_block_keys<D>() - 1) / paged_block_keys<D>(), items = (int64_t)a.T * a.Hk * a.chunks;
-  if (units <= B200_WHOLE || (units <= 2 * B200_WHOLE && items >= kPagedCtas))
-    return paged_decode_launch_t<D, NT, kF16, false>(a, (int)std::min<int64_t>(kPagedCtas, items), stream);
-  return paged_decode_launch_t<D, NT, kF16, true>(a, kPagedCtas, stream);
+  int cluster = 1;
+  while (cluster < 8 && ((2 * items * cluster <= 148 && units >= 4 * cluster) || (2 * items * cluster <= kPagedCtas && units >= 48 * cluster))) cluster *= 2;
+  if ((units > 128 * cluster && items < 8 * kPagedCtas) || (cluster == 8 && 16 * items <= kPagedCtas && units > 400))
+    return paged_decode_launch_t<D, NT, kF16, kShares>(a, kPagedCtas, 1, stream);
+  const int ctas = (int)std::min<int64_t>(kPagedCtas / cluster, items) * cluster;
+  if (cluster == 1) return paged_decode_launch_t<D, NT, kF16, kWhole>(a, ctas, 1, stream);
+  return paged_decode_launch_t<D, NT, kF16, kClusters>(a, ctas, cluster, stream);
 }
 
 inline int paged_decode_launch(PagedArgs a, int D, int dtype, void* workspace, cudaStream_t stream) {
