@@ -9,6 +9,9 @@ through flash_attn (``flash_attn_varlen_func`` for prefill, ``flash_attn_with_kv
 table for decode), as in the reference (``layers/attention.py:10-79``). The steps in between
 (residual add + RMSNorm, RoPE + cache store, SiLU * up) run as plain torch ops, or, with
 ``Decoder.fused_glue = True``, as the single-launch kernels of ``glue.py``.
+With ``DecoderConfig.paged_attention`` (which a sliding window implies) attention is ``attention.py``'s over the paged
+cache, for prompts, chunks of them and decode rows alike; with ``qk_norm`` every query and key head is RMS-normed ahead of
+the rotation.
 
 It exists to time a whole step with the multi-LoRA kernels in their real surroundings (one prefill
 step over all prompts, then decode steps replayed from a CUDA graph) and to compare it with the same
@@ -24,6 +27,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _native as N
+from . import attention as A
 from . import glue as G
 from . import layers as L
 from . import lora as LORA
@@ -48,6 +52,19 @@ class DecoderConfig:
     #: how the row-parallel layers (o, down) handle their LoRA delta under tensor parallelism
     #: (``layers.LoRARowParallelLinear``): "partial_y" (the reference's), "allreduce_tmp", "peer_exchange"
     lora_tp_mode: str = "partial_y"
+    #: RMS norm of every query and key head ahead of the rotation
+    qk_norm: bool = False
+    #: attention over the paged cache by ``attention.py`` instead of flash_attn
+    paged_attention: bool = False
+    #: keys that a token sees, its own among them (0: all), and first tokens that stay visible besides
+    sliding_window: int = 0
+    sink_tokens: int = 0
+
+    def __post_init__(self) -> None:
+        if self.sliding_window < 0 or self.sink_tokens < 0 or (self.sink_tokens and not self.sliding_window):
+            raise ValueError("sliding_window and sink_tokens must not be negative, and first tokens stay visible besides a window")
+        if self.sliding_window:
+            self.paged_attention = True
 
 
 @dataclass
@@ -63,6 +80,10 @@ class AttentionStep:
     #: mixed step (``is_prefill`` True and ``n_decode`` > 0): rows ``[0, n_decode)`` are single-token decode rows
     #: (``context_lens`` / ``block_tables`` describe them), the rest is a prefill chunk (``cu_seqlens``)
     n_decode: int = 0
+    #: with ``paged_attention``: int32 [B] tokens of the prefill requests, the new ones included (more than those where a prompt
+    #: comes in chunks), and their block tables
+    prefill_context_lens: torch.Tensor | None = None
+    prefill_block_tables: torch.Tensor | None = None
 
 
 def _rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
@@ -88,6 +109,9 @@ class DecoderAttention(nn.Module):
                                                 max_loras=cfg.max_loras, max_lora_rank=cfg.max_lora_rank)
         self.o_proj = L.LoRARowParallelLinear(cfg.num_heads * cfg.head_dim, cfg.hidden_size, max_loras=cfg.max_loras,
                                               max_lora_rank=cfg.max_lora_rank, lora_tp_mode=cfg.lora_tp_mode)
+        if cfg.qk_norm:
+            self.q_norm = nn.Parameter(torch.ones(cfg.head_dim))
+            self.k_norm = nn.Parameter(torch.ones(cfg.head_dim))
         self.k_cache = self.v_cache = None  # [blocks, block_size, kv_heads, head_dim], set by the harness
 
     def forward(self, positions, hidden, step: AttentionStep, cos_sin) -> torch.Tensor:
@@ -95,8 +119,11 @@ class DecoderAttention(nn.Module):
         qkv = self.qkv_proj(hidden)
         q, k, v = qkv.split([self.q_size, self.kv_size, self.kv_size], dim=-1)
         cos, sin = cos_sin
-        q = _rope(q.view(-1, self.heads, cfg.head_dim), cos, sin)
-        k = _rope(k.view(-1, self.kv_heads, cfg.head_dim), cos, sin)
+        q, k = q.view(-1, self.heads, cfg.head_dim), k.view(-1, self.kv_heads, cfg.head_dim)
+        if cfg.qk_norm:
+            q, k = _rms_norm(q, self.q_norm, cfg.rms_norm_eps), _rms_norm(k, self.k_norm, cfg.rms_norm_eps)
+        q = _rope(q, cos, sin)
+        k = _rope(k, cos, sin)
         v = v.reshape(-1, self.kv_heads, cfg.head_dim)
         flat_k = self.k_cache.view(-1, self.kv_heads, cfg.head_dim)
         flat_v = self.v_cache.view(-1, self.kv_heads, cfg.head_dim)
@@ -104,8 +131,23 @@ class DecoderAttention(nn.Module):
         flat_v.index_copy_(0, step.slot_mapping, v)
         return self.o_proj(self._attend(q, k, v, step).reshape(-1, self.q_size))
 
+    def _attend_paged(self, q, step: AttentionStep) -> torch.Tensor:
+        """``attention.py`` over the paged cache, which holds the new rows already."""
+        cfg = self.cfg
+        how = dict(scale=cfg.head_dim ** -0.5, window=cfg.sliding_window, sinks=cfg.sink_tokens)
+        nd = step.n_decode if step.is_prefill else q.size(0)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        if nd:
+            A.paged_decode_attention(q[:nd], self.k_cache, self.v_cache, step.block_tables, step.context_lens, out=out[:nd], **how)
+        if step.is_prefill:
+            A.paged_prefill_attention(q[nd:], self.k_cache, self.v_cache, step.prefill_block_tables, step.prefill_context_lens,
+                                      step.cu_seqlens, out=out[nd:], **how)
+        return out
+
     def _attend(self, q, k, v, step: AttentionStep) -> torch.Tensor:
         """flash_attn over the paged cache (decode rows) and / or the packed prompts (prefill rows)."""
+        if self.cfg.paged_attention:
+            return self._attend_paged(q, step)
         from flash_attn import flash_attn_varlen_func, flash_attn_with_kvcache
 
         scale = self.cfg.head_dim ** -0.5
@@ -122,8 +164,15 @@ class DecoderAttention(nn.Module):
     def forward_fused(self, positions, normed, step: AttentionStep, cos, sin, slot_mapping_i32) -> torch.Tensor:
         """Same as ``forward`` with RoPE and the cache store as one in-place kernel over the packed qkv rows."""
         cfg = self.cfg
-        q, k, v = G.rope_kv_store(self.qkv_proj(normed), self.heads, self.kv_heads, cfg.head_dim, positions=positions,
-                                  cos=cos, sin=sin, k_cache=self.k_cache, v_cache=self.v_cache, slot_mapping=slot_mapping_i32)
+        how = dict(positions=positions, cos=cos, sin=sin, k_cache=self.k_cache, v_cache=self.v_cache, slot_mapping=slot_mapping_i32)
+        qkv = self.qkv_proj(normed)
+        if cfg.qk_norm:
+            # (attention over the cache reads no k but the cache's: the packed rows need not have it)
+            q_out = torch.empty(qkv.size(0), self.heads, cfg.head_dim, dtype=qkv.dtype, device=qkv.device) if cfg.paged_attention else None
+            q, k, v = G.qk_norm_rope_kv_store(qkv, self.heads, self.kv_heads, cfg.head_dim, self.q_norm, self.k_norm, cfg.rms_norm_eps,
+                                              q_out=q_out, **how)
+        else:
+            q, k, v = G.rope_kv_store(qkv, self.heads, self.kv_heads, cfg.head_dim, **how)
         return self.o_proj(self._attend(q, k, v, step).reshape(-1, self.q_size))
 
 
@@ -195,7 +244,7 @@ class Decoder(nn.Module):
         128) one row 57 / 113, 85 / 119, 129 / 127; 64 rows 82 / 129, 111 / 163, 155 / 218. 4096-wide (8 of 128) one row 114 /
         194, 142 / 204, 187 / 207; 32 rows 191 / 241, 246 / 308, 334 / 414; 64 rows 232 / 277, 344 / 411."""
         cfg, T = self.cfg, embeds.size(0)
-        if step.is_prefill or not 1 <= T <= 128 or not embeds.is_cuda:
+        if step.is_prefill or not 1 <= T <= 128 or not embeds.is_cuda or cfg.qk_norm or cfg.paged_attention:
             return False
 
         def dense(t, dtype, *shape) -> bool:  # (the chain passes addresses on: a strided or foreign array would be misread)
@@ -356,6 +405,8 @@ class Decoder(nn.Module):
         for steps and layers that it does not cover (decode rows in the batch, tensor parallelism, biases, other types)."""
         cfg = self.cfg
         if not step.is_prefill or step.n_decode or step.cu_seqlens is None or embeds.dtype != torch.bfloat16:
+            return None
+        if cfg.qk_norm or cfg.paged_attention:
             return None
         backend = LORA.get_backend()
         if not isinstance(backend, LORA.B200LoRABackend) or backend.impl != N.IMPL_AUTO or L.FUSED_LINEAR or L.LORA_FIRST:
@@ -534,6 +585,9 @@ class BackboneRunner:
             cu = torch.tensor([0] + list(torch.tensor(lens).cumsum(0)), dtype=torch.int32, device=self.dev)
             embeds = torch.randn(T, self.model.cfg.hidden_size, device=self.dev, generator=gen).to(self.dtype)
             step = AttentionStep(True, self._cache_positions(req, pos), cu_seqlens=cu, max_seqlen=max(lens))
+            if self.model.cfg.paged_attention:
+                step.prefill_context_lens = cu[1:] - cu[:-1]
+                step.prefill_block_tables = self.block_tables[reqs[0]:reqs[-1] + 1]
             tts = torch.repeat_interleave(self.slots[torch.tensor(reqs)], torch.tensor(lens))
             ctx = None
             if self.use_lora:
@@ -636,6 +690,12 @@ def time_mixed_step(model: Decoder, n_decode: int, prefill_lens: list[int], slot
     step = AttentionStep(True, slot_mapping, cu_seqlens=cu, max_seqlen=max(prefill_lens),
                          context_lens=torch.full((n_decode,), context_len + 1, dtype=torch.int32, device=dev),
                          block_tables=block_tables, n_decode=n_decode)
+    if cfg.paged_attention:
+        tables, first = torch.full((len(prefill_lens), max(blocks_prefill)), -1, dtype=torch.int32), n_decode * per_decode
+        for i, nb in enumerate(blocks_prefill):
+            tables[i, :nb] = torch.arange(first, first + nb)
+            first += nb
+        step.prefill_context_lens, step.prefill_block_tables = cu[1:] - cu[:-1], tables.to(dev)
     gen = torch.Generator(device=dev).manual_seed(seed)
     embeds = torch.randn(n_decode + T_pre, cfg.hidden_size, device=dev, generator=gen).to(dtype)
     tts = torch.cat([torch.tensor(slots_decode, dtype=torch.int32),

@@ -111,3 +111,12 @@ def test_oracle_agrees_with_masked_softmax():
         torch.testing.assert_close(lse[row:row + n], s.logsumexp(-1).T)
         assert count[row:row + n].tolist() == [int(x) for x in (s[0] > float("-inf")).sum(-1)]
         row += n
+
+
+def test_decoder_config_refuses_what_attention_does():
+    from nanovllm_voxcpm_b200.backbone import DecoderConfig
+
+    assert DecoderConfig(sliding_window=64, sink_tokens=2).paged_attention and not DecoderConfig().paged_attention
+    for kw in (dict(sliding_window=-1), dict(sink_tokens=-1, sliding_window=4), dict(sink_tokens=2)):
+        with pytest.raises(ValueError):
+            DecoderConfig(**kw)
