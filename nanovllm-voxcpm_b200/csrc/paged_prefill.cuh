@@ -91,6 +91,20 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+// 2^x for x <= 8 or so on the FMA units: x = n + f with n whole and f in [-0.5, 0.5] (adding and subtracting 1.5 * 2^23 rounds to n), 2^f
+// by a polynomial with constant term 1, least in its largest relative error (1.7e-7 in fp32; weighted least squares until the
+// extrema are even), n added to the exponent. From -127 down exactly 0.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  constexpr float kRound = 12582912.f;
+  x = make_float2(fmaxf(x.x, -127.f), fmaxf(x.y, -127.f));
+  const float2 t = add2(x, make_float2(kRound, kRound)), f = fma2(add2(t, make_float2(-kRound, -kRound)), make_float2(-1.f, -1.f), x);
+  float2 y = fma2(f, make_float2(0x1.5bba14p-10f, 0x1.5bba14p-10f), make_float2(0x1.3cea88p-7f, 0x1.3cea88p-7f));
+  y = fma2(f, y, make_float2(0x1.c6b752p-5f, 0x1.c6b752p-5f));
+  y = fma2(f, y, make_float2(0x1.ebf9bcp-3f, 0x1.ebf9bcp-3f));
+  y = fma2(f, y, make_float2(0x1.62e42ap-1f, 0x1.62e42ap-1f));
+  y = fma2(f, y, make_float2(1.f, 1.f));
+  return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23)), __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23)));
+}
 // bits [0, n) of a word, n of any sign and size
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
 
@@ -200,9 +214,13 @@ template <int D, bool kF16, int kTiles, bool kSplit>
 __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_kernel(const __grid_constant__ PpMaps maps, const __grid_constant__ PpArgs a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   constexpr int kSt = pp_stages<D>(kTiles), kTile = pp_tile<D>(), kPanels = D / 64;
+  // Where the columns allow it P has its own, and S of the next tile is made while this one's softmax runs; the softmax is then all
+  // there is to wait for, and an eighth of the exponentials on the FMA units pays. (8192 tokens, 16 / 2 heads of 64: 208 us with P in
+  // S, 198 with columns of its own, 190 with an eighth, 197 with a quarter, 233 with half; heads of 128 gain from neither.)
+  constexpr bool kOwnP = kTiles == 1 && D == 64;
   constexpr int kLoader = 4 * kTiles, kIssuer = kLoader + 1, kTmem = 256 * kTiles, kO = kTiles * kPpKeys;  // warps; columns: all, the first of O
   enum { Q_FULL, Q_FREE, S_READY, P_READY = S_READY + 2, O_DONE = P_READY + 4, K_FULL = O_DONE + 2, K_FREE = K_FULL + kSt, V_FULL = K_FREE + kSt,
-         V_FREE = V_FULL + kSt, PIECE = V_FREE + kSt, TAKEN = PIECE + 2, N_BARS = TAKEN + 2 };
+         V_FREE = V_FULL + kSt, PIECE = V_FREE + kSt, TAKEN = PIECE + 2, S_TAKEN = TAKEN + 2, PV_DONE, N_BARS };
   __shared__ __align__(8) uint64_t bars[N_BARS];
   __shared__ uint32_t s_tmem, s_boxes[4];
   __shared__ PpPiece s_piece[2];
@@ -214,7 +232,7 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
 
   if (tid == 0) {
-    for (int i = 0; i < N_BARS; ++i) mbar_init(bar(i), i >= P_READY && i < O_DONE ? kPpRows : i >= TAKEN ? 4 * kTiles + 1 : 1);
+    for (int i = 0; i < N_BARS; ++i) mbar_init(bar(i), (i >= P_READY && i < O_DONE) || i == S_TAKEN ? kPpRows : i == TAKEN || i == TAKEN + 1 ? 4 * kTiles + 1 : 1);
     abort_flag = 0;
     mbar_fence_init();
   }
@@ -238,7 +256,7 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPpSoftmaxRegs));
     const int t = warp >> 2, row = (warp & 3) * 32 + lane, tok = t * per_tile + (row >> a.h_shift);
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + t * kPpKeys + lanes, o_at = tmem + kO + t * D + lanes;
+    const uint32_t s_at = tmem + t * kPpKeys + lanes, o_at = tmem + kO + t * D + lanes, p_at = kOwnP ? tmem + kO + D + lanes : s_at;
     const uint32_t all_boxes = bits_below(kPpKeys / a.box);
     const int box_shift = 31 - __clz(a.box);
     const uint32_t stage = out_u32 + warp * (32 * kPpOutPitch);  // 32 columns of the warp's rows on their way out
@@ -284,15 +302,23 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
             for (int j = 0; j < 32; j += 2) top4[j / 2 % 4] = max3(top4[j / 2 % 4], __uint_as_float(s[c][j]), __uint_as_float(s[c][j + 1]));
           }
         }
+        if (kOwnP) {
+          tc_fence_before_sync();
+          mbar_arrive(bar(S_TAKEN));
+        }
         const float mx = max3(max3(top4[0], top4[1], top4[2]), top4[3], top4[3]);
         // The maximum moves only where it would grow by more than 2^8: until then probabilities stay below that, and O as it is.
         const float top = mx * p.sc;
         const bool grows = !(top <= m + 8.f);  // (a NaN among the scores makes the maximum and with it the whole row NaN)
+        if (kOwnP && n > 0) {  // P and O of the tile before are done with
+          pp_wait(bar(PV_DONE), (n - 1) & 1, &abort_flag);
+          tc_fence_after_sync();
+        }
         if (__any_sync(0xffffffffu, grows)) {
           const float f = grows ? ex2(m - top) : 1.f;
           if (grows) m = top;
           l *= f;
-          if (i > w.i0) {  // (S of this tile came behind P V of the one before: O is complete)
+          if (i > w.i0) {  // (if P lies in S: S of this tile came behind P V of the one before, O is complete)
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) {
               uint32_t o[16];
@@ -313,11 +339,11 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
             const float2 x = fma2(make_float2(__uint_as_float(s[c][j]), __uint_as_float(s[c][j + 1])), scale2, base2);
-            const float2 y = make_float2(ex2(x.x), ex2(x.y));
+            const float2 y = kOwnP && j % 16 == 14 ? exp2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
             sum[j / 2 % 2] = add2(sum[j / 2 % 2], y);
             packed[j / 2] = pack_16x2<kF16>(y.x, y.y);  // (rounded to the type of V; the sum is that of the unrounded ones)
           }
-          tmem_st_32x16(s_at + 16 * c, packed);
+          tmem_st_32x16(p_at + 16 * c, packed);
           if (c & 1) {  // half of P: its products may begin
             tmem_st_wait();
             tc_fence_before_sync();
@@ -330,7 +356,8 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // (no visible key: zeros; NaN stays)
       const int64_t token0 = (int64_t)w.begin + w.q0;
       if (any) {
-        pp_wait(bar(O_DONE + t), pieces & 1, &abort_flag);
+        if (kOwnP) pp_wait(bar(PV_DONE), (n - 1) & 1, &abort_flag);
+        else pp_wait(bar(O_DONE + t), pieces & 1, &abort_flag);
         ++pieces;
         tc_fence_after_sync();
       }
@@ -343,16 +370,20 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
           const int of = (warp & 3) * 32 + 8 * r + (lane >> 2), its = t * per_tile + (of >> a.h_shift);
           dst[r] = its < w.n_here ? static_cast<char*>(p.out) + 2 * ((token0 + its) * p.out_token + (w.head0 + (of & ((1 << a.h_shift) - 1))) * p.out_head) + 16 * (lane & 3) : nullptr;
         }
+        uint32_t all[D / 32][32];
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
           if (any) {
-            tmem_ld_32x32(o_at + 32 * c, o);
-            tmem_ld_wait();
+            tmem_ld_32x32(o_at + 32 * c, all[c]);
           } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = 0;
+            for (int j = 0; j < 32; ++j) all[c][j] = 0;
           }
+        }
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          const uint32_t(&o)[32] = all[c];
 #pragma unroll
           for (int j = 0; j < 32; j += 8) {
             uint4 v;
@@ -492,12 +523,24 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
         pp_wait(bar(Q_FULL), pieces & 1, &abort_flag);
         ++pieces;
         pp_wait(bar(K_FULL + n % kSt), (n / kSt) & 1, &abort_flag);
+        if (kOwnP && n > 0) {
+          pp_wait(bar(S_TAKEN), (n - 1) & 1, &abort_flag);
+          tc_fence_after_sync();
+        }
         for (int t = 0; t < kTiles; ++t) scores(t, n % kSt);
         umma_commit_elected(bar(K_FREE + n % kSt), leader);
         if (w.i1 == w.i0 + 1) umma_commit_elected(bar(Q_FREE), leader);
         for (int i = w.i0; i < w.i1; ++i, ++n) {
           const int st = n % kSt, next = (n + 1) % kSt;
           const bool more = i + 1 < w.i1;
+          if (kOwnP && more) {
+            pp_wait(bar(K_FULL + next), ((n + 1) / kSt) & 1, &abort_flag);
+            pp_wait(bar(S_TAKEN), n & 1, &abort_flag);
+            tc_fence_after_sync();
+            scores(0, next);
+            umma_commit_elected(bar(K_FREE + next), leader);
+            if (i + 2 == w.i1) umma_commit_elected(bar(Q_FREE), leader);
+          }
           pp_wait(bar(V_FULL + st), (n / kSt) & 1, &abort_flag);
           // Rows of V that no token of this CTA sees may hold anything (a block's stale rows): they become zero, as 0 * V must.
           const int key0 = w.key0(i);
@@ -517,10 +560,12 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
                 pp_wait(bar(P_READY + 2 * t + k / 4), n & 1, &abort_flag);
                 tc_fence_after_sync();
               }
-              umma_ts_elected(tmem + kO + t * D, tmem + t * kPpKeys + 8 * k, lo_v(v_u32 + st * kTile + k * 2048), hi_k, idesc_o,
+              umma_ts_elected(tmem + kO + t * D, tmem + (kOwnP ? kO + D : t * kPpKeys) + 8 * k, lo_v(v_u32 + st * kTile + k * 2048), hi_k, idesc_o,
                               i > w.i0 || k > 0, leader);
             }
-            if (more) {
+            if (kOwnP) {
+              umma_commit_elected(bar(PV_DONE), leader);
+            } else if (more) {
               // (behind P V of this tile in the same thread: P has been read when S is written over it)
               if (t == 0) pp_wait(bar(K_FULL + next), ((n + 1) / kSt) & 1, &abort_flag);
               scores(t, next);
@@ -529,8 +574,8 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
             }
           }
           umma_commit_elected(bar(V_FREE + st), leader);
-          if (more) umma_commit_elected(bar(K_FREE + next), leader);
-          if (i + 2 == w.i1) umma_commit_elected(bar(Q_FREE), leader);
+          if (!kOwnP && more) umma_commit_elected(bar(K_FREE + next), leader);
+          if (!kOwnP && i + 2 == w.i1) umma_commit_elected(bar(Q_FREE), leader);
         }
       }
       // the last commits must have arrived before this CTA's shared memory is given up

@@ -63,9 +63,11 @@ def paged_attention(q, k_cache, v_cache, tables, context_lens, cu_seqlens, scale
             p = torch.exp(s - torch.where(total == -math.inf, torch.zeros_like(total), total)[:, None])
             # (a key that a row does not see has no part in it, whatever its value)
             vv = v[:, h // group]
-            for i in range(len(rows)):
-                mine = ~hidden[i]
-                out[rows[i], h] = p[i, mine] @ vv[mine]
-                size[rows[i], h] = p[i, mine] @ vv[mine].abs()
+            if vv.isfinite().all():
+                out[rows.start:rows.stop, h], size[rows.start:rows.stop, h] = p @ vv, p @ vv.abs()
+            else:
+                for i in range(len(rows)):
+                    mine = ~hidden[i]
+                    out[rows[i], h], size[rows[i], h] = p[i, mine] @ vv[mine], p[i, mine] @ vv[mine].abs()
             lse[rows.start:rows.stop, h] = total
     return out, lse, size, count
