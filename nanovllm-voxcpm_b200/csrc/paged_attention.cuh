@@ -57,16 +57,15 @@ __device__ __forceinline__ RowKeys row_keys(const PagedArgs& a, int row) {
   return r;
 }
 
-constexpr int kPagedWarps = 4;
-constexpr int kPagedThreads = 32 * kPagedWarps;
+constexpr int kJoinThreads = 128;
 constexpr int kPagedStages = 3;
-constexpr int kPagedCtas = 2 * 148;  // of a launch: two on every SM
+constexpr int kPagedCtas = 2 * 148;  // of a launch, of four warps: two on every SM
 template <int D>
 __host__ __device__ constexpr int paged_block_keys() { return D == 64 ? 32 : 16; }  // 8 KB of K and V rows
 template <int D>
 __host__ __device__ constexpr int paged_stage_bytes() { return 2 * paged_block_keys<D>() * (D * 2 + 16); }
 template <int D, int NT>
-__host__ __device__ constexpr int paged_smem() { return 2 * 8 * NT * (D * 2 + 16) + kPagedWarps * kPagedStages * paged_stage_bytes<D>(); }
+__host__ __device__ constexpr int paged_smem(int warps) { return 2 * 8 * NT * (D * 2 + 16) + warps * kPagedStages * paged_stage_bytes<D>(); }
 
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
   uint32_t r;
@@ -141,16 +140,17 @@ struct PagedWalk {
   }
 };
 
-// The warps of a CTA take the blocks of an item in turn, each through a ring of its own; the keys are the rows of the matrix
+// Four warps (two CTAs on an SM) or eight take the blocks of an item in turn, each through a ring of its own; the keys are the rows of the matrix
 // instruction (S^T = K Q^T, then O^T = V^T P^T), so that eight heads fill it. What the next piece needs first (its lengths, table
 // entries, queries, two blocks) is asked for ahead of the end of this one.
 // kWay: whose the items are
 constexpr int kWhole = 0, kShares = 1, kClusters = 2;  // one CTA's each; of a share of all blocks; a cluster's each, joined in its shared memory
 
-template <int D, int NT, bool kF16, int kWay>
-__global__ void __launch_bounds__(kPagedThreads, 2) paged_decode_kernel(const PagedArgs a) {
+template <int D, int NT, bool kF16, int kWay, int kPagedWarps>
+__global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decode_kernel(const PagedArgs a) {
   extern __shared__ __align__(16) uint8_t paged_smem_raw[];  // (a name of its own: 1024-byte alignment would cost heads of 64 the second CTA)
   uint8_t* const smem = paged_smem_raw;
+  constexpr int kPagedThreads = 32 * kPagedWarps;
   constexpr int kPitch = D * 2 + 16, kKeys = paged_block_keys<D>(), kStage = paged_stage_bytes<D>(), kPieces = D / 8;
   constexpr int kMT = kKeys / 16, kPerLoad = 32 / kPieces;  // rows of a load instruction
   constexpr int kQ = 8 * NT * kPitch, kQEach = (8 * NT * kPieces + kPagedThreads - 1) / kPagedThreads;
@@ -499,8 +499,8 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_decode_kernel(const Pa
 // Joins the parts of the item that begins in CTA blockIdx.x: its own, then the first one of every CTA up to the last; one of its
 // heads (blockIdx.y). D / 4 threads keep four columns each; groups of them take the parts in turn.
 template <int D, bool kF16>
-__global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const PagedArgs a) {
-  constexpr int kLanes = D / 4, kGroups = kPagedThreads / kLanes;
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArgs a) {
+  constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes;
   __shared__ float4 s_o[kGroups][kLanes];
   __shared__ float2 s_ml[kGroups];
   glue_enter();
@@ -542,15 +542,15 @@ inline size_t paged_workspace_bytes(int Hq, int Hk, int D) {
   return paged_parts_bytes(heads, D) + (size_t)2 * kPagedCtas * heads * 8 + kPagedCtas * sizeof(int4);
 }
 
-template <int D, int NT, bool kF16, int kWay>
+template <int D, int NT, bool kF16, int kWay, int kWarps>
 inline int paged_decode_launch_t(const PagedArgs& a, int ctas, int cluster, cudaStream_t stream) {
-  const auto kernel = paged_decode_kernel<D, NT, kF16, kWay>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, paged_smem<D, NT>());
+  const auto kernel = paged_decode_kernel<D, NT, kF16, kWay, kWarps>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, paged_smem<D, NT>(kWarps));
   if (e != cudaSuccess) return fail(B200_LORA_ECUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(kPagedThreads);
-  cfg.dynamicSmemBytes = paged_smem<D, NT>();
+  cfg.blockDim = dim3(32 * kWarps);
+  cfg.dynamicSmemBytes = paged_smem<D, NT>(kWarps);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -566,28 +566,31 @@ inline int paged_decode_launch_t(const PagedArgs& a, int ctas, int cluster, cuda
     return fail(B200_LORA_ECUDA, "paged_decode_kernel launch: %s", cudaGetErrorString(e));
   }
   if (kWay != kShares) return B200_LORA_OK;
-  return launch_dependent(paged_join_kernel<D, kF16>, "paged_join_kernel", dim3((unsigned)ctas, (unsigned)a.heads), kPagedThreads, 0, stream, a);
+  return launch_dependent(paged_join_kernel<D, kF16>, "paged_join_kernel", dim3((unsigned)ctas, (unsigned)a.heads), kJoinThreads, 0, stream, a);
 }
 
 // How the items (row, kv head, chunk) meet the CTAs, by what the host knows: their number, and the blocks of keys of one at most
-// (the table's width, the window). us, one CTA an item / clusters of 2, 4, 8 / equal shares:
-//   16 / 2 heads of 64: one request of 700 tokens (2 items, 22 blocks) 8.0 / 7.7, 6.7, 6.1 / 10.9; of 8000 48 / 28, 18, 12.4 / 15.9;
-//   of 32000 208 / 110, 62, 34 / 21; 64 of 1000 (128 items, 32 blocks) 11.9 / 12.7, 17, 34 / 16.7; 64 of 8000 64 / 51, 53, 81 / 53
-//   16 / 2 of 128: 16 of 4000 (32, 250) 56 / 34, 22, 18.7 / 23; 64 of 2000 (128, 125) 33 / 30, 33, 58 / 34; 128 of a window of 1024
-//   (256, 65) 28 / 35, 56, 95 / 35; 32 / 8 of 128: 8 of 300 (64, 19) 7.8 / 8.5, 8.5, 12.9 / 13.1; 8 of 2000 30 / 21, 18.3, 23 / 22;
-//   ragged, 48 of 500 to 8192 (384, 512) 204 / 171, 187, 258 / 140; 16 of 100 to 16000 (128, 1000) 208 / 134, 142, 137 / 110
+// (the table's width, the window). us, one CTA of four warps an item / of eight / clusters of 2, 4, 8 of eight / equal shares of four:
+//   16 / 2 heads of 64: one request of 700 tokens (2 items, 22 blocks) 8.2 / 7.1 / 7.4, 6.6, 6.3 / 10.9; of 8000 48 / 33 / 22, 15, 10.9 /
+//   15.9; of 32000 210 / 125 / 69, 39, 23.4 / 21.4; 64 of 1000 (128 items, 32 blocks) 11.9 / 10.0 / 16.5, 35, 66 / 16.7; 64 of 8000 64 / 48 /
+//   53, 84, 128 / 52; 32 / 8 of 128: 8 of 300 (64, 19) 7.9 / 7.4 / 8.4, 12.5, 30 / 13.1; 8 of 2000 30 / 22 / 18.9, 24, 42 / 22;
+//   16 / 2 of 128: 128 of 1000 (256, 63) 27.2 / 29.2 / 42, 97, 158 / 34
+//   ragged, 48 of 500 to 8192 (384, 512) 203 / 179 / 166, 273, 368 / 138; 16 of 100 to 16000 (128, 1000) 208 / 138 / 147, 146, 210 / 109
 template <int D, int NT, bool kF16>
 inline int paged_decode_launch_by(const PagedArgs& a, cudaStream_t stream) {
   int64_t keys = (int64_t)a.table_width * a.cache.block_size;
   if (a.window > 0) keys = std::min<int64_t>(keys, (int64_t)a.window + a.sinks);
   const int64_t units = (keys + paged_block_keys<D>() - 1) / paged_block_keys<D>(), items = (int64_t)a.T * a.Hk * a.chunks;
-  int cluster = 1;
-  while (cluster < 8 && ((2 * items * cluster <= 148 && units >= 4 * cluster) || (2 * items * cluster <= kPagedCtas && units >= 48 * cluster))) cluster *= 2;
-  if ((units > 128 * cluster && items < 8 * kPagedCtas) || (cluster == 8 && 16 * items <= kPagedCtas && units > 400))
-    return paged_decode_launch_t<D, NT, kF16, kShares>(a, kPagedCtas, 1, stream);
-  const int ctas = (int)std::min<int64_t>(kPagedCtas / cluster, items) * cluster;
-  if (cluster == 1) return paged_decode_launch_t<D, NT, kF16, kWhole>(a, ctas, 1, stream);
-  return paged_decode_launch_t<D, NT, kF16, kClusters>(a, ctas, cluster, stream);
+  int cluster = 8;
+  while (cluster > 1 && items * cluster > 148) cluster /= 2;
+  if (units < (cluster == 2 ? 64 : 20)) cluster = 1;
+  const int warps = items * cluster <= 148 ? 8 : 4;
+  if ((units > 32 * warps * cluster && items < 8 * kPagedCtas) || (cluster == 8 && units > 700))
+    return paged_decode_launch_t<D, NT, kF16, kShares, 4>(a, kPagedCtas, 1, stream);
+  const int ctas = (int)std::min<int64_t>((warps == 8 ? 148 : kPagedCtas) / cluster, items) * cluster;
+  if (cluster > 1) return paged_decode_launch_t<D, NT, kF16, kClusters, 8>(a, ctas, cluster, stream);
+  if (warps == 8) return paged_decode_launch_t<D, NT, kF16, kWhole, 8>(a, ctas, 1, stream);
+  return paged_decode_launch_t<D, NT, kF16, kWhole, 4>(a, ctas, 1, stream);
 }
 
 inline int paged_decode_launch(PagedArgs a, int D, int dtype, void* workspace, cudaStream_t stream) {
