@@ -16,6 +16,7 @@
 namespace b200lora {
 
 constexpr int kPpRows = 128, kPpKeys = 128;       // of a tile
+constexpr int kPpWindowBox = 32;
 constexpr int kPpOutPitch = 80;      // bytes of 32 columns of a row in shared memory, and 16 to spread the banks
 constexpr int kPpPanel = kPpKeys * 128;           // bytes of 128 rows of 64 columns
 // One softmax warpgroup per tile; one more with the loading warp and the MMA warp, which leaves its registers to them. Two tiles: 168
@@ -43,7 +44,7 @@ struct PpArgs {
   PagedArgs p;
   int h_shift, head_tiles;   // heads of a tile = 1 << h_shift; tiles over all heads
   int n_blocks;              // blocks of tokens that the launch has CTAs for
-  int box;                   // cache rows of a copy: 8 .. 128, a power of two that divides the block size
+  int box, box_shift;        // cache rows of a copy: 8 .. 128, a power of two that divides the block size; its logarithm
   float* parts; void* joins;  // split: partial results and what there is to join
   int k_heads_inner, v_heads_inner;  // order of the map's middle dimensions: (head, position) or (position, head)
 };
@@ -112,9 +113,13 @@ __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n 
 struct PpPiece {
   int head0, begin, q0, n_here;                // first head; first row of the sequence; first token and tokens of the block
   int req, pos0, held, key_end, lo_first, sink_end;  // position of the first token; keys that a row sees: [0, sink_end), [lo_first, key_end)
-  int first_tile, sink_tiles, i0, i1;
+  int first_box, sink_boxes, i0, i1;           // the keys in boxes: those of the first tokens, then from first_box on, side by side
   int parts;                                   // 0: no more pieces; 1: the whole item; else the item is in that many parts
-  __device__ __forceinline__ int key0(int i) const { return (i < sink_tiles ? i : i - sink_tiles + first_tile) * kPpKeys; }
+  // first key of box b of tile i, with 1 << shift keys in a box
+  __device__ __forceinline__ int key_of(int i, int b, int shift) const {
+    const int c = i * (kPpKeys >> shift) + b;
+    return (c < sink_boxes ? c : c - sink_boxes + first_box) << shift;
+  }
 };
 
 // New rows of request i, and its first one; a range that leaves the rows of q counts as none
@@ -196,10 +201,11 @@ __device__ __forceinline__ void pp_find(const PpArgs& a, int span, int item, int
   w->key_end = w->held;
   w->lo_first = p.window > 0 ? max(0, max(w->pos0, 0) - (p.window - 1)) : 0;
   w->sink_end = max(0, min(min(p.sinks, w->lo_first), w->key_end));
-  w->first_tile = w->lo_first / kPpKeys;
-  w->sink_tiles = min((w->sink_end + kPpKeys - 1) / kPpKeys, w->first_tile);
+  w->first_box = w->lo_first >> a.box_shift;
+  w->sink_boxes = min((w->sink_end + a.box - 1) >> a.box_shift, w->first_box);
   w->i0 = 0;
-  w->i1 = w->key_end <= 0 ? 0 : w->sink_tiles + max(0, (w->key_end + kPpKeys - 1) / kPpKeys - w->first_tile);
+  const int boxes = w->key_end <= 0 ? 0 : w->sink_boxes + max(0, ((w->key_end + a.box - 1) >> a.box_shift) - w->first_box);
+  w->i1 = (boxes + (kPpKeys >> a.box_shift) - 1) / (kPpKeys >> a.box_shift);
   w->parts = 1;
 }
 
@@ -258,7 +264,7 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + t * kPpKeys + lanes, o_at = tmem + kO + t * D + lanes, p_at = kOwnP ? tmem + kO + D + lanes : s_at;
     const uint32_t all_boxes = bits_below(kPpKeys / a.box);
-    const int box_shift = 31 - __clz(a.box);
+    const int tile_shift = 7 - a.box_shift;  // boxes of a tile, as a logarithm
     const uint32_t stage = out_u32 + warp * (32 * kPpOutPitch);  // 32 columns of the warp's rows on their way out
     uint32_t n = 0, pieces = 0;  // tiles and pieces with tiles so far: phases of the barriers
     PpPiece w;
@@ -266,16 +272,19 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
       const int pos = w.pos0 + tok;
       const int lo = p.window > 0 ? max(pos, 0) - (p.window - 1) : 0;
       const int tile_lo = w.pos0 + t * per_tile, tile_hi = tile_lo + per_tile - 1;  // positions of the tile
+      // tiles [clear0, clear1) need no mask: behind the first tokens, from where every row's window has begun, up to the first row
+      const int w_lo = p.window > 0 ? max(tile_hi, 0) - (p.window - 1) : 0;
+      const int clear0 = (w.sink_boxes + max(0, ((max(w_lo, 0) + a.box - 1) >> a.box_shift) - w.first_box) + (1 << tile_shift) - 1) >> tile_shift;
+      const int clear1 = (((tile_lo + 1) >> a.box_shift) + w.sink_boxes - w.first_box) >> tile_shift;
       float m = -INFINITY, l = 0.f;  // maximum that the probabilities refer to, in units of log2; their sum
       for (int i = w.i0; i < w.i1; ++i, ++n) {
-        const int key0 = w.key0(i);
         pp_wait(bar(S_READY + t), n & 1, &abort_flag);
         tc_fence_after_sync();
         uint32_t s[4][32];
 #pragma unroll
         for (int c = 0; c < 2; ++c) tmem_ld_32x32(s_at + 32 * c, s[c]);
         const uint32_t boxes = s_boxes[n & 3];
-        const bool masked = key0 + kPpKeys - 1 > tile_lo || (p.window > 0 && key0 < max(tile_hi, 0) - (p.window - 1) && key0 + kPpKeys > p.sinks) || boxes != all_boxes;
+        const bool masked = i < clear0 || i >= clear1 || boxes != all_boxes;
         float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -287,12 +296,15 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
 #pragma unroll
           for (int c = 2 * half; c < 2 * half + 2; ++c) {
             if (masked) {
-              const int at = key0 + 32 * c;
-              uint32_t seen = bits_below(pos + 1 - at) & (~bits_below(lo - at) | bits_below(p.sinks - at));
-              uint32_t there = 0;  // (a copy has 8 rows or more)
-#pragma unroll
-              for (int g = 0; g < 4; ++g) there |= (boxes >> ((32 * c + 8 * g) >> box_shift)) & 1u ? 0xffu << (8 * g) : 0u;
-              seen &= there;
+              auto seen_from = [&](int at) { return bits_below(pos + 1 - at) & (~bits_below(lo - at) | bits_below(p.sinks - at)); };
+              auto key_at = [&](int col) { return w.key_of(i, col >> a.box_shift, a.box_shift) + (col & (a.box - 1)); };
+              uint32_t seen = seen_from(key_at(32 * c));
+              if (boxes != all_boxes || key_at(32 * c + 31) != key_at(32 * c) + 31) {
+                seen = 0;
+#pragma unroll 1
+                for (int g = 0; g < 32; g += 8)  // (a box has 8 keys or more)
+                  if ((boxes >> ((32 * c + g) >> a.box_shift)) & 1u) seen |= (seen_from(key_at(32 * c + g)) & 0xffu) << g;
+              }
               asm volatile("" : "+r"(seen));  // (one word at a time: 128 tests at once cost 350 bytes of spills)
 #pragma unroll
               for (int j = 0; j < 32; ++j)
@@ -463,7 +475,7 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
         const int kvh = w.head0 / (p.Hq / p.Hk);
         const int32_t* table = p.tables + w.req * p.table_ld;
         for (int i = w.i0; i < w.i1; ++i, ++n) {
-          const int st = n % kSt, key = w.key0(i) + lane * a.box;
+          const int st = n % kSt, key = w.key_of(i, lane, a.box_shift);
           int block = -1, in_block = 0;
           if (lane < n_boxes && key < w.held) {
             const int page = key / p.cache.block_size;
@@ -543,10 +555,10 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
           }
           pp_wait(bar(V_FULL + st), (n / kSt) & 1, &abort_flag);
           // Rows of V that no token of this CTA sees may hold anything (a block's stale rows): they become zero, as 0 * V must.
-          const int key0 = w.key0(i);
-          if (!(key0 + kPpKeys <= w.sink_end || (key0 >= w.lo_first && key0 + kPpKeys <= w.key_end))) {
+          const int first_key = w.key_of(i, 0, a.box_shift), last_key = w.key_of(i, (kPpKeys >> a.box_shift) - 1, a.box_shift) + a.box - 1;
+          if (!(last_key < w.sink_end || (first_key >= w.lo_first && last_key < w.key_end))) {
             for (int x = lane; x < kPpKeys * kPanels * 8; x += 32) {
-              const int row = x / (kPanels * 8), key = key0 + row, c = x % (kPanels * 8);
+              const int row = x / (kPanels * 8), key = w.key_of(i, row >> a.box_shift, a.box_shift) + (row & (a.box - 1)), c = x % (kPanels * 8);
               if (!(key < w.sink_end || (key >= w.lo_first && key < w.key_end)))
                 sts128(v_u32 + st * kTile + (c >> 3) * kPpPanel + row * 128 + (c & 7) * 16, make_uint4(0, 0, 0, 0));
             }
@@ -673,7 +685,10 @@ inline bool paged_prefill_plan(const PagedArgs& p, int D, bool f16, int tiles, P
   if (p.cache.block_size % 8 != 0) return false;
   a->p = p;
   a->box = 8;
-  while (a->box < kPpKeys && p.cache.block_size % (2 * a->box) == 0) a->box *= 2;
+  // (a window's keys begin anywhere: short boxes leave little of the tiles ahead of it, and first tokens share a tile with it)
+  while (a->box < (p.window > 0 ? kPpWindowBox : kPpKeys) && p.cache.block_size % (2 * a->box) == 0) a->box *= 2;
+  a->box_shift = 0;
+  while ((1 << a->box_shift) < a->box) ++a->box_shift;
   a->h_shift = pp_h_shift(p.Hq / p.Hk);
   a->head_tiles = p.Hq >> a->h_shift;
   const int per_tile = kPpRows >> a->h_shift;
