@@ -16,7 +16,7 @@
 namespace b200lora {
 
 constexpr int kPpRows = 128, kPpKeys = 128;       // of a tile
-constexpr int kPpWindowBox = 32;
+constexpr int kPpSinkBox = 32;
 constexpr int kPpOutPitch = 80;      // bytes of 32 columns of a row in shared memory, and 16 to spread the banks
 constexpr int kPpPanel = kPpKeys * 128;           // bytes of 128 rows of 64 columns
 // One softmax warpgroup per tile; one more with the loading warp and the MMA warp, which leaves its registers to them. Two tiles: 168
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + t * kPpKeys + lanes, o_at = tmem + kO + t * D + lanes, p_at = kOwnP ? tmem + kO + D + lanes : s_at;
     const uint32_t all_boxes = bits_below(kPpKeys / a.box);
-    const int tile_shift = 7 - a.box_shift;  // boxes of a tile, as a logarithm
+    const int tile_shift = 7 - a.box_shift, step = min(a.box, 32);  // boxes of a tile, as a logarithm; columns of 32 that lie in one box
     const uint32_t stage = out_u32 + warp * (32 * kPpOutPitch);  // 32 columns of the warp's rows on their way out
     uint32_t n = 0, pieces = 0;  // tiles and pieces with tiles so far: phases of the barriers
     PpPiece w;
@@ -296,14 +296,12 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
 #pragma unroll
           for (int c = 2 * half; c < 2 * half + 2; ++c) {
             if (masked) {
-              auto seen_from = [&](int at) { return bits_below(pos + 1 - at) & (~bits_below(lo - at) | bits_below(p.sinks - at)); };
-              auto key_at = [&](int col) { return w.key_of(i, col >> a.box_shift, a.box_shift) + (col & (a.box - 1)); };
-              uint32_t seen = seen_from(key_at(32 * c));
-              if (boxes != all_boxes || key_at(32 * c + 31) != key_at(32 * c) + 31) {
-                seen = 0;
+              uint32_t seen = 0;
 #pragma unroll 1
-                for (int g = 0; g < 32; g += 8)  // (a box has 8 keys or more)
-                  if ((boxes >> ((32 * c + g) >> a.box_shift)) & 1u) seen |= (seen_from(key_at(32 * c + g)) & 0xffu) << g;
+              for (int g = 0; g < 32; g += step) {
+                const int col = 32 * c + g, b = col >> a.box_shift, at = w.key_of(i, b, a.box_shift) + (col & (a.box - 1));
+                const uint32_t bits = bits_below(pos + 1 - at) & (~bits_below(lo - at) | bits_below(p.sinks - at));
+                if ((boxes >> b) & 1u) seen |= (bits & bits_below(step)) << g;
               }
               asm volatile("" : "+r"(seen));  // (one word at a time: 128 tests at once cost 350 bytes of spills)
 #pragma unroll
@@ -685,8 +683,9 @@ inline bool paged_prefill_plan(const PagedArgs& p, int D, bool f16, int tiles, P
   if (p.cache.block_size % 8 != 0) return false;
   a->p = p;
   a->box = 8;
-  // (a window's keys begin anywhere: short boxes leave little of the tiles ahead of it, and first tokens share a tile with it)
-  while (a->box < (p.window > 0 ? kPpWindowBox : kPpKeys) && p.cache.block_size % (2 * a->box) == 0) a->box *= 2;
+  // Short boxes where first tokens stay visible: they share a tile with the window's begin (8001 tokens, window of 1024 and 4 first
+  // ones: 95 -> 89 us; without first ones whole tiles have the faster masks: window of 512 62 us, in short boxes 66).
+  while (a->box < (p.sinks > 0 ? kPpSinkBox : kPpKeys) && p.cache.block_size % (2 * a->box) == 0) a->box *= 2;
   a->box_shift = 0;
   while ((1 << a->box_shift) < a->box) ++a->box_shift;
   a->h_shift = pp_h_shift(p.Hq / p.Hk);
