@@ -1,8 +1,9 @@
 """Attention over the paged key-value cache that ``glue.rope_kv_store`` and ``glue.qk_norm_rope_kv_store`` fill: the next token
 of every request (``paged_decode_attention``) or packed runs of new tokens (``paged_prefill_attention``: whole prompts, chunks of
 them, a few tokens behind a long context). Causal, over everything or over a sliding window of the last keys plus a few first
-ones. Stands where the reference calls ``flash_attn_with_kvcache`` and ``flash_attn_varlen_func``
-(``nanovllm_voxcpm/layers/attention.py:70-79``); the kernels are ``csrc/paged_attention.cuh`` behind ``lora_b200_paged_*``.
+ones. Stands where the reference attends over its paged cache
+(``nanovllm_voxcpm/layers/attention.py:70-79``); the kernels are ``csrc/paged_attention.cuh`` and ``csrc/paged_prefill.cuh`` behind
+``lora_b200_paged_*``.
 CUDA tensors only, bf16 / fp16, heads of 64 or 128; there is no fallback path and no backward pass.
 """
 
@@ -102,5 +103,8 @@ def paged_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     """Packed new tokens: rows ``cu_seqlens[i] : cu_seqlens[i + 1]`` of ``q [tokens, heads, head_dim]`` are the last tokens of
     request ``i``, whose ``context_lens[i]`` counts them; keys and values of all of them are in the cache already. Every token
     sees what ``paged_decode_attention`` would show it at its position. Rows of ``out`` (and of
-    the log sums) before the first and behind the last sequence are not written: a given ``out`` keeps them. Other arguments as ``paged_decode_attention``."""
+    the log sums) before the first and behind the last sequence are not written: a given ``out`` keeps them. Other arguments as
+    ``paged_decode_attention``. Block sizes that are multiples of 8 go to the tensor-core kernel, others to the decode kernel, a token at
+    a time. A value that is not finite, of a key that some tokens of a block of a few see, may reach the block's other tokens; what no
+    token of the block sees (stale rows, returned blocks) never does."""
     return _paged_attention(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, scale, window, sinks, out, return_lse)

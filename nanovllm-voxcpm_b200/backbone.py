@@ -54,7 +54,7 @@ class DecoderConfig:
     lora_tp_mode: str = "partial_y"
     #: RMS norm of every query and key head ahead of the rotation
     qk_norm: bool = False
-    #: attention over the paged cache by ``attention.py`` instead of flash_attn
+    #: attention over the paged cache by ``attention.py``, for prompts too
     paged_attention: bool = False
     #: keys that a token sees, its own among them (0: all), and first tokens that stay visible besides
     sliding_window: int = 0

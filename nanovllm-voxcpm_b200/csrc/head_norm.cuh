@@ -2,7 +2,9 @@
 //
 //   y = x * rsqrt(mean(x^2) + eps) * w;  (y_j, y_{j + D/2}) turned by the angle of (position, j);  k and v rows to their cache slot
 //
-// Bound: the bytes of the rows, once in and once out.
+// Bound: the bytes of the rows, once in and once out. Measured: 8192 tokens, 32 / 8 heads of 128 (202 MB with the tables), 44 us = 4.6 TB/s, 0.70
+// of the measured copy bandwidth (16 warps on an SM by registers, each of them waiting for its sums a third of the time; a thread per
+// head's piece 62 to 81 us, two to eight heads a thread 49 to 88); one token 4.2 us.
 #pragma once
 
 #include "glue.cuh"
