@@ -86,6 +86,18 @@ def test_decode_strided(dtype):
     assert bool((wide[:, :, :8] == 7).all()) and bool((wide[:, :, 136:] == 7).all())
 
 
+@pytest.mark.parametrize("heads,contexts", [((16, 2, 128), [2500]), ((32, 8, 128), [700]), ((16, 2, 64), [900, 3, 0, 1024]), ((12, 1, 128), [1500] * 3),
+                                            ((40, 2, 64), [2100, 1]), ((16, 2, 64), [1000] * 40), ((16, 2, 64), [300] * 200), ((8, 8, 64), [5] * 60)])
+def test_decode_ways(heads, contexts):
+    """One CTA an item, clusters of them, with four and with eight warps; run to run the same."""
+    p = PP.make(*heads, 32, contexts, seed=len(contexts), poison=True)
+    out, lse = _decode(p, return_lse=True)
+    PP.check(p, out, lse)
+    for _ in range(3):
+        again, lse2 = _decode(p, return_lse=True)
+        assert torch.equal(again, out) and torch.equal(lse2, lse)
+
+
 @pytest.mark.parametrize("contexts", [[5000], [9000, 1, 30], [40] * 700, [3000] * 20, list(range(0, 640, 5))])
 def test_decode_shares_of_the_work(contexts):
     """One long request over many CTAs, many short ones over few, shares that begin and end inside requests; run to run the same."""
@@ -149,6 +161,28 @@ def test_prefill_pages_and_windows(page, window, sinks):
 def test_prefill_pages_that_the_tile_kernel_does_not_take(page):
     p = PP.make(8, 2, 64, page, [130, 61], [30, 61], window=40, sinks=3, seed=page, poison=True)
     PP.check(p, *_prefill(p, return_lse=True), f"pages of {page}")
+
+
+@pytest.mark.parametrize("heads", [(16, 2, 64), (8, 2, 128)])
+@pytest.mark.parametrize("n", [31, 32, 33, 70])
+def test_prefill_many_requests(n, heads):
+    """More requests than a warp has lanes, empty ones and prompts of several blocks among them, some behind a context."""
+    new = [(7 * i) % 41 if i % 9 else 150 + i for i in range(n)]
+    p = PP.make(*heads, 16, [x + (i % 3) * 60 for i, x in enumerate(new)], new, seed=n, poison=True, behind=1)
+    PP.check(p, *_prefill(p, return_lse=True), f"{n} requests")
+
+
+def test_prefill_ranges_outside_the_rows():
+    """Ranges that leave the rows of q, or run backwards, count as none; the others are served."""
+    p = PP.make(8, 2, 64, 16, [40, 50, 60], [40, 50, 60], seed=6)
+    q, k, v, tables, ctx, cu = p["args"]
+    want = _prefill(p)
+    for bad in ([0, 40, 90, 10 ** 6], [-5, 40, 90, 150], [0, 40, 30, 150], [200, 40, 90, 150]):
+        out = torch.full_like(q, 7.0)
+        A.paged_prefill_attention(q, k, v, tables, ctx, torch.tensor(bad, dtype=torch.int32, device="cuda"), scale=p["scale"], out=out)
+        torch.cuda.synchronize()
+        assert torch.equal(out[40:90], want[40:90]) or bad[2] == 30
+    assert N.device_status() == 0
 
 
 def test_prefill_tokens_ahead_of_their_context():
