@@ -485,12 +485,13 @@ int lora_b200_glue_qk_norm_rope_kv_store(void* qkv, int64_t qkv_ld, int32_t T, i
  * prefill: the tokens [cu_seqlens[i], cu_seqlens[i + 1]) of q are the last ones of sequence i (cu_seqlens ascending); rows of out
  *          (and lse) outside [cu_seqlens[0], cu_seqlens[n_seqs]) are left as they are.
  * head_dim 64 or 128, scale > 0, bf16 and fp16. workspace: device memory of the number of bytes that
- * lora_b200_paged_decode_workspace_bytes / _prefill_workspace_bytes give, 16-byte aligned, of this call alone until it has run. Counterpart in the reference: the two calls over the
+ * lora_b200_paged_decode_workspace_bytes / _prefill_workspace_bytes give (0: none, null will do), 16-byte aligned, of this call alone until it has run. Counterpart in the reference: the two calls over the
  * paged cache in Attention.forward (nanovllm_voxcpm/layers/attention.py:70-79); it has no window.
  * A value that is not finite, of a key that some rows of a prefill block of tokens see, may reach the block's other rows (a block: 128
  * or 256 rows of (token, head)); values of keys that no row of the block sees never do.
  */
-size_t lora_b200_paged_decode_workspace_bytes(int32_t num_heads, int32_t num_kv_heads, int32_t head_dim);
+size_t lora_b200_paged_decode_workspace_bytes(int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                              int32_t table_width, int32_t block_size, int32_t window, int32_t sinks);
 size_t lora_b200_paged_prefill_workspace_bytes(int32_t T, int32_t n_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                                                int32_t table_width, int32_t block_size, int32_t window);
 int lora_b200_paged_decode_attention(void* out, int64_t out_token, int64_t out_head, float* lse, const void* q, int64_t q_token,

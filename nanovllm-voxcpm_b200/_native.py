@@ -136,7 +136,7 @@ _SIGNATURES = {
         c_int32, [c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p,
                   c_int32, c_int32, c_int32, c_void_p, c_int64, POINTER(PagedCache), c_void_p, c_int32, c_void_p],
     ),
-    "lora_b200_paged_decode_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32]),
+    "lora_b200_paged_decode_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
     "lora_b200_paged_prefill_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
     "lora_b200_paged_decode_attention": (
         c_int32,

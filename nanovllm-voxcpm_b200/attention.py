@@ -67,12 +67,13 @@ def _paged_attention(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens
             out = torch.empty(T, heads, dim, dtype=q.dtype, device=q.device)
         lse = torch.empty(T, heads, dtype=torch.float32, device=q.device) if return_lse else None
         kv_heads = k_cache.size(2)
-        need = N.lib().lora_b200_paged_decode_workspace_bytes(heads, kv_heads, dim) if cu_seqlens is None else \
-            N.lib().lora_b200_paged_prefill_workspace_bytes(T, n, heads, kv_heads, dim, block_tables.size(1), k_cache.size(1), window)
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        shape = (heads, kv_heads, dim, block_tables.size(1), k_cache.size(1), window)
+        need = N.lib().lora_b200_paged_decode_workspace_bytes(T, *shape, sinks) if cu_seqlens is None else \
+            N.lib().lora_b200_paged_prefill_workspace_bytes(T, n, *shape)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
         head = (out.data_ptr(), out.stride(0), out.stride(1), N.ptr(lse), q.data_ptr(), q.stride(0), q.stride(1), T, heads, kv_heads, dim,
                 ctypes.byref(cache), block_tables.data_ptr(), block_tables.stride(0), block_tables.size(1), context_lens.data_ptr())
-        tail = (float(scale), int(window), int(sinks), N.dtype_code(q.dtype), workspace.data_ptr(), need, N.current_stream(q.device))
+        tail = (float(scale), int(window), int(sinks), N.dtype_code(q.dtype), N.ptr(workspace), need, N.current_stream(q.device))
         if cu_seqlens is None:
             N.check(N.lib().lora_b200_paged_decode_attention(*head, *tail))
         else:

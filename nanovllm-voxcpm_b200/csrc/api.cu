@@ -356,15 +356,17 @@ int lora_b200_glue_qk_norm_rope_kv_store(void* qkv, int64_t qkv_ld, int32_t T, i
   return head_norm_launch(p, dtype, static_cast<cudaStream_t>(stream));
 }
 
-size_t lora_b200_paged_decode_workspace_bytes(int32_t num_heads, int32_t num_kv_heads, int32_t head_dim) {
+size_t lora_b200_paged_decode_workspace_bytes(int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                              int32_t table_width, int32_t block_size, int32_t window, int32_t sinks) {
   if (num_kv_heads < 1 || num_heads < num_kv_heads || head_dim < 1) return 0;
-  return paged_workspace_bytes(num_heads, num_kv_heads, head_dim);
+  return paged_workspace_bytes(T, num_heads, num_kv_heads, head_dim, (int64_t)table_width * block_size, window, sinks);
 }
 
 size_t lora_b200_paged_prefill_workspace_bytes(int32_t T, int32_t n_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                                                int32_t table_width, int32_t block_size, int32_t window) {
   if (num_kv_heads < 1 || num_heads < num_kv_heads || head_dim < 1) return 0;
-  return paged_prefill_workspace_bytes(T, n_seqs, num_heads, num_kv_heads, head_dim, (int64_t)table_width * block_size, window);
+  if (block_size < 1) return 0;
+  return paged_prefill_workspace_bytes(T, n_seqs, num_heads, num_kv_heads, head_dim, block_size, (int64_t)table_width * block_size, window);
 }
 
 // What decode and prefill have in common; cu_seqlens null: decode
@@ -389,16 +391,16 @@ static int paged_attention_checked(const char* what, void* out, int64_t out_toke
     return fail(B200_LORA_EUNSUPPORTED, "%s: rows of q and out must start on 16-byte boundaries", what);
   if (!aligned16(workspace)) return fail(B200_LORA_EUNSUPPORTED, "%s: the workspace must be 16-byte aligned", what);
   const size_t need = prefill ? lora_b200_paged_prefill_workspace_bytes(T, n_seqs, num_heads, num_kv_heads, head_dim, table_width, cache->block_size, window)
-                              : lora_b200_paged_decode_workspace_bytes(num_heads, num_kv_heads, head_dim);
-  if (workspace == nullptr || workspace_bytes < need)
+                              : lora_b200_paged_decode_workspace_bytes(T, num_heads, num_kv_heads, head_dim, table_width, cache->block_size, window, sinks);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(B200_LORA_EWORKSPACE, "%s: %zu bytes of workspace, needs %zu", what, workspace == nullptr ? (size_t)0 : workspace_bytes, need);
   PagedArgs a = {};
   a.q = q; a.q_token = q_token; a.q_head = q_head; a.out = out; a.out_token = out_token; a.out_head = out_head; a.lse = lse;
   a.cache = *cache; a.tables = block_tables; a.table_ld = table_ld; a.table_width = table_width; a.context_lens = context_lens;
   a.cu_seqlens = cu_seqlens; a.n_req = n_seqs; a.T = T; a.Hq = num_heads; a.Hk = num_kv_heads; a.window = window; a.sinks = sinks;
   a.sc = scale * 1.4426950408889634f;
-  if (prefill) return paged_prefill_launch(a, head_dim, dtype, workspace, static_cast<cudaStream_t>(stream));
-  return paged_decode_launch(a, head_dim, dtype, workspace, static_cast<cudaStream_t>(stream));
+  if (prefill) return paged_prefill_launch(a, head_dim, dtype, need > 0 ? workspace : nullptr, static_cast<cudaStream_t>(stream));
+  return paged_decode_launch(a, head_dim, dtype, need > 0 ? workspace : nullptr, static_cast<cudaStream_t>(stream));
 }
 
 int lora_b200_paged_decode_attention(void* out, int64_t out_token, int64_t out_head, float* lse, const void* q, int64_t q_token,

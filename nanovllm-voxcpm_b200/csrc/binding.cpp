@@ -623,9 +623,11 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (out == nullptr || !on(*out, dev) || out->scalar_type() != dt || out->sizes() != q->sizes() || out->stride(2) != 1) return not_handled();
   }
   if (args[10] == Py_True) lse = at::empty({T, hq}, q->options().dtype(at::kFloat));
-  const size_t need = cu == nullptr ? p_decode_bytes((int)hq, (int)hk, (int)d)
+  const size_t need = cu == nullptr ? p_decode_bytes((int)T, (int)hq, (int)hk, (int)d, (int)tables->size(1), cache.block_size, (int)window, (int)sinks)
                                     : p_prefill_bytes((int)T, (int)n, (int)hq, (int)hk, (int)d, (int)tables->size(1), cache.block_size, (int)window);
-  const at::Tensor ws = at::empty({(int64_t)need}, q->options().dtype(at::kByte));
+  at::Tensor ws;
+  if (need > 0) ws = at::empty({(int64_t)need}, q->options().dtype(at::kByte));
+  void* const ws_ptr = need > 0 ? ws.data_ptr() : nullptr;
   void* stream = c10::cuda::getCurrentCUDAStream(dev).stream();
   float* lse_ptr = lse.defined() ? static_cast<float*>(lse.data_ptr()) : nullptr;
   int rc;
@@ -633,11 +635,11 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     rc = p_paged_prefill(out->data_ptr(), out->stride(0), out->stride(1), lse_ptr, q->data_ptr(), q->stride(0), q->stride(1), (int)T, (int)hq,
                          (int)hk, (int)d, &cache, static_cast<const int32_t*>(tables->data_ptr()), tables->stride(0), (int)tables->size(1),
                          static_cast<const int32_t*>(ctx->data_ptr()), static_cast<const int32_t*>(cu->data_ptr()), (int)n, (float)scale,
-                         (int)window, (int)sinks, code, ws.data_ptr(), need, stream);
+                         (int)window, (int)sinks, code, ws_ptr, need, stream);
   else
     rc = p_paged_decode(out->data_ptr(), out->stride(0), out->stride(1), lse_ptr, q->data_ptr(), q->stride(0), q->stride(1), (int)T, (int)hq,
                         (int)hk, (int)d, &cache, static_cast<const int32_t*>(tables->data_ptr()), tables->stride(0), (int)tables->size(1),
-                        static_cast<const int32_t*>(ctx->data_ptr()), (float)scale, (int)window, (int)sinks, code, ws.data_ptr(), need, stream);
+                        static_cast<const int32_t*>(ctx->data_ptr()), (float)scale, (int)window, (int)sinks, code, ws_ptr, need, stream);
   PyObject* lse_out = Py_None;
   if (lse.defined()) lse_out = THPVariable_Wrap(lse);
   else Py_INCREF(Py_None);

@@ -13,6 +13,8 @@
 // the longest request, 0.6 us each, behind 3.5 us of launch, look-ups and join).
 #pragma once
 
+#include <atomic>
+
 #include "decode_step.cuh"
 #include "glue.cuh"
 
@@ -542,8 +544,39 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArg
   *reinterpret_cast<uint32_t*>(static_cast<char*>(a.out) + 2 * (j.x * a.out_token + (j.y + (int)blockIdx.y) * a.out_head + 4 * c + 2)) = pack_16x2<kF16>(o.z * inv, o.w * inv);
 }
 
+// Dynamic shared memory of a kernel, set once on a device (`known`: the devices that have it; half a microsecond a call otherwise)
+inline int allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>* known) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev < 64 && (known->load(std::memory_order_relaxed) >> dev & 1u)) return B200_LORA_OK;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return fail(B200_LORA_ECUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  if (dev < 64) known->fetch_or(1ull << dev, std::memory_order_relaxed);
+  return B200_LORA_OK;
+}
+
+// How the items (row, kv head, chunk) meet the CTAs, by what the host knows: their number, and the blocks of keys of one at most
+// (the table's width, the window). us, one CTA of four warps an item / of eight / clusters of 2, 4, 8 of eight / equal shares of four:
+//   16 / 2 heads of 64: one request of 700 tokens (2 items, 22 blocks) 8.2 / 7.1 / 7.4, 6.6, 6.3 / 10.9; of 8000 48 / 33 / 22, 15, 10.9 /
+//   15.9; of 32000 210 / 125 / 69, 39, 23.4 / 21.4; 64 of 1000 (128 items, 32 blocks) 11.9 / 10.0 / 16.5, 35, 66 / 16.7; 64 of 8000 64 / 48 /
+//   53, 84, 128 / 52; 32 / 8 of 128: 8 of 300 (64, 19) 7.9 / 7.4 / 8.4, 12.5, 30 / 13.1; 8 of 2000 30 / 22 / 18.9, 24, 42 / 22;
+//   16 / 2 of 128: 128 of 1000 (256, 63) 27.2 / 29.2 / 42, 97, 158 / 34
+//   ragged, 48 of 500 to 8192 (384, 512) 203 / 179 / 166, 273, 368 / 138; 16 of 100 to 16000 (128, 1000) 208 / 138 / 147, 146, 210 / 109
+struct PagedWay { int cluster, warps; bool shares; };
+inline PagedWay paged_way(int T, int Hq, int Hk, int D, int64_t max_keys, int window, int sinks) {
+  const int64_t keys = window > 0 ? std::min<int64_t>(max_keys, (int64_t)window + sinks) : max_keys, block = D == 64 ? paged_block_keys<64>() : paged_block_keys<128>();
+  const int64_t units = (keys + block - 1) / block, items = (int64_t)T * Hk * ((Hq / Hk + 15) / 16);
+  PagedWay w = {8, 8, false};
+  while (w.cluster > 1 && items * w.cluster > 148) w.cluster /= 2;
+  if (units < (w.cluster == 2 ? 64 : 20)) w.cluster = 1;
+  if (items * w.cluster > 148) w.warps = 4;
+  w.shares = (units > 32 * w.warps * w.cluster && items < 8 * kPagedCtas) || (w.cluster == 8 && units > 700);
+  return w;
+}
+
 inline size_t paged_parts_bytes(int heads, int D) { return (size_t)2 * kPagedCtas * heads * D * 4; }
-inline size_t paged_workspace_bytes(int Hq, int Hk, int D) {
+inline size_t paged_workspace_bytes(int T, int Hq, int Hk, int D, int64_t max_keys, int window, int sinks) {
+  if (!paged_way(T, Hq, Hk, D, max_keys, window, sinks).shares) return 0;
   const int heads = std::min(Hq / Hk, 16);
   return paged_parts_bytes(heads, D) + (size_t)2 * kPagedCtas * heads * 8 + kPagedCtas * sizeof(int4);
 }
@@ -551,8 +584,8 @@ inline size_t paged_workspace_bytes(int Hq, int Hk, int D) {
 template <int D, int NT, bool kF16, int kWay, int kWarps>
 inline int paged_decode_launch_t(const PagedArgs& a, int ctas, int cluster, cudaStream_t stream) {
   const auto kernel = paged_decode_kernel<D, NT, kF16, kWay, kWarps>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, paged_smem<D, NT>(kWarps));
-  if (e != cudaSuccess) return fail(B200_LORA_ECUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  static std::atomic<uint64_t> known{0};
+  if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), paged_smem<D, NT>(kWarps), &known)) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(32 * kWarps);
@@ -566,7 +599,7 @@ inline int paged_decode_launch_t(const PagedArgs& a, int ctas, int cluster, cuda
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = bgmv_options().pdl ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, kernel, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return fail(B200_LORA_ECUDA, "paged_decode_kernel launch: %s", cudaGetErrorString(e));
@@ -575,27 +608,14 @@ inline int paged_decode_launch_t(const PagedArgs& a, int ctas, int cluster, cuda
   return launch_dependent(paged_join_kernel<D, kF16>, "paged_join_kernel", dim3((unsigned)ctas, (unsigned)a.heads), kJoinThreads, 0, stream, a);
 }
 
-// How the items (row, kv head, chunk) meet the CTAs, by what the host knows: their number, and the blocks of keys of one at most
-// (the table's width, the window). us, one CTA of four warps an item / of eight / clusters of 2, 4, 8 of eight / equal shares of four:
-//   16 / 2 heads of 64: one request of 700 tokens (2 items, 22 blocks) 8.2 / 7.1 / 7.4, 6.6, 6.3 / 10.9; of 8000 48 / 33 / 22, 15, 10.9 /
-//   15.9; of 32000 210 / 125 / 69, 39, 23.4 / 21.4; 64 of 1000 (128 items, 32 blocks) 11.9 / 10.0 / 16.5, 35, 66 / 16.7; 64 of 8000 64 / 48 /
-//   53, 84, 128 / 52; 32 / 8 of 128: 8 of 300 (64, 19) 7.9 / 7.4 / 8.4, 12.5, 30 / 13.1; 8 of 2000 30 / 22 / 18.9, 24, 42 / 22;
-//   16 / 2 of 128: 128 of 1000 (256, 63) 27.2 / 29.2 / 42, 97, 158 / 34
-//   ragged, 48 of 500 to 8192 (384, 512) 203 / 179 / 166, 273, 368 / 138; 16 of 100 to 16000 (128, 1000) 208 / 138 / 147, 146, 210 / 109
 template <int D, int NT, bool kF16>
 inline int paged_decode_launch_by(const PagedArgs& a, cudaStream_t stream) {
-  int64_t keys = (int64_t)a.table_width * a.cache.block_size;
-  if (a.window > 0) keys = std::min<int64_t>(keys, (int64_t)a.window + a.sinks);
-  const int64_t units = (keys + paged_block_keys<D>() - 1) / paged_block_keys<D>(), items = (int64_t)a.T * a.Hk * a.chunks;
-  int cluster = 8;
-  while (cluster > 1 && items * cluster > 148) cluster /= 2;
-  if (units < (cluster == 2 ? 64 : 20)) cluster = 1;
-  const int warps = items * cluster <= 148 ? 8 : 4;
-  if ((units > 32 * warps * cluster && items < 8 * kPagedCtas) || (cluster == 8 && units > 700))
-    return paged_decode_launch_t<D, NT, kF16, kShares, 4>(a, kPagedCtas, 1, stream);
-  const int ctas = (int)std::min<int64_t>((warps == 8 ? 148 : kPagedCtas) / cluster, items) * cluster;
-  if (cluster > 1) return paged_decode_launch_t<D, NT, kF16, kClusters, 8>(a, ctas, cluster, stream);
-  if (warps == 8) return paged_decode_launch_t<D, NT, kF16, kWhole, 8>(a, ctas, 1, stream);
+  const PagedWay w = paged_way(a.T, a.Hq, a.Hk, D, (int64_t)a.table_width * a.cache.block_size, a.window, a.sinks);
+  if (w.shares && a.part_o != nullptr) return paged_decode_launch_t<D, NT, kF16, kShares, 4>(a, kPagedCtas, 1, stream);
+  const int64_t items = (int64_t)a.T * a.Hk * a.chunks;
+  const int ctas = (int)std::min<int64_t>((w.warps == 8 ? 148 : kPagedCtas) / w.cluster, items) * w.cluster;
+  if (w.cluster > 1) return paged_decode_launch_t<D, NT, kF16, kClusters, 8>(a, ctas, w.cluster, stream);
+  if (w.warps == 8) return paged_decode_launch_t<D, NT, kF16, kWhole, 8>(a, ctas, 1, stream);
   return paged_decode_launch_t<D, NT, kF16, kWhole, 4>(a, ctas, 1, stream);
 }
 
@@ -603,10 +623,12 @@ inline int paged_decode_launch(PagedArgs a, int D, int dtype, void* workspace, c
   const int group = a.Hq / a.Hk;
   a.heads = std::min(group, 16);
   a.chunks = ceil_div_i(group, a.heads);
-  char* ws = static_cast<char*>(workspace);
-  a.part_o = reinterpret_cast<float*>(ws);
-  a.part_ml = reinterpret_cast<float*>(ws + paged_parts_bytes(a.heads, D));
-  a.joins = reinterpret_cast<int4*>(ws + paged_parts_bytes(a.heads, D) + (size_t)2 * kPagedCtas * a.heads * 8);
+  if (workspace != nullptr) {  // (null: no shares)
+    char* ws = static_cast<char*>(workspace);
+    a.part_o = reinterpret_cast<float*>(ws);
+    a.part_ml = reinterpret_cast<float*>(ws + paged_parts_bytes(a.heads, D));
+    a.joins = reinterpret_cast<int4*>(ws + paged_parts_bytes(a.heads, D) + (size_t)2 * kPagedCtas * a.heads * 8);
+  }
   const bool f16 = dtype == B200_LORA_F16, wide = a.heads > 8;
   if (D == 64) {
     if (wide) return f16 ? paged_decode_launch_by<64, 2, true>(a, stream) : paged_decode_launch_by<64, 2, false>(a, stream);

@@ -723,9 +723,10 @@ inline size_t pp_split_bytes(int D) {
   const int tiles = pp_tiles(D), ctas = 148 * (3 - tiles);
   return (size_t)ctas * tiles * kPpRows * (D + 2) * 4 + ctas * sizeof(PpJoin);
 }
-inline size_t paged_prefill_workspace_bytes(int T, int n_req, int Hq, int Hk, int D, int64_t max_context, int window) {
-  const size_t tokens = paged_workspace_bytes(Hq, Hk, D);
-  return pp_splits(T, n_req, Hq, pp_h_shift(Hq / Hk), pp_tiles(D), max_context, window) ? std::max(tokens, pp_split_bytes(D)) : tokens;
+// (blocks that the tile kernel does not take: what the decode kernel needs for as many rows)
+inline size_t paged_prefill_workspace_bytes(int T, int n_req, int Hq, int Hk, int D, int block_size, int64_t max_context, int window) {
+  if (block_size % 8 != 0) return paged_workspace_bytes(T, Hq, Hk, D, max_context, window, 0);
+  return pp_splits(T, n_req, Hq, pp_h_shift(Hq / Hk), pp_tiles(D), max_context, window) ? pp_split_bytes(D) : 0;
 }
 
 template <int D, bool kF16, bool kSplit>
@@ -733,8 +734,8 @@ inline int paged_prefill_launch_t(const PpMaps& maps, const PpArgs& a, cudaStrea
   constexpr int kTiles = pp_tiles(D), kCtas = 148 * (3 - kTiles);
   const auto kernel = paged_prefill_kernel<D, kF16, kTiles, kSplit>;
   constexpr int smem = pp_smem<D>(kTiles);
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return fail(B200_LORA_ECUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  static std::atomic<uint64_t> known{0};
+  if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), smem, &known)) return rc;
   const int ctas = kSplit ? kCtas : (int)std::min<int64_t>(kCtas, (int64_t)a.n_blocks * a.head_tiles);
   const int rc = launch_dependent(kernel, "paged_prefill_kernel", dim3((unsigned)ctas), pp_threads(kTiles), (size_t)smem, stream, maps, a);
   if (rc != B200_LORA_OK || !kSplit) return rc;
@@ -745,7 +746,7 @@ inline int paged_prefill_launch(const PagedArgs& p, int D, int dtype, void* work
   PpMaps maps;
   PpArgs a = {};
   const bool f16 = dtype == B200_LORA_F16;
-  if (!paged_prefill_plan(p, D, f16, pp_tiles(D), &maps, &a)) return paged_decode_launch(p, D, dtype, workspace, stream);
+  if (!paged_prefill_plan(p, D, f16, pp_tiles(D), &maps, &a)) return paged_decode_launch(p, D, dtype, p.cache.block_size % 8 != 0 ? workspace : nullptr, stream);
   if (pp_splits(p.T, p.n_req, p.Hq, a.h_shift, pp_tiles(D), (int64_t)p.table_width * p.cache.block_size, p.window)) {
     a.parts = static_cast<float*>(workspace);
     a.joins = static_cast<char*>(workspace) + pp_split_bytes(D) - 148 * (3 - pp_tiles(D)) * sizeof(PpJoin);

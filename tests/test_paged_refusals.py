@@ -43,7 +43,7 @@ BAD = [
     (dict(tables=None), N.E_INVAL), (dict(ctx=None), N.E_INVAL), (dict(cache=None), N.E_INVAL), (dict(cache=_cache(k=None)), N.E_INVAL),
     (dict(cache=_cache(v=None)), N.E_INVAL), (dict(cache=_cache(num_blocks=0)), N.E_INVAL), (dict(cache=_cache(block_size=0)), N.E_INVAL),
     (dict(cache=_cache(k=AT + 8)), N.E_UNSUPPORTED), (dict(cache=_cache(v_token=132)), N.E_UNSUPPORTED), (dict(q=AT + 2), N.E_UNSUPPORTED),
-    (dict(qh=68), N.E_UNSUPPORTED), (dict(ot=1028), N.E_UNSUPPORTED), (dict(ws=None), N.E_WORKSPACE), (dict(bytes=16), N.E_WORKSPACE),
+    (dict(qh=68), N.E_UNSUPPORTED), (dict(ot=1028), N.E_UNSUPPORTED), (dict(width=1 << 16, ws=None), N.E_WORKSPACE), (dict(width=1 << 16, bytes=16), N.E_WORKSPACE),
     (dict(ws=AT + 4), N.E_UNSUPPORTED),
 ]
 
