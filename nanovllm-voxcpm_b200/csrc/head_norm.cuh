@@ -2,9 +2,9 @@
 //
 //   y = x * rsqrt(mean(x^2) + eps) * w;  (y_j, y_{j + D/2}) turned by the angle of (position, j);  k and v rows to their cache slot
 //
-// Bound: the bytes of the rows, once in and once out. Measured: 8192 tokens, 32 / 8 heads of 128 (202 MB with the tables), 44 us = 4.6 TB/s, 0.70
-// of the measured copy bandwidth (16 warps on an SM by registers, each of them waiting for its sums a third of the time; a thread per
-// head's piece 62 to 81 us, two to eight heads a thread 49 to 88); one token 4.2 us.
+// Bound: the bytes of the rows, once in and once out. Measured: 8192 tokens, 32 / 8 heads of 128 (202 MB with the tables), 41 us = 4.9 TB/s, 0.75
+// of the measured copy bandwidth (24 warps on an SM by registers, each waiting for its sums much of the time; a thread per head's piece 62
+// to 81 us, two to eight heads a thread 49 to 88); one token 4.2 us.
 #pragma once
 
 #include "glue.cuh"
@@ -80,6 +80,7 @@ __device__ __forceinline__ float head_squares(const Vec8<T>& lo, const Vec8<T>& 
     sum = fma2(b, b, fma2(a, a, sum));
   }
   float ss = sum.x + sum.y;
+#pragma unroll
   for (int o = (1 << lane_shift) >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   return ss;
 }
@@ -147,11 +148,12 @@ __global__ void __launch_bounds__(kRopeThreads) head_norm_kernel(const HeadNormP
 }
 
 // Many tokens: the rows of `tokens` tokens and their table rows come by bulk copies into one of two stages while the other is
-// worked on, two CTAs on an SM; a thread keeps the angles and weights of its columns for all heads of its token that it takes.
+// worked on, three CTAs on an SM; a thread keeps the angles and weights of its columns for all heads of its token that it takes.
+constexpr int kHeadCtas = 3;  // on an SM (8192 wide tokens: 43 us with two, 41 with three, 59 with four, whose registers spill)
 struct HeadRing { int tokens, row_bytes, table_bytes, stage_bytes; };
 
-template <typename T>
-__global__ void __launch_bounds__(kRopeThreads, 2) head_norm_ring_kernel(const HeadNormParams p, const HeadRing ring, int lane_shift) {
+template <typename T, int lane_shift>
+__global__ void __launch_bounds__(kRopeThreads, kHeadCtas) head_norm_ring_kernel(const HeadNormParams p, const HeadRing ring) {
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(8) uint64_t full[2];
   __shared__ volatile int abort_flag;
@@ -224,10 +226,10 @@ __global__ void __launch_bounds__(kRopeThreads, 2) head_norm_ring_kernel(const H
   if (tid == 0 && abort_flag != 0) atomicOr(&g_b200_status, kStatusWaitGaveUp);
 }
 
-constexpr int kHeadStage = 52 << 10;  // bytes of a stage at most: two of them and two CTAs on an SM
+constexpr int kHeadStage = 36 << 10;  // bytes of a stage at most: two of them, and kHeadCtas CTAs on an SM
 // Rows of a call, in bytes, from which the copies pay: us, a thread per piece / stages, heads 16 / 2 of 64: 1024 tokens (2.6 MB) 3.6 /
-// 4.9, 2048 7.3 / 7.4, 4096 11.0 / 9.2, 8192 20 / 15.5; 32 / 8 of 128: 256 tokens (3.1 MB) 3.5 / 5.6, 512 7.0 / 7.1, 1024 12.6 / 8.9,
-// 8192 81 / 44.
+// 4.9, 2048 7.3 / 8.3, 4096 11.0 / 11.1, 8192 20 / 16.4; 32 / 8 of 128: 256 tokens (3.1 MB) 3.5 / 5.6, 512 7.0 / 7.9, 1024 12.6 / 10.4,
+// 8192 81 / 41.
 constexpr int64_t kHeadRingBytes = 5 << 20;
 
 inline int paged_cache_check(const lora_b200_paged_cache& c, const char* what) {
@@ -272,18 +274,27 @@ inline int head_norm_launch(const HeadNormParams& p, int dtype, cudaStream_t str
   ring.table_bytes = r.apply_rope ? r.table_dim * (r.table_dtype == B200_LORA_F32 ? 4 : 2) : 0;
   const int one = ring.row_bytes + 2 * ring.table_bytes;
   ring.tokens = 1;
-  while (2 * ring.tokens * one <= kHeadStage && 2 * ring.tokens <= (kRopeThreads >> lane_shift) && ceil_div_i(r.T, 2 * ring.tokens) >= 2 * 148) ring.tokens *= 2;
+  while (2 * ring.tokens * one <= kHeadStage && 2 * ring.tokens <= (kRopeThreads >> lane_shift) && ceil_div_i(r.T, 2 * ring.tokens) >= kHeadCtas * 148) ring.tokens *= 2;
   ring.stage_bytes = ring.tokens * one;
   if (2 * width * r.T >= kHeadRingBytes && one <= kHeadStage) {
-    const int smem = 2 * ring.stage_bytes, grid = std::min(2 * 148, ceil_div_i(r.T, ring.tokens));
-#define B200_HEAD_RING(TT)                                                                                                                           \
-  {                                                                                                                                                  \
-    const cudaError_t e = cudaFuncSetAttribute(head_norm_ring_kernel<TT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kHeadStage);              \
-    if (e != cudaSuccess) return fail(B200_LORA_ECUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));                                          \
-    return launch_dependent(head_norm_ring_kernel<TT>, "head_norm_ring_kernel", dim3((unsigned)grid), kRopeThreads, (size_t)smem, stream, p, ring, lane_shift); \
+    const int smem = 2 * ring.stage_bytes, grid = std::min(kHeadCtas * 148, ceil_div_i(r.T, ring.tokens));
+#define B200_HEAD_RING(TT, SHIFT)                                                                                                              \
+  {                                                                                                                                            \
+    const cudaError_t e = cudaFuncSetAttribute(head_norm_ring_kernel<TT, SHIFT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kHeadStage); \
+    if (e != cudaSuccess) return fail(B200_LORA_ECUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));                                    \
+    return launch_dependent(head_norm_ring_kernel<TT, SHIFT>, "head_norm_ring_kernel", dim3((unsigned)grid), kRopeThreads, (size_t)smem, stream, p, ring); \
   }
-    if (dtype == B200_LORA_BF16) B200_HEAD_RING(__nv_bfloat16)
-    B200_HEAD_RING(__half)
+#define B200_HEAD_RINGS(TT)                    \
+  {                                            \
+    if (lane_shift == 0) B200_HEAD_RING(TT, 0) \
+    if (lane_shift == 1) B200_HEAD_RING(TT, 1) \
+    if (lane_shift == 2) B200_HEAD_RING(TT, 2) \
+    if (lane_shift == 3) B200_HEAD_RING(TT, 3) \
+    B200_HEAD_RING(TT, 4)                      \
+  }
+    if (dtype == B200_LORA_BF16) B200_HEAD_RINGS(__nv_bfloat16)
+    B200_HEAD_RINGS(__half)
+#undef B200_HEAD_RINGS
 #undef B200_HEAD_RING
   }
   const int64_t units = (int64_t)r.T * heads;
