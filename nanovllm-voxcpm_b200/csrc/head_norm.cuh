@@ -230,7 +230,7 @@ constexpr int kHeadStage = 36 << 10;  // bytes of a stage at most: two of them, 
 // Rows of a call, in bytes, from which the copies pay: us, a thread per piece / stages, heads 16 / 2 of 64: 1024 tokens (2.6 MB) 3.6 /
 // 4.9, 2048 7.3 / 8.3, 4096 11.0 / 11.1, 8192 20 / 16.4; 32 / 8 of 128: 256 tokens (3.1 MB) 3.5 / 5.6, 512 7.0 / 7.9, 1024 12.6 / 10.4,
 // 8192 81 / 41.
-constexpr int64_t kHeadRingBytes = 5 << 20;
+constexpr int64_t kHeadRingBytes = 8 << 20;
 
 inline int paged_cache_check(const lora_b200_paged_cache& c, const char* what) {
   if (c.k == nullptr || c.v == nullptr) return fail(B200_LORA_EINVAL, "%s: a cache is null", what);

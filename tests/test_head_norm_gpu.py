@@ -34,9 +34,9 @@ def _near(got, want, size, dtype, what):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16])
-# (from 5 MB of rows on they come by bulk copies: the last seven; rows of more than a stage do not)
-@pytest.mark.parametrize("T,hq,hk,d,page", [(701, 32, 8, 128, 16), (5001, 16, 2, 64, 64), (1300, 7, 7, 96, 24), (3000, 3, 1, 192, 16), (2500, 5, 3, 112, 8),
-                                            (20011, 1, 1, 64, 256), (100, 90, 10, 256, 16), (1, 16, 2, 64, 256), (37, 16, 2, 128, 16), (300, 32, 8, 128, 16), (5, 3, 1, 80, 7), (9, 4, 4, 256, 3),
+# (from 8 MB of rows on they come by bulk copies: the first seven; rows of more than a stage do not)
+@pytest.mark.parametrize("T,hq,hk,d,page", [(701, 32, 8, 128, 16), (5001, 16, 2, 64, 64), (2300, 7, 7, 96, 24), (4800, 3, 1, 192, 16), (3700, 5, 3, 112, 8),
+                                            (23011, 1, 1, 64, 256), (160, 90, 10, 256, 16), (1, 16, 2, 64, 256), (37, 16, 2, 128, 16), (300, 32, 8, 128, 16), (5, 3, 1, 80, 7), (9, 4, 4, 256, 3),
                                             (2, 1, 1, 16, 1), (65, 7, 7, 96, 24), (1000, 8, 2, 64, 64)])
 @pytest.mark.parametrize("separate", [False, True])
 def test_against_64_bits(T, hq, hk, d, page, dtype, separate):
