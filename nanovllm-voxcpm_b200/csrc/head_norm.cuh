@@ -2,7 +2,7 @@
 //
 //   y = x * rsqrt(mean(x^2) + eps) * w;  (y_j, y_{j + D/2}) turned by the angle of (position, j);  k and v rows to their cache slot
 //
-// Bound: the bytes of the rows, once in and once out. Measured: 8192 tokens, 32 / 8 heads of 128 (202 MB with the tables), 41 us = 4.9 TB/s, 0.75
+// Bound: the bytes of the rows, once in and once out. Measured: 8192 tokens, 32 / 8 heads of 128 (202 MB with the tables), 42 us = 4.8 TB/s, 0.73
 // of the measured copy bandwidth (24 warps on an SM by registers, each waiting for its sums much of the time; a thread per head's piece 62
 // to 81 us, two to eight heads a thread 49 to 88); one token 4.2 us.
 #pragma once
@@ -19,7 +19,10 @@ struct HeadNormParams {
   lora_b200_paged_cache cache;
 };
 
-// Weights and rotation of a thread's columns as one: lo' = rstd (a1 lo + b1 hi), hi' = rstd (a2 lo + b2 hi)
+// Weights and rotation of a thread's columns as one: with x = rstd lo and y = rstd hi, lo' = a1 x + b1 y, hi' = a2 x + b2 y. (rstd first:
+// of a head whose sum of squares is infinite it is 0, and so is rstd times any finite element, while an element times its factor may
+// have overflowed by then. The sum is fp32: 8192 wide tokens take 42.4 us so, 41.4 with rstd last.) Without a rotation lo' = a1 x and
+// hi' = b2 y alone: 0 times an infinite element would be NaN in its opposite column.
 struct HeadTurn {
   float2 a1[4], b1[4], a2[4], b2[4];
   // at `tb` of the tables: the angles of the first of the thread's columns; w1, w2: its weights in the two halves
@@ -50,13 +53,21 @@ struct HeadTurn {
     }
   }
   template <typename T>
-  __device__ __forceinline__ void apply(Vec8<T>& lo, Vec8<T>& hi, float rstd) const {
+  __device__ __forceinline__ void apply(Vec8<T>& lo, Vec8<T>& hi, float rstd, bool rotate) const {
     const float2 r2 = make_float2(rstd, rstd);
+    if (rotate) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 a = lo.pair(e), b = hi.pair(e);
-      lo.set_pair(e, mul2(r2, fma2(b, b1[e], mul2(a, a1[e]))));
-      hi.set_pair(e, mul2(r2, fma2(b, b2[e], mul2(a, a2[e]))));
+      for (int e = 0; e < 4; ++e) {
+        const float2 x = mul2(r2, lo.pair(e)), y = mul2(r2, hi.pair(e));
+        lo.set_pair(e, fma2(y, b1[e], mul2(x, a1[e])));
+        hi.set_pair(e, fma2(y, b2[e], mul2(x, a2[e])));
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        lo.set_pair(e, mul2(mul2(r2, lo.pair(e)), a1[e]));
+        hi.set_pair(e, mul2(mul2(r2, hi.pair(e)), b2[e]));
+      }
     }
   }
 };
@@ -140,7 +151,7 @@ __global__ void __launch_bounds__(kRopeThreads) head_norm_kernel(const HeadNormP
     HeadTurn turn;
     const T* w = static_cast<const T*>(head < p.r.Hq ? p.q_weight : p.k_weight) + j;
     turn.load(p.r, load8(w), load8(w + half), p.r.cos, p.r.sin, p.r.apply_rope ? table_row(p.r, tok) + j : 0);
-    turn.apply(lo, hi, rsqrtf(ss / (float)p.r.D + p.eps));
+    turn.apply(lo, hi, rsqrtf(ss / (float)p.r.D + p.eps), p.r.apply_rope);
   }
   int64_t at_k, at_v;
   cache_rows(p, tok, &at_k, &at_v);
@@ -216,7 +227,7 @@ __global__ void __launch_bounds__(kRopeThreads, kHeadCtas) head_norm_ring_kernel
           turn.load(p.r, load8(w), load8(w + half), at + ring.row_bytes, at + ring.row_bytes + ring.table_bytes, j);
         }
         kind = want;
-        turn.apply(lo, hi, rsqrtf(ss / (float)p.r.D + p.eps));
+        turn.apply(lo, hi, rsqrtf(ss / (float)p.r.D + p.eps), p.r.apply_rope);
       }
       store_head(p, tok, h, j, at_k, at_v, lo, hi);
     }

@@ -124,6 +124,38 @@ def test_rows_of_zeros_and_of_infinities():
     assert bool((q[2] == 0).all())  # the sum of squares is infinite, as in any fp32 norm
 
 
+@pytest.mark.parametrize("T", [3, 24000])  # (a thread a piece; rows by bulk copies)
+@pytest.mark.parametrize("rotate", [False, True])
+def test_heads_of_an_infinite_sum_of_squares(rotate, T):
+    """Their factor is 0 (the sum is fp32), and 0 times an element, its weight and its angle is 0 for finite elements whatever the order
+    of the products gives on the way; only the infinite element is NaN, with a rotation its opposite column too."""
+    hq, hk, d = 2, 1, 64
+    wide = torch.zeros(T, hq + 2 * hk, d, dtype=BF16)
+    wide[0, 0, 5] = float("inf")
+    wide[0, 0, 6:] = 3.0
+    wide[0, 2, 40] = -float("inf")
+    wide[1] = 3.0e38
+    wide[2, :, ::2], wide[2, :, 1::2] = -3.0e38, 2.0e38
+    wide[-1, 1, 3] = float("inf")
+    weight = torch.linspace(1.5, 40.0, d).to(BF16)
+    angle = torch.linspace(0.1, 3.0, d // 2).expand(8, -1)
+    turn = dict(positions=(torch.arange(T) % 8).cuda(), cos=angle.cos().contiguous().cuda(), sin=angle.sin().contiguous().cuda()) if rotate else {}
+    q, k, v = G.qk_norm_rope_kv_store(wide.cuda().view(T, -1), hq, hk, d, weight.cuda(), weight.cuda(), 1e-6, **turn)
+    for got, head, at in ((q, 0, (0, 5)), (k, 2, (0, 40)), (q, 1, (T - 1, 3))):
+        row = got[at[0], head if got is q else 0].cpu()
+        nan = torch.zeros(d, dtype=torch.bool)
+        nan[at[1]] = True
+        if rotate:
+            nan[(at[1] + d // 2) % d] = True
+        assert torch.equal(row.isnan(), nan) and bool((row[~nan] == 0).all()), (head, row)
+    assert bool((q[1] == 0).all()) and bool((k[1] == 0).all())
+    if T > 3:
+        assert bool((q[2] == 0).all()) and bool((k[2] == 0).all())
+    else:
+        assert bool((q[2, 0] == 0).all()) and bool((k[2] == 0).all())
+    assert torch.equal(v.cpu(), wide[:, hq + hk:])
+
+
 def test_graph_and_empty_batch():
     T, hq, hk, d = 12, 16, 2, 64
     wide, qw, kw, cos, sin, pos, slots, (kc, vc) = (t.cuda() if torch.is_tensor(t) else [c.cuda() for c in t] for t in _make(T, hq, hk, d, 16, BF16))
