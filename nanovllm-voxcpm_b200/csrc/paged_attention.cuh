@@ -107,7 +107,7 @@ struct PagedWalk {
   long long at, end, row_at;  // share: units; first unit of `row`
   int row, step;              // step > 0: items `at`, at + step, ..., of each the rank-th of `ranks` parts
   int rank, ranks;
-  static __device__ __forceinline__ int units(const RowKeys& r) { return r.n_keys < 0 ? 0 : max(1, (r.n_keys + kKeys - 1) / kKeys); }
+  static __device__ __forceinline__ int units(const RowKeys& r) { return r.n_keys < 0 ? 0 : max(1, (int)(((unsigned)r.n_keys + kKeys - 1u) / kKeys)); }
   __device__ __forceinline__ PagedPiece next(const PagedArgs& a) {
     const int per_row = a.Hk * a.chunks, group = a.Hq / a.Hk;
     PagedPiece w;

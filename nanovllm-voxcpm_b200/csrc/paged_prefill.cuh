@@ -116,16 +116,22 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
 // bits [0, n) of a word, n of any sign and size
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
 
+// Keys of a block table at most: indexes of keys, rounded up to tiles and with the columns of one added, are ints.
+constexpr int kPpMaxKeys = INT32_MAX - 255;
+// (positions that are not ints are those of rows behind the last token)
+__device__ __forceinline__ int pp_position(int first, int n) { return (int)min((int64_t)first + n, (int64_t)INT32_MAX - 1); }
+
 // A piece of work: tiles [i0, i1) of the keys that a block of tokens sees, for one set of heads.
 struct PpPiece {
   int head0, begin, q0, n_here;                // first head; first row of the sequence; first token and tokens of the block
   int req, pos0, held, key_end, lo_first, sink_end;  // position of the first token; keys that a row sees: [0, sink_end), [lo_first, key_end)
   int first_box, sink_boxes, i0, i1;           // the keys in boxes: those of the first tokens, then from first_box on, side by side
   int parts;                                   // 0: no more pieces; 1: the whole item; else the item is in that many parts
-  // first key of box b of tile i, with 1 << shift keys in a box
+  // first key of box b of tile i, with 1 << shift keys in a box; boxes from kPpMaxKeys on (of the last tile of a position next to
+  // 2^31: no table reaches them) all begin there, where the sum would no longer fit
   __device__ __forceinline__ int key_of(int i, int b, int shift) const {
     const int c = i * (kPpKeys >> shift) + b;
-    return (c < sink_boxes ? c : c - sink_boxes + first_box) << shift;
+    return (int)min((uint32_t)(c < sink_boxes ? c : c - sink_boxes + first_box) << shift, (uint32_t)kPpMaxKeys);
   }
 };
 
@@ -204,7 +210,7 @@ __device__ __forceinline__ void pp_find(const PpArgs& a, int span, int item, int
   w->q0 = block * span;
   w->n_here = min(span, len - w->q0);
   w->pos0 = __shfl_sync(0xffffffffu, q.ctx, who) - len + w->q0;
-  w->held = (int)min((int64_t)min(w->pos0 + w->n_here, INT32_MAX - 255), (int64_t)p.table_width * p.cache.block_size);
+  w->held = (int)min((int64_t)w->pos0 + w->n_here, (int64_t)p.table_width * p.cache.block_size);
   w->key_end = w->held;
   w->lo_first = p.window > 0 ? max(0, max(w->pos0, 0) - (p.window - 1)) : 0;
   w->sink_end = max(0, min(min(p.sinks, w->lo_first), w->key_end));
@@ -276,12 +282,12 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
     uint32_t n = 0, pieces = 0;  // tiles and pieces with tiles so far: phases of the barriers
     PpPiece w;
     for (int k = 0; take(k, &w); ++k) {
-      const int pos = w.pos0 + tok;
+      const int pos = pp_position(w.pos0, tok);
       const int lo = p.window > 0 ? max(pos, 0) - (p.window - 1) : 0;
-      const int tile_lo = w.pos0 + t * per_tile, tile_hi = tile_lo + per_tile - 1;  // positions of the tile
+      const int tile_lo = pp_position(w.pos0, t * per_tile), tile_hi = pp_position(tile_lo, per_tile - 1);  // positions of the tile
       // tiles [clear0, clear1) need no mask: behind the first tokens, from where every row's window has begun, up to the first row
       const int w_lo = p.window > 0 ? max(tile_hi, 0) - (p.window - 1) : 0;
-      const int clear0 = (w.sink_boxes + max(0, ((max(w_lo, 0) + a.box - 1) >> a.box_shift) - w.first_box) + (1 << tile_shift) - 1) >> tile_shift;
+      const int clear0 = (w.sink_boxes + max(0, (int)(((uint32_t)max(w_lo, 0) + a.box - 1u) >> a.box_shift) - w.first_box) + (1 << tile_shift) - 1) >> tile_shift;
       const int clear1 = (((tile_lo + 1) >> a.box_shift) + w.sink_boxes - w.first_box) >> tile_shift;
       float m = -INFINITY, l = 0.f;  // maximum that the probabilities refer to, in units of log2; their sum
       for (int i = w.i0; i < w.i1; ++i, ++n) {
@@ -685,9 +691,10 @@ inline int pp_h_shift(int group) {
   return s;
 }
 
-// Whether the tensor-core kernel takes a call: copies of 8 cache rows or more that lie in one block, and strides that its maps take.
+// Whether the tensor-core kernel takes a call: copies of 8 cache rows or more that lie in one block, a table of which every key has an
+// int, and strides that its maps take.
 inline bool paged_prefill_plan(const PagedArgs& p, int D, bool f16, int tiles, PpMaps* maps, PpArgs* a) {
-  if (p.cache.block_size % 8 != 0) return false;
+  if (p.cache.block_size % 8 != 0 || (int64_t)p.table_width * p.cache.block_size > kPpMaxKeys) return false;
   a->p = p;
   a->box = 8;
   // Short boxes where first tokens stay visible: they share a tile with the window's begin (8001 tokens, window of 1024 and 4 first

@@ -309,3 +309,44 @@ def test_refusals_leave_the_device_healthy():
     assert N.device_status() == 0
     PP.check(p, _decode(p))
     assert A.paged_decode_attention(q[:0], k, v, tables[:0], ctx[:0]).shape == (0, 8, 64)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(64, 4), (1, 40), (2 ** 31 - 21, 0), (2 ** 31 - 21, 9), (2 ** 31 - 1, 3)])
+def test_positions_next_to_two_to_the_31(window, sinks, dim):
+    """Contexts of 2^31 - 1 behind a short table: the first tokens alone, or a window whose begin lies inside the table for the last rows
+    and ahead of it for the others."""
+    last = 2 ** 31 - 1
+    for page in (8, 16):
+        p = PP.make(8, 2, dim, page, [64, 64], [150, 3], window=window, sinks=sinks, seed=dim + sinks)
+        p["contexts"] = [last, last - 40]
+        args = list(p["args"])
+        args[4] = torch.tensor(p["contexts"], dtype=torch.int32, device="cuda")
+        how = dict(scale=p["scale"], window=window, sinks=sinks, return_lse=True)
+        out, lse = A.paged_prefill_attention(*args, **how)
+        assert N.device_status() == 0
+        PP.check(p, out, lse)
+        p["q"], p["cu"] = p["q"][[149, 152]], None  # the last token of each
+        out, lse = A.paged_decode_attention(args[0][[149, 152]], *args[1:5], **how)
+        PP.check(p, out, lse)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("window", [0, 100])
+def test_tables_of_two_to_the_31_keys(window, dim):
+    """The last pages of a table of 2^31 keys, the others missing: what the same pages give alone."""
+    blocks, page, tail = 2 ** 23, 256, 3
+    near = 2 ** 31 - 1 - (blocks - tail) * page
+    p = PP.make(2, 1, dim, page, [near], [5], window=window, seed=dim)
+    q, k, v, tables, _, cu = p["args"]
+    wide = torch.full((1, blocks), -1, dtype=torch.int32, device="cuda")
+    wide[:, blocks - tail:] = tables
+    ctx = torch.tensor([2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    how = dict(scale=p["scale"], window=window, return_lse=True)
+    if window:  # (without one every row walks the whole table)
+        out, lse = A.paged_prefill_attention(q, k, v, wide, ctx, cu, **how)
+        PP.check(p, out, lse)
+    p["q"], p["cu"] = p["q"][4:], None
+    out, lse = A.paged_decode_attention(q[4:], k, v, wide, ctx, **how)
+    PP.check(p, out, lse)
+    assert N.device_status() == 0
