@@ -127,11 +127,10 @@ struct PpPiece {
   int req, pos0, held, key_end, lo_first, sink_end;  // position of the first token; keys that a row sees: [0, sink_end), [lo_first, key_end)
   int first_box, sink_boxes, i0, i1;           // the keys in boxes: those of the first tokens, then from first_box on, side by side
   int parts;                                   // 0: no more pieces; 1: the whole item; else the item is in that many parts
-  // first key of box b of tile i, with 1 << shift keys in a box; boxes from kPpMaxKeys on (of the last tile of a position next to
-  // 2^31: no table reaches them) all begin there, where the sum would no longer fit
+  // first key of box b of tile i, with 1 << shift keys in a box
   __device__ __forceinline__ int key_of(int i, int b, int shift) const {
     const int c = i * (kPpKeys >> shift) + b;
-    return (int)min((uint32_t)(c < sink_boxes ? c : c - sink_boxes + first_box) << shift, (uint32_t)kPpMaxKeys);
+    return (c < sink_boxes ? c : c - sink_boxes + first_box) << shift;
   }
 };
 
@@ -214,7 +213,8 @@ __device__ __forceinline__ void pp_find(const PpArgs& a, int span, int item, int
   w->key_end = w->held;
   w->lo_first = p.window > 0 ? max(0, max(w->pos0, 0) - (p.window - 1)) : 0;
   w->sink_end = max(0, min(min(p.sinks, w->lo_first), w->key_end));
-  w->first_box = w->lo_first >> a.box_shift;
+  // (a window behind the table's end has no box; its first one is at the end, since a key next to 2^31 and its tile need not fit an int)
+  w->first_box = min(w->lo_first, max(w->held, 0) + a.box - 1) >> a.box_shift;
   w->sink_boxes = min((w->sink_end + a.box - 1) >> a.box_shift, w->first_box);
   w->i0 = 0;
   const int boxes = w->key_end <= 0 ? 0 : w->sink_boxes + max(0, ((w->key_end + a.box - 1) >> a.box_shift) - w->first_box);
