@@ -65,6 +65,15 @@ __device__ __forceinline__ RowKeys row_keys(const PagedArgs& a, int row) {
   return r;
 }
 
+// Probabilities are 2^(score - m) of a reference m that any value near the maximum may be, since it leaves with the sum. It moves, to
+// kProbUp below the maximum, where the maximum has grown to more than kProbSlack + kProbUp above it: until then O stays as it is and
+// probabilities stay below 2^(kProbSlack + kProbUp). In fp16 they go up to 2^15 of its 2^16, so that those from 2^-21 of the largest
+// on are normal numbers and what rounding does to smaller ones is at most 2^-32 of it: keys of a long context that one outweighs by
+// 2^25 would else count in the sum and be zero in the product. (Slack 8, 6, 4 of these 15: a window of 1024 over 8001 tokens, heads of
+// 128, 91, 93, 96 us.)
+template <bool kF16> constexpr float kProbUp = kF16 ? 7.f : 0.f;
+constexpr float kProbSlack = 8.f;
+
 constexpr int kJoinThreads = 128;
 constexpr int kPagedStages = 3;
 constexpr int kPagedCtas = 2 * 148;  // of a launch, of four warps: two on every SM
@@ -340,8 +349,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
           for (int n = 0; n < NT; ++n) mma_16816<kF16>(s[n][i], kf[0], kf[1], kf[2], kf[3], qf[n][k][0], qf[n][k][1]);
         }
       }
-      // scores, masked; the maximum moves only where it would grow by more than 2^8 (probabilities stay below that)
-      bool grows = false;
+      bool grows = false;  // scores, masked
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -350,7 +358,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
           for (int x = 0; x < 4; ++x) {
             const bool seen = (live >> (16 * i + g + 8 * (x >> 1))) & 1u;
             s[n][i][x] = seen ? s[n][i][x] * a.sc : -INFINITY;
-            grows |= s[n][i][x] > m[n][x & 1] + 8.f;
+            grows |= s[n][i][x] > m[n][x & 1] + (kProbSlack + kProbUp<kF16>);
           }
       if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
@@ -359,7 +367,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
           for (int c = 0; c < 2; ++c) {
             float mx = m[n][c];
 #pragma unroll
-            for (int i = 0; i < kMT; ++i) mx = fmaxf(mx, fmaxf(s[n][i][c], s[n][i][c + 2]));
+            for (int i = 0; i < kMT; ++i) mx = fmaxf(mx, fmaxf(s[n][i][c], s[n][i][c + 2]) - kProbUp<kF16>);
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));

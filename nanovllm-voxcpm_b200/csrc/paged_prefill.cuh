@@ -99,7 +99,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// 2^x for x <= 8 or so on the FMA units: x = n + f with n whole and f in [-0.5, 0.5] (adding and subtracting 1.5 * 2^23 rounds to n), 2^f
+// 2^x for x up to 2^7 on the FMA units: x = n + f with n whole and f in [-0.5, 0.5] (adding and subtracting 1.5 * 2^23 rounds to n), 2^f
 // by a polynomial with constant term 1, least in its largest relative error (1.7e-7 in fp32; weighted least squares until the
 // extrema are even), n added to the exponent. From -127 down exactly 0.
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
       const int w_lo = p.window > 0 ? max(tile_hi, 0) - (p.window - 1) : 0;
       const int clear0 = (w.sink_boxes + max(0, (int)(((uint32_t)max(w_lo, 0) + a.box - 1u) >> a.box_shift) - w.first_box) + (1 << tile_shift) - 1) >> tile_shift;
       const int clear1 = (((tile_lo + 1) >> a.box_shift) + w.sink_boxes - w.first_box) >> tile_shift;
-      float m = -INFINITY, l = 0.f;  // maximum that the probabilities refer to, in units of log2; their sum
+      float m = -INFINITY, l = 0.f;  // what the probabilities refer to, in units of log2; their sum
       for (int i = w.i0; i < w.i1; ++i, ++n) {
         pp_wait(bar(S_READY + t), n & 1, &abort_flag);
         tc_fence_after_sync();
@@ -330,16 +330,15 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
           mbar_arrive(bar(S_TAKEN));
         }
         const float mx = max3(max3(top4[0], top4[1], top4[2]), top4[3], top4[3]);
-        // The maximum moves only where it would grow by more than 2^8: until then probabilities stay below that, and O as it is.
         const float top = mx * p.sc;
-        const bool grows = !(top <= m + 8.f);  // (a NaN among the scores makes the maximum and with it the whole row NaN)
+        const bool grows = !(top <= m + (kProbSlack + kProbUp<kF16>));  // (a NaN among the scores makes the maximum and with it the whole row NaN)
         if (kOwnP && n > 0) {  // P and O of the tile before are done with
           pp_wait(bar(PV_DONE), (n - 1) & 1, &abort_flag);
           tc_fence_after_sync();
         }
         if (__any_sync(0xffffffffu, grows)) {
-          const float f = grows ? ex2(m - top) : 1.f;
-          if (grows) m = top;
+          const float up = top - kProbUp<kF16>, f = grows ? ex2(m - up) : 1.f;
+          if (grows) m = up;
           l *= f;
           if (i > w.i0) {  // (if P lies in S: S of this tile came behind P V of the one before, O is complete)
 #pragma unroll

@@ -350,3 +350,33 @@ def test_tables_of_two_to_the_31_keys(window, dim):
     out, lse = A.paged_decode_attention(q[4:], k, v, wide, ctx, **how)
     PP.check(p, out, lse)
     assert N.device_status() == 0
+
+
+@pytest.mark.parametrize("prefill", [False, True])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("spread", [0.0, 3.0])
+def test_one_key_outweighs_a_long_context(spread, dim, prefill):
+    """One key with 2^25 to 2^26 times the weight of any other of 60000, and a value of zero: the result is what the others add up to.
+    Roundings in fp16: u of every probability (those from 2^-21 of the largest on are normal numbers) or, below that, 2^-32 of the largest;
+    their sum is not rounded, the result once. The rest as in ``paged_problem.check``: scores are one product here (2^-24 of at most 20,
+    twice), exponentials and running sums 2^-18 and keys 2^-23."""
+    n = 60000
+    p = PP.make(2, 1, dim, 64, [n], [2] if prefill else None, dtype=FP16, seed=3)
+    flat = torch.tensor(p["tables"][0])
+    k, v = torch.zeros_like(p["k"]), torch.rand(p["v"].shape, generator=torch.Generator().manual_seed(1)).add_(0.5).to(FP16)
+    k[..., 1] = (torch.rand(k.shape[:3], generator=torch.Generator().manual_seed(2)) * -spread).to(FP16)
+    k[flat[0], 0, 0, 0], k[flat[0], 0, 0, 1], v[flat[0], 0] = 8.0, 0.0, 0.0
+    q = torch.zeros_like(p["q"])
+    q[..., 0] = 17.5 / 8 / p["scale"]
+    q[..., 1] = 0.25 / p["scale"]
+    p.update(q=q, k=k, v=v)
+    args = [q.cuda(), k.cuda(), v.cuda(), *p["args"][3:]]
+    out, lse = (A.paged_prefill_attention if prefill else A.paged_decode_attention)(*args, scale=p["scale"], return_lse=True)
+    want, want_lse, size, _ = PP.PO.paged_attention(q, k, v, p["tables"], p["contexts"], p["cu"], p["scale"], 0, 0)
+    assert float(want.min()) > 5e-4
+    u = 2.0 ** -11
+    eps = 2 * 20 * 2.0 ** -24 + 2.0 ** -18 + n * 2.0 ** -23
+    bound = u * want + (u * (1 + u) + eps) * size + n * 2.0 ** -32 * 1.5
+    err = (out.double().cpu() - want).abs()
+    assert bool((err <= bound).all()), f"worst {float((err / bound).max()):.3g} of the bound, {float((err / want).max()):.3g} of the result"
+    assert bool(((lse.double().cpu() - want_lse).abs() <= 20 * 2.0 ** -24 + 2.0 ** -19 * 20 + n * 2.0 ** -24).all())
