@@ -108,4 +108,6 @@ def paged_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     ``paged_decode_attention``. Block sizes that are multiples of 8 go to the tensor-core kernel, others (and tables of 2^31 keys) to the
     decode kernel, a token at a time. A value that is not finite, of a key that some tokens of a block of a few see, may reach the block's other tokens; what no
     token of the block sees (stale rows, returned blocks) never does."""
+    if cu_seqlens is None:
+        raise ValueError("cu_seqlens says which rows of q are whose: paged_prefill_attention needs it")
     return _paged_attention(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, scale, window, sinks, out, return_lse)

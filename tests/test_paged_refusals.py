@@ -120,3 +120,10 @@ def test_decoder_config_refuses_what_attention_does():
     for kw in (dict(sliding_window=-1), dict(sink_tokens=-1, sliding_window=4), dict(sink_tokens=2)):
         with pytest.raises(ValueError):
             DecoderConfig(**kw)
+
+
+def test_prefill_without_cu_seqlens_is_refused_by_name():
+    """As many rows as requests would pass for a decode batch otherwise."""
+    q, k = torch.zeros(2, 16, 64, dtype=torch.bfloat16), torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        A.paged_prefill_attention(q, k, k, torch.zeros(2, 4, dtype=torch.int32), torch.ones(2, dtype=torch.int32), None)
