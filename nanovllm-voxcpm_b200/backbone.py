@@ -136,6 +136,10 @@ class DecoderAttention(nn.Module):
         cfg = self.cfg
         how = dict(scale=cfg.head_dim ** -0.5, window=cfg.sliding_window, sinks=cfg.sink_tokens)
         nd = step.n_decode if step.is_prefill else q.size(0)
+        needs = ("prefill_context_lens", "prefill_block_tables", "cu_seqlens") if step.is_prefill else ()
+        for name in (("context_lens", "block_tables") if nd else ()) + needs:
+            if getattr(step, name) is None:
+                raise ValueError(f"attention over the paged cache (DecoderConfig.paged_attention, sliding_window) needs AttentionStep.{name}")
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         if nd:
             A.paged_decode_attention(q[:nd], self.k_cache, self.v_cache, step.block_tables, step.context_lens, out=out[:nd], **how)

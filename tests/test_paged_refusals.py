@@ -127,3 +127,22 @@ def test_prefill_without_cu_seqlens_is_refused_by_name():
     q, k = torch.zeros(2, 16, 64, dtype=torch.bfloat16), torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="cu_seqlens"):
         A.paged_prefill_attention(q, k, k, torch.zeros(2, 4, dtype=torch.int32), torch.ones(2, dtype=torch.int32), None)
+
+
+@pytest.mark.parametrize("missing", ["prefill_context_lens", "prefill_block_tables", "cu_seqlens", "context_lens", "block_tables"])
+def test_steps_without_what_paged_attention_needs(missing):
+    from nanovllm_voxcpm_b200 import backbone as BB
+
+    cfg = BB.DecoderConfig(hidden_size=128, num_heads=2, num_kv_heads=1, head_dim=64, intermediate_size=128, num_layers=1, max_loras=2,
+                           max_lora_rank=16, max_position=64, sliding_window=8)
+    layer = BB.DecoderAttention(cfg)
+    ints = torch.ones(1, dtype=torch.int32)
+    step = BB.AttentionStep(True, torch.arange(3), cu_seqlens=torch.tensor([0, 2], dtype=torch.int32), max_seqlen=2, context_lens=ints,
+                            block_tables=ints.view(1, 1), n_decode=1, prefill_context_lens=2 * ints, prefill_block_tables=ints.view(1, 1))
+    setattr(step, missing, None)
+    with pytest.raises(ValueError, match=missing):
+        layer._attend_paged(torch.zeros(3, 2, 64, dtype=torch.bfloat16), step)
+    if missing in ("context_lens", "block_tables"):
+        with pytest.raises(ValueError, match=missing):
+            layer._attend_paged(torch.zeros(1, 2, 64, dtype=torch.bfloat16), BB.AttentionStep(False, torch.arange(1), **{
+                "context_lens": ints, "block_tables": ints.view(1, 1), missing: None}))
