@@ -494,6 +494,11 @@ size_t lora_b200_paged_decode_workspace_bytes(int32_t T, int32_t num_heads, int3
                                               int32_t table_width, int32_t block_size, int32_t window, int32_t sinks);
 size_t lora_b200_paged_prefill_workspace_bytes(int32_t T, int32_t n_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                                                int32_t table_width, int32_t block_size, int32_t window);
+/* How a decode call meets the GPU: CTAs that take an item (a row, a kv head and up to 16 of its heads) together, 1, 2, 4 or 8, times 16,
+ * plus the warps of a CTA, 4 or 8; 0: equal shares of all blocks of keys, joined by a second launch (with the workspace). Host code, for
+ * tests and tuning. No counterpart in the reference. */
+int32_t lora_b200_paged_decode_way(int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t table_width,
+                                   int32_t block_size, int32_t window, int32_t sinks);
 int lora_b200_paged_decode_attention(void* out, int64_t out_token, int64_t out_head, float* lse, const void* q, int64_t q_token,
                                      int64_t q_head, int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                                      const lora_b200_paged_cache* cache, const int32_t* block_tables, int64_t table_ld,

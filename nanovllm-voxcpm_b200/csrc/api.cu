@@ -369,6 +369,13 @@ size_t lora_b200_paged_prefill_workspace_bytes(int32_t T, int32_t n_seqs, int32_
   return paged_prefill_workspace_bytes(T, n_seqs, num_heads, num_kv_heads, head_dim, block_size, (int64_t)table_width * block_size, window);
 }
 
+int32_t lora_b200_paged_decode_way(int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t table_width,
+                                   int32_t block_size, int32_t window, int32_t sinks) {
+  if (num_kv_heads < 1 || num_heads < num_kv_heads) return fail(B200_LORA_EINVAL, "paged_decode_way: %d heads over %d kv heads", num_heads, num_kv_heads);
+  const PagedWay w = paged_way(T, num_heads, num_kv_heads, head_dim, (int64_t)table_width * block_size, window, sinks);
+  return w.shares ? 0 : 16 * w.cluster + w.warps;
+}
+
 // What decode and prefill have in common; cu_seqlens null: decode
 static int paged_attention_checked(const char* what, void* out, int64_t out_token, int64_t out_head, float* lse, const void* q, int64_t q_token,
                                    int64_t q_head, int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
