@@ -482,8 +482,8 @@ int lora_b200_glue_qk_norm_rope_kv_store(void* qkv, int64_t qkv_ld, int32_t T, i
  *                caller may have given the block back), as are keys behind the table. Entries of blocks without a seen key are not used
  *  context_lens  int32 [n_seqs]: tokens of the sequence, the new ones included (< 0: none)
  * decode:  T = n_seqs, token t is the last of its sequence.
- * prefill: the tokens [cu_seqlens[i], cu_seqlens[i + 1]) of q are the last ones of sequence i (cu_seqlens ascending); rows of out
- *          (and lse) outside [cu_seqlens[0], cu_seqlens[n_seqs]) are left as they are.
+ * prefill: the tokens [cu_seqlens[i], cu_seqlens[i + 1]) of q are the last ones of sequence i (cu_seqlens ascending; a range that
+ *          leaves the T rows counts as none); rows of out (and lse) of no sequence are left as they are.
  * head_dim 64 or 128, scale > 0, bf16 and fp16. workspace: device memory of the number of bytes that
  * lora_b200_paged_decode_workspace_bytes / _prefill_workspace_bytes give (0: none, null will do), 16-byte aligned, of this call alone until it has run. Counterpart in the reference: the two calls over the
  * paged cache in Attention.forward (nanovllm_voxcpm/layers/attention.py:70-79); it has no window.

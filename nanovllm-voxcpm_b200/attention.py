@@ -102,12 +102,12 @@ def paged_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
                             context_lens: torch.Tensor, cu_seqlens: torch.Tensor, *, scale: float | None = None, window: int = 0,
                             sinks: int = 0, out: torch.Tensor | None = None, return_lse: bool = False):
     """Packed new tokens: rows ``cu_seqlens[i] : cu_seqlens[i + 1]`` of ``q [tokens, heads, head_dim]`` are the last tokens of
-    request ``i``, whose ``context_lens[i]`` counts them; keys and values of all of them are in the cache already. Every token
-    sees what ``paged_decode_attention`` would show it at its position. Rows of ``out`` (and of
-    the log sums) before the first and behind the last sequence are not written: a given ``out`` keeps them. Other arguments as
+    request ``i``, whose ``context_lens[i]`` counts them (ascending; a range that leaves the rows of q counts as none); keys and values
+    of all of them are in the cache already. Every token sees what ``paged_decode_attention`` would show it at its position. Rows of
+    ``out`` (and of the log sums) of no sequence are not written: a given ``out`` keeps them. Other arguments as
     ``paged_decode_attention``. Block sizes that are multiples of 8 go to the tensor-core kernel, others (and tables of 2^31 keys) to the
-    decode kernel, a token at a time. A value that is not finite, of a key that some tokens of a block of a few see, may reach the block's other tokens; what no
-    token of the block sees (stale rows, returned blocks) never does."""
+    decode kernel, a token at a time. A value that is not finite, of a key that some tokens of a block of a few see, may reach the
+    block's other tokens; what no token of the block sees (stale rows, returned blocks) never does."""
     if cu_seqlens is None:
         raise ValueError("cu_seqlens says which rows of q are whose: paged_prefill_attention needs it")
     return _paged_attention(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, scale, window, sinks, out, return_lse)

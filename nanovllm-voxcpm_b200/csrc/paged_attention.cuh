@@ -53,8 +53,10 @@ __device__ __forceinline__ RowKeys row_keys(const PagedArgs& a, int row) {
       if (a.cu_seqlens[mid] <= row) lo = mid;
       else hi = mid;
     }
+    const int begin = a.cu_seqlens[lo], end = a.cu_seqlens[lo + 1];
+    if (begin < 0 || end > a.T) return r;  // (a range that leaves the rows of q counts as none)
     r.req = lo;
-    ctx = (int64_t)a.context_lens[lo] - (a.cu_seqlens[lo + 1] - 1 - row);
+    ctx = (int64_t)a.context_lens[lo] - (end - 1 - row);
   }
   ctx = ctx < 0 ? 0 : ctx;
   const int64_t held = min(ctx, (int64_t)a.table_width * a.cache.block_size);
