@@ -1,5 +1,7 @@
 // C ABI of the B200 multi-LoRA library: argument checks + kernel dispatch.
 // Declarations and the reference interface each entry point replaces: include/b200_lora.h
+#include <cmath>
+
 #include "common.cuh"
 #include "generic.cuh"
 #include "bgmv_fused.cuh"
@@ -387,7 +389,8 @@ static int paged_attention_checked(const char* what, void* out, int64_t out_toke
     return fail(B200_LORA_EINVAL, "%s: T=%d, %d sequences, %d table entries, window %d, sinks %d", what, T, n_seqs, table_width, window, sinks);
   if (num_kv_heads < 1 || num_heads < 1 || num_heads % num_kv_heads != 0)
     return fail(B200_LORA_EINVAL, "%s: %d heads over %d kv heads", what, num_heads, num_kv_heads);
-  if (!(scale > 0.f) || scale > 3.0e38f) return fail(B200_LORA_EINVAL, "%s: scale must be positive and finite", what);
+  const float sc = scale * 1.4426950408889634f;  // log2(e)
+  if (!(scale > 0.f) || !std::isfinite(sc)) return fail(B200_LORA_EINVAL, "%s: scale must be positive and finite, in units of log2 too", what);
   if (dtype != B200_LORA_BF16 && dtype != B200_LORA_F16) return fail(B200_LORA_EUNSUPPORTED, "%s: bf16 and fp16 only", what);
   if (head_dim != 64 && head_dim != 128) return fail(B200_LORA_EUNSUPPORTED, "%s: head_dim %d (64 and 128 only)", what, head_dim);
   if (T == 0 || n_seqs == 0) return B200_LORA_OK;
@@ -405,7 +408,7 @@ static int paged_attention_checked(const char* what, void* out, int64_t out_toke
   a.q = q; a.q_token = q_token; a.q_head = q_head; a.out = out; a.out_token = out_token; a.out_head = out_head; a.lse = lse;
   a.cache = *cache; a.tables = block_tables; a.table_ld = table_ld; a.table_width = table_width; a.context_lens = context_lens;
   a.cu_seqlens = cu_seqlens; a.n_req = n_seqs; a.T = T; a.Hq = num_heads; a.Hk = num_kv_heads; a.window = window; a.sinks = sinks;
-  a.sc = scale * 1.4426950408889634f;
+  a.sc = sc;
   if (prefill) return paged_prefill_launch(a, head_dim, dtype, need > 0 ? workspace : nullptr, static_cast<cudaStream_t>(stream));
   return paged_decode_launch(a, head_dim, dtype, need > 0 ? workspace : nullptr, static_cast<cudaStream_t>(stream));
 }

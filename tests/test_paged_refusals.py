@@ -146,3 +146,10 @@ def test_steps_without_what_paged_attention_needs(missing):
         with pytest.raises(ValueError, match=missing):
             layer._attend_paged(torch.zeros(1, 2, 64, dtype=torch.bfloat16), BB.AttentionStep(False, torch.arange(1), **{
                 "context_lens": ints, "block_tables": ints.view(1, 1), missing: None}))
+
+
+@pytest.mark.parametrize("call", [_decode, _prefill])
+def test_scales_that_overflow_in_units_of_log2(call):
+    """Scores are kept in units of log2: a scale that is finite, but not times log2(e), would turn scores of zero into NaN."""
+    assert call(scale=2.9e38) == N.E_INVAL and call(scale=2.4e38) == N.E_INVAL and b"log2" in N.lib().lora_b200_last_error()
+    assert call(scale=2.3e38, T=0) == 0
