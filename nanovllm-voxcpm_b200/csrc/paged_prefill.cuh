@@ -680,7 +680,7 @@ inline bool pp_cache_map(CUtensorMap* out, const lora_b200_paged_cache& c, bool 
   const cuuint64_t strides[3] = {(cuuint64_t)(inner ? (Hk == 1 ? D : head) : token) * 2, (cuuint64_t)(inner ? token : head) * 2,
                                  (cuuint64_t)(c.num_blocks == 1 ? (int64_t)c.block_size * Hk * D : block) * 2};
   const cuuint32_t b[4] = {64, (cuuint32_t)(inner ? 1 : box), (cuuint32_t)(inner ? box : 1), 1};
-  return head >= 0 && token >= 0 && block >= 0 && pp_map(out, v ? c.v : c.k, f16, 4, dims, strides, b);
+  return (Hk == 1 || head > 0) && (c.block_size == 1 || token > 0) && (c.num_blocks == 1 || block > 0) && pp_map(out, v ? c.v : c.k, f16, 4, dims, strides, b);
 }
 
 // Heads of a tile, as a power of two: they divide a group
@@ -691,7 +691,7 @@ inline int pp_h_shift(int group) {
 }
 
 // Whether the tensor-core kernel takes a call: copies of 8 cache rows or more that lie in one block, a table of which every key has an
-// int, and strides that its maps take.
+// int, and strides that its maps take (not 0, as of heads that are expanded from one).
 inline bool paged_prefill_plan(const PagedArgs& p, int D, bool f16, int tiles, PpMaps* maps, PpArgs* a) {
   if (p.cache.block_size % 8 != 0 || (int64_t)p.table_width * p.cache.block_size > kPpMaxKeys) return false;
   a->p = p;
@@ -710,7 +710,7 @@ inline bool paged_prefill_plan(const PagedArgs& p, int D, bool f16, int tiles, P
   const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)p.Hq, (cuuint64_t)p.T};
   const cuuint64_t strides[2] = {(cuuint64_t)(p.Hq == 1 ? D : p.q_head) * 2, (cuuint64_t)(p.T == 1 ? (int64_t)p.Hq * D : p.q_token) * 2};
   const cuuint32_t box[3] = {64, 1u << a->h_shift, (cuuint32_t)per_tile};
-  return p.q_head >= 0 && p.q_token >= 0 && pp_map(&maps->q, p.q, f16, 3, dims, strides, box) &&
+  return (p.Hq == 1 || p.q_head > 0) && (p.T == 1 || p.q_token > 0) && pp_map(&maps->q, p.q, f16, 3, dims, strides, box) &&
          pp_cache_map(&maps->k, p.cache, false, p.Hk, D, a->box, f16, &a->k_heads_inner) &&
          pp_cache_map(&maps->v, p.cache, true, p.Hk, D, a->box, f16, &a->v_heads_inner);
 }

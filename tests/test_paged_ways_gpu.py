@@ -280,3 +280,55 @@ def test_prefill_ranges_that_do_not_count(page, dim):
         for a, b in stay:
             assert bool((out[a:b] == 7).all()), bad
     assert N.device_status() == 0
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads_first", [False, True])
+def test_prefill_expanded_and_transposed(heads_first, dim):
+    """q with heads ahead of tokens; one query row, one kv head or one block that stands for many."""
+    p = PP.make(8, 2, dim, 16, [90, 200], [40, 33], seed=dim)
+    q, k, v, *rest = p["args"]
+    if heads_first:
+        q = q.transpose(0, 1).contiguous().transpose(0, 1)
+    want = A.paged_prefill_attention(q, k, v, *rest, **_how(p))
+    PP.check(p, want)
+    one = k[:, :, :1].expand_as(k), v[:, :, :1].expand_as(v)
+    q1 = q[:1].expand_as(q)
+    for args, same in (((q, *one), (q, *(x.contiguous() for x in one))), ((q1, k, v), (q1.contiguous(), k, v)),
+                       ((q, k[:1].expand_as(k), v), (q, k[:1].expand_as(k).contiguous(), v))):
+        p["q"], p["k"], p["v"] = (x.cpu() for x in same)
+        PP.check(p, A.paged_prefill_attention(*args, *rest, **_how(p)))
+        PP.check(p, A.paged_prefill_attention(*same, *rest, **_how(p)))
+    assert N.device_status() == 0
+
+
+@pytest.mark.parametrize("heads,contexts,new,keys", [((16, 2, 64), [5000], None, 23000), ((16, 2, 64), [2000, 5], None, 0), ((32, 8, 128), [700] * 40, None, 0),
+                                                     ((16, 2, 64), [70, 900, 33], [70, 300, 1], 0), ((16, 2, 128), [3000, 40], [20, 40], 9000), ((8, 2, 64), [90, 61], [90, 33], 0)])
+def test_results_in_place_of_the_queries(heads, contexts, new, keys):
+    p = PP.make(*heads, 32, contexts, new, seed=len(contexts), behind=0 if new is None else 1)
+    args, call = _widened(p, keys), A.paged_decode_attention if new is None else A.paged_prefill_attention
+    rows = slice(0, len(contexts) if new is None else sum(new))
+    want, want_lse = call(*args, **_how(p), return_lse=True)
+    for _ in range(5):
+        q = args[0].clone()
+        out, lse = call(q, *args[1:], **_how(p), out=q, return_lse=True)
+        assert out is q and torch.equal(q[rows], want[rows]) and torch.equal(lse[rows], want_lse[rows])
+        assert torch.equal(q[rows.stop:], args[0][rows.stop:])
+
+
+def test_large_calls_on_two_streams():
+    """Cut prefills, shares of decodes and stores next to one another, each with tensors of its own stream."""
+    ps = [PP.make(16, 2, 64, 64, [7000, 900], [90, 33], seed=1), PP.make(16, 2, 64, 64, [23500, 40], seed=2), PP.make(16, 2, 128, 64, [9000], [300], seed=3)]
+    calls = [A.paged_prefill_attention, A.paged_decode_attention, A.paged_prefill_attention]
+    want = [c(*p["args"], **_how(p)) for c, p in zip(calls, ps)]
+    streams = [torch.cuda.Stream() for _ in ps]
+    torch.cuda.synchronize()
+    got = [[] for _ in ps]
+    for _ in range(10):
+        for i, (c, p, s) in enumerate(zip(calls, ps, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(c(*p["args"], **_how(p)))
+    torch.cuda.synchronize()
+    for w, gs in zip(want, got):
+        assert all(torch.equal(g, w) for g in gs)
+    assert N.device_status() == 0
