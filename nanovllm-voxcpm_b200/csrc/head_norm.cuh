@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(kRopeThreads) head_norm_kernel(const HeadNormP
 
 // Many tokens: the rows of `tokens` tokens and their table rows come by bulk copies into one of two stages while the other is
 // worked on, three CTAs on an SM; a thread keeps the angles and weights of its columns for all heads of its token that it takes.
-constexpr int kHeadCtas = 3;  // on an SM (8192 wide tokens: 43 us with two, 41 with three, 59 with four, whose registers spill)
+constexpr int kHeadCtas = 3;  // on an SM (8192 wide tokens: 43 us with two, 41 with three, 59 with four; ptxas spills one word of three's 80 registers, many of four's 64)
 struct HeadRing { int tokens, row_bytes, table_bytes, stage_bytes; };
 
 template <typename T, int lane_shift>

@@ -9,8 +9,10 @@
 // mma.sync, since eight or sixteen heads do not fill a tcgen05 tile and the arithmetic is a few per cent of the time.
 // Measured (bytes that must be read, of the measured copy bandwidth): 256 requests of 1000 tokens, 32 / 8 heads of 128, 173 us (93 %); 48 of
 // 500 to 8192 139 us (87 %); one of 100003 79 us (79 %: 62.5 at the bandwidth, the rest is the sums over the rows, the first
-// blocks and the join); 64 of 2000, 16 / 2 of 128, 27 us (74 %); 64 of 128 to 1024, 16 / 2 of 64, 8.7 us (31 %: eight blocks a warp of
-// the longest request, 0.6 us each, behind 3.5 us of launch, look-ups and join).
+// blocks and the join); 64 of 2000, 16 / 2 of 128, 27 us (74 %); 128 with a window of 1024, 16 / 2 of 128, 28 us (71 %: 64 to 148 such
+// requests 16.9 to 31.5 us, which is 6.0 TB/s behind 5.7 us of launch, first blocks and join); 64 of 128 to 1024, 16 / 2 of 64, 8.2 us
+// (33 %: bound by the longest request, whose eight warps have four blocks each, 1.3 us a block behind 3.9 us of launch, look-ups and
+// join; 38 requests of 1024 each take 9.0 us, 64 9.3; of 512 6.6 and 6.9, of 256 4.9 and 5.3, of 32 3.9 and 4.0).
 #pragma once
 
 #include <atomic>

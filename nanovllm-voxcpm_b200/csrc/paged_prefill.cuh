@@ -12,9 +12,11 @@
 // Bound: the products where contexts are long, else the chain S - softmax - P V of a tile. A pair of tiles of heads of 128 takes 3000
 // cycles where its products take 2048, of which a row's softmax is 2000 (128 exponentials, latency of tensor memory, one warp to a
 // scheduler at a time). Measured: 8192 tokens, 16 / 2 heads of 128, 228 us = 1.20 PFLOP/s (0.73 of the measured GEMM rate), heads of 64
-// 190 to 205 us (0.44); 4096 behind 12288, 32 / 8 of 128, 760 us = 1.27 PFLOP/s (870 among other work, at the clock that the power cap
-// leaves); 8001 tokens with a window of 1024, 16 / 2 of 128, 89 us = 0.71 PFLOP/s (an item is nine tiles of 1.8 us and 5 us of its own;
-// four waves of items where 3.4 would do); 12 prompts of 100 to 1000, heads of 64, 35 us.
+// 190 to 205 us (0.44); 4096 behind 12288, 32 / 8 of 128, 875 us = 1.10 PFLOP/s one after another, at the clock that the power cap leaves
+// (760 us, 1.27 PFLOP/s, alone); 8001 tokens with a window of 1024, 16 / 2 of 128, 90 us = 0.70 PFLOP/s: 22.6 us for a wave of 148 items
+// behind 6.3 us (2368, 4736 and 7104 tokens are one to three waves: 28.9, 51.5 and 74.1 us), and of 3.4 waves the last costs 17; 12
+// prompts of 100 to 1200, heads of 64, 37 us: 3.3 us, then 1.8 us a tile (the other CTA of the SM at work too; 1.4 alone) and 2.7 us an
+// item, of which the fullest CTA has 13 tiles in 3 items (960 items of 3.4 tiles; 12 equal prompts of 16 to 1200 tokens fit within 2 us).
 #pragma once
 
 #include "paged_attention.cuh"
@@ -169,7 +171,8 @@ __device__ __forceinline__ int pp_items(const PpArgs& a, int span, const PpLane&
 }
 
 // Item `item` of the n_items, longest contexts first as far as one warp can tell (up to 32 requests: blocks by the position that
-// they end at; more: the last block of the last sequence first), the sets of heads of a block one after another. A whole warp calls
+// they end at; more: the last block of the last sequence first; 32 requests of 30 to 400 tokens, heads of 64, 27.2 us, 33 of them 33.3;
+// of 100 each 13.9 and 14.5), the sets of heads of a block one after another. A whole warp calls
 // it, with the first 32 requests in hand.
 __device__ __forceinline__ void pp_find(const PpArgs& a, int span, int item, int n_items, const PpLane& lanes0, PpPiece* w) {
   const PagedArgs& p = a.p;
