@@ -511,6 +511,36 @@ int lora_b200_paged_prefill_attention(void* out, int64_t out_token, int64_t out_
                                       int32_t n_seqs, float scale, int32_t window, int32_t sinks, int32_t dtype,
                                       void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Differential attention over a paged cache: the halves of a head's columns of q and k (head_dim / 2 each) make two softmax maps over
+ * the same keys, and with S1, S2 their results over the whole columns of v
+ *   out[t, h] = S1 - lam[t, h] * S2,  with norm_weight: y / sqrt(mean(y^2) + eps) * norm_weight, y that difference
+ * (fp32 throughout, rounded once). lam float, [T, num_heads] by strides in elements (0: one for all); norm_weight [head_dim] of the
+ * type of q, 16-byte aligned, or null. A token without a visible key gives zeros. cu_seqlens null: decode (n_seqs = T), else packed
+ * as lora_b200_paged_prefill_attention; everything else as there. packed (of the workspace's size): with cu_seqlens.
+ * No counterpart in the reference (Ye et al., "Differential Transformer", 2024).
+ */
+size_t lora_b200_differential_workspace_bytes(int32_t T, int32_t n_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                              int32_t table_width, int32_t block_size, int32_t window, int32_t sinks, int32_t packed);
+int lora_b200_differential_attention(void* out, int64_t out_token, int64_t out_head, const void* q, int64_t q_token, int64_t q_head,
+                                     int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                     const lora_b200_paged_cache* cache, const int32_t* block_tables, int64_t table_ld,
+                                     int32_t table_width, const int32_t* context_lens, const int32_t* cu_seqlens, int32_t n_seqs,
+                                     const float* lam, int64_t lam_token, int64_t lam_head, const void* norm_weight, float eps,
+                                     float scale, int32_t window, int32_t sinks, int32_t dtype, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
+/*
+ * Joins attention over n_parts (up to 64) parts of a context: outs[i] [T, num_heads, head_dim] and lses[i] float [T, num_heads] are a
+ * part's result and the logarithm of its sum (as the calls above give them; -inf: no key, its values count for nothing), host arrays
+ * of device addresses, the strides (in elements) the same for all parts. out = the result over all of them, lse [T, num_heads] the
+ * logarithm of the whole sum, or null. bf16, fp16, fp32; rows of head_dim adjacent elements that start on 16-byte boundaries. out may
+ * be one of the parts. No counterpart in the reference.
+ */
+int lora_b200_join_attention(void* out, int64_t out_token, int64_t out_head, float* lse, const void* const* outs, const float* const* lses,
+                             int32_t n_parts, int64_t part_token, int64_t part_head, int64_t lse_token, int64_t lse_head, int32_t T,
+                             int32_t num_heads, int32_t head_dim, int32_t dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -149,6 +149,20 @@ _SIGNATURES = {
         [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, POINTER(PagedCache),
          c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_int32, c_float, c_int32, c_int32, c_int32, c_void_p, c_size_t, c_void_p],
     ),
+    "lora_b200_differential_workspace_bytes": (
+        c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32],
+    ),
+    "lora_b200_differential_attention": (
+        c_int32,
+        [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, POINTER(PagedCache), c_void_p, c_int64,
+         c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_float, c_float, c_int32, c_int32, c_int32, c_void_p,
+         c_size_t, c_void_p],
+    ),
+    "lora_b200_join_attention": (
+        c_int32,
+        [c_void_p, c_int64, c_int64, c_void_p, POINTER(c_void_p), POINTER(c_void_p), c_int32, c_int64, c_int64, c_int64, c_int64, c_int32,
+         c_int32, c_int32, c_int32, c_void_p],
+    ),
     "lora_b200_tp_allreduce": (
         c_int32, [c_void_p, c_void_p, c_int32, POINTER(c_void_p), c_int32, c_int32, c_int32, c_void_p],
     ),

@@ -2,8 +2,10 @@
 of every request (``paged_decode_attention``) or packed runs of new tokens (``paged_prefill_attention``: whole prompts, chunks of
 them, a few tokens behind a long context). Causal, over everything or over a sliding window of the last keys plus a few first
 ones. Stands where the reference attends over its paged cache
-(``nanovllm_voxcpm/layers/attention.py:70-79``); the kernels are ``csrc/paged_attention.cuh`` and ``csrc/paged_prefill.cuh`` behind
-``lora_b200_paged_*``.
+(``nanovllm_voxcpm/layers/attention.py:70-79``). Besides: the difference of two softmax maps (``differential_decode_attention``,
+``differential_prefill_attention``), and what joins results over parts of a context (``join_attention``). The kernels are
+``csrc/paged_attention.cuh``, ``csrc/paged_prefill.cuh`` and ``csrc/attention_join.cuh`` behind ``lora_b200_paged_*``,
+``lora_b200_differential_attention`` and ``lora_b200_join_attention``.
 CUDA tensors only, bf16 / fp16, heads of 64 or 128; there is no fallback path and no backward pass.
 """
 
@@ -24,20 +26,13 @@ def _int32(t: torch.Tensor, name: str, shape: tuple) -> torch.Tensor:
     return t
 
 
-def _paged_attention(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, scale, window, sinks, out, return_lse):
-    if scale is None:
-        scale = q.size(-1) ** -0.5
-    got = N.native().paged_attention(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, scale, window, sinks, out,
-                                     bool(return_lse))
-    if got is not None:
-        N.check(got[0])
-        return (got[1], got[2]) if return_lse else got[1]
-    # what the compiled path leaves: a tensor on another device than the current one, or something to refuse
-    N.require_cuda(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, out)
+def _checked(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, scale, window, sinks, out, *others) -> N.PagedCache:
+    """The checks that the compiled path leaves to be named: it takes tensors on the current device and gives back the rest."""
+    N.require_cuda(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, out, *others)
     if q.dim() != 3 or q.stride(2) != 1:
         raise ValueError("q must be [tokens, heads, head_dim] with adjacent elements in a head")
-    T, heads, dim = q.shape
-    cache = paged_cache(k_cache, v_cache, q.dtype, None, dim)
+    T = q.size(0)
+    cache = paged_cache(k_cache, v_cache, q.dtype, None, q.size(2))
     if context_lens.dim() != 1 or not context_lens.is_contiguous():
         raise ValueError("context_lens must be a contiguous vector")
     n = context_lens.numel()
@@ -59,9 +54,24 @@ def _paged_attention(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens
         raise ValueError("sinks are the first tokens outside a window: they need one")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1):
         raise ValueError("out must have the shape and dtype of q, and adjacent elements in a head")
-    devices = {t.device for t in (q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, out) if t is not None}
+    devices = {t.device for t in (q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, out, *others) if t is not None}
     if len(devices) > 1:
         raise ValueError(f"tensors on several devices: {sorted(map(str, devices))}")
+    return cache
+
+
+def _paged_attention(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, scale, window, sinks, out, return_lse):
+    if scale is None:
+        scale = q.size(-1) ** -0.5
+    got = N.native().paged_attention(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, scale, window, sinks, out,
+                                     bool(return_lse))
+    if got is not None:
+        N.check(got[0])
+        return (got[1], got[2]) if return_lse else got[1]
+    # what the compiled path leaves: a tensor on another device than the current one, or something to refuse
+    cache = _checked(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, scale, window, sinks, out)
+    T, heads, dim = q.shape
+    n = context_lens.numel()
     with N.on_device(q.device):
         if out is None:
             out = torch.empty(T, heads, dim, dtype=q.dtype, device=q.device)
@@ -111,3 +121,99 @@ def paged_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     if cu_seqlens is None:
         raise ValueError("cu_seqlens says which rows of q are whose: paged_prefill_attention needs it")
     return _paged_attention(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, scale, window, sinks, out, return_lse)
+
+
+def _differential(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, lam, norm_weight, eps, scale, window, sinks, out):
+    if scale is None:
+        scale = (q.size(-1) // 2) ** -0.5
+    got = N.native().differential_attention(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, lam, norm_weight, eps, scale,
+                                            window, sinks, out)
+    if got is not None:
+        N.check(got[0])
+        return got[1]
+    cache = _checked(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, scale, window, sinks, out, lam, norm_weight)
+    T, heads, dim = q.shape
+    if lam.dtype != torch.float32 or tuple(lam.shape) not in ((heads,), (T, heads)):
+        raise ValueError(f"lam must be a float32 tensor [heads] or [tokens, heads], got {lam.dtype} {tuple(lam.shape)}")
+    if norm_weight is not None:
+        if norm_weight.dtype != q.dtype or tuple(norm_weight.shape) != (dim,) or not norm_weight.is_contiguous():
+            raise ValueError("norm_weight must be a contiguous [head_dim] vector of the dtype of q")
+        if not (math.isfinite(eps) and eps > 0):
+            raise ValueError("eps must be positive and finite")
+    with N.on_device(q.device):
+        if out is None:
+            out = torch.empty(T, heads, dim, dtype=q.dtype, device=q.device)
+        n, kv_heads, width, page = context_lens.numel(), k_cache.size(2), block_tables.size(1), k_cache.size(1)
+        need = N.lib().lora_b200_differential_workspace_bytes(T, n, heads, kv_heads, dim, width, page, window, sinks, cu_seqlens is not None)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        N.check(N.lib().lora_b200_differential_attention(
+            out.data_ptr(), out.stride(0), out.stride(1), q.data_ptr(), q.stride(0), q.stride(1), T, heads, kv_heads, dim, ctypes.byref(cache),
+            block_tables.data_ptr(), block_tables.stride(0), width, context_lens.data_ptr(), N.ptr(cu_seqlens), n, lam.data_ptr(),
+            lam.stride(0) if lam.dim() == 2 else 0, lam.stride(-1), N.ptr(norm_weight), float(eps), float(scale), int(window), int(sinks),
+            N.dtype_code(q.dtype), N.ptr(workspace), need, N.current_stream(q.device)))
+    return out
+
+
+def differential_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                                  context_lens: torch.Tensor, lam: torch.Tensor, *, norm_weight: torch.Tensor | None = None,
+                                  eps: float = 1e-5, scale: float | None = None, window: int = 0, sinks: int = 0,
+                                  out: torch.Tensor | None = None):
+    """Differential attention (Ye et al., "Differential Transformer", 2024) of one new token of every request. The halves of a head's
+    columns of q and k make two softmax maps over the keys that ``paged_decode_attention`` would show the token; with ``S1`` and ``S2``
+    their results over the whole columns of v, a head gives ``S1 - lam * S2``. With ``norm_weight [head_dim]`` that difference is
+    RMS-normed over the head and scaled by it (a constant factor, ``1 - lambda_init``, belongs into it). All of it fp32, rounded once.
+
+    ``lam`` float32 ``[heads]`` or, of every token its own, ``[requests, heads]``; ``scale`` defaults to that of half a head. The halves
+    are rotated as heads of their own: ``rope_kv_store`` fills such a cache as one of twice the heads of half the size. Other
+    arguments, strides, missing blocks and contexts of no key as ``paged_decode_attention``."""
+    return _differential(q, k_cache, v_cache, block_tables, context_lens, None, lam, norm_weight, eps, scale, window, sinks, out)
+
+
+def differential_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                                   context_lens: torch.Tensor, cu_seqlens: torch.Tensor, lam: torch.Tensor, *,
+                                   norm_weight: torch.Tensor | None = None, eps: float = 1e-5, scale: float | None = None,
+                                   window: int = 0, sinks: int = 0, out: torch.Tensor | None = None):
+    """``differential_decode_attention`` of packed new tokens, packed as ``paged_prefill_attention``'s (rows of no sequence are not
+    written); ``lam`` float32 ``[heads]`` or ``[tokens, heads]``."""
+    if cu_seqlens is None:
+        raise ValueError("cu_seqlens says which rows of q are whose: differential_prefill_attention needs it")
+    return _differential(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, lam, norm_weight, eps, scale, window, sinks, out)
+
+
+def join_attention(outs, lses, *, out: torch.Tensor | None = None, return_lse: bool = False):
+    """The result over a whole context of results over its parts (each token's keys lie in one part each).
+
+    ``outs`` ``[parts, tokens, heads, head_dim]`` or a sequence of ``[tokens, heads, head_dim]`` tensors of one shape and one set of
+    strides, bf16, fp16 or fp32, up to 64 of them; ``lses`` the fp32 ``[tokens, heads]`` logarithms of their sums that came with them
+    (``return_lse``), as ``[parts, ...]`` or a sequence. A part without a key (``-inf``) counts for nothing, whatever its values; a row
+    that has none in any part gives zeros. ``out`` may be one of the parts. Returns ``out``, with ``return_lse`` also the logarithm of
+    the whole sum."""
+    outs, lses = tuple(outs), tuple(lses)
+    got = N.native().join_attention(outs, lses, out, bool(return_lse))
+    if got is not None:
+        N.check(got[0])
+        return (got[1], got[2]) if return_lse else got[1]
+    N.require_cuda(*outs, *lses, out)
+    if not outs or len(outs) != len(lses):
+        raise ValueError(f"{len(outs)} results and {len(lses)} logarithms: a part has one of each")
+    first, lse0 = outs[0], lses[0]
+    if first.dim() != 3 or first.stride(2) != 1:
+        raise ValueError("a part must be [tokens, heads, head_dim] with adjacent elements in a head")
+    if any(o.shape != first.shape or o.dtype != first.dtype or o.stride() != first.stride() for o in outs):
+        raise ValueError("the parts must have one shape, dtype and set of strides")
+    T, heads, dim = first.shape
+    if any(x.dtype != torch.float32 or tuple(x.shape) != (T, heads) or x.stride() != lse0.stride() for x in lses):
+        raise ValueError(f"the logarithms must be float32 tensors {(T, heads)} of one set of strides")
+    if out is not None and (out.shape != first.shape or out.dtype != first.dtype or out.stride(2) != 1):
+        raise ValueError("out must have the shape and dtype of a part, and adjacent elements in a head")
+    devices = {t.device for t in (*outs, *lses, out) if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f"tensors on several devices: {sorted(map(str, devices))}")
+    with N.on_device(first.device):
+        if out is None:
+            out = torch.empty(T, heads, dim, dtype=first.dtype, device=first.device)
+        lse = torch.empty(T, heads, dtype=torch.float32, device=first.device) if return_lse else None
+        N.check(N.lib().lora_b200_join_attention(
+            out.data_ptr(), out.stride(0), out.stride(1), N.ptr(lse), N.ptr_array(outs), N.ptr_array(lses), len(outs), first.stride(0),
+            first.stride(1), lse0.stride(0), lse0.stride(1), T, heads, dim, N.dtype_code(first.dtype), N.current_stream(first.device)))
+    return (out, lse) if return_lse else out

@@ -17,6 +17,7 @@
 #include "decode_step.cuh"
 #include "prefill_attention.cuh"
 #include "head_norm.cuh"
+#include "attention_join.cuh"
 #include "paged_attention.cuh"
 #include "paged_prefill.cuh"
 
@@ -378,13 +379,13 @@ int32_t lora_b200_paged_decode_way(int32_t T, int32_t num_heads, int32_t num_kv_
   return w.shares ? 0 : 16 * w.cluster + w.warps;
 }
 
-// What decode and prefill have in common; cu_seqlens null: decode
-static int paged_attention_checked(const char* what, void* out, int64_t out_token, int64_t out_head, float* lse, const void* q, int64_t q_token,
-                                   int64_t q_head, int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                                   const lora_b200_paged_cache* cache, const int32_t* block_tables, int64_t table_ld,
-                                   int32_t table_width, const int32_t* context_lens, const int32_t* cu_seqlens, int32_t n_seqs,
-                                   bool prefill, float scale, int32_t window, int32_t sinks, int32_t dtype, void* workspace,
-                                   size_t workspace_bytes, void* stream) {
+// What the attentions over a paged cache have in common: `a` is filled but for what the caller's form has besides. `packed`:
+// cu_seqlens must be there. nothing: there are no rows, the call is done.
+static int paged_args(const char* what, PagedArgs* a, bool* nothing, void* out, int64_t out_token, int64_t out_head, float* lse, const void* q, int64_t q_token,
+                      int64_t q_head, int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, const lora_b200_paged_cache* cache,
+                      const int32_t* block_tables, int64_t table_ld, int32_t table_width, const int32_t* context_lens, const int32_t* cu_seqlens,
+                      int32_t n_seqs, bool packed, float scale, int32_t window, int32_t sinks, int32_t dtype, const void* workspace) {
+  *nothing = false;
   if (T < 0 || n_seqs < 0 || table_width < 0 || window < 0 || sinks < 0)
     return fail(B200_LORA_EINVAL, "%s: T=%d, %d sequences, %d table entries, window %d, sinks %d", what, T, n_seqs, table_width, window, sinks);
   if (num_kv_heads < 1 || num_heads < 1 || num_heads % num_kv_heads != 0)
@@ -393,22 +394,43 @@ static int paged_attention_checked(const char* what, void* out, int64_t out_toke
   if (!(scale > 0.f) || !std::isfinite(sc)) return fail(B200_LORA_EINVAL, "%s: scale must be positive and finite, in units of log2 too", what);
   if (dtype != B200_LORA_BF16 && dtype != B200_LORA_F16) return fail(B200_LORA_EUNSUPPORTED, "%s: bf16 and fp16 only", what);
   if (head_dim != 64 && head_dim != 128) return fail(B200_LORA_EUNSUPPORTED, "%s: head_dim %d (64 and 128 only)", what, head_dim);
-  if (T == 0 || n_seqs == 0) return B200_LORA_OK;
-  if (!out || !q || !cache || (!block_tables && table_width > 0) || !context_lens || (prefill && !cu_seqlens)) return fail(B200_LORA_EINVAL, "%s: null pointer", what);
+  if (T == 0 || n_seqs == 0) {
+    *nothing = true;
+    return B200_LORA_OK;
+  }
+  if (!out || !q || !cache || (!block_tables && table_width > 0) || !context_lens || (packed && !cu_seqlens)) return fail(B200_LORA_EINVAL, "%s: null pointer", what);
   int rc = paged_cache_check(*cache, what);
   if (rc != B200_LORA_OK) return rc;
   if (!aligned16(q) || !aligned16(out) || q_token % 8 || q_head % 8 || out_token % 8 || out_head % 8)
     return fail(B200_LORA_EUNSUPPORTED, "%s: rows of q and out must start on 16-byte boundaries", what);
   if (!aligned16(workspace)) return fail(B200_LORA_EUNSUPPORTED, "%s: the workspace must be 16-byte aligned", what);
+  *a = PagedArgs{};
+  a->q = q; a->q_token = q_token; a->q_head = q_head; a->out = out; a->out_token = out_token; a->out_head = out_head; a->lse = lse;
+  a->cache = *cache; a->tables = block_tables; a->table_ld = table_ld; a->table_width = table_width; a->context_lens = context_lens;
+  a->cu_seqlens = cu_seqlens; a->n_req = n_seqs; a->T = T; a->Hq = num_heads; a->Hk = num_kv_heads; a->window = window; a->sinks = sinks;
+  a->sc = sc;
+  return B200_LORA_OK;
+}
+static int workspace_short(const char* what, size_t need, const void* workspace, size_t bytes) {
+  if (need == 0 || (workspace != nullptr && bytes >= need)) return B200_LORA_OK;
+  return fail(B200_LORA_EWORKSPACE, "%s: %zu bytes of workspace, needs %zu", what, workspace == nullptr ? (size_t)0 : bytes, need);
+}
+
+// cu_seqlens null: decode
+static int paged_attention_checked(const char* what, void* out, int64_t out_token, int64_t out_head, float* lse, const void* q, int64_t q_token,
+                                   int64_t q_head, int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                   const lora_b200_paged_cache* cache, const int32_t* block_tables, int64_t table_ld,
+                                   int32_t table_width, const int32_t* context_lens, const int32_t* cu_seqlens, int32_t n_seqs,
+                                   bool prefill, float scale, int32_t window, int32_t sinks, int32_t dtype, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  PagedArgs a;
+  bool nothing;
+  int rc = paged_args(what, &a, &nothing, out, out_token, out_head, lse, q, q_token, q_head, T, num_heads, num_kv_heads, head_dim, cache, block_tables,
+                      table_ld, table_width, context_lens, cu_seqlens, n_seqs, prefill, scale, window, sinks, dtype, workspace);
+  if (rc != B200_LORA_OK || nothing) return rc;
   const size_t need = prefill ? lora_b200_paged_prefill_workspace_bytes(T, n_seqs, num_heads, num_kv_heads, head_dim, table_width, cache->block_size, window)
                               : lora_b200_paged_decode_workspace_bytes(T, num_heads, num_kv_heads, head_dim, table_width, cache->block_size, window, sinks);
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
-    return fail(B200_LORA_EWORKSPACE, "%s: %zu bytes of workspace, needs %zu", what, workspace == nullptr ? (size_t)0 : workspace_bytes, need);
-  PagedArgs a = {};
-  a.q = q; a.q_token = q_token; a.q_head = q_head; a.out = out; a.out_token = out_token; a.out_head = out_head; a.lse = lse;
-  a.cache = *cache; a.tables = block_tables; a.table_ld = table_ld; a.table_width = table_width; a.context_lens = context_lens;
-  a.cu_seqlens = cu_seqlens; a.n_req = n_seqs; a.T = T; a.Hq = num_heads; a.Hk = num_kv_heads; a.window = window; a.sinks = sinks;
-  a.sc = sc;
+  if ((rc = workspace_short(what, need, workspace, workspace_bytes)) != B200_LORA_OK) return rc;
   if (prefill) return paged_prefill_launch(a, head_dim, dtype, need > 0 ? workspace : nullptr, static_cast<cudaStream_t>(stream));
   return paged_decode_launch(a, head_dim, dtype, need > 0 ? workspace : nullptr, static_cast<cudaStream_t>(stream));
 }
@@ -432,6 +454,65 @@ int lora_b200_paged_prefill_attention(void* out, int64_t out_token, int64_t out_
   return paged_attention_checked("paged_prefill_attention", out, out_token, out_head, lse, q, q_token, q_head, T, num_heads, num_kv_heads,
                                  head_dim, cache, block_tables, table_ld, table_width, context_lens, cu_seqlens, n_seqs, true, scale, window,
                                  sinks, dtype, workspace, workspace_bytes, stream);
+}
+
+size_t lora_b200_differential_workspace_bytes(int32_t T, int32_t n_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                              int32_t table_width, int32_t block_size, int32_t window, int32_t sinks, int32_t packed) {
+  if (num_kv_heads < 1 || num_heads < num_kv_heads || head_dim < 1 || block_size < 1) return 0;
+  return paged_workspace_bytes<kDiff>(T, num_heads, num_kv_heads, head_dim, (int64_t)table_width * block_size, window, sinks);
+}
+
+int lora_b200_differential_attention(void* out, int64_t out_token, int64_t out_head, const void* q, int64_t q_token, int64_t q_head,
+                                     int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                     const lora_b200_paged_cache* cache, const int32_t* block_tables, int64_t table_ld,
+                                     int32_t table_width, const int32_t* context_lens, const int32_t* cu_seqlens, int32_t n_seqs,
+                                     const float* lam, int64_t lam_token, int64_t lam_head, const void* norm_weight, float eps,
+                                     float scale, int32_t window, int32_t sinks, int32_t dtype, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  const char* what = "differential_attention";
+  PagedArgs a;
+  bool nothing;
+  int rc = paged_args(what, &a, &nothing, out, out_token, out_head, nullptr, q, q_token, q_head, T, num_heads, num_kv_heads, head_dim, cache,
+                      block_tables, table_ld, table_width, context_lens, cu_seqlens, n_seqs, false, scale, window, sinks, dtype, workspace);
+  if (rc != B200_LORA_OK) return rc;
+  if (norm_weight != nullptr && !(eps > 0.f && std::isfinite(eps))) return fail(B200_LORA_EINVAL, "%s: eps must be positive and finite", what);
+  if (nothing) return B200_LORA_OK;
+  if (lam == nullptr) return fail(B200_LORA_EINVAL, "%s: null pointer", what);
+  if (cu_seqlens == nullptr && n_seqs != T) return fail(B200_LORA_EINVAL, "%s: %d tokens, %d sequences: a decode batch has one of each", what, T, n_seqs);
+  if (!aligned16(norm_weight)) return fail(B200_LORA_EUNSUPPORTED, "%s: norm_weight must be 16-byte aligned", what);
+  const size_t need = lora_b200_differential_workspace_bytes(T, n_seqs, num_heads, num_kv_heads, head_dim, table_width, cache->block_size, window,
+                                                             sinks, cu_seqlens != nullptr);
+  if ((rc = workspace_short(what, need, workspace, workspace_bytes)) != B200_LORA_OK) return rc;
+  a.lam = lam; a.lam_token = lam_token; a.lam_head = lam_head; a.norm_weight = norm_weight; a.eps = eps;
+  void* const ws = need > 0 ? workspace : nullptr;
+  return paged_decode_launch<kDiff>(a, head_dim, dtype, ws, static_cast<cudaStream_t>(stream));
+}
+
+int lora_b200_join_attention(void* out, int64_t out_token, int64_t out_head, float* lse, const void* const* outs, const float* const* lses,
+                             int32_t n_parts, int64_t part_token, int64_t part_head, int64_t lse_token, int64_t lse_head, int32_t T,
+                             int32_t num_heads, int32_t head_dim, int32_t dtype, void* stream) {
+  const char* what = "join_attention";
+  if (T < 0 || num_heads < 1 || head_dim < 1 || n_parts < 1)
+    return fail(B200_LORA_EINVAL, "%s: T=%d, %d heads of %d, %d parts", what, T, num_heads, head_dim, n_parts);
+  if (n_parts > kJoinParts) return fail(B200_LORA_EUNSUPPORTED, "%s: %d parts (%d at most)", what, n_parts, kJoinParts);
+  if (dtype != B200_LORA_BF16 && dtype != B200_LORA_F16 && dtype != B200_LORA_F32) return fail(B200_LORA_EUNSUPPORTED, "%s: bf16, fp16 and fp32 only", what);
+  const int each = dtype == B200_LORA_F32 ? 4 : 8;  // elements of 16 bytes
+  if (head_dim % each != 0) return fail(B200_LORA_EUNSUPPORTED, "%s: head_dim %d (a multiple of %d)", what, head_dim, each);
+  if (T == 0) return B200_LORA_OK;
+  if (!out || !outs || !lses) return fail(B200_LORA_EINVAL, "%s: null pointer", what);
+  JoinArgs a = {};
+  for (int i = 0; i < n_parts; ++i) {
+    if (!outs[i] || !lses[i]) return fail(B200_LORA_EINVAL, "%s: null pointer", what);
+    if (!aligned16(outs[i])) return fail(B200_LORA_EUNSUPPORTED, "%s: rows must start on 16-byte boundaries", what);
+    a.outs[i] = outs[i];
+    a.lses[i] = lses[i];
+  }
+  if (!aligned16(out) || part_token % each || part_head % each || out_token % each || out_head % each)
+    return fail(B200_LORA_EUNSUPPORTED, "%s: rows must start on 16-byte boundaries", what);
+  a.part_token = part_token; a.part_head = part_head; a.lse_token = lse_token; a.lse_head = lse_head;
+  a.out = out; a.out_token = out_token; a.out_head = out_head; a.lse = lse;
+  a.n_parts = n_parts; a.T = T; a.H = num_heads; a.vecs = head_dim / each;
+  return join_attention_launch(a, dtype, static_cast<cudaStream_t>(stream));
 }
 
 size_t lora_b200_tp_exchange_bytes(int32_t tp, int32_t capacity) { return tp_exchange_bytes(tp, capacity); }

@@ -45,6 +45,9 @@ decltype(&lora_b200_paged_decode_workspace_bytes) p_decode_bytes = nullptr;
 decltype(&lora_b200_paged_prefill_workspace_bytes) p_prefill_bytes = nullptr;
 decltype(&lora_b200_paged_decode_attention) p_paged_decode = nullptr;
 decltype(&lora_b200_paged_prefill_attention) p_paged_prefill = nullptr;
+decltype(&lora_b200_differential_workspace_bytes) p_differential_bytes = nullptr;
+decltype(&lora_b200_differential_attention) p_differential = nullptr;
+decltype(&lora_b200_join_attention) p_join = nullptr;
 PyObject* scratch_for = nullptr;  // lora.scratch_for(device, bytes)
 PyObject *s_weight, *s_lora_a, *s_tts, *s_sorted, *s_ids, *s_counts, *s_offsets, *s_num_active;
 
@@ -581,69 +584,180 @@ PyObject* qk_norm_rope_kv_store(PyObject*, PyObject* const* args, Py_ssize_t nar
   END_HANDLE_TH_ERRORS
 }
 
+// What the attentions over a paged cache are given: q, k_cache, v_cache, block_tables, context_lens, cu_seqlens | None
+struct PagedCall {
+  const at::Tensor *q = nullptr, *tables = nullptr, *ctx = nullptr, *cu = nullptr, *out = nullptr;
+  lora_b200_paged_cache cache;
+  int dev = 0, code = -1, width = 0;
+  int64_t T = 0, hq = 0, hk = 0, d = 0, n = 0;
+  at::Tensor fresh, ws;
+
+  bool read(PyObject* const* args) {  // false = not handled
+    q = tensor_of(args[0]); tables = tensor_of(args[3]); ctx = tensor_of(args[4]);
+    if (!q || !tables || !ctx || !q->is_cuda() || q->dim() != 3 || q->stride(2) != 1) return false;
+    dev = q->get_device();
+    code = dtype_code(q->scalar_type());
+    T = q->size(0); hq = q->size(1); d = q->size(2);
+    if (code < 0 || dev != c10::cuda::current_device() || T > INT32_MAX || hq < 1 || hq > 65536 || d > 65536) return false;
+    if (!read_cache(args[1], args[2], q->scalar_type(), -1, d, dev, &cache)) return false;
+    hk = tensor_of(args[1])->size(2);
+    if (hk < 1 || hk > 65536) return false;
+    for (const at::Tensor* t : {tables, ctx})
+      if (!on(*t, dev) || t->scalar_type() != at::kInt) return false;
+    n = ctx->numel();
+    if (ctx->dim() != 1 || !ctx->is_contiguous() || tables->dim() != 2 || tables->size(0) != n || tables->size(1) > INT32_MAX || n > INT32_MAX ||
+        (tables->size(1) > 1 && tables->stride(1) != 1))
+      return false;
+    width = (int)tables->size(1);
+    if (args[5] != Py_None) {
+      cu = tensor_of(args[5]);
+      if (cu == nullptr || !on(*cu, dev) || cu->scalar_type() != at::kInt || cu->dim() != 1 || !cu->is_contiguous() || cu->numel() != n + 1)
+        return false;
+    } else if (n != T) {
+      return false;
+    }
+    return true;
+  }
+  // The given tensor of the shape of q, or a fresh one
+  bool result(PyObject* o) {
+    out = &fresh;
+    if (o == Py_None) {
+      fresh = at::empty({T, hq, d}, q->options());
+    } else {
+      out = tensor_of(o);
+      if (out == nullptr || !on(*out, dev) || out->scalar_type() != q->scalar_type() || out->sizes() != q->sizes() || out->stride(2) != 1) return false;
+    }
+    return true;
+  }
+  void* workspace(size_t need) {
+    if (need == 0) return nullptr;
+    ws = at::empty({(int64_t)need}, q->options().dtype(at::kByte));
+    return ws.data_ptr();
+  }
+  const int32_t* ints(const at::Tensor* t) const { return t == nullptr ? nullptr : static_cast<const int32_t*>(t->data_ptr()); }
+  void* stream() const { return c10::cuda::getCurrentCUDAStream(dev).stream(); }
+  PyObject* wrapped(PyObject* o) const {
+    if (o == Py_None) return THPVariable_Wrap(fresh);
+    Py_INCREF(o);
+    return o;
+  }
+};
+
+// window and sinks as the attentions take them; false = not handled
+bool read_window(PyObject* wo, PyObject* so, int64_t* window, int64_t* sinks) {
+  *window = PyLong_AsLongLong(wo);
+  *sinks = PyLong_AsLongLong(so);
+  if (PyErr_Occurred()) { PyErr_Clear(); return false; }
+  return *window >= 0 && *sinks >= 0 && *window <= INT32_MAX && *sinks <= INT32_MAX && (*sinks == 0 || *window > 0);
+}
+
 // paged_attention(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens | None, scale, window, sinks, out | None, lse?)
 // -> (status, out, lse | None), or None
 PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   if (nargs != 11) { PyErr_SetString(PyExc_TypeError, "paged_attention takes 11 arguments"); return nullptr; }
-  const at::Tensor *q = tensor_of(args[0]), *tables = tensor_of(args[3]), *ctx = tensor_of(args[4]), *cu = nullptr;
-  if (!q || !tables || !ctx || !q->is_cuda() || q->dim() != 3 || q->stride(2) != 1) return not_handled();
-  const int dev = q->get_device();
-  const at::ScalarType dt = q->scalar_type();
-  const int code = dtype_code(dt);
-  const int64_t T = q->size(0), hq = q->size(1), d = q->size(2);
-  if (code < 0 || dev != c10::cuda::current_device() || T > INT32_MAX || hq < 1 || hq > 65536 || d > 65536) return not_handled();
-  lora_b200_paged_cache cache;
-  if (!read_cache(args[1], args[2], dt, -1, d, dev, &cache)) return not_handled();
-  const int64_t hk = tensor_of(args[1])->size(2);
-  if (hk < 1 || hk > 65536) return not_handled();
-  for (const at::Tensor* t : {tables, ctx})
-    if (!on(*t, dev) || t->scalar_type() != at::kInt) return not_handled();
-  const int64_t n = ctx->numel();
-  if (ctx->dim() != 1 || !ctx->is_contiguous() || tables->dim() != 2 || tables->size(0) != n || tables->size(1) > INT32_MAX || n > INT32_MAX ||
-      (tables->size(1) > 1 && tables->stride(1) != 1))
-    return not_handled();
-  if (args[5] != Py_None) {
-    cu = tensor_of(args[5]);
-    if (cu == nullptr || !on(*cu, dev) || cu->scalar_type() != at::kInt || cu->dim() != 1 || !cu->is_contiguous() || cu->numel() != n + 1)
-      return not_handled();
-  } else if (n != T) {
-    return not_handled();
-  }
+  PagedCall c;
+  if (!c.read(args)) return not_handled();
   const double scale = PyFloat_AsDouble(args[6]);
-  const int64_t window = PyLong_AsLongLong(args[7]), sinks = PyLong_AsLongLong(args[8]);
   if (PyErr_Occurred()) { PyErr_Clear(); return not_handled(); }
-  if (window < 0 || sinks < 0 || window > INT32_MAX || sinks > INT32_MAX || (sinks > 0 && window == 0)) return not_handled();
-  at::Tensor fresh, lse;
-  const at::Tensor* out = &fresh;
-  if (args[9] == Py_None) {
-    fresh = at::empty({T, hq, d}, q->options());
-  } else {
-    out = tensor_of(args[9]);
-    if (out == nullptr || !on(*out, dev) || out->scalar_type() != dt || out->sizes() != q->sizes() || out->stride(2) != 1) return not_handled();
-  }
-  if (args[10] == Py_True) lse = at::empty({T, hq}, q->options().dtype(at::kFloat));
-  const size_t need = cu == nullptr ? p_decode_bytes((int)T, (int)hq, (int)hk, (int)d, (int)tables->size(1), cache.block_size, (int)window, (int)sinks)
-                                    : p_prefill_bytes((int)T, (int)n, (int)hq, (int)hk, (int)d, (int)tables->size(1), cache.block_size, (int)window);
-  at::Tensor ws;
-  if (need > 0) ws = at::empty({(int64_t)need}, q->options().dtype(at::kByte));
-  void* const ws_ptr = need > 0 ? ws.data_ptr() : nullptr;
-  void* stream = c10::cuda::getCurrentCUDAStream(dev).stream();
+  int64_t window, sinks;
+  if (!read_window(args[7], args[8], &window, &sinks) || !c.result(args[9])) return not_handled();
+  at::Tensor lse;
+  if (args[10] == Py_True) lse = at::empty({c.T, c.hq}, c.q->options().dtype(at::kFloat));
+  const size_t need = c.cu == nullptr ? p_decode_bytes((int)c.T, (int)c.hq, (int)c.hk, (int)c.d, c.width, c.cache.block_size, (int)window, (int)sinks)
+                                      : p_prefill_bytes((int)c.T, (int)c.n, (int)c.hq, (int)c.hk, (int)c.d, c.width, c.cache.block_size, (int)window);
+  void* const ws = c.workspace(need);
   float* lse_ptr = lse.defined() ? static_cast<float*>(lse.data_ptr()) : nullptr;
   int rc;
-  if (cu != nullptr)
-    rc = p_paged_prefill(out->data_ptr(), out->stride(0), out->stride(1), lse_ptr, q->data_ptr(), q->stride(0), q->stride(1), (int)T, (int)hq,
-                         (int)hk, (int)d, &cache, static_cast<const int32_t*>(tables->data_ptr()), tables->stride(0), (int)tables->size(1),
-                         static_cast<const int32_t*>(ctx->data_ptr()), static_cast<const int32_t*>(cu->data_ptr()), (int)n, (float)scale,
-                         (int)window, (int)sinks, code, ws_ptr, need, stream);
+  if (c.cu != nullptr)
+    rc = p_paged_prefill(c.out->data_ptr(), c.out->stride(0), c.out->stride(1), lse_ptr, c.q->data_ptr(), c.q->stride(0), c.q->stride(1), (int)c.T,
+                         (int)c.hq, (int)c.hk, (int)c.d, &c.cache, c.ints(c.tables), c.tables->stride(0), c.width, c.ints(c.ctx), c.ints(c.cu),
+                         (int)c.n, (float)scale, (int)window, (int)sinks, c.code, ws, need, c.stream());
   else
-    rc = p_paged_decode(out->data_ptr(), out->stride(0), out->stride(1), lse_ptr, q->data_ptr(), q->stride(0), q->stride(1), (int)T, (int)hq,
-                        (int)hk, (int)d, &cache, static_cast<const int32_t*>(tables->data_ptr()), tables->stride(0), (int)tables->size(1),
-                        static_cast<const int32_t*>(ctx->data_ptr()), (float)scale, (int)window, (int)sinks, code, ws_ptr, need, stream);
+    rc = p_paged_decode(c.out->data_ptr(), c.out->stride(0), c.out->stride(1), lse_ptr, c.q->data_ptr(), c.q->stride(0), c.q->stride(1), (int)c.T,
+                        (int)c.hq, (int)c.hk, (int)c.d, &c.cache, c.ints(c.tables), c.tables->stride(0), c.width, c.ints(c.ctx), (float)scale,
+                        (int)window, (int)sinks, c.code, ws, need, c.stream());
   PyObject* lse_out = Py_None;
   if (lse.defined()) lse_out = THPVariable_Wrap(lse);
   else Py_INCREF(Py_None);
-  if (args[9] != Py_None) return Py_BuildValue("(iON)", rc, args[9], lse_out);
+  return Py_BuildValue("(iNN)", rc, c.wrapped(args[9]), lse_out);
+  END_HANDLE_TH_ERRORS
+}
+
+// differential_attention(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens | None, lam, norm_weight | None, eps, scale, window,
+// sinks, out | None) -> (status, out), or None
+PyObject* differential_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 13) { PyErr_SetString(PyExc_TypeError, "differential_attention takes 13 arguments"); return nullptr; }
+  PagedCall c;
+  if (!c.read(args)) return not_handled();
+  const at::Tensor *lam = tensor_of(args[6]), *weight = nullptr;
+  if (lam == nullptr || !on(*lam, c.dev) || lam->scalar_type() != at::kFloat || lam->dim() < 1 || lam->dim() > 2 || lam->size(-1) != c.hq ||
+      (lam->dim() == 2 && lam->size(0) != c.T))
+    return not_handled();
+  if (args[7] != Py_None) {
+    weight = tensor_of(args[7]);
+    if (weight == nullptr || !on(*weight, c.dev) || weight->scalar_type() != c.q->scalar_type() || weight->dim() != 1 || weight->size(0) != c.d ||
+        !weight->is_contiguous())
+      return not_handled();
+  }
+  const double eps = PyFloat_AsDouble(args[8]), scale = PyFloat_AsDouble(args[9]);
+  if (PyErr_Occurred()) { PyErr_Clear(); return not_handled(); }
+  int64_t window, sinks;
+  if (!read_window(args[10], args[11], &window, &sinks) || !c.result(args[12])) return not_handled();
+  const size_t need = p_differential_bytes((int)c.T, (int)c.n, (int)c.hq, (int)c.hk, (int)c.d, c.width, c.cache.block_size, (int)window, (int)sinks,
+                                           c.cu != nullptr);
+  void* const ws = c.workspace(need);
+  const int rc = p_differential(c.out->data_ptr(), c.out->stride(0), c.out->stride(1), c.q->data_ptr(), c.q->stride(0), c.q->stride(1), (int)c.T,
+                                (int)c.hq, (int)c.hk, (int)c.d, &c.cache, c.ints(c.tables), c.tables->stride(0), c.width, c.ints(c.ctx), c.ints(c.cu),
+                                (int)c.n, static_cast<const float*>(lam->data_ptr()), lam->dim() == 2 ? lam->stride(0) : 0, lam->stride(-1),
+                                weight == nullptr ? nullptr : weight->data_ptr(), (float)eps, (float)scale, (int)window, (int)sinks, c.code, ws, need,
+                                c.stream());
+  return Py_BuildValue("(iN)", rc, c.wrapped(args[12]));
+  END_HANDLE_TH_ERRORS
+}
+
+// join_attention(outs, lses, out | None, lse?) -> (status, out, lse | None), or None; outs and lses: tuples of tensors
+PyObject* join_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 4) { PyErr_SetString(PyExc_TypeError, "join_attention takes 4 arguments"); return nullptr; }
+  constexpr Py_ssize_t kMost = 64;
+  if (!PyTuple_CheckExact(args[0]) || !PyTuple_CheckExact(args[1])) return not_handled();
+  const Py_ssize_t parts = PyTuple_GET_SIZE(args[0]);
+  if (parts < 1 || parts > kMost || PyTuple_GET_SIZE(args[1]) != parts) return not_handled();
+  const at::Tensor *first = tensor_of(PyTuple_GET_ITEM(args[0], 0)), *lse0 = tensor_of(PyTuple_GET_ITEM(args[1], 0));
+  if (!first || !lse0 || !first->is_cuda() || first->dim() != 3 || first->stride(2) != 1) return not_handled();
+  const int dev = first->get_device(), code = dtype_code(first->scalar_type());
+  const int64_t T = first->size(0), heads = first->size(1), d = first->size(2);
+  if (code < 0 || dev != c10::cuda::current_device() || T > INT32_MAX || heads < 1 || heads > 65536 || d < 1 || d > 65536) return not_handled();
+  const void* outs[kMost];
+  const float* lses[kMost];
+  for (Py_ssize_t i = 0; i < parts; ++i) {
+    const at::Tensor *o = tensor_of(PyTuple_GET_ITEM(args[0], i)), *x = tensor_of(PyTuple_GET_ITEM(args[1], i));
+    if (!o || !x || !on(*o, dev) || !on(*x, dev) || o->scalar_type() != first->scalar_type() || o->sizes() != first->sizes() ||
+        o->strides() != first->strides() || x->scalar_type() != at::kFloat || x->dim() != 2 || x->size(0) != T || x->size(1) != heads ||
+        x->strides() != lse0->strides())
+      return not_handled();
+    outs[i] = o->data_ptr();
+    lses[i] = static_cast<const float*>(x->data_ptr());
+  }
+  at::Tensor fresh, lse;
+  const at::Tensor* out = &fresh;
+  if (args[2] == Py_None) {
+    fresh = at::empty({T, heads, d}, first->options());
+  } else {
+    out = tensor_of(args[2]);
+    if (out == nullptr || !on(*out, dev) || out->scalar_type() != first->scalar_type() || out->sizes() != first->sizes() || out->stride(2) != 1)
+      return not_handled();
+  }
+  if (args[3] == Py_True) lse = at::empty({T, heads}, first->options().dtype(at::kFloat));
+  const int rc = p_join(out->data_ptr(), out->stride(0), out->stride(1), lse.defined() ? static_cast<float*>(lse.data_ptr()) : nullptr, outs, lses,
+                        (int)parts, first->stride(0), first->stride(1), lse0->stride(0), lse0->stride(1), (int)T, (int)heads, (int)d, code,
+                        c10::cuda::getCurrentCUDAStream(dev).stream());
+  PyObject* lse_out = Py_None;
+  if (lse.defined()) lse_out = THPVariable_Wrap(lse);
+  else Py_INCREF(Py_None);
+  if (args[2] != Py_None) return Py_BuildValue("(iON)", rc, args[2], lse_out);
   return Py_BuildValue("(iNN)", rc, THPVariable_Wrap(fresh), lse_out);
   END_HANDLE_TH_ERRORS
 }
@@ -991,6 +1105,9 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   B200_BIND(p_prefill_bytes, lora_b200_paged_prefill_workspace_bytes)
   B200_BIND(p_paged_decode, lora_b200_paged_decode_attention)
   B200_BIND(p_paged_prefill, lora_b200_paged_prefill_attention)
+  B200_BIND(p_differential_bytes, lora_b200_differential_workspace_bytes)
+  B200_BIND(p_differential, lora_b200_differential_attention)
+  B200_BIND(p_join, lora_b200_join_attention)
 #undef B200_BIND
   Py_INCREF(args[1]);
   Py_XDECREF(scratch_for);
@@ -1000,7 +1117,7 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 #define B200_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {B200_METHOD(add), B200_METHOD(shrink), B200_METHOD(expand), B200_METHOD(linear), B200_METHOD(add_rms_norm), B200_METHOD(silu_mul),
-                         B200_METHOD(rope_kv_store), B200_METHOD(qk_norm_rope_kv_store), B200_METHOD(paged_attention), B200_METHOD(prefill_layers), B200_METHOD(bucket_lists), B200_METHOD(pack_lists), B200_METHOD(bind), {nullptr, nullptr, 0, nullptr}};
+                         B200_METHOD(rope_kv_store), B200_METHOD(qk_norm_rope_kv_store), B200_METHOD(paged_attention), B200_METHOD(differential_attention), B200_METHOD(join_attention), B200_METHOD(prefill_layers), B200_METHOD(bucket_lists), B200_METHOD(pack_lists), B200_METHOD(bind), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "b200lora_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -40,7 +40,16 @@ struct PagedArgs {
   int window, sinks;
   float sc;                                    // scale * log2(e): scores and maxima are in units of log2
   float *part_o, *part_ml; int4* joins;        // partial results of CTA boundaries, and what there is to join
+  // differential heads: what the second map counts, [T, Hq] by strides; weight [D] of the heads' norm or null
+  const float* lam; int64_t lam_token, lam_head;
+  const void* norm_weight; float eps;
 };
+
+// What a kernel makes of a head: one softmax map; or two, of the halves of its columns of q and k over the whole of v, and of them the
+// difference a - lam b, normed.
+constexpr int kPlain = 0, kDiff = 1;
+template <int kForm> constexpr int kMaps = kForm == kDiff ? 2 : 1;
+template <int kForm> constexpr int kItemHeads = kForm == kDiff ? 8 : 16;  // q heads of an item at most
 
 __device__ __forceinline__ RowKeys row_keys(const PagedArgs& a, int row) {
   RowKeys r = {row, 0, 0, -1};
@@ -99,13 +108,35 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+__device__ __forceinline__ float over(float l) { return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l); }  // (no visible key: zeros; NaN stays)
 // Joined or single result of a head's two columns
 template <bool kF16>
 __device__ __forceinline__ void store_result(const PagedArgs& a, int row, int head, int d, float x, float y, float m, float l) {
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // (no visible key: zeros; NaN stays)
+  const float inv = over(l);
   char* dst = static_cast<char*>(a.out) + 2 * (row * a.out_token + head * a.out_head + d);
   *reinterpret_cast<uint32_t*>(dst) = pack_16x2<kF16>(x * inv, y * inv);
   if (a.lse != nullptr && d == 0) a.lse[(int64_t)row * a.Hq + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+// Four columns (4 c on) of a differential head from the sums of its maps. The lanes of a head, D / 4 side by side, call it together
+// (`live`: this lane has a head). Difference and norm in fp32, of what has not been rounded.
+template <int D, bool kF16>
+__device__ __forceinline__ void store_difference(const PagedArgs& a, bool live, int64_t row, int head, int c, const float4 (&x)[2], const float (&l)[2]) {
+  const float one = over(l[0]), two = live ? a.lam[row * a.lam_token + head * a.lam_head] * over(l[1]) : 0.f;
+  auto sub = [&](float p, float q) { return __fmul_rn(p, one) - __fmul_rn(q, two); };  // (both products rounded: equal maps cancel)
+  float4 y = make_float4(sub(x[0].x, x[1].x), sub(x[0].y, x[1].y), sub(x[0].z, x[1].z), sub(x[0].w, x[1].w));
+  if (a.norm_weight != nullptr) {
+    float ss = (y.x * y.x + y.y * y.y) + (y.z * y.z + y.w * y.w);
+#pragma unroll
+    for (int d = 1; d < D / 4; d *= 2) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+    const float r = rsqrtf(ss * (1.f / D) + a.eps);
+    const uint2 w = live ? *reinterpret_cast<const uint2*>(static_cast<const char*>(a.norm_weight) + 8 * c) : make_uint2(0, 0);
+    const float2 w0 = unpack_16x2<kF16>(w.x), w1 = unpack_16x2<kF16>(w.y);
+    y = make_float4(y.x * r * w0.x, y.y * r * w0.y, y.z * r * w1.x, y.w * r * w1.y);
+  }
+  if (live)
+    *reinterpret_cast<uint2*>(static_cast<char*>(a.out) + 2 * (row * a.out_token + head * a.out_head + 4 * c)) =
+        make_uint2(pack_16x2<kF16>(y.x, y.y), pack_16x2<kF16>(y.z, y.w));
 }
 
 // Blocks [u0, u1) of the keys of one (row, kv head, chunk of its q heads)
@@ -167,14 +198,17 @@ struct PagedWalk {
 // kWay: whose the items are
 constexpr int kWhole = 0, kShares = 1, kClusters = 2;  // one CTA's each; of a share of all blocks; a cluster's each, joined in its shared memory
 
-template <int D, int NT, bool kF16, int kWay, int kPagedWarps>
+// kForm kDiff: the tiles of eight heads are the two maps of the same eight, whose scores take half of the columns each.
+template <int D, int NT, bool kF16, int kWay, int kPagedWarps, int kForm>
 __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decode_kernel(const PagedArgs a) {
   extern __shared__ __align__(16) uint8_t paged_smem_raw[];  // (a name of its own: 1024-byte alignment would cost heads of 64 the second CTA)
   uint8_t* const smem = paged_smem_raw;
   constexpr int kPagedThreads = 32 * kPagedWarps;
   constexpr int kPitch = D * 2 + 16, kKeys = paged_block_keys<D>(), kStage = paged_stage_bytes<D>(), kPieces = D / 8;
   constexpr int kMT = kKeys / 16, kPerLoad = 32 / kPieces;  // rows of a load instruction
-  constexpr int kQ = 8 * NT * kPitch, kQEach = (8 * NT * kPieces + kPagedThreads - 1) / kPagedThreads;
+  static_assert(kForm != kDiff || NT == 2, "a tile for each map");
+  constexpr int kQRows = 8 * NT / kMaps<kForm>, kSteps = D / 16 / kMaps<kForm>;  // rows of q; steps of a score
+  constexpr int kQ = 8 * NT * kPitch, kQEach = (kQRows * kPieces + kPagedThreads - 1) / kPagedThreads;
   static_assert(8 * NT * (D + 2) * 4 <= kStage, "a warp's result lies in one stage");
   __shared__ int s_row;
   __shared__ long long s_at, s_sum[kPagedWarps];
@@ -291,7 +325,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
 #pragma unroll
     for (int e = 0; e < kQEach; ++e) {
       const int i = tid + e * kPagedThreads, h = i / kPieces, p = i - h * kPieces;
-      if (h < 8 * NT) sts128(q_u32 + (uint32_t)(buf * kQ + h * kPitch + p * 16), q_piece[e]);
+      if (h < kQRows) sts128(q_u32 + (uint32_t)(buf * kQ + h * kPitch + p * 16), q_piece[e]);
     }
   };
 
@@ -316,13 +350,14 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
     } else {
       __syncthreads();  // q is there; the stages that held results may be filled again
     }
-    uint32_t qf[NT][D / 16][2];
+    uint32_t qf[NT][kSteps][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int k = 0; k < D / 32; ++k) {
+      for (int k = 0; k < kSteps / 2; ++k) {
         uint32_t r[4];
-        ldsm_x4(q_u32 + (uint32_t)(buf * kQ + (8 * n + (lane & 7)) * kPitch + (lane >> 3) * 16 + 64 * k), r);
+        const int q_row = (kForm == kDiff ? 0 : 8 * n) + (lane & 7), q_col = kForm == kDiff ? n * D : 0;
+        ldsm_x4(q_u32 + (uint32_t)(buf * kQ + q_row * kPitch + q_col + (lane >> 3) * 16 + 64 * k), r);
         qf[n][2 * k][0] = r[0]; qf[n][2 * k][1] = r[1];
         qf[n][2 * k + 1][0] = r[2]; qf[n][2 * k + 1][1] = r[3];
       }
@@ -350,7 +385,8 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
           uint32_t kf[4];
           ldsm_x4(ks + (uint32_t)((16 * i + (lane & 15)) * kPitch + (lane >> 4) * 16 + 32 * k), kf);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_16816<kF16>(s[n][i], kf[0], kf[1], kf[2], kf[3], qf[n][k][0], qf[n][k][1]);
+          for (int n = 0; n < NT; ++n)
+            if (kForm != kDiff || k / kSteps == n) mma_16816<kF16>(s[n][i], kf[0], kf[1], kf[2], kf[3], qf[n][k % kSteps][0], qf[n][k % kSteps][1]);
         }
       }
       bool grows = false;  // scores, masked
@@ -441,7 +477,39 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
     __shared__ float2 s_ml[8 * NT];
     const bool whole = !kShare || (w.u0 == 0 && w.u1 == w.n_units);
     const int slot = 2 * blockIdx.x + (first_piece ? 0 : 1);
-    for (int i = tid; i < w.n_heads * (D / 2); i += kPagedThreads) {
+    // (differential: four columns of a head a lane, of both maps)
+    for (int i = tid; kForm == kDiff && i < 8 * (D / 4); i += kPagedThreads) {
+      const int h = i / (D / 4), c = i - h * (D / 4);
+      float4 x[2];
+      float sum[2];
+#pragma unroll
+      for (int map = 0; map < 2; ++map) {
+        const int vh = 8 * map + h;
+        float top = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < kPagedWarps; ++k) top = fmaxf(top, part[k][8 * NT * D + 2 * vh]);
+        sum[map] = 0.f;
+        x[map] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < kPagedWarps; ++k) {
+          const float2 ml = *reinterpret_cast<const float2*>(part[k] + 8 * NT * D + 2 * vh);
+          const float4 v = *reinterpret_cast<const float4*>(part[k] + vh * D + 4 * c);
+          const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+          sum[map] += f * ml.y;
+          x[map] = make_float4(x[map].x + f * v.x, x[map].y + f * v.y, x[map].z + f * v.z, x[map].w + f * v.w);
+        }
+        if (kWay == kClusters) {
+          *reinterpret_cast<float4*>(const_cast<float*>(part[0]) + vh * D + 4 * c) = x[map];
+          if (c == 0) s_ml[vh] = make_float2(top, sum[map]);
+        } else if (!whole && h < w.n_heads) {
+          const int64_t at_slot = ((int64_t)slot * 2 + map) * a.heads + h;
+          *reinterpret_cast<float4*>(a.part_o + at_slot * D + 4 * c) = x[map];
+          if (c == 0) *reinterpret_cast<float2*>(a.part_ml + at_slot * 2) = make_float2(top, sum[map]);
+        }
+      }
+      if (kWay != kClusters && whole) store_difference<D, kF16>(a, h < w.n_heads, w.row, w.head0 + h, c, x, sum);
+    }
+    for (int i = tid; kForm != kDiff && i < w.n_heads * (D / 2); i += kPagedThreads) {
       const int h = i / (D / 2), d = 2 * (i - h * (D / 2));
       float top = -INFINITY;
 #pragma unroll
@@ -470,7 +538,43 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
       // the cluster's parts: every CTA joins some of the columns
       cluster_arrive();
       cluster_wait();
-      const int all = w.n_heads * (D / 2);
+      if (kForm == kDiff) {  // (whole heads, for their norm; whole warps, for its sum)
+        const int h0 = (int)(8 * rank / ranks), h1 = (int)(8 * (rank + 1) / ranks);
+        for (int i = tid; i < ((h1 - h0) * (D / 4) + 31) / 32 * 32; i += kPagedThreads) {
+          const int its = h0 + i / (D / 4), h = min(its, 7), c = i % (D / 4);
+          float4 x[2];
+          float sum[2];
+#pragma unroll
+          for (int map = 0; map < 2; ++map) {
+            const int vh = 8 * map + h;
+            float2 ml[8], v0[8], v1[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              ml[k] = make_float2(-INFINITY, 0.f);
+              v0[k] = v1[k] = make_float2(0.f, 0.f);
+              if (k < (int)ranks) {
+                ml[k] = ld_cluster_f32x2(mapa_shared(smem_u32(&s_ml[vh]), k));
+                const uint32_t at = mapa_shared(q_u32 + 2 * kQ + ld_cluster_u32(mapa_shared(smem_u32(&s_third[0]), k)) * kStage + 4 * (vh * D + 4 * c), k);
+                v0[k] = ld_cluster_f32x2(at);
+                v1[k] = ld_cluster_f32x2(at + 8);
+              }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
+            sum[map] = 0.f;
+            x[map] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float f = ml[k].x == -INFINITY ? 0.f : ex2(ml[k].x - top);
+              sum[map] += f * ml[k].y;
+              x[map] = make_float4(x[map].x + f * v0[k].x, x[map].y + f * v0[k].y, x[map].z + f * v1[k].x, x[map].w + f * v1[k].y);
+            }
+          }
+          store_difference<D, kF16>(a, its < h1 && h < w.n_heads, w.row, w.head0 + h, c, x, sum);
+        }
+      }
+      const int all = kForm == kDiff ? 0 : w.n_heads * (D / 2);
       for (int i = (int)((int64_t)all * rank / ranks) + tid, to = (int)((int64_t)all * (rank + 1) / ranks); i < to; i += kPagedThreads) {
         const int h = i / (D / 2), d = 2 * (i - h * (D / 2));
         float2 ml[8], v[8];
@@ -518,7 +622,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
 
 // Joins the parts of the item that begins in CTA blockIdx.x: its own, then the first one of every CTA up to the last; one of its
 // heads (blockIdx.y). D / 4 threads keep four columns each; groups of them take the parts in turn.
-template <int D, bool kF16>
+template <int D, bool kF16, int kForm>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArgs a) {
   constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes;
   __shared__ float4 s_o[kGroups][kLanes];
@@ -528,32 +632,44 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArg
   const int group = a.Hq / a.Hk, in_group = j.y % group, n_heads = min(a.heads, group - in_group);
   if (j.x < 0 || (int)blockIdx.y >= n_heads) return;
   const int parts = j.w - (int)blockIdx.x + 1, c = threadIdx.x % kLanes, mine = threadIdx.x / kLanes;
-  auto slot_of = [&](int k) { return (int64_t)(k == 0 ? j.z : 2 * ((int)blockIdx.x + k)) * a.heads + blockIdx.y; };
-  auto stats = [&](int k) { return *reinterpret_cast<const float2*>(a.part_ml + slot_of(k) * 2); };
-  float top = -INFINITY, sum = 0.f;
+  float4 x[kMaps<kForm>];
+  float l[kMaps<kForm>], top;
+#pragma unroll
+  for (int map = 0; map < kMaps<kForm>; ++map) {
+    auto slot_of = [&](int k) { return ((int64_t)(k == 0 ? j.z : 2 * ((int)blockIdx.x + k)) * kMaps<kForm> + map) * a.heads + blockIdx.y; };
+    auto stats = [&](int k) { return *reinterpret_cast<const float2*>(a.part_ml + slot_of(k) * 2); };
+    float sum = 0.f;
+    top = -INFINITY;
 #pragma unroll 8
-  for (int k = 0; k < parts; ++k) top = fmaxf(top, stats(k).x);
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < parts; ++k) top = fmaxf(top, stats(k).x);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-  for (int k = mine; k < parts; k += kGroups) {
-    const float2 ml = stats(k);
-    const float4 v = *reinterpret_cast<const float4*>(a.part_o + slot_of(k) * D + 4 * c);
-    const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
-    sum += f * ml.y;
-    o = make_float4(o.x + f * v.x, o.y + f * v.y, o.z + f * v.z, o.w + f * v.w);
+    for (int k = mine; k < parts; k += kGroups) {
+      const float2 ml = stats(k);
+      const float4 v = *reinterpret_cast<const float4*>(a.part_o + slot_of(k) * D + 4 * c);
+      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+      sum += f * ml.y;
+      o = make_float4(o.x + f * v.x, o.y + f * v.y, o.z + f * v.z, o.w + f * v.w);
+    }
+    if (map > 0) __syncthreads();
+    s_o[mine][c] = o;
+    if (c == 0) s_ml[mine].y = sum;
+    __syncthreads();
+    for (int k = 1; mine == 0 && k < kGroups; ++k) {
+      const float4 v = s_o[k][c];
+      sum += s_ml[k].y;
+      o = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+    }
+    x[map] = o;
+    l[map] = sum;
   }
-  s_o[mine][c] = o;
-  if (c == 0) s_ml[mine].y = sum;
-  __syncthreads();
-  if (mine != 0) return;
-  for (int k = 1; k < kGroups; ++k) {
-    const float4 v = s_o[k][c];
-    sum += s_ml[k].y;
-    o = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+  if constexpr (kForm == kDiff) {
+    if (threadIdx.x < 32) store_difference<D, kF16>(a, mine == 0, j.x, j.y + (int)blockIdx.y, c, x, l);
+  } else if (mine == 0) {
+    store_result<kF16>(a, j.x, j.y + blockIdx.y, 4 * c, x[0].x, x[0].y, top, l[0]);
+    const float inv = over(l[0]);
+    *reinterpret_cast<uint32_t*>(static_cast<char*>(a.out) + 2 * (j.x * a.out_token + (j.y + (int)blockIdx.y) * a.out_head + 4 * c + 2)) = pack_16x2<kF16>(x[0].z * inv, x[0].w * inv);
   }
-  store_result<kF16>(a, j.x, j.y + blockIdx.y, 4 * c, o.x, o.y, top, sum);
-  const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
-  *reinterpret_cast<uint32_t*>(static_cast<char*>(a.out) + 2 * (j.x * a.out_token + (j.y + (int)blockIdx.y) * a.out_head + 4 * c + 2)) = pack_16x2<kF16>(o.z * inv, o.w * inv);
 }
 
 // Dynamic shared memory of a kernel, set once on a device (`known`: the devices that have it; half a microsecond a call otherwise)
@@ -575,9 +691,9 @@ inline int allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>* know
 //   16 / 2 of 128: 128 of 1000 (256, 63) 27.2 / 29.2 / 42, 97, 158 / 34
 //   ragged, 48 of 500 to 8192 (384, 512) 203 / 179 / 166, 273, 368 / 138; 16 of 100 to 16000 (128, 1000) 208 / 138 / 147, 146, 210 / 109
 struct PagedWay { int cluster, warps; bool shares; };
-inline PagedWay paged_way(int T, int Hq, int Hk, int D, int64_t max_keys, int window, int sinks) {
+inline PagedWay paged_way(int T, int Hq, int Hk, int D, int64_t max_keys, int window, int sinks, int item_heads = kItemHeads<kPlain>) {
   const int64_t keys = window > 0 ? std::min<int64_t>(max_keys, (int64_t)window + sinks) : max_keys, block = D == 64 ? paged_block_keys<64>() : paged_block_keys<128>();
-  const int64_t units = (keys + block - 1) / block, items = (int64_t)T * Hk * ((Hq / Hk + 15) / 16);
+  const int64_t units = (keys + block - 1) / block, items = (int64_t)T * Hk * ((Hq / Hk + item_heads - 1) / item_heads);
   PagedWay w = {8, 8, false};
   while (w.cluster > 1 && items * w.cluster > 148) w.cluster /= 2;
   if (units < (w.cluster == 2 ? 64 : 20)) w.cluster = 1;
@@ -587,15 +703,17 @@ inline PagedWay paged_way(int T, int Hq, int Hk, int D, int64_t max_keys, int wi
 }
 
 inline size_t paged_parts_bytes(int heads, int D) { return (size_t)2 * kPagedCtas * heads * D * 4; }
+// (heads: sets of sums, of one head or of one map of a head)
+template <int kForm = kPlain>
 inline size_t paged_workspace_bytes(int T, int Hq, int Hk, int D, int64_t max_keys, int window, int sinks) {
-  if (!paged_way(T, Hq, Hk, D, max_keys, window, sinks).shares) return 0;
-  const int heads = std::min(Hq / Hk, 16);
+  if (!paged_way(T, Hq, Hk, D, max_keys, window, sinks, kItemHeads<kForm>).shares) return 0;
+  const int heads = std::min(Hq / Hk, kItemHeads<kForm>) * kMaps<kForm>;
   return paged_parts_bytes(heads, D) + (size_t)2 * kPagedCtas * heads * 8 + kPagedCtas * sizeof(int4);
 }
 
-template <int D, int NT, bool kF16, int kWay, int kWarps>
+template <int D, int NT, bool kF16, int kWay, int kWarps, int kForm>
 inline int paged_decode_launch_t(const PagedArgs& a, int ctas, int cluster, cudaStream_t stream) {
-  const auto kernel = paged_decode_kernel<D, NT, kF16, kWay, kWarps>;
+  const auto kernel = paged_decode_kernel<D, NT, kF16, kWay, kWarps, kForm>;
   static std::atomic<uint64_t> known{0};
   if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), paged_smem<D, NT>(kWarps), &known)) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -617,37 +735,41 @@ inline int paged_decode_launch_t(const PagedArgs& a, int ctas, int cluster, cuda
     return fail(B200_LORA_ECUDA, "paged_decode_kernel launch: %s", cudaGetErrorString(e));
   }
   if (kWay != kShares) return B200_LORA_OK;
-  return launch_dependent(paged_join_kernel<D, kF16>, "paged_join_kernel", dim3((unsigned)ctas, (unsigned)a.heads), kJoinThreads, 0, stream, a);
+  return launch_dependent(paged_join_kernel<D, kF16, kForm>, "paged_join_kernel", dim3((unsigned)ctas, (unsigned)a.heads), kJoinThreads, 0, stream, a);
 }
 
-template <int D, int NT, bool kF16>
+template <int D, int NT, bool kF16, int kForm>
 inline int paged_decode_launch_by(const PagedArgs& a, cudaStream_t stream) {
-  const PagedWay w = paged_way(a.T, a.Hq, a.Hk, D, (int64_t)a.table_width * a.cache.block_size, a.window, a.sinks);
-  if (w.shares && a.part_o != nullptr) return paged_decode_launch_t<D, NT, kF16, kShares, 4>(a, kPagedCtas, 1, stream);
+  const PagedWay w = paged_way(a.T, a.Hq, a.Hk, D, (int64_t)a.table_width * a.cache.block_size, a.window, a.sinks, kItemHeads<kForm>);
+  if (w.shares && a.part_o != nullptr) return paged_decode_launch_t<D, NT, kF16, kShares, 4, kForm>(a, kPagedCtas, 1, stream);
   const int64_t items = (int64_t)a.T * a.Hk * a.chunks;
   const int ctas = (int)std::min<int64_t>((w.warps == 8 ? 148 : kPagedCtas) / w.cluster, items) * w.cluster;
-  if (w.cluster > 1) return paged_decode_launch_t<D, NT, kF16, kClusters, 8>(a, ctas, w.cluster, stream);
-  if (w.warps == 8) return paged_decode_launch_t<D, NT, kF16, kWhole, 8>(a, ctas, 1, stream);
-  return paged_decode_launch_t<D, NT, kF16, kWhole, 4>(a, ctas, 1, stream);
+  if (w.cluster > 1) return paged_decode_launch_t<D, NT, kF16, kClusters, 8, kForm>(a, ctas, w.cluster, stream);
+  if (w.warps == 8) return paged_decode_launch_t<D, NT, kF16, kWhole, 8, kForm>(a, ctas, 1, stream);
+  return paged_decode_launch_t<D, NT, kF16, kWhole, 4, kForm>(a, ctas, 1, stream);
 }
 
+template <int D, int kForm>
+inline int paged_decode_launch_d(const PagedArgs& a, bool f16, cudaStream_t stream) {
+  if (kForm == kDiff || a.heads > 8) return f16 ? paged_decode_launch_by<D, 2, true, kForm>(a, stream) : paged_decode_launch_by<D, 2, false, kForm>(a, stream);
+  constexpr int NT = kForm == kDiff ? 2 : 1;
+  return f16 ? paged_decode_launch_by<D, NT, true, kForm>(a, stream) : paged_decode_launch_by<D, NT, false, kForm>(a, stream);
+}
+
+template <int kForm = kPlain>
 inline int paged_decode_launch(PagedArgs a, int D, int dtype, void* workspace, cudaStream_t stream) {
   const int group = a.Hq / a.Hk;
-  a.heads = std::min(group, 16);
+  a.heads = std::min(group, kItemHeads<kForm>);
   a.chunks = ceil_div_i(group, a.heads);
   if (workspace != nullptr) {  // (null: no shares)
+    const int sums = a.heads * kMaps<kForm>;
     char* ws = static_cast<char*>(workspace);
     a.part_o = reinterpret_cast<float*>(ws);
-    a.part_ml = reinterpret_cast<float*>(ws + paged_parts_bytes(a.heads, D));
-    a.joins = reinterpret_cast<int4*>(ws + paged_parts_bytes(a.heads, D) + (size_t)2 * kPagedCtas * a.heads * 8);
+    a.part_ml = reinterpret_cast<float*>(ws + paged_parts_bytes(sums, D));
+    a.joins = reinterpret_cast<int4*>(ws + paged_parts_bytes(sums, D) + (size_t)2 * kPagedCtas * sums * 8);
   }
-  const bool f16 = dtype == B200_LORA_F16, wide = a.heads > 8;
-  if (D == 64) {
-    if (wide) return f16 ? paged_decode_launch_by<64, 2, true>(a, stream) : paged_decode_launch_by<64, 2, false>(a, stream);
-    return f16 ? paged_decode_launch_by<64, 1, true>(a, stream) : paged_decode_launch_by<64, 1, false>(a, stream);
-  }
-  if (wide) return f16 ? paged_decode_launch_by<128, 2, true>(a, stream) : paged_decode_launch_by<128, 2, false>(a, stream);
-  return f16 ? paged_decode_launch_by<128, 1, true>(a, stream) : paged_decode_launch_by<128, 1, false>(a, stream);
+  const bool f16 = dtype == B200_LORA_F16;
+  return D == 64 ? paged_decode_launch_d<64, kForm>(a, f16, stream) : paged_decode_launch_d<128, kForm>(a, f16, stream);
 }
 
 }  // namespace b200lora

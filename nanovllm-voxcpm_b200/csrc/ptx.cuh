@@ -272,6 +272,10 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 __device__ __forceinline__ float2 unpack_f16x2(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
 template <bool kF16>
 __device__ __forceinline__ uint32_t pack_16x2(float lo, float hi) { return kF16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi); }
+template <bool kF16>
+__device__ __forceinline__ float2 unpack_16x2(uint32_t v) {
+  return kF16 ? unpack_f16x2(v) : make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
 // what the two numbers of `packed` = pack_16x2(lo, hi) left over, rounded to the same type
 template <bool kF16>
 __device__ __forceinline__ uint32_t pack_rest(float lo, float hi, uint32_t packed) {
