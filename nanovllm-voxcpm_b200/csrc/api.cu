@@ -459,7 +459,9 @@ int lora_b200_paged_prefill_attention(void* out, int64_t out_token, int64_t out_
 size_t lora_b200_differential_workspace_bytes(int32_t T, int32_t n_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                                               int32_t table_width, int32_t block_size, int32_t window, int32_t sinks, int32_t packed) {
   if (num_kv_heads < 1 || num_heads < num_kv_heads || head_dim < 1 || block_size < 1) return 0;
-  return paged_workspace_bytes<kDiff>(T, num_heads, num_kv_heads, head_dim, (int64_t)table_width * block_size, window, sinks);
+  const int64_t keys = (int64_t)table_width * block_size;
+  if (packed) return paged_prefill_workspace_bytes<kDiff>(T, n_seqs, num_heads, num_kv_heads, head_dim, block_size, keys, window);
+  return paged_workspace_bytes<kDiff>(T, num_heads, num_kv_heads, head_dim, keys, window, sinks);
 }
 
 int lora_b200_differential_attention(void* out, int64_t out_token, int64_t out_head, const void* q, int64_t q_token, int64_t q_head,
@@ -485,6 +487,7 @@ int lora_b200_differential_attention(void* out, int64_t out_token, int64_t out_h
   if ((rc = workspace_short(what, need, workspace, workspace_bytes)) != B200_LORA_OK) return rc;
   a.lam = lam; a.lam_token = lam_token; a.lam_head = lam_head; a.norm_weight = norm_weight; a.eps = eps;
   void* const ws = need > 0 ? workspace : nullptr;
+  if (cu_seqlens != nullptr) return paged_prefill_launch<kDiff>(a, head_dim, dtype, ws, static_cast<cudaStream_t>(stream));
   return paged_decode_launch<kDiff>(a, head_dim, dtype, ws, static_cast<cudaStream_t>(stream));
 }
 

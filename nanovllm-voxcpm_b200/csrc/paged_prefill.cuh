@@ -37,8 +37,11 @@ template <int D>
 __host__ __device__ constexpr int pp_stages(int tiles) { return (D == 64 ? 1 : 0) + tiles; }
 template <int D>
 __host__ __device__ constexpr int pp_tile() { return kPpKeys * D * 2; }
+// Tiles of a CTA, and how many of them have rows of their own: the two maps of differential heads are two tiles of the same rows.
+__host__ __device__ constexpr int pp_tiles(int D, int form) { return D == 64 && form != kDiff ? 1 : 2; }
+__host__ __device__ constexpr int pp_row_tiles(int D, int form) { return form == kDiff ? 1 : pp_tiles(D, form); }
 template <int D>
-__host__ __device__ constexpr int pp_smem(int tiles) { return (2 * pp_stages<D>(tiles) + tiles) * pp_tile<D>() + tiles * kPpRows * kPpOutPitch + 1024; }
+__host__ __device__ constexpr int pp_smem(int tiles, int row_tiles) { return (2 * pp_stages<D>(tiles) + row_tiles) * pp_tile<D>() + tiles * kPpRows * kPpOutPitch + 1024; }
 
 // Items that do not fill a wave of CTAs may be cut into parts along the keys, joined by a second launch: us, whole / cut, 16 / 2 heads,
 // 16 tokens behind 8192 keys (heads of 128) 112 / 29, behind 65536 844 / 56, 500 behind 3000 (64) 42 / 25; 32 / 8 of 128, 4096 behind
@@ -232,29 +235,32 @@ __host__ __device__ constexpr int pp_slot_floats(int tiles) { return tiles * kPp
 // Of the item whose parts the CTAs c, c + stride, ... (`parts` of them) hold; parts < 2: none
 struct PpJoin { int head0, token0, n_here, parts, stride, pad[3]; };
 
-template <int D, bool kF16, int kTiles, bool kSplit>
-__global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_kernel(const __grid_constant__ PpMaps maps, const __grid_constant__ PpArgs a) {
+// kForm kDiff: the tiles are the two maps of the same rows, over the same K and V: scores take half of the columns each, a warpgroup
+// ends with half of the columns of both maps' O.
+template <int D, bool kF16, bool kSplit, int kForm>
+__global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D, kForm)) paged_prefill_kernel(const __grid_constant__ PpMaps maps, const __grid_constant__ PpArgs a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  constexpr int kSt = pp_stages<D>(kTiles), kTile = pp_tile<D>(), kPanels = D / 64;
+  constexpr int kTiles = pp_tiles(D, kForm), kRowTiles = pp_row_tiles(D, kForm), kSt = pp_stages<D>(kTiles), kTile = pp_tile<D>(), kPanels = D / 64;
   // Where the columns allow it P has its own, and S of the next tile is made while this one's softmax runs; the softmax is then all
   // there is to wait for, and an eighth of the exponentials on the FMA units pays. (8192 tokens, 16 / 2 heads of 64: 208 us with P in
   // S, 198 with columns of its own, 190 with an eighth, 197 with a quarter, 233 with half; heads of 128 gain from neither.)
   constexpr bool kOwnP = kTiles == 1 && D == 64;
   constexpr int kLoader = 4 * kTiles, kIssuer = kLoader + 1, kTmem = 256 * kTiles, kO = kTiles * kPpKeys;  // warps; columns: all, the first of O
   enum { Q_FULL, Q_FREE, S_READY, P_READY = S_READY + 2, O_DONE = P_READY + 4, K_FULL = O_DONE + 2, K_FREE = K_FULL + kSt, V_FULL = K_FREE + kSt,
-         V_FREE = V_FULL + kSt, PIECE = V_FREE + kSt, TAKEN = PIECE + 2, S_TAKEN = TAKEN + 2, PV_DONE, N_BARS };
+         V_FREE = V_FULL + kSt, PIECE = V_FREE + kSt, TAKEN = PIECE + 2, S_TAKEN = TAKEN + 2, PV_DONE, SHARED, N_BARS };
   __shared__ __align__(8) uint64_t bars[N_BARS];
   __shared__ uint32_t s_tmem, s_boxes[4];
   __shared__ PpPiece s_piece[2];
   __shared__ volatile int abort_flag;
+  __shared__ float s_sums[kForm == kDiff ? 2 : 1][kTiles][kPpRows];  // what the maps tell each other: sums, sums of squares
   const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
   const PagedArgs& p = a.p;
   // (V first: what a wrong stride of its descriptor could reach stays inside the allocation)
-  const uint32_t raw = smem_u32(smem_raw), v_u32 = (raw + 1023u) & ~1023u, k_u32 = v_u32 + kSt * kTile, q_u32 = k_u32 + kSt * kTile, out_u32 = q_u32 + kTiles * kTile;
+  const uint32_t raw = smem_u32(smem_raw), v_u32 = (raw + 1023u) & ~1023u, k_u32 = v_u32 + kSt * kTile, q_u32 = k_u32 + kSt * kTile, out_u32 = q_u32 + kRowTiles * kTile;
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
 
   if (tid == 0) {
-    for (int i = 0; i < N_BARS; ++i) mbar_init(bar(i), (i >= P_READY && i < O_DONE) || i == S_TAKEN ? kPpRows : i == TAKEN || i == TAKEN + 1 ? 4 * kTiles + 1 : 1);
+    for (int i = 0; i < N_BARS; ++i) mbar_init(bar(i), (i >= P_READY && i < O_DONE) || i == S_TAKEN ? kPpRows : i == SHARED ? 2 * kPpRows : i == TAKEN || i == TAKEN + 1 ? 4 * kTiles + 1 : 1);
     abort_flag = 0;
     mbar_fence_init();
   }
@@ -264,7 +270,7 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
   tc_fence_after_sync();
   glue_enter();  // (dependents may start: every CTA of this launch holds its tensor memory by then)
   const uint32_t tmem = s_tmem;
-  const int per_tile = kPpRows >> a.h_shift, span = kTiles * per_tile;
+  const int per_tile = kPpRows >> a.h_shift, span = kRowTiles * per_tile;
 
   // Pieces come from the loading warp through two places in shared memory.
   auto take = [&](int k, PpPiece* w) {
@@ -276,18 +282,18 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
   };
   if (warp < kLoader) {  // ------------------------------------------------------------------- softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPpSoftmaxRegs));
-    const int t = warp >> 2, row = (warp & 3) * 32 + lane, tok = t * per_tile + (row >> a.h_shift);
+    const int t = warp >> 2, row = (warp & 3) * 32 + lane, tok0 = (kForm == kDiff ? 0 : t) * per_tile, tok = tok0 + (row >> a.h_shift);
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + t * kPpKeys + lanes, o_at = tmem + kO + t * D + lanes, p_at = kOwnP ? tmem + kO + D + lanes : s_at;
     const uint32_t all_boxes = bits_below(kPpKeys / a.box);
     const int tile_shift = 7 - a.box_shift, step = min(a.box, 32);  // boxes of a tile, as a logarithm; columns of 32 that lie in one box
     const uint32_t stage = out_u32 + warp * (32 * kPpOutPitch);  // 32 columns of the warp's rows on their way out
-    uint32_t n = 0, pieces = 0;  // tiles and pieces with tiles so far: phases of the barriers
+    uint32_t n = 0, pieces = 0, exchanges = 0;  // tiles and pieces with tiles so far: phases of the barriers
     PpPiece w;
     for (int k = 0; take(k, &w); ++k) {
       const int pos = pp_position(w.pos0, tok);
       const int lo = p.window > 0 ? max(pos, 0) - (p.window - 1) : 0;
-      const int tile_lo = pp_position(w.pos0, t * per_tile), tile_hi = pp_position(tile_lo, per_tile - 1);  // positions of the tile
+      const int tile_lo = pp_position(w.pos0, tok0), tile_hi = pp_position(tile_lo, per_tile - 1);  // positions of the tile
       // tiles [clear0, clear1) need no mask: behind the first tokens, from where every row's window has begun, up to the first row
       const int w_lo = p.window > 0 ? max(tile_hi, 0) - (p.window - 1) : 0;
       const int clear0 = (w.sink_boxes + max(0, (int)(((uint32_t)max(w_lo, 0) + a.box - 1u) >> a.box_shift) - w.first_box) + (1 << tile_shift) - 1) >> tile_shift;
@@ -383,18 +389,89 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
       if (any) {
         if (kOwnP) pp_wait(bar(PV_DONE), (n - 1) & 1, &abort_flag);
         else pp_wait(bar(O_DONE + t), pieces & 1, &abort_flag);
+        if (kForm == kDiff && whole) pp_wait(bar(O_DONE + (t ^ 1)), pieces & 1, &abort_flag);
         ++pieces;
         tc_fence_after_sync();
       }
-      if (whole) {
+      auto whose = [&](int r) { return (warp & 3) * 32 + 8 * r + (lane >> 2); };  // row that the lane stores in round r
+      auto stored = [&](int r, int col) {  // its columns from `col` on in out, null: not there
+        const int of = whose(r), its = tok0 + (of >> a.h_shift);
+        return its < w.n_here ? static_cast<char*>(p.out) + 2 * ((token0 + its) * p.out_token + (w.head0 + (of & ((1 << a.h_shift) - 1))) * p.out_head + col) + 16 * (lane & 3) : nullptr;
+      };
+      if (kForm == kDiff && whole) {
+        // Half of the columns of both maps: their sums go through shared memory, then the sums of squares of the halves. Behind the
+        // second exchange every thread has its columns of O, which the next piece may then overwrite.
+        auto exchange = [&](int which, float v) {
+          s_sums[which][t][row] = v;
+          tc_fence_before_sync();
+          mbar_arrive(bar(SHARED));
+          pp_wait(bar(SHARED), exchanges & 1, &abort_flag);
+          ++exchanges;
+          tc_fence_after_sync();
+          return s_sums[which][t ^ 1][row];
+        };
+        const float other = over(exchange(0, l));
+        const float lam = live ? p.lam[(token0 + tok) * p.lam_token + (w.head0 + (row & ((1 << a.h_shift) - 1))) * p.lam_head] : 0.f;
+        const float one = t == 0 ? inv : other, two = lam * (t == 0 ? other : inv);
+        float y[D / 2], ss = 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          uint32_t o1[32], o2[32];
+          const uint32_t at = tmem + kO + t * (D / 2) + 32 * c + lanes;
+          if (any) {
+            tmem_ld_32x32(at, o1);
+            tmem_ld_32x32(at + D, o2);
+            tmem_ld_wait();
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {  // (both products rounded: equal maps cancel)
+            y[32 * c + j] = any ? __fmul_rn(__uint_as_float(o1[j]), one) - __fmul_rn(__uint_as_float(o2[j]), two) : 0.f;
+            ss += y[32 * c + j] * y[32 * c + j];
+          }
+        }
+        ss += exchange(1, ss);
+        const float r = p.norm_weight != nullptr ? rsqrtf(ss * (1.f / D) + p.eps) : 1.f;
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          const int col = t * (D / 2) + 32 * c;
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            float f[8];
+            if (p.norm_weight != nullptr) {
+              const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const char*>(p.norm_weight) + 2 * (col + j));
+              const uint32_t raw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float2 u = unpack_16x2<kF16>(raw[i]);
+                f[2 * i] = r * u.x;
+                f[2 * i + 1] = r * u.y;
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) f[i] = 1.f;
+            }
+            const float* const x = y + 32 * c + j;
+            uint4 v;
+            v.x = pack_16x2<kF16>(x[0] * f[0], x[1] * f[1]);
+            v.y = pack_16x2<kF16>(x[2] * f[2], x[3] * f[3]);
+            v.z = pack_16x2<kF16>(x[4] * f[4], x[5] * f[5]);
+            v.w = pack_16x2<kF16>(x[6] * f[6], x[7] * f[7]);
+            sts128(stage + lane * kPpOutPitch + 2 * j, v);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            char* const dst = stored(i, col);
+            if (dst != nullptr) stg128(dst, lds128(stage + (8 * i + (lane >> 2)) * kPpOutPitch + 16 * (lane & 3)));
+          }
+          __syncwarp();
+        }
+      } else if (whole) {
         // Through shared memory, so that four lanes write 64 adjacent bytes of a row. (A row's pieces straight from its thread: 32
         // half-used sectors a store, 3200 cycles for a tile of 128 columns.)
         char* dst[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int of = (warp & 3) * 32 + 8 * r + (lane >> 2), its = t * per_tile + (of >> a.h_shift);
-          dst[r] = its < w.n_here ? static_cast<char*>(p.out) + 2 * ((token0 + its) * p.out_token + (w.head0 + (of & ((1 << a.h_shift) - 1))) * p.out_head) + 16 * (lane & 3) : nullptr;
-        }
+        for (int r = 0; r < 4; ++r) dst[r] = stored(r, 0);
         uint32_t all[D / 32][32];
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
@@ -499,8 +576,8 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
             if (pieces > 0) pp_wait(bar(Q_FREE), (pieces - 1) & 1, &abort_flag);
             ++pieces;
             if (leader) {
-              mbar_arrive_expect_tx(bar(Q_FULL), kTiles * kTile);
-              for (int t = 0; t < kTiles; ++t)
+              mbar_arrive_expect_tx(bar(Q_FULL), kRowTiles * kTile);
+              for (int t = 0; t < kRowTiles; ++t)
                 for (int c = 0; c < kPanels; ++c)
                   tma_load_3d_at(q_u32 + t * kTile + c * kPpPanel, &maps.q, 64 * c, w.head0, w.begin + w.q0 + t * per_tile, bar(Q_FULL));
             }
@@ -534,10 +611,12 @@ __global__ void __launch_bounds__(pp_threads(kTiles), 3 - kTiles) paged_prefill_
       auto lo_k = [](uint32_t addr) { return ((addr & 0x3FFFF) >> 4) | (1u << 16); };
       auto lo_v = [](uint32_t addr) { return ((addr & 0x3FFFF) >> 4) | ((uint32_t)(kPpPanel >> 4) << 16); };  // 64-column panels
       auto scores = [&](int t, int st) {
+        constexpr int kSteps = D / 16 / kMaps<kForm>;
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
+        for (int i = 0; i < kSteps; ++i) {
+          const int k = (kForm == kDiff ? t * kSteps : 0) + i;
           const uint32_t at = (k >> 2) * kPpPanel + (k & 3) * 32;
-          umma_elected(tmem + t * kPpKeys, lo_k(q_u32 + t * kTile + at), lo_k(k_u32 + st * kTile + at), hi_k, idesc_s, k > 0, leader);
+          umma_elected(tmem + t * kPpKeys, lo_k(q_u32 + (kForm == kDiff ? 0 : t * kTile) + at), lo_k(k_u32 + st * kTile + at), hi_k, idesc_s, i > 0, leader);
         }
         umma_commit_elected(bar(S_READY + t), leader);
       };
@@ -664,6 +743,76 @@ __global__ void __launch_bounds__(kTiles * kPpRows) paged_prefill_join_kernel(co
   if (c0 == 0 && p.lse != nullptr) p.lse[token * p.Hq + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
+// The same for differential heads: 32 rows of the item (blockIdx.y), a warp per 16 columns, of both maps (the tiles of a part); the sums
+// of squares of a row meet in shared memory.
+template <int D, bool kF16>
+__global__ void __launch_bounds__(2 * D) paged_prefill_join_maps_kernel(const __grid_constant__ PpArgs a) {
+  __shared__ float s_squares[D / 16][32];
+  glue_enter();
+  const PpJoin j = static_cast<const PpJoin*>(a.joins)[blockIdx.x];
+  if (j.parts < 2) return;
+  const PagedArgs& p = a.p;
+  const int lane = threadIdx.x & 31, group = threadIdx.x >> 5, row = 32 * blockIdx.y + lane, tok = row >> a.h_shift, c0 = 4 * group;
+  const bool live = tok < j.n_here;
+  const int head = j.head0 + (row & ((1 << a.h_shift) - 1));
+  const int64_t token = (int64_t)j.token0 + tok;
+  const float* const first = a.parts + (int64_t)blockIdx.x * pp_slot_floats<D>(2);
+  const int64_t step = (int64_t)j.stride * pp_slot_floats<D>(2);
+  float y[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) y[i] = 0.f;
+  for (int map = 0; live && map < 2; ++map) {
+    auto stats = [&](int k) { return reinterpret_cast<const float2*>(first + k * step + 2 * kPpRows * D)[map * kPpRows + row]; };
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < j.parts; ++k) top = fmaxf(top, stats(k).x);
+    float4 o[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int k = 0; k < j.parts; ++k) {
+      const float2 ml = stats(k);
+      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+      sum += f * ml.y;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float4 v = reinterpret_cast<const float4*>(first + k * step)[(map * (D / 4) + c0 + c) * kPpRows + row];
+        o[c] = make_float4(o[c].x + f * v.x, o[c].y + f * v.y, o[c].z + f * v.z, o[c].w + f * v.w);
+      }
+    }
+    const float f = map == 0 ? over(sum) : p.lam[token * p.lam_token + head * p.lam_head] * over(sum);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float x[4] = {o[c].x, o[c].y, o[c].z, o[c].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[4 * c + i] = map == 0 ? __fmul_rn(x[i], f) : y[4 * c + i] - __fmul_rn(x[i], f);
+    }
+  }
+  if (p.norm_weight != nullptr) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) ss += y[i] * y[i];
+    s_squares[group][lane] = ss;
+    __syncthreads();
+    ss = 0.f;
+#pragma unroll
+    for (int g = 0; g < D / 16; ++g) ss += s_squares[g][lane];
+    const float r = rsqrtf(ss * (1.f / D) + p.eps);
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      const float2 w = unpack_16x2<kF16>(*reinterpret_cast<const uint32_t*>(static_cast<const char*>(p.norm_weight) + 2 * (4 * c0 + i)));
+      y[i] *= r * w.x;
+      y[i + 1] *= r * w.y;
+    }
+  }
+  if (!live) return;
+  char* const dst = static_cast<char*>(p.out) + 2 * (token * p.out_token + head * p.out_head + 4 * c0);
+#pragma unroll
+  for (int i = 0; i < 16; i += 8)
+    stg128(dst + 2 * i, make_uint4(pack_16x2<kF16>(y[i], y[i + 1]), pack_16x2<kF16>(y[i + 2], y[i + 3]), pack_16x2<kF16>(y[i + 4], y[i + 5]),
+                                   pack_16x2<kF16>(y[i + 6], y[i + 7])));
+}
+
 // ------------------------------------------------------------------ host
 inline bool pp_map(CUtensorMap* out, const void* base, bool f16, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
   const EncodeTiledFn fn = encode_tiled_fn();
@@ -695,7 +844,7 @@ inline int pp_h_shift(int group) {
 
 // Whether the tensor-core kernel takes a call: copies of 8 cache rows or more that lie in one block, a table of which every key has an
 // int, and strides that its maps take (not 0, as of heads that are expanded from one).
-inline bool paged_prefill_plan(const PagedArgs& p, int D, bool f16, int tiles, PpMaps* maps, PpArgs* a) {
+inline bool paged_prefill_plan(const PagedArgs& p, int D, bool f16, int row_tiles, PpMaps* maps, PpArgs* a) {
   if (p.cache.block_size % 8 != 0 || (int64_t)p.table_width * p.cache.block_size > kPpMaxKeys) return false;
   a->p = p;
   a->box = 8;
@@ -707,7 +856,7 @@ inline bool paged_prefill_plan(const PagedArgs& p, int D, bool f16, int tiles, P
   a->h_shift = pp_h_shift(p.Hq / p.Hk);
   a->head_tiles = p.Hq >> a->h_shift;
   const int per_tile = kPpRows >> a->h_shift;
-  const int64_t blocks = (int64_t)p.T / (tiles * per_tile) + p.n_req;
+  const int64_t blocks = (int64_t)p.T / (row_tiles * per_tile) + p.n_req;
   if (blocks * a->head_tiles > INT32_MAX) return false;
   a->n_blocks = (int)blocks;
   const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)p.Hq, (cuuint64_t)p.T};
@@ -720,50 +869,54 @@ inline bool paged_prefill_plan(const PagedArgs& p, int D, bool f16, int tiles, P
 
 // Whether a launch cuts the items that do not fill a wave of CTAs into parts, as told by what the host knows: items at most, and
 // tiles of an item at most.
-inline bool pp_splits(int T, int n_req, int Hq, int h_shift, int tiles, int64_t max_context, int window) {
-  const int span = tiles * (kPpRows >> h_shift);
+inline bool pp_splits(int T, int n_req, int Hq, int h_shift, int row_tiles, int ctas, int64_t max_context, int window) {
+  const int span = row_tiles * (kPpRows >> h_shift);
   const int64_t items = ((int64_t)T / span + n_req) * (Hq >> h_shift);
   const int64_t keys = window > 0 ? std::min<int64_t>(max_context, (int64_t)window + span) : max_context;
-  const int wave = 148 * (3 - tiles);
-  return keys / kPpKeys >= kPpSplitTiles && (2 * items <= wave || (items <= kPpSplitWaves * wave && keys >= 2 * (int64_t)T));
+  return keys / kPpKeys >= kPpSplitTiles && (2 * items <= ctas || (items <= kPpSplitWaves * ctas && keys >= 2 * (int64_t)T));
 }
-constexpr int pp_tiles(int D) { return D == 64 ? 1 : 2; }
-inline size_t pp_split_bytes(int D) {
-  const int tiles = pp_tiles(D), ctas = 148 * (3 - tiles);
-  return (size_t)ctas * tiles * kPpRows * (D + 2) * 4 + ctas * sizeof(PpJoin);
+constexpr int pp_ctas(int D, int form) { return 148 * (3 - pp_tiles(D, form)); }
+inline size_t pp_split_bytes(int D, int form) {
+  return (size_t)pp_ctas(D, form) * pp_tiles(D, form) * kPpRows * (D + 2) * 4 + pp_ctas(D, form) * sizeof(PpJoin);
 }
 // (blocks that the tile kernel does not take: what the decode kernel needs for as many rows)
+template <int kForm = kPlain>
 inline size_t paged_prefill_workspace_bytes(int T, int n_req, int Hq, int Hk, int D, int block_size, int64_t max_context, int window) {
-  if (block_size % 8 != 0) return paged_workspace_bytes(T, Hq, Hk, D, max_context, window, 0);
-  return pp_splits(T, n_req, Hq, pp_h_shift(Hq / Hk), pp_tiles(D), max_context, window) ? pp_split_bytes(D) : 0;
+  if (block_size % 8 != 0) return paged_workspace_bytes<kForm>(T, Hq, Hk, D, max_context, window, 0);
+  return pp_splits(T, n_req, Hq, pp_h_shift(Hq / Hk), pp_row_tiles(D, kForm), pp_ctas(D, kForm), max_context, window) ? pp_split_bytes(D, kForm) : 0;
 }
 
-template <int D, bool kF16, bool kSplit>
+template <int D, bool kF16, bool kSplit, int kForm>
 inline int paged_prefill_launch_t(const PpMaps& maps, const PpArgs& a, cudaStream_t stream) {
-  constexpr int kTiles = pp_tiles(D), kCtas = 148 * (3 - kTiles);
-  const auto kernel = paged_prefill_kernel<D, kF16, kTiles, kSplit>;
-  constexpr int smem = pp_smem<D>(kTiles);
+  constexpr int kTiles = pp_tiles(D, kForm), kCtas = pp_ctas(D, kForm);
+  const auto kernel = paged_prefill_kernel<D, kF16, kSplit, kForm>;
+  constexpr int smem = pp_smem<D>(kTiles, pp_row_tiles(D, kForm));
   static std::atomic<uint64_t> known{0};
   if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), smem, &known)) return rc;
   const int ctas = kSplit ? kCtas : (int)std::min<int64_t>(kCtas, (int64_t)a.n_blocks * a.head_tiles);
   const int rc = launch_dependent(kernel, "paged_prefill_kernel", dim3((unsigned)ctas), pp_threads(kTiles), (size_t)smem, stream, maps, a);
   if (rc != B200_LORA_OK || !kSplit) return rc;
-  return launch_dependent(paged_prefill_join_kernel<D, kF16, kTiles>, "paged_prefill_join_kernel", dim3((unsigned)ctas, D / 16), kTiles * kPpRows, 0, stream, a);
+  if constexpr (kForm == kDiff)
+    return launch_dependent(paged_prefill_join_maps_kernel<D, kF16>, "paged_prefill_join_maps_kernel", dim3((unsigned)ctas, kPpRows / 32), 2 * D, 0, stream, a);
+  else
+    return launch_dependent(paged_prefill_join_kernel<D, kF16, kTiles>, "paged_prefill_join_kernel", dim3((unsigned)ctas, D / 16), kTiles * kPpRows, 0, stream, a);
 }
 
+template <int kForm = kPlain>
 inline int paged_prefill_launch(const PagedArgs& p, int D, int dtype, void* workspace, cudaStream_t stream) {
   PpMaps maps;
   PpArgs a = {};
   const bool f16 = dtype == B200_LORA_F16;
-  if (!paged_prefill_plan(p, D, f16, pp_tiles(D), &maps, &a)) return paged_decode_launch(p, D, dtype, p.cache.block_size % 8 != 0 ? workspace : nullptr, stream);
-  if (pp_splits(p.T, p.n_req, p.Hq, a.h_shift, pp_tiles(D), (int64_t)p.table_width * p.cache.block_size, p.window)) {
+  if (!paged_prefill_plan(p, D, f16, pp_row_tiles(D, kForm), &maps, &a))
+    return paged_decode_launch<kForm>(p, D, dtype, p.cache.block_size % 8 != 0 ? workspace : nullptr, stream);
+  if (pp_splits(p.T, p.n_req, p.Hq, a.h_shift, pp_row_tiles(D, kForm), pp_ctas(D, kForm), (int64_t)p.table_width * p.cache.block_size, p.window)) {
     a.parts = static_cast<float*>(workspace);
-    a.joins = static_cast<char*>(workspace) + pp_split_bytes(D) - 148 * (3 - pp_tiles(D)) * sizeof(PpJoin);
-    if (D == 64) return f16 ? paged_prefill_launch_t<64, true, true>(maps, a, stream) : paged_prefill_launch_t<64, false, true>(maps, a, stream);
-    return f16 ? paged_prefill_launch_t<128, true, true>(maps, a, stream) : paged_prefill_launch_t<128, false, true>(maps, a, stream);
+    a.joins = static_cast<char*>(workspace) + pp_split_bytes(D, kForm) - pp_ctas(D, kForm) * sizeof(PpJoin);
+    if (D == 64) return f16 ? paged_prefill_launch_t<64, true, true, kForm>(maps, a, stream) : paged_prefill_launch_t<64, false, true, kForm>(maps, a, stream);
+    return f16 ? paged_prefill_launch_t<128, true, true, kForm>(maps, a, stream) : paged_prefill_launch_t<128, false, true, kForm>(maps, a, stream);
   }
-  if (D == 64) return f16 ? paged_prefill_launch_t<64, true, false>(maps, a, stream) : paged_prefill_launch_t<64, false, false>(maps, a, stream);
-  return f16 ? paged_prefill_launch_t<128, true, false>(maps, a, stream) : paged_prefill_launch_t<128, false, false>(maps, a, stream);
+  if (D == 64) return f16 ? paged_prefill_launch_t<64, true, false, kForm>(maps, a, stream) : paged_prefill_launch_t<64, false, false, kForm>(maps, a, stream);
+  return f16 ? paged_prefill_launch_t<128, true, false, kForm>(maps, a, stream) : paged_prefill_launch_t<128, false, false, kForm>(maps, a, stream);
 }
 
 }  // namespace b200lora
