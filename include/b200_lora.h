@@ -531,6 +531,26 @@ int lora_b200_differential_attention(void* out, int64_t out_token, int64_t out_h
                                      size_t workspace_bytes, void* stream);
 
 /*
+ * Attention over a paged cache for requests that begin alike: the results of lora_b200_paged_decode_attention (cu_seqlens null, n_seqs
+ * = T) or lora_b200_paged_prefill_attention without a window, for which the common keys are read once a group instead of once a
+ * request. The sequences [cu_groups[g], cu_groups[g + 1]) have the same keys and values at their first prefix_lens[g] positions; where
+ * those lie is read from the block table of the group's first sequence, and what follows from each one's own. prefix_lens int32
+ * [n_groups], cu_groups int32 [n_groups + 1], ascending; a sequence in no group (or in one that leaves the sequences) shares nothing, a
+ * prefix of zero (or less) is none. Tokens inside the prefix see it up to themselves. A value that is not finite, of a key of the prefix
+ * that some rows of a block see, may reach the block's other rows (as in a prefill call; a block may hold rows of several sequences of
+ * the group). Sharing takes block sizes that are multiples of 8; other calls, and those without two sequences in a group, run as those
+ * two do. No counterpart in the reference.
+ */
+size_t lora_b200_shared_prefix_workspace_bytes(int32_t T, int32_t n_seqs, int32_t n_groups, int32_t num_heads, int32_t num_kv_heads,
+                                               int32_t head_dim, int32_t table_width, int32_t block_size, int32_t packed);
+int lora_b200_shared_prefix_attention(void* out, int64_t out_token, int64_t out_head, float* lse, const void* q, int64_t q_token,
+                                      int64_t q_head, int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                      const lora_b200_paged_cache* cache, const int32_t* block_tables, int64_t table_ld,
+                                      int32_t table_width, const int32_t* context_lens, const int32_t* cu_seqlens, int32_t n_seqs,
+                                      const int32_t* prefix_lens, const int32_t* cu_groups, int32_t n_groups, float scale,
+                                      int32_t dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Joins attention over n_parts (up to 64) parts of a context: outs[i] [T, num_heads, head_dim] and lses[i] float [T, num_heads] are a
  * part's result and the logarithm of its sum (as the calls above give them; -inf: no key, its values count for nothing), host arrays
  * of device addresses, the strides (in elements) the same for all parts. out = the result over all of them, lse [T, num_heads] the

@@ -158,6 +158,14 @@ _SIGNATURES = {
          c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_float, c_float, c_int32, c_int32, c_int32, c_void_p,
          c_size_t, c_void_p],
     ),
+    "lora_b200_shared_prefix_workspace_bytes": (
+        c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32],
+    ),
+    "lora_b200_shared_prefix_attention": (
+        c_int32,
+        [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, POINTER(PagedCache), c_void_p,
+         c_int64, c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_int32, c_float, c_int32, c_void_p, c_size_t, c_void_p],
+    ),
     "lora_b200_join_attention": (
         c_int32,
         [c_void_p, c_int64, c_int64, c_void_p, POINTER(c_void_p), POINTER(c_void_p), c_int32, c_int64, c_int64, c_int64, c_int64, c_int32,

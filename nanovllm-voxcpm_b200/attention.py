@@ -2,10 +2,11 @@
 of every request (``paged_decode_attention``) or packed runs of new tokens (``paged_prefill_attention``: whole prompts, chunks of
 them, a few tokens behind a long context). Causal, over everything or over a sliding window of the last keys plus a few first
 ones. Stands where the reference attends over its paged cache
-(``nanovllm_voxcpm/layers/attention.py:70-79``). Besides: the difference of two softmax maps (``differential_decode_attention``,
+(``nanovllm_voxcpm/layers/attention.py:70-79``). Besides: both for requests that begin alike, whose common keys are read once
+(``shared_prefix_decode_attention``, ``shared_prefix_prefill_attention``); the difference of two softmax maps (``differential_decode_attention``,
 ``differential_prefill_attention``), and what joins results over parts of a context (``join_attention``). The kernels are
 ``csrc/paged_attention.cuh``, ``csrc/paged_prefill.cuh`` and ``csrc/attention_join.cuh`` behind ``lora_b200_paged_*``,
-``lora_b200_differential_attention`` and ``lora_b200_join_attention``.
+``lora_b200_shared_prefix_attention``, ``lora_b200_differential_attention`` and ``lora_b200_join_attention``.
 CUDA tensors only, bf16 / fp16, heads of 64 or 128; there is no fallback path and no backward pass.
 """
 
@@ -121,6 +122,62 @@ def paged_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     if cu_seqlens is None:
         raise ValueError("cu_seqlens says which rows of q are whose: paged_prefill_attention needs it")
     return _paged_attention(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, scale, window, sinks, out, return_lse)
+
+
+def _shared_prefix(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, prefix_lens, cu_groups, scale, out, return_lse):
+    if scale is None:
+        scale = q.size(-1) ** -0.5
+    got = N.native().shared_prefix_attention(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, prefix_lens, cu_groups, scale,
+                                             out, bool(return_lse))
+    if got is not None:
+        N.check(got[0])
+        return (got[1], got[2]) if return_lse else got[1]
+    cache = _checked(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, scale, 0, 0, out, prefix_lens, cu_groups)
+    if prefix_lens.dim() != 1 or not prefix_lens.is_contiguous() or not cu_groups.is_contiguous():
+        raise ValueError("prefix_lens and cu_groups must be contiguous vectors")
+    groups = prefix_lens.numel()
+    _int32(prefix_lens, "prefix_lens", (groups,))
+    _int32(cu_groups, "cu_groups", (groups + 1,))
+    T, heads, dim = q.shape
+    with N.on_device(q.device):
+        if out is None:
+            out = torch.empty(T, heads, dim, dtype=q.dtype, device=q.device)
+        lse = torch.empty(T, heads, dtype=torch.float32, device=q.device) if return_lse else None
+        n, kv_heads, width, page = context_lens.numel(), k_cache.size(2), block_tables.size(1), k_cache.size(1)
+        need = N.lib().lora_b200_shared_prefix_workspace_bytes(T, n, groups, heads, kv_heads, dim, width, page, cu_seqlens is not None)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        N.check(N.lib().lora_b200_shared_prefix_attention(
+            out.data_ptr(), out.stride(0), out.stride(1), N.ptr(lse), q.data_ptr(), q.stride(0), q.stride(1), T, heads, kv_heads, dim,
+            ctypes.byref(cache), block_tables.data_ptr(), block_tables.stride(0), width, context_lens.data_ptr(), N.ptr(cu_seqlens), n,
+            prefix_lens.data_ptr(), cu_groups.data_ptr(), groups, float(scale), N.dtype_code(q.dtype), N.ptr(workspace), need,
+            N.current_stream(q.device)))
+    return (out, lse) if return_lse else out
+
+
+def shared_prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                                   context_lens: torch.Tensor, prefix_lens: torch.Tensor, cu_groups: torch.Tensor, *,
+                                   scale: float | None = None, out: torch.Tensor | None = None, return_lse: bool = False):
+    """``paged_decode_attention`` (without a window) of requests that begin alike: the keys that the requests of a group have in common
+    are read once for all of them. Same result, but for the order of its sums.
+
+    Requests ``cu_groups[g] : cu_groups[g + 1]`` have the same keys and values at their first ``prefix_lens[g]`` positions (any number:
+    a prefix may end inside a block, of which every request has a copy of its own). Where those lie is read from the table of the group's
+    first request, what follows from each one's own. ``prefix_lens`` int32 ``[groups]``, ``cu_groups`` int32 ``[groups + 1]``, ascending;
+    requests of no group share nothing, a prefix of zero is none. Other arguments, strides, missing blocks, contexts of no key and the
+    log sums as ``paged_decode_attention``. Block sizes that are multiples of 8; others (and calls with one request a group) are attended
+    request by request. A value that is not finite, of a key of the prefix that some requests of a group see, may reach the group's others."""
+    return _shared_prefix(q, k_cache, v_cache, block_tables, context_lens, None, prefix_lens, cu_groups, scale, out, return_lse)
+
+
+def shared_prefix_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                                    context_lens: torch.Tensor, cu_seqlens: torch.Tensor, prefix_lens: torch.Tensor,
+                                    cu_groups: torch.Tensor, *, scale: float | None = None, out: torch.Tensor | None = None,
+                                    return_lse: bool = False):
+    """``paged_prefill_attention`` (without a window) of requests that begin alike, grouped as in ``shared_prefix_decode_attention``;
+    tokens inside a prefix see it up to themselves. Rows of no sequence are not written."""
+    if cu_seqlens is None:
+        raise ValueError("cu_seqlens says which rows of q are whose: shared_prefix_prefill_attention needs it")
+    return _shared_prefix(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, prefix_lens, cu_groups, scale, out, return_lse)
 
 
 def _differential(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, lam, norm_weight, eps, scale, window, sinks, out):

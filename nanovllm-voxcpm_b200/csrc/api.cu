@@ -491,6 +491,35 @@ int lora_b200_differential_attention(void* out, int64_t out_token, int64_t out_h
   return paged_decode_launch<kDiff>(a, head_dim, dtype, ws, static_cast<cudaStream_t>(stream));
 }
 
+size_t lora_b200_shared_prefix_workspace_bytes(int32_t T, int32_t n_seqs, int32_t n_groups, int32_t num_heads, int32_t num_kv_heads,
+                                               int32_t head_dim, int32_t table_width, int32_t block_size, int32_t packed) {
+  if (num_kv_heads < 1 || num_heads < num_kv_heads || head_dim < 1 || block_size < 1 || T < 1) return 0;
+  return shared_prefix_workspace_bytes(T, n_seqs, n_groups, num_heads, num_kv_heads, head_dim, block_size, (int64_t)table_width * block_size, packed != 0);
+}
+
+int lora_b200_shared_prefix_attention(void* out, int64_t out_token, int64_t out_head, float* lse, const void* q, int64_t q_token,
+                                      int64_t q_head, int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                      const lora_b200_paged_cache* cache, const int32_t* block_tables, int64_t table_ld,
+                                      int32_t table_width, const int32_t* context_lens, const int32_t* cu_seqlens, int32_t n_seqs,
+                                      const int32_t* prefix_lens, const int32_t* cu_groups, int32_t n_groups, float scale,
+                                      int32_t dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "shared_prefix_attention";
+  PagedArgs a;
+  bool nothing;
+  int rc = paged_args(what, &a, &nothing, out, out_token, out_head, lse, q, q_token, q_head, T, num_heads, num_kv_heads, head_dim, cache,
+                      block_tables, table_ld, table_width, context_lens, cu_seqlens, n_seqs, false, scale, 0, 0, dtype, workspace);
+  if (rc != B200_LORA_OK) return rc;
+  if (n_groups < 0) return fail(B200_LORA_EINVAL, "%s: %d groups", what, n_groups);
+  if (nothing) return B200_LORA_OK;
+  if (n_groups > 0 && (prefix_lens == nullptr || cu_groups == nullptr)) return fail(B200_LORA_EINVAL, "%s: null pointer", what);
+  if (cu_seqlens == nullptr && n_seqs != T) return fail(B200_LORA_EINVAL, "%s: %d tokens, %d sequences: a decode batch has one of each", what, T, n_seqs);
+  const size_t need = lora_b200_shared_prefix_workspace_bytes(T, n_seqs, n_groups, num_heads, num_kv_heads, head_dim, table_width, cache->block_size,
+                                                              cu_seqlens != nullptr);
+  if ((rc = workspace_short(what, need, workspace, workspace_bytes)) != B200_LORA_OK) return rc;
+  a.prefix_lens = prefix_lens; a.cu_groups = cu_groups; a.n_groups = n_groups;
+  return shared_prefix_launch(a, head_dim, dtype, cu_seqlens != nullptr, need > 0 ? workspace : nullptr, static_cast<cudaStream_t>(stream));
+}
+
 int lora_b200_join_attention(void* out, int64_t out_token, int64_t out_head, float* lse, const void* const* outs, const float* const* lses,
                              int32_t n_parts, int64_t part_token, int64_t part_head, int64_t lse_token, int64_t lse_head, int32_t T,
                              int32_t num_heads, int32_t head_dim, int32_t dtype, void* stream) {

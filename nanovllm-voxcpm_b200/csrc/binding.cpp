@@ -48,6 +48,8 @@ decltype(&lora_b200_paged_prefill_attention) p_paged_prefill = nullptr;
 decltype(&lora_b200_differential_workspace_bytes) p_differential_bytes = nullptr;
 decltype(&lora_b200_differential_attention) p_differential = nullptr;
 decltype(&lora_b200_join_attention) p_join = nullptr;
+decltype(&lora_b200_shared_prefix_workspace_bytes) p_shared_bytes = nullptr;
+decltype(&lora_b200_shared_prefix_attention) p_shared = nullptr;
 PyObject* scratch_for = nullptr;  // lora.scratch_for(device, bytes)
 PyObject *s_weight, *s_lora_a, *s_tts, *s_sorted, *s_ids, *s_counts, *s_offsets, *s_num_active;
 
@@ -717,6 +719,37 @@ PyObject* differential_attention(PyObject*, PyObject* const* args, Py_ssize_t na
   END_HANDLE_TH_ERRORS
 }
 
+// shared_prefix_attention(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens | None, prefix_lens, cu_groups, scale, out | None,
+// lse?) -> (status, out, lse | None), or None
+PyObject* shared_prefix_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 11) { PyErr_SetString(PyExc_TypeError, "shared_prefix_attention takes 11 arguments"); return nullptr; }
+  PagedCall c;
+  if (!c.read(args)) return not_handled();
+  const at::Tensor *lens = tensor_of(args[6]), *groups = tensor_of(args[7]);
+  if (!lens || !groups) return not_handled();
+  for (const at::Tensor* t : {lens, groups})
+    if (!on(*t, c.dev) || t->scalar_type() != at::kInt || t->dim() != 1 || !t->is_contiguous()) return not_handled();
+  if (groups->numel() != lens->numel() + 1 || lens->numel() > INT32_MAX - 1) return not_handled();
+  const double scale = PyFloat_AsDouble(args[8]);
+  if (PyErr_Occurred()) { PyErr_Clear(); return not_handled(); }
+  if (!c.result(args[9])) return not_handled();
+  at::Tensor lse;
+  if (args[10] == Py_True) lse = at::empty({c.T, c.hq}, c.q->options().dtype(at::kFloat));
+  const int n_groups = (int)lens->numel();
+  const size_t need = p_shared_bytes((int)c.T, (int)c.n, n_groups, (int)c.hq, (int)c.hk, (int)c.d, c.width, c.cache.block_size, c.cu != nullptr);
+  void* const ws = c.workspace(need);
+  const int rc = p_shared(c.out->data_ptr(), c.out->stride(0), c.out->stride(1), lse.defined() ? static_cast<float*>(lse.data_ptr()) : nullptr,
+                          c.q->data_ptr(), c.q->stride(0), c.q->stride(1), (int)c.T, (int)c.hq, (int)c.hk, (int)c.d, &c.cache, c.ints(c.tables),
+                          c.tables->stride(0), c.width, c.ints(c.ctx), c.ints(c.cu), (int)c.n, c.ints(lens), c.ints(groups), n_groups, (float)scale,
+                          c.code, ws, need, c.stream());
+  PyObject* lse_out = Py_None;
+  if (lse.defined()) lse_out = THPVariable_Wrap(lse);
+  else Py_INCREF(Py_None);
+  return Py_BuildValue("(iNN)", rc, c.wrapped(args[9]), lse_out);
+  END_HANDLE_TH_ERRORS
+}
+
 // join_attention(outs, lses, out | None, lse?) -> (status, out, lse | None), or None; outs and lses: tuples of tensors
 PyObject* join_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -1108,6 +1141,8 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   B200_BIND(p_differential_bytes, lora_b200_differential_workspace_bytes)
   B200_BIND(p_differential, lora_b200_differential_attention)
   B200_BIND(p_join, lora_b200_join_attention)
+  B200_BIND(p_shared_bytes, lora_b200_shared_prefix_workspace_bytes)
+  B200_BIND(p_shared, lora_b200_shared_prefix_attention)
 #undef B200_BIND
   Py_INCREF(args[1]);
   Py_XDECREF(scratch_for);
@@ -1117,7 +1152,7 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 #define B200_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {B200_METHOD(add), B200_METHOD(shrink), B200_METHOD(expand), B200_METHOD(linear), B200_METHOD(add_rms_norm), B200_METHOD(silu_mul),
-                         B200_METHOD(rope_kv_store), B200_METHOD(qk_norm_rope_kv_store), B200_METHOD(paged_attention), B200_METHOD(differential_attention), B200_METHOD(join_attention), B200_METHOD(prefill_layers), B200_METHOD(bucket_lists), B200_METHOD(pack_lists), B200_METHOD(bind), {nullptr, nullptr, 0, nullptr}};
+                         B200_METHOD(rope_kv_store), B200_METHOD(qk_norm_rope_kv_store), B200_METHOD(paged_attention), B200_METHOD(differential_attention), B200_METHOD(join_attention), B200_METHOD(shared_prefix_attention), B200_METHOD(prefill_layers), B200_METHOD(bucket_lists), B200_METHOD(pack_lists), B200_METHOD(bind), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "b200lora_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

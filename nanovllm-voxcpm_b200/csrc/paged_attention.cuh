@@ -43,17 +43,69 @@ struct PagedArgs {
   // differential heads: what the second map counts, [T, Hq] by strides; weight [D] of the heads' norm or null
   const float* lam; int64_t lam_token, lam_head;
   const void* norm_weight; float eps;
+  // prefixes that groups of requests share: requests [cu_groups[g], cu_groups[g + 1]) begin with the same prefix_lens[g] keys. What a
+  // launch ahead leaves of them: sums over px_chunk tiles of keys each, [part, T, Hq, D] and (reference, sum) [part, T, Hq]
+  const int32_t *prefix_lens, *cu_groups; int n_groups;
+  int px_most;                                 // parts of a prefix at most
+  int* px_chunk; float2* px_ml; float* px_o;
 };
 
 // What a kernel makes of a head: one softmax map; or two, of the halves of its columns of q and k over the whole of v, and of them the
 // difference a - lam b, normed.
-constexpr int kPlain = 0, kDiff = 1;
+// Or, of requests with a common prefix: the keys of the prefix, all requests of a group side by side; the keys behind it, and the join.
+constexpr int kPlain = 0, kDiff = 1, kPrefix = 2, kSuffix = 3;
 template <int kForm> constexpr int kMaps = kForm == kDiff ? 2 : 1;
 template <int kForm> constexpr int kItemHeads = kForm == kDiff ? 8 : 16;  // q heads of an item at most
 
+// Keys of a prefix in a tile of the launch that attends to it
+constexpr int kPrefixTile = 128;
+
+// A group as both launches see it; one that leaves the requests, or whose rows leave those of q, counts as none (keys 0).
+struct PxGroup { int r0, r1, begin, end, keys; };  // requests; rows; keys of the prefix
+// (the second launch runs beside the first: it reads what earlier launches wrote past its SM's L1)
+__device__ __forceinline__ PxGroup px_group(const PagedArgs& a, int g) {
+  PxGroup p = {0, 0, 0, 0, 0};
+  if (g < 0 || g >= a.n_groups) return p;
+  const int r0 = __ldcg(a.cu_groups + g), r1 = __ldcg(a.cu_groups + g + 1), keys = __ldcg(a.prefix_lens + g);
+  if (r0 < 0 || r1 > a.n_req || r0 >= r1) return p;
+  const int begin = a.cu_seqlens == nullptr ? r0 : __ldcg(a.cu_seqlens + r0), end = a.cu_seqlens == nullptr ? r1 : __ldcg(a.cu_seqlens + r1);
+  if (begin < 0 || end > a.T || begin >= end) return p;
+  p = {r0, r1, begin, end, (int)min((int64_t)max(keys, 0), (int64_t)a.table_width * a.cache.block_size)};
+  return p;
+}
+// Keys of the prefix that request `req` shares; a whole warp calls it. Up to 32 groups are looked at side by side.
+__device__ __forceinline__ int px_keys(const PagedArgs& a, int req) {
+  if (a.n_groups <= 32) {
+    const PxGroup p = px_group(a, (int)(threadIdx.x & 31));
+    const uint32_t hit = __ballot_sync(0xffffffffu, p.r0 <= req && req < p.r1);
+    return hit == 0 ? 0 : __shfl_sync(0xffffffffu, p.keys, __ffs(hit) - 1);
+  }
+  int lo = 0, hi = a.n_groups;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldcg(a.cu_groups + mid) <= req) lo = mid;
+    else hi = mid;
+  }
+  const PxGroup p = px_group(a, lo);
+  return p.r0 <= req && req < p.r1 ? p.keys : 0;
+}
+// (behind the wait for the launch that wrote it)
+__device__ __forceinline__ int px_parts(const PagedArgs& a, int keys) {
+  const int tiles = (int)(((unsigned)keys + kPrefixTile - 1u) / kPrefixTile), chunk = max(1, __ldcg(a.px_chunk));
+  return min(a.px_most, (tiles + chunk - 1) / chunk);
+}
+
+template <int kForm>
 __device__ __forceinline__ RowKeys row_keys(const PagedArgs& a, int row) {
   RowKeys r = {row, 0, 0, -1};
   int64_t ctx;
+  if constexpr (kForm == kSuffix) {  // (one row a request)
+    ctx = max(__ldcg(a.context_lens + row), 0);
+    const int64_t held = min(ctx, (int64_t)a.table_width * a.cache.block_size);
+    r.first = px_keys(a, row);
+    r.n_keys = (int)max((int64_t)0, held - r.first);
+    return r;
+  }
   if (a.cu_seqlens == nullptr) {
     ctx = a.context_lens[row];
   } else {
@@ -145,6 +197,32 @@ __device__ __forceinline__ void store_difference(const PagedArgs& a, bool live, 
         make_uint2(pack_16x2<kF16>(y.x, y.y), pack_16x2<kF16>(y.z, y.w));
 }
 
+// Four columns of a head over the keys behind the prefix, joined with the parts over the prefix (none: 0 of them). A part without a key that
+// the row sees has no sums.
+template <int D, bool kF16>
+__device__ __forceinline__ void store_behind_prefix(const PagedArgs& a, int64_t row, int head, int c, int parts, float4 x, float m, float l) {
+  const int64_t at = row * a.Hq + head, step = (int64_t)a.T * a.Hq;
+  float top = m;
+#pragma unroll 8
+  for (int k = 0; k < parts; ++k) top = fmaxf(top, __ldcg(a.px_ml + at + k * step).x);
+  const float own = m == -INFINITY ? 0.f : ex2(m - top);
+  x = make_float4(x.x * own, x.y * own, x.z * own, x.w * own);
+  l *= own;
+#pragma unroll 8
+  for (int k = 0; k < parts; ++k) {
+    const float2 ml = __ldcg(a.px_ml + at + k * step);
+    const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+    float4 v = __ldcg(reinterpret_cast<const float4*>(a.px_o + (at + k * step) * D) + c);
+    if (ml.x == -INFINITY) v = make_float4(0.f, 0.f, 0.f, 0.f);
+    l += f * ml.y;
+    x = make_float4(x.x + f * v.x, x.y + f * v.y, x.z + f * v.z, x.w + f * v.w);
+  }
+  const float inv = over(l);
+  *reinterpret_cast<uint2*>(static_cast<char*>(a.out) + 2 * (row * a.out_token + head * a.out_head + 4 * c)) =
+      make_uint2(pack_16x2<kF16>(x.x * inv, x.y * inv), pack_16x2<kF16>(x.z * inv, x.w * inv));
+  if (a.lse != nullptr && c == 0) a.lse[at] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+}
+
 // Blocks [u0, u1) of the keys of one (row, kv head, chunk of its q heads)
 struct PagedPiece {
   int row, kvh, head0, n_heads, u0, u1, n_units;  // n_units: of the whole item; row < 0: none
@@ -152,7 +230,7 @@ struct PagedPiece {
 };
 
 // Walks the pieces of a CTA: whole items in turn, or an equal share of the blocks of all items.
-template <int kKeys>
+template <int kKeys, int kForm>
 struct PagedWalk {
   long long at, end, row_at;  // share: units; first unit of `row`
   int row, step;              // step > 0: items `at`, at + step, ..., of each the rank-th of `ranks` parts
@@ -168,13 +246,13 @@ struct PagedWalk {
         row = (int)(at / per_row);
         item = (int)(at - (long long)row * per_row);
         at += step;
-        w.keys = row_keys(a, row);
+        w.keys = row_keys<kForm>(a, row);
         w.n_units = units(w.keys);
         if (w.n_units == 0) continue;
         w.u0 = (int)((int64_t)w.n_units * rank / ranks);
         w.u1 = (int)((int64_t)w.n_units * (rank + 1) / ranks);
       } else {
-        w.keys = row_keys(a, row);
+        w.keys = row_keys<kForm>(a, row);
         w.n_units = units(w.keys);
         if (at >= row_at + (long long)w.n_units * per_row) {
           row_at += (long long)w.n_units * per_row;
@@ -221,14 +299,16 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
   __shared__ uint32_t s_live[kPagedWarps][kPagedStages];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int per_row = a.Hk * a.chunks;
-  using Walk = PagedWalk<kKeys>;
+  using Walk = PagedWalk<kKeys, kForm>;
   constexpr bool kShare = kWay == kShares;
   uint32_t rank = 0, ranks = 1;
   if (kWay == kClusters) {
     rank = cluster_ctarank();
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
   }
-  glue_enter();
+  // (Behind the prefix launch, which lets this one start once all of its CTAs have waited for what lies ahead of both: only the join
+  // waits for it.)
+  if (kForm != kSuffix) glue_enter();
 
   Walk walk;
   long long total = 0;
@@ -243,7 +323,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
     // where this CTA's share begins: sums over the rows, a thread a run of them
     const int rows_each = (a.T + kPagedThreads - 1) / kPagedThreads;
     long long sum = 0;
-    for (int i = 0, row = tid * rows_each; i < rows_each && row < a.T; ++i, ++row) sum += Walk::units(row_keys(a, row));
+    for (int i = 0, row = tid * rows_each; i < rows_each && row < a.T; ++i, ++row) sum += Walk::units(row_keys<kForm>(a, row));
     long long upto = sum;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
@@ -270,7 +350,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
       long long at = from;
       int row = tid * rows_each;
       for (;; ++row) {
-        const long long n = (long long)Walk::units(row_keys(a, row)) * per_row;
+        const long long n = (long long)Walk::units(row_keys<kForm>(a, row)) * per_row;
         if (walk.at < at + n) break;
         at += n;
       }
@@ -289,7 +369,8 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
   auto entry = [&](const PagedPiece& w, int u) {
     const int i = u * kKeys + lane;
     if (w.row < 0 || u >= w.u1 || lane >= kKeys || i >= w.keys.n_keys) return -1;
-    return a.tables[w.keys.req * a.table_ld + w.keys.key(i) / a.cache.block_size];
+    const int32_t* const at = a.tables + (w.keys.req * a.table_ld + w.keys.key(i) / a.cache.block_size);
+    return kForm == kSuffix ? __ldcg(at) : *at;
   };
   auto load = [&](const PagedPiece& w, int u, int blk, int stage) {
     if (w.row >= 0 && u < w.u1) {
@@ -323,8 +404,10 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
     for (int e = 0; e < kQEach; ++e) {
       const int i = tid + e * kPagedThreads, h = i / kPieces, p = i - h * kPieces;
       q_piece[e] = make_uint4(0, 0, 0, 0);
-      if (w.row >= 0 && h < w.n_heads)
-        q_piece[e] = *reinterpret_cast<const uint4*>(static_cast<const char*>(a.q) + 2 * (w.row * a.q_token + (w.head0 + h) * a.q_head + p * 8));
+      if (w.row >= 0 && h < w.n_heads) {
+        const uint4* const at = reinterpret_cast<const uint4*>(static_cast<const char*>(a.q) + 2 * (w.row * a.q_token + (w.head0 + h) * a.q_head + p * 8));
+        q_piece[e] = kForm == kSuffix ? __ldcg(at) : *at;
+      }
     }
   };
   auto put_q = [&](int buf) {
@@ -494,15 +577,22 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
     __shared__ float2 s_ml[8 * NT];
     const bool whole = !kShare || (w.u0 == 0 && w.u1 == w.n_units);
     const int slot = 2 * blockIdx.x + (first_piece ? 0 : 1);
-    // (differential: four columns of a head a lane, of both maps)
-    for (int i = tid; kForm == kDiff && i < 8 * (D / 4); i += kPagedThreads) {
+    // (differential: four columns of a head a lane, of both maps; behind a prefix the same, of one)
+    constexpr bool kFour = kForm != kPlain;
+    constexpr int kSumHeads = 8 * NT / kMaps<kForm>;
+    int prefix_parts = 0;
+    if (kForm == kSuffix && kWay != kClusters) {
+      if (first_piece) glue_enter();
+      prefix_parts = px_parts(a, w.keys.first);
+    }
+    for (int i = tid; kFour && i < kSumHeads * (D / 4); i += kPagedThreads) {
       const int h = i / (D / 4), c = i - h * (D / 4);
-      float4 x[2];
-      float sum[2];
+      float4 x[kMaps<kForm>];
+      float sum[kMaps<kForm>], top;
 #pragma unroll
-      for (int map = 0; map < 2; ++map) {
+      for (int map = 0; map < kMaps<kForm>; ++map) {
         const int vh = 8 * map + h;
-        float top = -INFINITY;
+        top = -INFINITY;
 #pragma unroll
         for (int k = 0; k < kPagedWarps; ++k) top = fmaxf(top, part[k][8 * NT * D + 2 * vh]);
         sum[map] = 0.f;
@@ -519,14 +609,17 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
           *reinterpret_cast<float4*>(const_cast<float*>(part[0]) + vh * D + 4 * c) = x[map];
           if (c == 0) s_ml[vh] = make_float2(top, sum[map]);
         } else if (!whole && h < w.n_heads) {
-          const int64_t at_slot = ((int64_t)slot * 2 + map) * a.heads + h;
+          const int64_t at_slot = ((int64_t)slot * kMaps<kForm> + map) * a.heads + h;
           *reinterpret_cast<float4*>(a.part_o + at_slot * D + 4 * c) = x[map];
           if (c == 0) *reinterpret_cast<float2*>(a.part_ml + at_slot * 2) = make_float2(top, sum[map]);
         }
       }
-      if (kWay != kClusters && whole) store_difference<D, kF16>(a, h < w.n_heads, w.row, w.head0 + h, c, x, sum);
+      if (kWay != kClusters && whole) {
+        if constexpr (kForm == kDiff) store_difference<D, kF16>(a, h < w.n_heads, w.row, w.head0 + h, c, x, sum);
+        else if (kForm == kSuffix && h < w.n_heads) store_behind_prefix<D, kF16>(a, w.row, w.head0 + h, c, prefix_parts, x[0], top, sum[0]);
+      }
     }
-    for (int i = tid; kForm != kDiff && i < w.n_heads * (D / 2); i += kPagedThreads) {
+    for (int i = tid; !kFour && i < w.n_heads * (D / 2); i += kPagedThreads) {
       const int h = i / (D / 2), d = 2 * (i - h * (D / 2));
       float top = -INFINITY;
 #pragma unroll
@@ -555,14 +648,18 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
       // the cluster's parts: every CTA joins some of the columns
       cluster_arrive();
       cluster_wait();
-      if (kForm == kDiff) {  // (whole heads, for their norm; whole warps, for its sum)
-        const int h0 = (int)(8 * rank / ranks), h1 = (int)(8 * (rank + 1) / ranks);
+      if (kForm == kSuffix) {
+        if (first_piece) glue_enter();
+        prefix_parts = px_parts(a, w.keys.first);
+      }
+      if (kFour) {  // (whole heads, for their norm; whole warps, for its sum)
+        const int h0 = (int)(kSumHeads * rank / ranks), h1 = (int)(kSumHeads * (rank + 1) / ranks);
         for (int i = tid; i < ((h1 - h0) * (D / 4) + 31) / 32 * 32; i += kPagedThreads) {
-          const int its = h0 + i / (D / 4), h = min(its, 7), c = i % (D / 4);
-          float4 x[2];
-          float sum[2];
+          const int its = h0 + i / (D / 4), h = min(its, kSumHeads - 1), c = i % (D / 4);
+          float4 x[kMaps<kForm>];
+          float sum[kMaps<kForm>], top;
 #pragma unroll
-          for (int map = 0; map < 2; ++map) {
+          for (int map = 0; map < kMaps<kForm>; ++map) {
             const int vh = 8 * map + h;
             float2 ml[8], v0[8], v1[8];
 #pragma unroll
@@ -576,7 +673,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
                 v1[k] = ld_cluster_f32x2(at + 8);
               }
             }
-            float top = -INFINITY;
+            top = -INFINITY;
 #pragma unroll
             for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
             sum[map] = 0.f;
@@ -588,10 +685,12 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
               x[map] = make_float4(x[map].x + f * v0[k].x, x[map].y + f * v0[k].y, x[map].z + f * v1[k].x, x[map].w + f * v1[k].y);
             }
           }
-          store_difference<D, kF16>(a, its < h1 && h < w.n_heads, w.row, w.head0 + h, c, x, sum);
+          const bool live = its < h1 && h < w.n_heads;
+          if constexpr (kForm == kDiff) store_difference<D, kF16>(a, live, w.row, w.head0 + h, c, x, sum);
+          else if (live) store_behind_prefix<D, kF16>(a, w.row, w.head0 + h, c, prefix_parts, x[0], top, sum[0]);
         }
       }
-      const int all = kForm == kDiff ? 0 : w.n_heads * (D / 2);
+      const int all = kFour ? 0 : w.n_heads * (D / 2);
       for (int i = (int)((int64_t)all * rank / ranks) + tid, to = (int)((int64_t)all * (rank + 1) / ranks); i < to; i += kPagedThreads) {
         const int h = i / (D / 2), d = 2 * (i - h * (D / 2));
         float2 ml[8], v[8];
@@ -631,6 +730,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
     w = following;
   }
   cp_async_wait_group<0>();
+  if (kForm == kSuffix && first_piece) glue_enter();  // (this launch ends behind the one ahead whatever its CTAs find)
   if (kWay == kClusters) {  // (no CTA leaves while another reads its part)
     cluster_arrive();
     cluster_wait();
@@ -751,14 +851,15 @@ inline int paged_decode_launch_t(const PagedArgs& a, int ctas, int cluster, cuda
     cudaGetLastError();
     return fail(B200_LORA_ECUDA, "paged_decode_kernel launch: %s", cudaGetErrorString(e));
   }
-  if (kWay != kShares) return B200_LORA_OK;
-  return launch_dependent(paged_join_kernel<D, kF16, kForm>, "paged_join_kernel", dim3((unsigned)ctas, (unsigned)a.heads), kJoinThreads, 0, stream, a);
+  if constexpr (kWay != kShares) return B200_LORA_OK;
+  else return launch_dependent(paged_join_kernel<D, kF16, kForm>, "paged_join_kernel", dim3((unsigned)ctas, (unsigned)a.heads), kJoinThreads, 0, stream, a);
 }
 
 template <int D, int NT, bool kF16, int kForm>
 inline int paged_decode_launch_by(const PagedArgs& a, cudaStream_t stream) {
   const PagedWay w = paged_way(a.T, a.Hq, a.Hk, D, (int64_t)a.table_width * a.cache.block_size, a.window, a.sinks, kItemHeads<kForm>);
-  if (w.shares && a.part_o != nullptr) return paged_decode_launch_t<D, NT, kF16, kShares, 4, kForm>(a, kPagedCtas, 1, stream);
+  if constexpr (kForm != kSuffix)
+    if (w.shares && a.part_o != nullptr) return paged_decode_launch_t<D, NT, kF16, kShares, 4, kForm>(a, kPagedCtas, 1, stream);
   const int64_t items = (int64_t)a.T * a.Hk * a.chunks;
   const int ctas = (int)std::min<int64_t>((w.warps == 8 ? 148 : kPagedCtas) / w.cluster, items) * w.cluster;
   if (w.cluster > 1) return paged_decode_launch_t<D, NT, kF16, kClusters, 8, kForm>(a, ctas, w.cluster, stream);

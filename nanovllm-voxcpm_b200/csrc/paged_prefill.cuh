@@ -38,6 +38,7 @@ __host__ __device__ constexpr int pp_stages(int tiles) { return (D == 64 ? 1 : 0
 template <int D>
 __host__ __device__ constexpr int pp_tile() { return kPpKeys * D * 2; }
 // Tiles of a CTA, and how many of them have rows of their own: the two maps of differential heads are two tiles of the same rows.
+static_assert(kPpKeys == kPrefixTile, "parts of a prefix are whole tiles");
 __host__ __device__ constexpr int pp_tiles(int D, int form) { return D == 64 && form != kDiff ? 1 : 2; }
 __host__ __device__ constexpr int pp_row_tiles(int D, int form) { return form == kDiff ? 1 : pp_tiles(D, form); }
 template <int D>
@@ -49,6 +50,7 @@ __host__ __device__ constexpr int pp_smem(int tiles, int row_tiles) { return (2 
 // wave: their last items are their shortest (8192 tokens 223 / 239).
 constexpr int kPpSplitTiles = 8;     // tiles of an item, at least
 constexpr int kPpSplitWaves = 6;     // waves of CTAs at most
+constexpr int kPxChunk = 2;          // tiles of a part of a prefix, at least
 constexpr int kPpShare = 2, kPpParts = 32;  // tiles of a part at least, parts at most (the join reads them one after another)
 
 struct PpMaps { CUtensorMap q, k, v; };
@@ -58,6 +60,7 @@ struct PpArgs {
   int n_blocks;              // blocks of tokens that the launch has CTAs for
   int box, box_shift;        // cache rows of a copy: 8 .. 128, a power of two that divides the block size; its logarithm
   float* parts; void* joins;  // split: partial results and what there is to join
+  int px_ctas;               // CTAs that the parts of prefixes are to fill
   int k_heads_inner, v_heads_inner;  // order of the map's middle dimensions: (head, position) or (position, head)
 };
 
@@ -132,12 +135,30 @@ struct PpPiece {
   int req, pos0, held, key_end, lo_first, sink_end;  // position of the first token; keys that a row sees: [0, sink_end), [lo_first, key_end)
   int first_box, sink_boxes, i0, i1;           // the keys in boxes: those of the first tokens, then from first_box on, side by side
   int parts;                                   // 0: no more pieces; 1: the whole item; else the item is in that many parts
+  int part, r1, keys;                              // of a prefix: which part of it; its keys. Behind a prefix: the keys of that
   // first key of box b of tile i, with 1 << shift keys in a box
   __device__ __forceinline__ int key_of(int i, int b, int shift) const {
     const int c = i * (kPpKeys >> shift) + b;
     return (c < sink_boxes ? c : c - sink_boxes + first_box) << shift;
   }
 };
+
+// Of the requests [r0, r1), the one that begins at or before the row last
+__device__ __forceinline__ int px_request(const PagedArgs& p, int row, int r0, int r1) {
+  while (r1 - r0 > 1) {
+    const int mid = (r0 + r1) >> 1;
+    if (p.cu_seqlens[mid] <= row) r0 = mid;
+    else r1 = mid;
+  }
+  return r0;
+}
+// Position of a row of the group that begins with request r0; -1 if its request's rows leave those of q
+__device__ __forceinline__ int px_position(const PagedArgs& p, int row, int r0, int r1) {
+  if (p.cu_seqlens == nullptr) return p.context_lens[row] - 1;
+  const int r = px_request(p, row, r0, r1), end = p.cu_seqlens[r + 1];
+  if (p.cu_seqlens[r] < 0 || end > p.T || row >= end) return -1;
+  return (int)max((int64_t)p.context_lens[r] - (end - row), (int64_t)-1);
+}
 
 // New rows of request i, and its first one; a range that leaves the rows of q counts as none
 __device__ __forceinline__ int pp_rows(const PagedArgs& p, int i, int* begin) {
@@ -177,6 +198,7 @@ __device__ __forceinline__ int pp_items(const PpArgs& a, int span, const PpLane&
 // they end at; more: the last block of the last sequence first; 32 requests of 30 to 400 tokens, heads of 64, 27.2 us, 33 of them 33.3;
 // of 100 each 13.9 and 14.5), the sets of heads of a block one after another. A whole warp calls
 // it, with the first 32 requests in hand.
+template <int kForm>
 __device__ __forceinline__ void pp_find(const PpArgs& a, int span, int item, int n_items, const PpLane& lanes0, PpPiece* w) {
   const PagedArgs& p = a.p;
   const int lane = threadIdx.x & 31, back = item / a.head_tiles;
@@ -218,6 +240,7 @@ __device__ __forceinline__ void pp_find(const PpArgs& a, int span, int item, int
   w->held = (int)min((int64_t)w->pos0 + w->n_here, (int64_t)p.table_width * p.cache.block_size);
   w->key_end = w->held;
   w->lo_first = p.window > 0 ? max(0, max(w->pos0, 0) - (p.window - 1)) : 0;
+  if (kForm == kSuffix) w->lo_first = w->keys = px_keys(p, w->req);
   w->sink_end = max(0, min(min(p.sinks, w->lo_first), w->key_end));
   // (a window behind the table's end has no box; its first one is at the end, since a key next to 2^31 and its tile need not fit an int)
   w->first_box = min(w->lo_first, max(w->held, 0) + a.box - 1) >> a.box_shift;
@@ -228,12 +251,128 @@ __device__ __forceinline__ void pp_find(const PpArgs& a, int span, int item, int
   w->parts = 1;
 }
 
+// Of a prefix launch: tiles of a part, so that the parts of all prefixes are as many as the CTAs that the launch is to fill, or more; items
+// over all groups (a block of rows, a set of heads, a part). 32 groups, one a lane, at a time.
+struct PxLane { PxGroup g; int blocks, tiles; };
+__device__ __forceinline__ PxLane px_lane(const PpArgs& a, int span, int g) {
+  PxLane q;
+  q.g = px_group(a.p, g);
+  q.tiles = (int)(((unsigned)q.g.keys + kPpKeys - 1u) / kPpKeys);
+  q.blocks = q.tiles == 0 ? 0 : (q.g.end - q.g.begin + span - 1) / span;
+  return q;
+}
+__device__ __forceinline__ int px_chunk_tiles(const PpArgs& a, int span, const PxLane& lanes0) {
+  long long work = 0;
+  int longest = 0;
+  for (int base = 0; base < a.p.n_groups; base += 32) {
+    const PxLane q = base == 0 ? lanes0 : px_lane(a, span, base + (int)(threadIdx.x & 31));
+    work += (long long)q.blocks * q.tiles;
+    longest = max(longest, q.tiles);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d /= 2) {
+    work += __shfl_xor_sync(0xffffffffu, work, d);
+    longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, d));
+  }
+  work *= a.head_tiles;
+  const long long even = (work + a.px_ctas - 1) / a.px_ctas, least = max(kPxChunk, (longest + a.p.px_most - 1) / a.p.px_most);
+  return (int)min(max(even, least), (long long)INT32_MAX);
+}
+// Items of a group, at most INT32_MAX over all (the host sees to that for groups that do not overlap)
+__device__ __forceinline__ int px_items_of(const PpArgs& a, const PxLane& q, int chunk) {
+  return (int)min((long long)q.blocks * a.head_tiles * ((q.tiles + chunk - 1) / chunk), (long long)(INT32_MAX >> 6));
+}
+// Item `item` of the launch, or parts = 0
+__device__ __forceinline__ void px_find(const PpArgs& a, int span, int chunk, int item, const PxLane& lanes0, PpPiece* w) {
+  const PagedArgs& p = a.p;
+  const int lane = threadIdx.x & 31;
+  w->parts = 0;
+  for (int base = 0; base < p.n_groups; base += 32) {
+    const PxLane q = base == 0 ? lanes0 : px_lane(a, span, base + lane);
+    const int mine = px_items_of(a, q, chunk), upto = warp_upto(mine);
+    const uint32_t hit = __ballot_sync(0xffffffffu, upto > item);
+    if (hit == 0) {
+      item -= __shfl_sync(0xffffffffu, upto, 31);
+      continue;
+    }
+    const int who = __ffs(hit) - 1;
+    const int at = item - __shfl_sync(0xffffffffu, upto - mine, who), blocks = __shfl_sync(0xffffffffu, q.blocks, who);
+    const int r0 = __shfl_sync(0xffffffffu, q.g.r0, who), r1 = __shfl_sync(0xffffffffu, q.g.r1, who);
+    const int begin = __shfl_sync(0xffffffffu, q.g.begin, who), end = __shfl_sync(0xffffffffu, q.g.end, who);
+    w->keys = __shfl_sync(0xffffffffu, q.g.keys, who);
+    // (the blocks of rows over one part and set of heads side by side: they read the same keys)
+    const int block = at % blocks, rest = at / blocks, set = rest % a.head_tiles;
+    w->part = rest / a.head_tiles;
+    w->head0 = set << a.h_shift;
+    w->req = r0;
+    w->r1 = r1;
+    w->begin = begin;
+    w->q0 = block * span;
+    w->n_here = min(span, end - begin - w->q0);
+    // No key behind the contexts of the block's requests: rows there may hold anything.
+    int first = begin + w->q0, last = first + w->n_here - 1, most = 0;  // requests of the block
+    if (p.cu_seqlens != nullptr) {
+      first = px_request(p, first, r0, r1);
+      last = px_request(p, last, r0, r1);
+    }
+    for (int r = first + lane; r <= last; r += 32) most = max(most, p.context_lens[r]);
+    most = __reduce_max_sync(0xffffffffu, most);
+    w->pos0 = 0;
+    w->held = w->key_end = min(w->keys, most);
+    w->lo_first = w->sink_end = w->first_box = w->sink_boxes = 0;
+    w->i0 = w->part * chunk;
+    w->i1 = min(w->i0 + chunk, (w->key_end + kPpKeys - 1) / kPpKeys);
+    w->parts = 1;
+    return;
+  }
+}
+
+// Sums (m, l) of a row and head over the keys behind the prefix, joined with those over its parts: the common reference, what the own
+// numerators count, 1 / sum, the logarithm
+struct PxJoined { float top, own, inv, lse; };
+__device__ __forceinline__ PxJoined px_join(const PagedArgs& p, int64_t at, int parts, float m, float l) {
+  const int64_t step = (int64_t)p.T * p.Hq;
+  PxJoined j;
+  j.top = m;
+#pragma unroll 4
+  for (int k = 0; k < parts; ++k) j.top = fmaxf(j.top, __ldcg(p.px_ml + at + k * step).x);
+  j.own = m == -INFINITY ? 0.f : ex2(m - j.top);
+  l *= j.own;
+#pragma unroll 4
+  for (int k = 0; k < parts; ++k) {
+    const float2 ml = __ldcg(p.px_ml + at + k * step);
+    l += (ml.x == -INFINITY ? 0.f : ex2(ml.x - j.top)) * ml.y;
+  }
+  j.inv = over(l);
+  j.lse = l == 0.f ? -INFINITY : (j.top + log2f(l)) * 0.6931471805599453f;
+  return j;
+}
+// Adds the parts' numerators of N columns, `col` on; a part without a key that the row sees has none.
+template <int D, int N>
+__device__ __forceinline__ void px_add(const PagedArgs& p, int64_t at, int parts, float top, int col, float (&x)[N]) {
+  const int64_t step = (int64_t)p.T * p.Hq;
+  for (int k = 0; k < parts; ++k) {
+    const float reference = __ldcg(p.px_ml + at + k * step).x;
+    if (reference == -INFINITY) continue;
+    const float f = ex2(reference - top);
+    const float4* const src = reinterpret_cast<const float4*>(p.px_o + (at + k * step) * D + col);
+#pragma unroll
+    for (int c = 0; c < N / 4; ++c) {
+      const float4 v = __ldcg(src + c);
+      x[4 * c] += f * v.x;
+      x[4 * c + 1] += f * v.y;
+      x[4 * c + 2] += f * v.z;
+      x[4 * c + 3] += f * v.w;
+    }
+  }
+}
+
 // The part of an item that CTA c leaves for the join (slot c): numerators [row / 128][column / 4][row % 128] of four columns, then
 // maximum and sum of every row.
 template <int D>
 __host__ __device__ constexpr int pp_slot_floats(int tiles) { return tiles * kPpRows * (D + 2); }
 // Of the item whose parts the CTAs c, c + stride, ... (`parts` of them) hold; parts < 2: none
-struct PpJoin { int head0, token0, n_here, parts, stride, pad[3]; };
+struct PpJoin { int head0, token0, n_here, parts, stride, keys, pad[2]; };  // keys: of the prefix
 
 // kForm kDiff: the tiles are the two maps of the same rows, over the same K and V: scores take half of the columns each, a warpgroup
 // ends with half of the columns of both maps' O.
@@ -273,7 +412,8 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  glue_enter();  // (dependents may start: every CTA of this launch holds its tensor memory by then)
+  // (Dependents may start: every CTA of this launch holds its tensor memory by then. Behind a prefix launch only the join waits for it.)
+  if (kForm != kSuffix) glue_enter();
   const uint32_t tmem = s_tmem;
   const int per_tile = kPpRows >> a.h_shift, span = kRowTiles * per_tile;
 
@@ -293,14 +433,20 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
     const uint32_t all_boxes = bits_below(kPpKeys / a.box);
     const int tile_shift = 7 - a.box_shift, step = min(a.box, 32);  // boxes of a tile, as a logarithm; columns of 32 that lie in one box
     const uint32_t stage = out_u32 + warp * (32 * kPpOutPitch);  // 32 columns of the warp's rows on their way out
+    bool waited = false;
     uint32_t n = 0, pieces = 0, exchanges = 0;  // tiles and pieces with tiles so far: phases of the barriers
     PpPiece w;
     for (int k = 0; take(k, &w); ++k) {
-      const int pos = pp_position(w.pos0, tok);
-      const int lo = p.window > 0 ? max(pos, 0) - (p.window - 1) : 0;
-      const int tile_lo = pp_position(w.pos0, tok0), tile_hi = pp_position(tile_lo, per_tile - 1);  // positions of the tile
+      int pos = pp_position(w.pos0, tok);
+      const int lo = kForm == kSuffix ? w.lo_first : p.window > 0 ? max(pos, 0) - (p.window - 1) : 0;
+      int tile_lo = pp_position(w.pos0, tok0);
+      if (kForm == kPrefix) {  // (rows have positions of their own, most of them behind the prefix; the first key that some row of the warp does not see)
+        pos = tok < w.n_here && w.i1 > w.i0 ? min(px_position(p, w.begin + w.q0 + tok, w.req, w.r1), w.keys - 1) : w.keys - 1;
+        tile_lo = __reduce_min_sync(0xffffffffu, pos);
+      }
+      const int tile_hi = pp_position(tile_lo, per_tile - 1);  // positions of the tile
       // tiles [clear0, clear1) need no mask: behind the first tokens, from where every row's window has begun, up to the first row
-      const int w_lo = p.window > 0 ? max(tile_hi, 0) - (p.window - 1) : 0;
+      const int w_lo = kForm == kSuffix ? w.lo_first : p.window > 0 ? max(tile_hi, 0) - (p.window - 1) : 0;
       const int clear0 = (w.sink_boxes + max(0, (int)(((uint32_t)max(w_lo, 0) + a.box - 1u) >> a.box_shift) - w.first_box) + (1 << tile_shift) - 1) >> tile_shift;
       const int clear1 = (((tile_lo + 1) >> a.box_shift) + w.sink_boxes - w.first_box) >> tile_shift;
       float m = -INFINITY, l = 0.f;  // what the probabilities refer to, in units of log2; their sum
@@ -396,7 +542,7 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
         }
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }
-      const bool live = tok < w.n_here, any = w.i1 > w.i0, whole = !kSplit || w.parts == 1;
+      const bool live = tok < w.n_here, any = w.i1 > w.i0, whole = kForm != kPrefix && (!kSplit || w.parts == 1);
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // (no visible key: zeros; NaN stays)
       const int64_t token0 = (int64_t)w.begin + w.q0;
       if (any) {
@@ -479,6 +625,62 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
           }
           __syncwarp();
         }
+      } else if (kForm == kPrefix) {
+        // The part's sums as they are, through shared memory for the same reason as below, 16 columns of fp32 at a time.
+        const int64_t part_at = ((int64_t)w.part * p.T + token0) * p.Hq;
+#pragma unroll
+        for (int c = 0; any && c < D / 16; ++c) {
+          uint32_t o[16];
+          tmem_ld_32x16(o_at + 16 * c, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; j += 4) sts128(stage + lane * kPpOutPitch + 4 * j, make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]));
+          __syncwarp();
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int of = whose(r), its = tok0 + (of >> a.h_shift);
+            if (its < w.n_here)
+              stg128(p.px_o + (part_at + (int64_t)its * p.Hq + w.head0 + (of & ((1 << a.h_shift) - 1))) * D + 16 * c + 4 * (lane & 3),
+                     lds128(stage + (8 * r + (lane >> 2)) * kPpOutPitch + 16 * (lane & 3)));
+          }
+          __syncwarp();
+        }
+        if (live) p.px_ml[part_at + (int64_t)tok * p.Hq + w.head0 + (row & ((1 << a.h_shift) - 1))] = make_float2(m, l);
+      } else if (kForm == kSuffix && whole) {
+        if (!waited) glue_enter();  // (the prefix's parts)
+        waited = true;
+        const int64_t at = (token0 + (live ? tok : 0)) * p.Hq + w.head0 + (row & ((1 << a.h_shift) - 1));
+        const int parts = live ? px_parts(p, w.keys) : 0;
+        const PxJoined j = px_join(p, at, parts, m, l);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          if (any) {
+            tmem_ld_32x32(o_at + 32 * c, o);
+            tmem_ld_wait();
+          }
+          float x[32];
+#pragma unroll
+          for (int k = 0; k < 32; ++k) x[k] = any ? __uint_as_float(o[k]) * j.own : 0.f;
+          px_add<D>(p, at, parts, j.top, 32 * c, x);
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) {
+            uint4 v;
+            v.x = pack_16x2<kF16>(x[k] * j.inv, x[k + 1] * j.inv);
+            v.y = pack_16x2<kF16>(x[k + 2] * j.inv, x[k + 3] * j.inv);
+            v.z = pack_16x2<kF16>(x[k + 4] * j.inv, x[k + 5] * j.inv);
+            v.w = pack_16x2<kF16>(x[k + 6] * j.inv, x[k + 7] * j.inv);
+            sts128(stage + lane * kPpOutPitch + 2 * k, v);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            char* const dst = stored(r, 32 * c);
+            if (dst != nullptr) stg128(dst, lds128(stage + (8 * r + (lane >> 2)) * kPpOutPitch + 16 * (lane & 3)));
+          }
+          __syncwarp();
+        }
+        if (live && p.lse != nullptr) p.lse[at] = j.lse;
       } else if (whole) {
         // Through shared memory, so that four lanes write 64 adjacent bytes of a row. (A row's pieces straight from its thread: 32
         // half-used sectors a store, 3200 cycles for a tile of 128 columns.)
@@ -538,8 +740,19 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
       const uint32_t leader = elect_one();
       const int n_boxes = kPpKeys / a.box;
       uint32_t n = 0, pieces = 0;
-      const PpLane lanes0 = pp_lane(a, span, lane);
-      const int n_items = pp_items(a, span, lanes0), G = gridDim.x, waves = n_items / G, rest = n_items - waves * G;
+      const int G = gridDim.x;
+      PpLane lanes0 = {0, 0, 0, 0, 0};
+      PxLane groups0 = {{0, 0, 0, 0, 0}, 0, 0};
+      int n_items = 0, chunk = 1;
+      if constexpr (kForm == kPrefix) {
+        groups0 = px_lane(a, span, lane);
+        chunk = px_chunk_tiles(a, span, groups0);
+        if (blockIdx.x == 0 && leader) *p.px_chunk = chunk;
+      } else {
+        lanes0 = pp_lane(a, span, lane);
+        n_items = pp_items(a, span, lanes0);
+      }
+      const int waves = n_items / G, rest = n_items - waves * G;
       // Split: the items that do not fill a wave are cut into parts, CTA i + s * rest has part s of item i.
       const int most = kSplit && rest > 0 ? G / rest : 1;
       if (kSplit && leader) static_cast<PpJoin*>(a.joins)[blockIdx.x].parts = 0;
@@ -549,23 +762,25 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
         w.parts = 0;
         // (every other wave backwards: contexts get shorter from item to item)
         const int c = k & 1 ? G - 1 - (int)blockIdx.x : (int)blockIdx.x;
-        if (k < waves) {
-          pp_find(a, span, k * G + c, n_items, lanes0, &w);
+        if constexpr (kForm == kPrefix) {
+          px_find(a, span, chunk, k * G + (int)blockIdx.x, groups0, &w);
+        } else if (k < waves) {
+          pp_find<kForm>(a, span, k * G + c, n_items, lanes0, &w);
         } else if (k == waves && most >= 2) {
           const int i = blockIdx.x % rest, s = blockIdx.x / rest;
           if (s < most) {
-            pp_find(a, span, k * G + i, n_items, lanes0, &w);
+            pp_find<kForm>(a, span, k * G + i, n_items, lanes0, &w);
             const int tiles = w.i1;
             w.parts = max(1, min(min(most, kPpParts), tiles / kPpShare));
             if (s >= w.parts) w.parts = 0;
             if (w.parts > 1) {
               w.i0 = (int)((int64_t)tiles * s / w.parts);
               w.i1 = (int)((int64_t)tiles * (s + 1) / w.parts);
-              if (s == 0 && leader) static_cast<PpJoin*>(a.joins)[i] = {w.head0, w.begin + w.q0, w.n_here, w.parts, rest, {0, 0, 0}};
+              if (s == 0 && leader) static_cast<PpJoin*>(a.joins)[i] = {w.head0, w.begin + w.q0, w.n_here, w.parts, rest, kForm == kSuffix ? w.keys : 0, {0, 0}};
             }
           }
         } else if (k == waves && c < rest) {
-          pp_find(a, span, k * G + c, n_items, lanes0, &w);
+          pp_find<kForm>(a, span, k * G + c, n_items, lanes0, &w);
         }
         more_pieces = w.parts > 0;
         if (k >= 2) pp_wait(bar(TAKEN + (k & 1)), (uint32_t)((k >> 1) - 1) & 1, &abort_flag);
@@ -704,6 +919,7 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
       }
     }
   }
+  if (kForm == kSuffix) glue_enter();  // (this launch ends behind the one ahead, whatever its CTAs found)
   __syncthreads();
   if (warp == kIssuer) {
     tc_fence_after_sync();
@@ -714,7 +930,7 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
 
 // Joins the parts of the item that CTA blockIdx.x has the first part of. A thread per row of the item, 16 columns (blockIdx.y): eight
 // parts' worth of them are under way at a time.
-template <int D, bool kF16, int kTiles>
+template <int D, bool kF16, int kTiles, int kForm>
 __global__ void __launch_bounds__(kTiles * kPpRows) paged_prefill_join_kernel(const __grid_constant__ PpArgs a) {
   glue_enter();
   const PpJoin j = static_cast<const PpJoin*>(a.joins)[blockIdx.x];
@@ -743,8 +959,26 @@ __global__ void __launch_bounds__(kTiles * kPpRows) paged_prefill_join_kernel(co
       o[c] = make_float4(o[c].x + f * v.x, o[c].y + f * v.y, o[c].z + f * v.z, o[c].w + f * v.w);
     }
   }
-  const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
   const int64_t token = (int64_t)j.token0 + tok;
+  float inv = over(sum), lse = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+  if constexpr (kForm == kSuffix) {
+    const int64_t at = token * p.Hq + head;
+    const int parts = px_parts(p, j.keys);
+    const PxJoined both = px_join(p, at, parts, top, sum);
+    float x[16];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      x[4 * c] = o[c].x * both.own;
+      x[4 * c + 1] = o[c].y * both.own;
+      x[4 * c + 2] = o[c].z * both.own;
+      x[4 * c + 3] = o[c].w * both.own;
+    }
+    px_add<D>(p, at, parts, both.top, 4 * c0, x);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] = make_float4(x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
+    inv = both.inv;
+    lse = both.lse;
+  }
   char* const dst = static_cast<char*>(p.out) + 2 * (token * p.out_token + head * p.out_head + 4 * c0);
 #pragma unroll
   for (int c = 0; c < 4; c += 2) {
@@ -755,7 +989,7 @@ __global__ void __launch_bounds__(kTiles * kPpRows) paged_prefill_join_kernel(co
     v.w = pack_16x2<kF16>(o[c + 1].z * inv, o[c + 1].w * inv);
     stg128(dst + 8 * c, v);
   }
-  if (c0 == 0 && p.lse != nullptr) p.lse[token * p.Hq + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+  if (c0 == 0 && p.lse != nullptr) p.lse[token * p.Hq + head] = lse;
 }
 
 // The same for differential heads: 32 rows of the item (blockIdx.y), a warp per 16 columns, of both maps (the tiles of a part); the sums
@@ -908,13 +1142,13 @@ inline int paged_prefill_launch_t(const PpMaps& maps, const PpArgs& a, cudaStrea
   constexpr int smem = pp_smem<D>(kTiles, pp_row_tiles(D, kForm));
   static std::atomic<uint64_t> known{0};
   if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), smem, &known)) return rc;
-  const int ctas = kSplit ? kCtas : (int)std::min<int64_t>(kCtas, (int64_t)a.n_blocks * a.head_tiles);
+  const int ctas = kForm == kPrefix ? a.px_ctas : kSplit ? kCtas : (int)std::min<int64_t>(kCtas, (int64_t)a.n_blocks * a.head_tiles);
   const int rc = launch_dependent(kernel, "paged_prefill_kernel", dim3((unsigned)ctas), pp_threads(kTiles), (size_t)smem, stream, maps, a);
   if (rc != B200_LORA_OK || !kSplit) return rc;
   if constexpr (kForm == kDiff)
     return launch_dependent(paged_prefill_join_maps_kernel<D, kF16>, "paged_prefill_join_maps_kernel", dim3((unsigned)ctas, kPpRows / 32), 2 * D, 0, stream, a);
   else
-    return launch_dependent(paged_prefill_join_kernel<D, kF16, kTiles>, "paged_prefill_join_kernel", dim3((unsigned)ctas, D / 16), kTiles * kPpRows, 0, stream, a);
+    return launch_dependent(paged_prefill_join_kernel<D, kF16, kTiles, kForm>, "paged_prefill_join_kernel", dim3((unsigned)ctas, D / 16), kTiles * kPpRows, 0, stream, a);
 }
 
 template <int kForm = kPlain>
@@ -922,8 +1156,10 @@ inline int paged_prefill_launch(const PagedArgs& p, int D, int dtype, void* work
   PpMaps maps;
   PpArgs a = {};
   const bool f16 = dtype == B200_LORA_F16;
-  if (!paged_prefill_plan(p, D, f16, pp_row_tiles(D, kForm), &maps, &a))
-    return paged_decode_launch<kForm>(p, D, dtype, p.cache.block_size % 8 != 0 ? workspace : nullptr, stream);
+  if (!paged_prefill_plan(p, D, f16, pp_row_tiles(D, kForm), &maps, &a)) {
+    if constexpr (kForm == kSuffix) return fail(B200_LORA_EUNSUPPORTED, "shared_prefix_attention: no tensor map");  // (the prefix launch had one)
+    else return paged_decode_launch<kForm>(p, D, dtype, p.cache.block_size % 8 != 0 ? workspace : nullptr, stream);
+  }
   if (pp_splits(p.T, p.n_req, p.Hq, a.h_shift, pp_row_tiles(D, kForm), pp_ctas(D, kForm), (int64_t)p.table_width * p.cache.block_size, p.window)) {
     a.parts = static_cast<float*>(workspace);
     a.joins = static_cast<char*>(workspace) + pp_split_bytes(D, kForm) - pp_ctas(D, kForm) * sizeof(PpJoin);
@@ -932,6 +1168,59 @@ inline int paged_prefill_launch(const PagedArgs& p, int D, int dtype, void* work
   }
   if (D == 64) return f16 ? paged_prefill_launch_t<64, true, false, kForm>(maps, a, stream) : paged_prefill_launch_t<64, false, false, kForm>(maps, a, stream);
   return f16 ? paged_prefill_launch_t<128, true, false, kForm>(maps, a, stream) : paged_prefill_launch_t<128, false, false, kForm>(maps, a, stream);
+}
+
+// Requests with common prefixes: a launch over the prefixes, the requests of a group side by side, and one over the keys behind them that
+// joins. Host code; what the device makes of the lengths is at px_chunk_tiles.
+struct PxPlan { int most, ctas; size_t own_bytes, ml_bytes, o_bytes; };  // parts of a prefix at most; CTAs that they are to fill
+inline PxPlan px_plan(int T, int n_req, int Hq, int Hk, int D, int block_size, int64_t max_keys, bool packed) {
+  PxPlan x;
+  const int h_shift = pp_h_shift(Hq / Hk), span = pp_row_tiles(D, kPrefix) * (kPpRows >> h_shift);
+  x.ctas = 148;
+  const int64_t blocks = (int64_t)ceil_div_i(T, span) * (Hq >> h_shift);
+  x.most = (int)std::max<int64_t>(1, std::min<int64_t>(kPpParts, (2 * x.ctas + blocks - 1) / blocks));
+  x.own_bytes = packed ? paged_prefill_workspace_bytes<kSuffix>(T, n_req, Hq, Hk, D, block_size, max_keys, 0) : 0;
+  x.own_bytes = (x.own_bytes + 15) / 16 * 16;
+  x.ml_bytes = ((size_t)x.most * T * Hq * 8 + 15) / 16 * 16;
+  x.o_bytes = (size_t)x.most * T * Hq * D * 4;
+  return x;
+}
+// Whether requests are attended by group: where a group has more than one, and copies of the cache's rows take tiles of them.
+inline bool px_shares(int T, int n_req, int n_groups, int block_size, int64_t max_keys) {
+  return n_groups > 0 && n_req > n_groups && block_size % 8 == 0 && max_keys > 0 && max_keys <= kPpMaxKeys && (int64_t)T < (1 << 24);
+}
+inline size_t shared_prefix_workspace_bytes(int T, int n_req, int n_groups, int Hq, int Hk, int D, int block_size, int64_t max_keys, bool packed) {
+  // (a call whose strides a map refuses goes without sharing)
+  const size_t plain = packed ? paged_prefill_workspace_bytes(T, n_req, Hq, Hk, D, block_size, max_keys, 0) : paged_workspace_bytes(T, Hq, Hk, D, max_keys, 0, 0);
+  if (!px_shares(T, n_req, n_groups, block_size, max_keys)) return plain;
+  const PxPlan x = px_plan(T, n_req, Hq, Hk, D, block_size, max_keys, packed);
+  return std::max(plain, 16 + x.own_bytes + x.ml_bytes + x.o_bytes);
+}
+
+template <int D, bool kF16>
+inline int shared_prefix_launch_t(PagedArgs p, bool packed, void* workspace, cudaStream_t stream) {
+  const int64_t max_keys = (int64_t)p.table_width * p.cache.block_size;
+  const int dtype = kF16 ? B200_LORA_F16 : B200_LORA_BF16;
+  PpMaps maps;
+  PpArgs a = {};
+  if (!px_shares(p.T, p.n_req, p.n_groups, p.cache.block_size, max_keys) || !paged_prefill_plan(p, D, kF16, pp_row_tiles(D, kPrefix), &maps, &a))
+    return packed ? paged_prefill_launch(p, D, dtype, workspace, stream) : paged_decode_launch(p, D, dtype, workspace, stream);
+  const PxPlan x = px_plan(p.T, p.n_req, p.Hq, p.Hk, D, p.cache.block_size, max_keys, packed);
+  char* const ws = static_cast<char*>(workspace);
+  p.px_most = x.most;
+  p.px_chunk = reinterpret_cast<int*>(ws);
+  p.px_ml = reinterpret_cast<float2*>(ws + 16 + x.own_bytes);
+  p.px_o = reinterpret_cast<float*>(ws + 16 + x.own_bytes + x.ml_bytes);
+  a.p = p;
+  a.px_ctas = x.ctas;
+  const int rc = paged_prefill_launch_t<D, kF16, false, kPrefix>(maps, a, stream);
+  if (rc != B200_LORA_OK) return rc;
+  return packed ? paged_prefill_launch<kSuffix>(p, D, dtype, ws + 16, stream) : paged_decode_launch<kSuffix>(p, D, dtype, nullptr, stream);
+}
+inline int shared_prefix_launch(const PagedArgs& p, int D, int dtype, bool packed, void* workspace, cudaStream_t stream) {
+  const bool f16 = dtype == B200_LORA_F16;
+  if (D == 64) return f16 ? shared_prefix_launch_t<64, true>(p, packed, workspace, stream) : shared_prefix_launch_t<64, false>(p, packed, workspace, stream);
+  return f16 ? shared_prefix_launch_t<128, true>(p, packed, workspace, stream) : shared_prefix_launch_t<128, false>(p, packed, workspace, stream);
 }
 
 }  // namespace b200lora

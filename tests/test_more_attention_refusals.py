@@ -1,4 +1,4 @@
-"""What differential attention and the join refuse before any launch: in Python on CPU tensors, and behind the C ABI with addresses
+"""What attention behind a shared prefix, differential attention and the join refuse before any launch: in Python on CPU tensors, and behind the C ABI with addresses
 that are never read."""
 
 import ctypes
@@ -43,6 +43,27 @@ def test_differential_statuses(kw, code):
     assert _differential(**kw) == code
 
 
+def _shared(**kw):
+    a = dict(out=AT, ot=1024, oh=64, lse=None, q=AT, qt=1024, qh=64, T=2, heads=16, kv=2, dim=64, cache=_cache(), tables=AT, ld=4, width=4, ctx=AT,
+             cu=None, n=2, prefix=AT, cu_groups=AT, groups=1, scale=0.125, dtype=N.DT_BF16, ws=AT, bytes=1 << 30, stream=None)
+    a.update(kw)
+    a["cache"] = ctypes.byref(a["cache"]) if a["cache"] is not None else None
+    return N.lib().lora_b200_shared_prefix_attention(*a.values())
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(T=-1), N.E_INVAL), (dict(n=-1), N.E_INVAL), (dict(groups=-1), N.E_INVAL), (dict(width=-1), N.E_INVAL), (dict(kv=0), N.E_INVAL),
+    (dict(heads=15), N.E_INVAL), (dict(scale=0.0), N.E_INVAL), (dict(scale=float("inf")), N.E_INVAL), (dict(dtype=N.DT_F32), N.E_UNSUPPORTED),
+    (dict(dim=96), N.E_UNSUPPORTED), (dict(out=None), N.E_INVAL), (dict(q=None), N.E_INVAL), (dict(tables=None), N.E_INVAL),
+    (dict(ctx=None), N.E_INVAL), (dict(cache=None), N.E_INVAL), (dict(cache=_cache(v=None)), N.E_INVAL), (dict(cache=_cache(num_blocks=0)), N.E_INVAL),
+    (dict(cache=_cache(k=AT + 8)), N.E_UNSUPPORTED), (dict(q=AT + 2), N.E_UNSUPPORTED), (dict(oh=68), N.E_UNSUPPORTED), (dict(prefix=None), N.E_INVAL),
+    (dict(cu_groups=None), N.E_INVAL), (dict(n=3), N.E_INVAL), (dict(ws=None), N.E_WORKSPACE), (dict(bytes=16), N.E_WORKSPACE),
+    (dict(ws=AT + 4), N.E_UNSUPPORTED), (dict(cu=AT, ws=None), N.E_WORKSPACE), (dict(T=0), 0), (dict(n=0), 0), (dict(T=0, prefix=None), 0),
+])
+def test_shared_prefix_statuses(kw, code):
+    assert _shared(**kw) == code
+
+
 def _join(parts=2, **kw):
     a = dict(out=AT, ot=1024, oh=64, lse=None, outs=[AT] * parts, lses=[AT] * parts, n=parts, pt=1024, ph=64, lt=16, lh=1, T=2, heads=16, dim=64,
              dtype=N.DT_BF16, stream=None)
@@ -71,6 +92,11 @@ def test_python_refusals_without_a_gpu():
         A.differential_decode_attention(q, cache, cache, ints, ints[:, 0].contiguous(), torch.zeros(16))
     with pytest.raises(ValueError, match="cu_seqlens"):
         A.differential_prefill_attention(q, cache, cache, ints, ints[:, 0].contiguous(), None, torch.zeros(16))
+    groups = torch.tensor([0, 2], dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        A.shared_prefix_decode_attention(q, cache, cache, ints, ints[:, 0].contiguous(), groups[:1], groups)
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        A.shared_prefix_prefill_attention(q, cache, cache, ints, ints[:, 0].contiguous(), None, groups[:1], groups)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         A.join_attention(torch.zeros(2, 2, 4, 64), torch.zeros(2, 2, 4))
     with pytest.raises(ValueError, match="one of each"):
@@ -109,6 +135,15 @@ def test_python_refusals_on_a_gpu():
         A.differential_prefill_attention(q, cache, cache, tables, lens, lens, lam)
     with pytest.raises(RuntimeError, match="head_dim"):
         call(q[..., :32].contiguous(), cache[..., :32].contiguous(), cache[..., :32].contiguous(), tables, lens, lam)
+    groups = torch.tensor([0, 2, 2], dtype=torch.int32, device="cuda")
+    for prefix, cu, what in ((lens[:1], groups, "cu_groups"), (lens, groups[:2], "cu_groups"), (lens.long(), groups, "prefix_lens"),
+                             (lens, groups.long(), "cu_groups"), (lens[None], groups, "vectors"), (groups[::2], groups, "vectors")):
+        with pytest.raises(ValueError, match=what):
+            A.shared_prefix_decode_attention(q, cache, cache, tables, lens, prefix, cu)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        A.shared_prefix_decode_attention(q, cache, cache, tables, lens, lens.cpu(), groups)
+    with pytest.raises(ValueError, match="one of each"):
+        A.shared_prefix_decode_attention(q, cache, cache, tables[:1], lens[:1], lens, groups)
     outs, lses = torch.zeros(2, 3, 4, 64, device="cuda"), torch.zeros(2, 3, 4, device="cuda")
     for args, what in (((outs, lses[:1]), "one of each"), (([outs[0], outs[1, :2]], lses), "shape"), (([outs[0], outs[1].half()], lses), "dtype"),
                        ((outs, lses.double()), "float32"), ((outs[0], lses), "one of each|must be"), ((outs, lses[:, :, :2]), "float32")):
