@@ -161,6 +161,7 @@ _SIGNATURES = {
     "lora_b200_shared_prefix_workspace_bytes": (
         c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32],
     ),
+    "lora_b200_shared_prefix_way": (c_int32, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
     "lora_b200_shared_prefix_attention": (
         c_int32,
         [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, POINTER(PagedCache), c_void_p,

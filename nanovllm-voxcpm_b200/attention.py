@@ -164,8 +164,8 @@ def shared_prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cac
     a prefix may end inside a block, of which every request has a copy of its own). Where those lie is read from the table of the group's
     first request, what follows from each one's own. ``prefix_lens`` int32 ``[groups]``, ``cu_groups`` int32 ``[groups + 1]``, ascending;
     requests of no group share nothing, a prefix of zero is none. Other arguments, strides, missing blocks, contexts of no key and the
-    log sums as ``paged_decode_attention``. Block sizes that are multiples of 8; others (and calls with one request a group) are attended
-    request by request. A value that is not finite, of a key of the prefix that some requests of a group see, may reach the group's others."""
+    log sums as ``paged_decode_attention``. Calls whose tables are too narrow for a second launch to pay, block sizes that are no
+    multiples of 8 and groups of one request are attended request by request. A value that is not finite, of a key of the prefix that some requests of a group see, may reach the group's others."""
     return _shared_prefix(q, k_cache, v_cache, block_tables, context_lens, None, prefix_lens, cu_groups, scale, out, return_lse)
 
 
@@ -245,11 +245,11 @@ def join_attention(outs, lses, *, out: torch.Tensor | None = None, return_lse: b
     (``return_lse``), as ``[parts, ...]`` or a sequence. A part without a key (``-inf``) counts for nothing, whatever its values; a row
     that has none in any part gives zeros. ``out`` may be one of the parts. Returns ``out``, with ``return_lse`` also the logarithm of
     the whole sum."""
-    outs, lses = tuple(outs), tuple(lses)
     got = N.native().join_attention(outs, lses, out, bool(return_lse))
     if got is not None:
         N.check(got[0])
         return (got[1], got[2]) if return_lse else got[1]
+    outs, lses = tuple(outs), tuple(lses)
     N.require_cuda(*outs, *lses, out)
     if not outs or len(outs) != len(lses):
         raise ValueError(f"{len(outs)} results and {len(lses)} logarithms: a part has one of each")

@@ -497,6 +497,12 @@ size_t lora_b200_shared_prefix_workspace_bytes(int32_t T, int32_t n_seqs, int32_
   return shared_prefix_workspace_bytes(T, n_seqs, n_groups, num_heads, num_kv_heads, head_dim, block_size, (int64_t)table_width * block_size, packed != 0);
 }
 
+int32_t lora_b200_shared_prefix_way(int32_t T, int32_t n_seqs, int32_t n_groups, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                    int32_t table_width, int32_t block_size, int32_t packed) {
+  if (num_kv_heads < 1 || num_heads < num_kv_heads || head_dim < 1 || block_size < 1 || T < 1) return 0;
+  return px_shares(T, n_seqs, n_groups, num_heads, num_kv_heads, head_dim, block_size, (int64_t)table_width * block_size, packed != 0) ? 1 : 0;
+}
+
 int lora_b200_shared_prefix_attention(void* out, int64_t out_token, int64_t out_head, float* lse, const void* q, int64_t q_token,
                                       int64_t q_head, int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                                       const lora_b200_paged_cache* cache, const int32_t* block_tables, int64_t table_ld,

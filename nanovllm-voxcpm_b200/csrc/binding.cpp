@@ -750,42 +750,66 @@ PyObject* shared_prefix_attention(PyObject*, PyObject* const* args, Py_ssize_t n
   END_HANDLE_TH_ERRORS
 }
 
-// join_attention(outs, lses, out | None, lse?) -> (status, out, lse | None), or None; outs and lses: tuples of tensors
+// The parts of a join: one tensor stacked along its first dimension, or a list or tuple of tensors of one shape, type and set of strides
+struct Parts {
+  static constexpr Py_ssize_t kMost = 64;
+  const at::Tensor* first = nullptr;  // the stack, or the first part
+  int64_t n = 0, stacked = 0;         // 1: the parts' own dimensions begin behind the stack's
+  void* at[kMost];
+
+  int64_t size(int64_t d) const { return first->size(d + stacked); }
+  int64_t stride(int64_t d) const { return first->stride(d + stacked); }
+  bool read(PyObject* o, int64_t dims, int dev) {  // false = not handled
+    first = tensor_of(o);
+    if (first != nullptr) {
+      stacked = 1;
+      n = first->dim() == dims + 1 ? first->size(0) : 0;
+      if (n < 1 || n > kMost || !first->is_cuda() || (dev >= 0 && first->get_device() != dev)) return false;
+      char* const base = static_cast<char*>(first->data_ptr());
+      for (int64_t i = 0; i < n; ++i) at[i] = base + i * first->stride(0) * (int64_t)first->element_size();
+      return true;
+    }
+    PyObject** each;
+    n = items(o, &each);
+    if (n < 1 || n > kMost) return false;
+    first = tensor_of(each[0]);
+    if (first == nullptr || first->dim() != dims || !first->is_cuda() || (dev >= 0 && first->get_device() != dev)) return false;
+    for (int64_t i = 0; i < n; ++i) {
+      const at::Tensor* t = tensor_of(each[i]);
+      if (t == nullptr || !on(*t, first->get_device()) || t->scalar_type() != first->scalar_type() || t->sizes() != first->sizes() ||
+          t->strides() != first->strides())
+        return false;
+      at[i] = t->data_ptr();
+    }
+    return true;
+  }
+};
+
+// join_attention(outs, lses, out | None, lse?) -> (status, out, lse | None), or None
 PyObject* join_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   if (nargs != 4) { PyErr_SetString(PyExc_TypeError, "join_attention takes 4 arguments"); return nullptr; }
-  constexpr Py_ssize_t kMost = 64;
-  if (!PyTuple_CheckExact(args[0]) || !PyTuple_CheckExact(args[1])) return not_handled();
-  const Py_ssize_t parts = PyTuple_GET_SIZE(args[0]);
-  if (parts < 1 || parts > kMost || PyTuple_GET_SIZE(args[1]) != parts) return not_handled();
-  const at::Tensor *first = tensor_of(PyTuple_GET_ITEM(args[0], 0)), *lse0 = tensor_of(PyTuple_GET_ITEM(args[1], 0));
-  if (!first || !lse0 || !first->is_cuda() || first->dim() != 3 || first->stride(2) != 1) return not_handled();
+  Parts outs, lses;
+  if (!outs.read(args[0], 3, -1) || outs.stride(2) != 1) return not_handled();
+  const at::Tensor* const first = outs.first;
   const int dev = first->get_device(), code = dtype_code(first->scalar_type());
-  const int64_t T = first->size(0), heads = first->size(1), d = first->size(2);
+  const int64_t T = outs.size(0), heads = outs.size(1), d = outs.size(2);
   if (code < 0 || dev != c10::cuda::current_device() || T > INT32_MAX || heads < 1 || heads > 65536 || d < 1 || d > 65536) return not_handled();
-  const void* outs[kMost];
-  const float* lses[kMost];
-  for (Py_ssize_t i = 0; i < parts; ++i) {
-    const at::Tensor *o = tensor_of(PyTuple_GET_ITEM(args[0], i)), *x = tensor_of(PyTuple_GET_ITEM(args[1], i));
-    if (!o || !x || !on(*o, dev) || !on(*x, dev) || o->scalar_type() != first->scalar_type() || o->sizes() != first->sizes() ||
-        o->strides() != first->strides() || x->scalar_type() != at::kFloat || x->dim() != 2 || x->size(0) != T || x->size(1) != heads ||
-        x->strides() != lse0->strides())
-      return not_handled();
-    outs[i] = o->data_ptr();
-    lses[i] = static_cast<const float*>(x->data_ptr());
-  }
+  if (!lses.read(args[1], 2, dev) || lses.n != outs.n || lses.first->scalar_type() != at::kFloat || lses.size(0) != T || lses.size(1) != heads)
+    return not_handled();
   at::Tensor fresh, lse;
   const at::Tensor* out = &fresh;
   if (args[2] == Py_None) {
     fresh = at::empty({T, heads, d}, first->options());
   } else {
     out = tensor_of(args[2]);
-    if (out == nullptr || !on(*out, dev) || out->scalar_type() != first->scalar_type() || out->sizes() != first->sizes() || out->stride(2) != 1)
+    if (out == nullptr || !on(*out, dev) || out->scalar_type() != first->scalar_type() || out->dim() != 3 || out->size(0) != T ||
+        out->size(1) != heads || out->size(2) != d || out->stride(2) != 1)
       return not_handled();
   }
   if (args[3] == Py_True) lse = at::empty({T, heads}, first->options().dtype(at::kFloat));
-  const int rc = p_join(out->data_ptr(), out->stride(0), out->stride(1), lse.defined() ? static_cast<float*>(lse.data_ptr()) : nullptr, outs, lses,
-                        (int)parts, first->stride(0), first->stride(1), lse0->stride(0), lse0->stride(1), (int)T, (int)heads, (int)d, code,
+  const int rc = p_join(out->data_ptr(), out->stride(0), out->stride(1), lse.defined() ? static_cast<float*>(lse.data_ptr()) : nullptr, outs.at,
+                        reinterpret_cast<const float* const*>(lses.at), (int)outs.n, outs.stride(0), outs.stride(1), lses.stride(0), lses.stride(1), (int)T, (int)heads, (int)d, code,
                         c10::cuda::getCurrentCUDAStream(dev).stream());
   PyObject* lse_out = Py_None;
   if (lse.defined()) lse_out = THPVariable_Wrap(lse);

@@ -28,6 +28,9 @@ struct RowKeys {
   __device__ __forceinline__ int key(int i) const { return i < n_sink ? i : i - n_sink + first; }
 };
 
+// What two launches over a prefix and behind it tell each other: tiles of keys in a part; the next item that no CTA has taken
+struct PxHead { int chunk, next_item, pad[2]; };
+
 struct PagedArgs {
   const void* q; int64_t q_token, q_head;      // [T, Hq, D], strides in elements
   void* out; int64_t out_token, out_head;
@@ -44,10 +47,10 @@ struct PagedArgs {
   const float* lam; int64_t lam_token, lam_head;
   const void* norm_weight; float eps;
   // prefixes that groups of requests share: requests [cu_groups[g], cu_groups[g + 1]) begin with the same prefix_lens[g] keys. What a
-  // launch ahead leaves of them: sums over px_chunk tiles of keys each, [part, T, Hq, D] and (reference, sum) [part, T, Hq]
+  // launch ahead leaves of them: sums over px_head->chunk tiles of keys each, [part, T, Hq, D] and (reference, sum) [part, T, Hq]
   const int32_t *prefix_lens, *cu_groups; int n_groups;
   int px_most;                                 // parts of a prefix at most
-  int* px_chunk; float2* px_ml; float* px_o;
+  PxHead* px_head; float2* px_ml; float* px_o;
 };
 
 // What a kernel makes of a head: one softmax map; or two, of the halves of its columns of q and k over the whole of v, and of them the
@@ -73,13 +76,9 @@ __device__ __forceinline__ PxGroup px_group(const PagedArgs& a, int g) {
   p = {r0, r1, begin, end, (int)min((int64_t)max(keys, 0), (int64_t)a.table_width * a.cache.block_size)};
   return p;
 }
-// Keys of the prefix that request `req` shares; a whole warp calls it. Up to 32 groups are looked at side by side.
-__device__ __forceinline__ int px_keys(const PagedArgs& a, int req) {
-  if (a.n_groups <= 32) {
-    const PxGroup p = px_group(a, (int)(threadIdx.x & 31));
-    const uint32_t hit = __ballot_sync(0xffffffffu, p.r0 <= req && req < p.r1);
-    return hit == 0 ? 0 : __shfl_sync(0xffffffffu, p.keys, __ffs(hit) - 1);
-  }
+// Keys of the prefix that request `req` shares: of the first 32 groups that of the first one which has it, where they are all; else of the
+// last one that begins at or before it. A whole warp calls it; `lanes`: group `lane` of the first 32, looked up once.
+__device__ __forceinline__ int px_keys_of_many(const PagedArgs& a, int req) {
   int lo = 0, hi = a.n_groups;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -89,20 +88,42 @@ __device__ __forceinline__ int px_keys(const PagedArgs& a, int req) {
   const PxGroup p = px_group(a, lo);
   return p.r0 <= req && req < p.r1 ? p.keys : 0;
 }
+__device__ __forceinline__ int px_keys(const PagedArgs& a, const PxGroup& lanes, int req) {
+  if (a.n_groups > 32) return px_keys_of_many(a, req);
+  const uint32_t hit = __ballot_sync(0xffffffffu, lanes.r0 <= req && req < lanes.r1);
+  return hit == 0 ? 0 : __shfl_sync(0xffffffffu, lanes.keys, __ffs(hit) - 1);
+}
 // (behind the wait for the launch that wrote it)
 __device__ __forceinline__ int px_parts(const PagedArgs& a, int keys) {
-  const int tiles = (int)(((unsigned)keys + kPrefixTile - 1u) / kPrefixTile), chunk = max(1, __ldcg(a.px_chunk));
+  const int tiles = (int)(((unsigned)keys + kPrefixTile - 1u) / kPrefixTile), chunk = max(1, __ldcg(&a.px_head->chunk));
   return min(a.px_most, (tiles + chunk - 1) / chunk);
 }
 
+// (kForm kSuffix: a whole warp calls it, with the same row)
 template <int kForm>
-__device__ __forceinline__ RowKeys row_keys(const PagedArgs& a, int row) {
+__device__ __forceinline__ RowKeys row_keys(const PagedArgs& a, const PxGroup& groups, int row) {
   RowKeys r = {row, 0, 0, -1};
   int64_t ctx;
-  if constexpr (kForm == kSuffix) {  // (one row a request)
-    ctx = max(__ldcg(a.context_lens + row), 0);
-    const int64_t held = min(ctx, (int64_t)a.table_width * a.cache.block_size);
-    r.first = px_keys(a, row);
+  if constexpr (kForm == kSuffix) {
+    if (a.cu_seqlens == nullptr) {
+      ctx = __ldcg(a.context_lens + row);
+    } else {
+      // the last request that begins at or before the row, 32 looked at side by side
+      int lo = 0, n = a.n_req;
+      while (n > 1) {
+        const int step = (n + 31) / 32, at = (int)(threadIdx.x & 31) * step;
+        const uint32_t before = __ballot_sync(0xffffffffu, at < n && __ldcg(a.cu_seqlens + lo + min(at, n - 1)) <= row);
+        const int k = max(0, 31 - __clz(before)) * step;
+        lo += k;
+        n = min(step, n - k);
+      }
+      const int begin = __ldcg(a.cu_seqlens + lo), end = __ldcg(a.cu_seqlens + lo + 1);
+      if (begin < 0 || end > a.T || row < begin || row >= end) return r;
+      r.req = lo;
+      ctx = (int64_t)__ldcg(a.context_lens + lo) - (end - 1 - row);
+    }
+    const int64_t held = min(max(ctx, (int64_t)0), (int64_t)a.table_width * a.cache.block_size);
+    r.first = px_keys(a, groups, r.req);
     r.n_keys = (int)max((int64_t)0, held - r.first);
     return r;
   }
@@ -197,25 +218,38 @@ __device__ __forceinline__ void store_difference(const PagedArgs& a, bool live, 
         make_uint2(pack_16x2<kF16>(y.x, y.y), pack_16x2<kF16>(y.z, y.w));
 }
 
-// Four columns of a head over the keys behind the prefix, joined with the parts over the prefix (none: 0 of them). A part without a key that
-// the row sees has no sums.
+// Four columns of a head over the keys behind the prefix, joined with the parts over the prefix (none: 0 of them), of which kPxAtOnce are
+// under way at a time. A part without a key that the row sees has no sums.
+constexpr int kPxAtOnce = 8;
 template <int D, bool kF16>
 __device__ __forceinline__ void store_behind_prefix(const PagedArgs& a, int64_t row, int head, int c, int parts, float4 x, float m, float l) {
   const int64_t at = row * a.Hq + head, step = (int64_t)a.T * a.Hq;
   float top = m;
-#pragma unroll 8
-  for (int k = 0; k < parts; ++k) top = fmaxf(top, __ldcg(a.px_ml + at + k * step).x);
-  const float own = m == -INFINITY ? 0.f : ex2(m - top);
-  x = make_float4(x.x * own, x.y * own, x.z * own, x.w * own);
-  l *= own;
-#pragma unroll 8
-  for (int k = 0; k < parts; ++k) {
-    const float2 ml = __ldcg(a.px_ml + at + k * step);
-    const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
-    float4 v = __ldcg(reinterpret_cast<const float4*>(a.px_o + (at + k * step) * D) + c);
-    if (ml.x == -INFINITY) v = make_float4(0.f, 0.f, 0.f, 0.f);
-    l += f * ml.y;
-    x = make_float4(x.x + f * v.x, x.y + f * v.y, x.z + f * v.z, x.w + f * v.w);
+  for (int k0 = 0; k0 < parts; k0 += kPxAtOnce) {
+    float2 ml[kPxAtOnce];
+    float4 v[kPxAtOnce];
+#pragma unroll
+    for (int k = 0; k < kPxAtOnce; ++k) {
+      ml[k] = make_float2(-INFINITY, 0.f);
+      if (k0 + k < parts) {
+        ml[k] = __ldcg(a.px_ml + at + (k0 + k) * step);
+        v[k] = __ldcg(reinterpret_cast<const float4*>(a.px_o + (at + (k0 + k) * step) * D) + c);
+      }
+    }
+    float up = top;
+#pragma unroll
+    for (int k = 0; k < kPxAtOnce; ++k) up = fmaxf(up, ml[k].x);
+    const float own = top == -INFINITY ? 0.f : ex2(top - up);
+    top = up;
+    l *= own;
+    x = make_float4(x.x * own, x.y * own, x.z * own, x.w * own);
+#pragma unroll
+    for (int k = 0; k < kPxAtOnce; ++k) {
+      if (ml[k].x == -INFINITY) continue;
+      const float f = ex2(ml[k].x - top);
+      l += f * ml[k].y;
+      x = make_float4(x.x + f * v[k].x, x.y + f * v[k].y, x.z + f * v[k].z, x.w + f * v[k].w);
+    }
   }
   const float inv = over(l);
   *reinterpret_cast<uint2*>(static_cast<char*>(a.out) + 2 * (row * a.out_token + head * a.out_head + 4 * c)) =
@@ -233,6 +267,7 @@ struct PagedPiece {
 template <int kKeys, int kForm>
 struct PagedWalk {
   long long at, end, row_at;  // share: units; first unit of `row`
+  PxGroup groups;             // behind a prefix: of the first 32 groups the lane's
   int row, step;              // step > 0: items `at`, at + step, ..., of each the rank-th of `ranks` parts
   int rank, ranks;
   static __device__ __forceinline__ int units(const RowKeys& r) { return r.n_keys < 0 ? 0 : max(1, (int)(((unsigned)r.n_keys + kKeys - 1u) / kKeys)); }
@@ -245,14 +280,14 @@ struct PagedWalk {
       if (step > 0) {
         row = (int)(at / per_row);
         item = (int)(at - (long long)row * per_row);
-        at += step;
-        w.keys = row_keys<kForm>(a, row);
+        at = kForm == kSuffix && ranks == 1 ? end : at + step;  // (there the caller says what is next)
+        w.keys = row_keys<kForm>(a, groups, row);
         w.n_units = units(w.keys);
-        if (w.n_units == 0) continue;
+        if (w.n_units == 0 && !(kForm == kSuffix && ranks == 1)) continue;  // (else: a piece of no heads, for the caller asks once an item)
         w.u0 = (int)((int64_t)w.n_units * rank / ranks);
         w.u1 = (int)((int64_t)w.n_units * (rank + 1) / ranks);
       } else {
-        w.keys = row_keys<kForm>(a, row);
+        w.keys = row_keys<kForm>(a, groups, row);
         w.n_units = units(w.keys);
         if (at >= row_at + (long long)w.n_units * per_row) {
           row_at += (long long)w.n_units * per_row;
@@ -269,7 +304,7 @@ struct PagedWalk {
       w.kvh = item / a.chunks;
       const int chunk = item - w.kvh * a.chunks;
       w.head0 = w.kvh * group + chunk * a.heads;
-      w.n_heads = min(a.heads, group - chunk * a.heads);
+      w.n_heads = w.keys.n_keys < 0 ? 0 : min(a.heads, group - chunk * a.heads);
       return w;
     }
     return w;
@@ -297,6 +332,10 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
   __shared__ int s_row;
   __shared__ long long s_at, s_sum[kPagedWarps];
   __shared__ uint32_t s_live[kPagedWarps][kPagedStages];
+  // Behind a prefix a CTA has one item to begin with, and then takes what nobody has: items are of any length, and some CTAs start late,
+  // where CTAs of the prefix launch have been. (Which CTA has an item changes nothing in it.)
+  constexpr bool kQueue = kForm == kSuffix && kWay == kWhole;
+  __shared__ int s_next;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int per_row = a.Hk * a.chunks;
   using Walk = PagedWalk<kKeys, kForm>;
@@ -311,6 +350,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
   if (kForm != kSuffix) glue_enter();
 
   Walk walk;
+  if constexpr (kForm == kSuffix) walk.groups = px_group(a, lane);
   long long total = 0;
   int G = gridDim.x;
   if (!kShare) {
@@ -323,7 +363,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
     // where this CTA's share begins: sums over the rows, a thread a run of them
     const int rows_each = (a.T + kPagedThreads - 1) / kPagedThreads;
     long long sum = 0;
-    for (int i = 0, row = tid * rows_each; i < rows_each && row < a.T; ++i, ++row) sum += Walk::units(row_keys<kForm>(a, row));
+    for (int i = 0, row = tid * rows_each; i < rows_each && row < a.T; ++i, ++row) sum += Walk::units(row_keys<kForm>(a, walk.groups, row));
     long long upto = sum;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
@@ -350,7 +390,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
       long long at = from;
       int row = tid * rows_each;
       for (;; ++row) {
-        const long long n = (long long)Walk::units(row_keys<kForm>(a, row)) * per_row;
+        const long long n = (long long)Walk::units(row_keys<kForm>(a, walk.groups, row)) * per_row;
         if (walk.at < at + n) break;
         at += n;
       }
@@ -418,6 +458,9 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
     }
   };
 
+  auto take = [&]() { return (int)gridDim.x + atomicAdd(&a.px_head->next_item, 1); };
+  int taken = 0;
+  if (kQueue && tid == 0) taken = take();
   PagedPiece w = walk.next(a);
   int stage = 0, buf = 0;
   bool first_piece = true;
@@ -427,16 +470,21 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
     load(w, w.u0 + warp, e0, 0);
     load(w, w.u0 + warp + kPagedWarps, e1, 1);
     put_q(0);
+    if (kQueue && tid == 0) s_next = taken;
   }
   while (w.row >= 0) {
     int e = entry(w, w.u0 + warp + 2 * kPagedWarps);
+    if (kQueue) {
+      __syncthreads();  // (q is there, too)
+      walk.at = s_next;
+    }
     const PagedPiece following = walk.next(a);
     const int e0 = entry(following, following.u0 + warp), e1 = entry(following, following.u0 + warp + kPagedWarps);
     load_q(following);
     if (kWay == kClusters) {
       cluster_arrive();
       cluster_wait();
-    } else {
+    } else if (!kQueue) {
       __syncthreads();  // q is there; the stages that held results may be filled again
     }
     uint32_t qf[NT][kSteps][2];
@@ -556,6 +604,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
         l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 8);
         l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 16);
       }
+    if (kQueue && tid == 0) taken = take();
     // the warps' results, each in the third stage of its ring, where nothing is under way
     __shared__ int s_third[kPagedWarps];
     float* const mine = reinterpret_cast<float*>(smem + ring_at + after(stage, 2) * kStage);
@@ -581,8 +630,8 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
     constexpr bool kFour = kForm != kPlain;
     constexpr int kSumHeads = 8 * NT / kMaps<kForm>;
     int prefix_parts = 0;
-    if (kForm == kSuffix && kWay != kClusters) {
-      if (first_piece) glue_enter();
+    if (kForm == kSuffix && kWay != kClusters && whole) {
+      glue_enter();
       prefix_parts = px_parts(a, w.keys.first);
     }
     for (int i = tid; kFour && i < kSumHeads * (D / 4); i += kPagedThreads) {
@@ -649,7 +698,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
       cluster_arrive();
       cluster_wait();
       if (kForm == kSuffix) {
-        if (first_piece) glue_enter();
+        glue_enter();
         prefix_parts = px_parts(a, w.keys.first);
       }
       if (kFour) {  // (whole heads, for their norm; whole warps, for its sum)
@@ -725,12 +774,13 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
       while (total * last / G >= item_end) --last;
       a.joins[blockIdx.x] = make_int4(w.row, w.head0, slot, last);
     }
+    if (kQueue && tid == 0) s_next = taken;
     first_piece = false;
     buf ^= 1;
     w = following;
   }
   cp_async_wait_group<0>();
-  if (kForm == kSuffix && first_piece) glue_enter();  // (this launch ends behind the one ahead whatever its CTAs find)
+  if (kForm == kSuffix) glue_enter();  // (this launch ends behind the one ahead whatever its CTAs find)
   if (kWay == kClusters) {  // (no CTA leaves while another reads its part)
     cluster_arrive();
     cluster_wait();
@@ -861,6 +911,13 @@ inline int paged_decode_launch_by(const PagedArgs& a, cudaStream_t stream) {
   if constexpr (kForm != kSuffix)
     if (w.shares && a.part_o != nullptr) return paged_decode_launch_t<D, NT, kF16, kShares, 4, kForm>(a, kPagedCtas, 1, stream);
   const int64_t items = (int64_t)a.T * a.Hk * a.chunks;
+  // Behind a prefix, items that CTAs take as they come: four warps, for which an SM has room beside a CTA of the prefix launch (64 requests
+  // of 10 to 600 keys behind 2000, 16 / 2 heads of 64, 13.9 us, eight warps 18.5). Shares would be even where the keys behind the prefix
+  // are many, which the host does not know: 48 requests, 32 / 8 heads of 128, of 500 / 3000 keys behind 8000, items 48 / 168 us, shares 65 / 138.
+  if constexpr (kForm == kSuffix) {
+    if (w.cluster > 1) return paged_decode_launch_t<D, NT, kF16, kClusters, 8, kForm>(a, (int)std::min<int64_t>(148 / w.cluster, items) * w.cluster, w.cluster, stream);
+    return paged_decode_launch_t<D, NT, kF16, kWhole, 4, kForm>(a, (int)std::min<int64_t>(kPagedCtas, items), 1, stream);
+  }
   const int ctas = (int)std::min<int64_t>((w.warps == 8 ? 148 : kPagedCtas) / w.cluster, items) * w.cluster;
   if (w.cluster > 1) return paged_decode_launch_t<D, NT, kF16, kClusters, 8, kForm>(a, ctas, w.cluster, stream);
   if (w.warps == 8) return paged_decode_launch_t<D, NT, kF16, kWhole, 8, kForm>(a, ctas, 1, stream);

@@ -39,7 +39,8 @@ template <int D>
 __host__ __device__ constexpr int pp_tile() { return kPpKeys * D * 2; }
 // Tiles of a CTA, and how many of them have rows of their own: the two maps of differential heads are two tiles of the same rows.
 static_assert(kPpKeys == kPrefixTile, "parts of a prefix are whole tiles");
-__host__ __device__ constexpr int pp_tiles(int D, int form) { return D == 64 && form != kDiff ? 1 : 2; }
+// (The rows over a prefix seldom fill two, and one leaves an SM room for a CTA of the launch over the keys behind it.)
+__host__ __device__ constexpr int pp_tiles(int D, int form) { return (D == 128 && form == kPlain) || form == kDiff ? 2 : 1; }
 __host__ __device__ constexpr int pp_row_tiles(int D, int form) { return form == kDiff ? 1 : pp_tiles(D, form); }
 template <int D>
 __host__ __device__ constexpr int pp_smem(int tiles, int row_tiles) { return (2 * pp_stages<D>(tiles) + row_tiles) * pp_tile<D>() + tiles * kPpRows * kPpOutPitch + 1024; }
@@ -135,7 +136,7 @@ struct PpPiece {
   int req, pos0, held, key_end, lo_first, sink_end;  // position of the first token; keys that a row sees: [0, sink_end), [lo_first, key_end)
   int first_box, sink_boxes, i0, i1;           // the keys in boxes: those of the first tokens, then from first_box on, side by side
   int parts;                                   // 0: no more pieces; 1: the whole item; else the item is in that many parts
-  int part, r1, keys;                              // of a prefix: which part of it; its keys. Behind a prefix: the keys of that
+  int part, r1, keys;                          // of a prefix: which part of it, the request behind the group's, its keys
   // first key of box b of tile i, with 1 << shift keys in a box
   __device__ __forceinline__ int key_of(int i, int b, int shift) const {
     const int c = i * (kPpKeys >> shift) + b;
@@ -198,7 +199,6 @@ __device__ __forceinline__ int pp_items(const PpArgs& a, int span, const PpLane&
 // they end at; more: the last block of the last sequence first; 32 requests of 30 to 400 tokens, heads of 64, 27.2 us, 33 of them 33.3;
 // of 100 each 13.9 and 14.5), the sets of heads of a block one after another. A whole warp calls
 // it, with the first 32 requests in hand.
-template <int kForm>
 __device__ __forceinline__ void pp_find(const PpArgs& a, int span, int item, int n_items, const PpLane& lanes0, PpPiece* w) {
   const PagedArgs& p = a.p;
   const int lane = threadIdx.x & 31, back = item / a.head_tiles;
@@ -240,7 +240,6 @@ __device__ __forceinline__ void pp_find(const PpArgs& a, int span, int item, int
   w->held = (int)min((int64_t)w->pos0 + w->n_here, (int64_t)p.table_width * p.cache.block_size);
   w->key_end = w->held;
   w->lo_first = p.window > 0 ? max(0, max(w->pos0, 0) - (p.window - 1)) : 0;
-  if (kForm == kSuffix) w->lo_first = w->keys = px_keys(p, w->req);
   w->sink_end = max(0, min(min(p.sinks, w->lo_first), w->key_end));
   // (a window behind the table's end has no box; its first one is at the end, since a key next to 2^31 and its tile need not fit an int)
   w->first_box = min(w->lo_first, max(w->held, 0) + a.box - 1) >> a.box_shift;
@@ -261,22 +260,38 @@ __device__ __forceinline__ PxLane px_lane(const PpArgs& a, int span, int g) {
   q.blocks = q.tiles == 0 ? 0 : (q.g.end - q.g.begin + span - 1) / span;
   return q;
 }
+// A part of `chunk` tiles each: one wave of CTAs where that is possible, since ceil(t / c) <= t / c + 1, so that with R items of one part
+// each and W tiles over them W / c + R <= CTAs; then the least c near it that still fits.
 __device__ __forceinline__ int px_chunk_tiles(const PpArgs& a, int span, const PxLane& lanes0) {
-  long long work = 0;
+  long long work = 0, rows = 0;
   int longest = 0;
   for (int base = 0; base < a.p.n_groups; base += 32) {
     const PxLane q = base == 0 ? lanes0 : px_lane(a, span, base + (int)(threadIdx.x & 31));
     work += (long long)q.blocks * q.tiles;
+    rows += q.blocks;
     longest = max(longest, q.tiles);
   }
 #pragma unroll
   for (int d = 16; d > 0; d /= 2) {
     work += __shfl_xor_sync(0xffffffffu, work, d);
-    longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, d));
+    rows += __shfl_xor_sync(0xffffffffu, rows, d);
   }
+  longest = __reduce_max_sync(0xffffffffu, longest);
   work *= a.head_tiles;
-  const long long even = (work + a.px_ctas - 1) / a.px_ctas, least = max(kPxChunk, (longest + a.p.px_most - 1) / a.p.px_most);
-  return (int)min(max(even, least), (long long)INT32_MAX);
+  rows *= a.head_tiles;
+  const int once = a.px_ctas / 2;  // (a CTA an SM leaves room beside it; two where that is long, too)
+  const long long one = work > 8ll * once ? a.px_ctas : once;
+  const long long ctas = one * max(1ll, (2 * rows + one - 1) / one);  // (as many waves as leave half of the places to cuts)
+  const int least = max(kPxChunk, (longest + a.p.px_most - 1) / a.p.px_most);
+  int chunk = (int)min((work + max(1ll, ctas - rows) - 1) / max(1ll, ctas - rows), (long long)INT32_MAX);
+  if (a.p.n_groups <= 32) {
+    for (int k = 0; k < 8 && chunk > least; ++k) {
+      const unsigned mine = (unsigned)min((long long)lanes0.blocks * a.head_tiles * ((lanes0.tiles + chunk - 2) / (chunk - 1)), 1ll << 26);
+      if (__reduce_add_sync(0xffffffffu, mine) > ctas) break;
+      --chunk;
+    }
+  }
+  return max(chunk, least);
 }
 // Items of a group, at most INT32_MAX over all (the host sees to that for groups that do not overlap)
 __device__ __forceinline__ int px_items_of(const PpArgs& a, const PxLane& q, int chunk) {
@@ -327,52 +342,12 @@ __device__ __forceinline__ void px_find(const PpArgs& a, int span, int chunk, in
   }
 }
 
-// Sums (m, l) of a row and head over the keys behind the prefix, joined with those over its parts: the common reference, what the own
-// numerators count, 1 / sum, the logarithm
-struct PxJoined { float top, own, inv, lse; };
-__device__ __forceinline__ PxJoined px_join(const PagedArgs& p, int64_t at, int parts, float m, float l) {
-  const int64_t step = (int64_t)p.T * p.Hq;
-  PxJoined j;
-  j.top = m;
-#pragma unroll 4
-  for (int k = 0; k < parts; ++k) j.top = fmaxf(j.top, __ldcg(p.px_ml + at + k * step).x);
-  j.own = m == -INFINITY ? 0.f : ex2(m - j.top);
-  l *= j.own;
-#pragma unroll 4
-  for (int k = 0; k < parts; ++k) {
-    const float2 ml = __ldcg(p.px_ml + at + k * step);
-    l += (ml.x == -INFINITY ? 0.f : ex2(ml.x - j.top)) * ml.y;
-  }
-  j.inv = over(l);
-  j.lse = l == 0.f ? -INFINITY : (j.top + log2f(l)) * 0.6931471805599453f;
-  return j;
-}
-// Adds the parts' numerators of N columns, `col` on; a part without a key that the row sees has none.
-template <int D, int N>
-__device__ __forceinline__ void px_add(const PagedArgs& p, int64_t at, int parts, float top, int col, float (&x)[N]) {
-  const int64_t step = (int64_t)p.T * p.Hq;
-  for (int k = 0; k < parts; ++k) {
-    const float reference = __ldcg(p.px_ml + at + k * step).x;
-    if (reference == -INFINITY) continue;
-    const float f = ex2(reference - top);
-    const float4* const src = reinterpret_cast<const float4*>(p.px_o + (at + k * step) * D + col);
-#pragma unroll
-    for (int c = 0; c < N / 4; ++c) {
-      const float4 v = __ldcg(src + c);
-      x[4 * c] += f * v.x;
-      x[4 * c + 1] += f * v.y;
-      x[4 * c + 2] += f * v.z;
-      x[4 * c + 3] += f * v.w;
-    }
-  }
-}
-
 // The part of an item that CTA c leaves for the join (slot c): numerators [row / 128][column / 4][row % 128] of four columns, then
 // maximum and sum of every row.
 template <int D>
 __host__ __device__ constexpr int pp_slot_floats(int tiles) { return tiles * kPpRows * (D + 2); }
 // Of the item whose parts the CTAs c, c + stride, ... (`parts` of them) hold; parts < 2: none
-struct PpJoin { int head0, token0, n_here, parts, stride, keys, pad[2]; };  // keys: of the prefix
+struct PpJoin { int head0, token0, n_here, parts, stride, pad[3]; };
 
 // kForm kDiff: the tiles are the two maps of the same rows, over the same K and V: scores take half of the columns each, a warpgroup
 // ends with half of the columns of both maps' O.
@@ -412,8 +387,16 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  // (Dependents may start: every CTA of this launch holds its tensor memory by then. Behind a prefix launch only the join waits for it.)
-  if (kForm != kSuffix) glue_enter();
+  if (kForm == kPrefix) {
+    // The launch behind this one starts once all CTAs have let it, and takes its items from a counter that is there by then.
+    griddep_wait();
+    if (blockIdx.x == 0 && tid == 0) {
+      p.px_head->next_item = 0;
+      __threadfence();
+    }
+    __syncthreads();
+  }
+  glue_enter();  // (dependents may start: every CTA of this launch holds its tensor memory by then)
   const uint32_t tmem = s_tmem;
   const int per_tile = kPpRows >> a.h_shift, span = kRowTiles * per_tile;
 
@@ -433,12 +416,11 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
     const uint32_t all_boxes = bits_below(kPpKeys / a.box);
     const int tile_shift = 7 - a.box_shift, step = min(a.box, 32);  // boxes of a tile, as a logarithm; columns of 32 that lie in one box
     const uint32_t stage = out_u32 + warp * (32 * kPpOutPitch);  // 32 columns of the warp's rows on their way out
-    bool waited = false;
     uint32_t n = 0, pieces = 0, exchanges = 0;  // tiles and pieces with tiles so far: phases of the barriers
     PpPiece w;
     for (int k = 0; take(k, &w); ++k) {
       int pos = pp_position(w.pos0, tok);
-      const int lo = kForm == kSuffix ? w.lo_first : p.window > 0 ? max(pos, 0) - (p.window - 1) : 0;
+      const int lo = p.window > 0 ? max(pos, 0) - (p.window - 1) : 0;
       int tile_lo = pp_position(w.pos0, tok0);
       if (kForm == kPrefix) {  // (rows have positions of their own, most of them behind the prefix; the first key that some row of the warp does not see)
         pos = tok < w.n_here && w.i1 > w.i0 ? min(px_position(p, w.begin + w.q0 + tok, w.req, w.r1), w.keys - 1) : w.keys - 1;
@@ -446,7 +428,7 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
       }
       const int tile_hi = pp_position(tile_lo, per_tile - 1);  // positions of the tile
       // tiles [clear0, clear1) need no mask: behind the first tokens, from where every row's window has begun, up to the first row
-      const int w_lo = kForm == kSuffix ? w.lo_first : p.window > 0 ? max(tile_hi, 0) - (p.window - 1) : 0;
+      const int w_lo = p.window > 0 ? max(tile_hi, 0) - (p.window - 1) : 0;
       const int clear0 = (w.sink_boxes + max(0, (int)(((uint32_t)max(w_lo, 0) + a.box - 1u) >> a.box_shift) - w.first_box) + (1 << tile_shift) - 1) >> tile_shift;
       const int clear1 = (((tile_lo + 1) >> a.box_shift) + w.sink_boxes - w.first_box) >> tile_shift;
       float m = -INFINITY, l = 0.f;  // what the probabilities refer to, in units of log2; their sum
@@ -646,41 +628,6 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
           __syncwarp();
         }
         if (live) p.px_ml[part_at + (int64_t)tok * p.Hq + w.head0 + (row & ((1 << a.h_shift) - 1))] = make_float2(m, l);
-      } else if (kForm == kSuffix && whole) {
-        if (!waited) glue_enter();  // (the prefix's parts)
-        waited = true;
-        const int64_t at = (token0 + (live ? tok : 0)) * p.Hq + w.head0 + (row & ((1 << a.h_shift) - 1));
-        const int parts = live ? px_parts(p, w.keys) : 0;
-        const PxJoined j = px_join(p, at, parts, m, l);
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          if (any) {
-            tmem_ld_32x32(o_at + 32 * c, o);
-            tmem_ld_wait();
-          }
-          float x[32];
-#pragma unroll
-          for (int k = 0; k < 32; ++k) x[k] = any ? __uint_as_float(o[k]) * j.own : 0.f;
-          px_add<D>(p, at, parts, j.top, 32 * c, x);
-#pragma unroll
-          for (int k = 0; k < 32; k += 8) {
-            uint4 v;
-            v.x = pack_16x2<kF16>(x[k] * j.inv, x[k + 1] * j.inv);
-            v.y = pack_16x2<kF16>(x[k + 2] * j.inv, x[k + 3] * j.inv);
-            v.z = pack_16x2<kF16>(x[k + 4] * j.inv, x[k + 5] * j.inv);
-            v.w = pack_16x2<kF16>(x[k + 6] * j.inv, x[k + 7] * j.inv);
-            sts128(stage + lane * kPpOutPitch + 2 * k, v);
-          }
-          __syncwarp();
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            char* const dst = stored(r, 32 * c);
-            if (dst != nullptr) stg128(dst, lds128(stage + (8 * r + (lane >> 2)) * kPpOutPitch + 16 * (lane & 3)));
-          }
-          __syncwarp();
-        }
-        if (live && p.lse != nullptr) p.lse[at] = j.lse;
       } else if (whole) {
         // Through shared memory, so that four lanes write 64 adjacent bytes of a row. (A row's pieces straight from its thread: 32
         // half-used sectors a store, 3200 cycles for a tile of 128 columns.)
@@ -747,7 +694,7 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
       if constexpr (kForm == kPrefix) {
         groups0 = px_lane(a, span, lane);
         chunk = px_chunk_tiles(a, span, groups0);
-        if (blockIdx.x == 0 && leader) *p.px_chunk = chunk;
+        if (blockIdx.x == 0 && leader) p.px_head->chunk = chunk;
       } else {
         lanes0 = pp_lane(a, span, lane);
         n_items = pp_items(a, span, lanes0);
@@ -765,22 +712,22 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
         if constexpr (kForm == kPrefix) {
           px_find(a, span, chunk, k * G + (int)blockIdx.x, groups0, &w);
         } else if (k < waves) {
-          pp_find<kForm>(a, span, k * G + c, n_items, lanes0, &w);
+          pp_find(a, span, k * G + c, n_items, lanes0, &w);
         } else if (k == waves && most >= 2) {
           const int i = blockIdx.x % rest, s = blockIdx.x / rest;
           if (s < most) {
-            pp_find<kForm>(a, span, k * G + i, n_items, lanes0, &w);
+            pp_find(a, span, k * G + i, n_items, lanes0, &w);
             const int tiles = w.i1;
             w.parts = max(1, min(min(most, kPpParts), tiles / kPpShare));
             if (s >= w.parts) w.parts = 0;
             if (w.parts > 1) {
               w.i0 = (int)((int64_t)tiles * s / w.parts);
               w.i1 = (int)((int64_t)tiles * (s + 1) / w.parts);
-              if (s == 0 && leader) static_cast<PpJoin*>(a.joins)[i] = {w.head0, w.begin + w.q0, w.n_here, w.parts, rest, kForm == kSuffix ? w.keys : 0, {0, 0}};
+              if (s == 0 && leader) static_cast<PpJoin*>(a.joins)[i] = {w.head0, w.begin + w.q0, w.n_here, w.parts, rest, {0, 0, 0}};
             }
           }
         } else if (k == waves && c < rest) {
-          pp_find<kForm>(a, span, k * G + c, n_items, lanes0, &w);
+          pp_find(a, span, k * G + c, n_items, lanes0, &w);
         }
         more_pieces = w.parts > 0;
         if (k >= 2) pp_wait(bar(TAKEN + (k & 1)), (uint32_t)((k >> 1) - 1) & 1, &abort_flag);
@@ -919,7 +866,6 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
       }
     }
   }
-  if (kForm == kSuffix) glue_enter();  // (this launch ends behind the one ahead, whatever its CTAs found)
   __syncthreads();
   if (warp == kIssuer) {
     tc_fence_after_sync();
@@ -930,7 +876,7 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
 
 // Joins the parts of the item that CTA blockIdx.x has the first part of. A thread per row of the item, 16 columns (blockIdx.y): eight
 // parts' worth of them are under way at a time.
-template <int D, bool kF16, int kTiles, int kForm>
+template <int D, bool kF16, int kTiles>
 __global__ void __launch_bounds__(kTiles * kPpRows) paged_prefill_join_kernel(const __grid_constant__ PpArgs a) {
   glue_enter();
   const PpJoin j = static_cast<const PpJoin*>(a.joins)[blockIdx.x];
@@ -960,25 +906,7 @@ __global__ void __launch_bounds__(kTiles * kPpRows) paged_prefill_join_kernel(co
     }
   }
   const int64_t token = (int64_t)j.token0 + tok;
-  float inv = over(sum), lse = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
-  if constexpr (kForm == kSuffix) {
-    const int64_t at = token * p.Hq + head;
-    const int parts = px_parts(p, j.keys);
-    const PxJoined both = px_join(p, at, parts, top, sum);
-    float x[16];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      x[4 * c] = o[c].x * both.own;
-      x[4 * c + 1] = o[c].y * both.own;
-      x[4 * c + 2] = o[c].z * both.own;
-      x[4 * c + 3] = o[c].w * both.own;
-    }
-    px_add<D>(p, at, parts, both.top, 4 * c0, x);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) o[c] = make_float4(x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
-    inv = both.inv;
-    lse = both.lse;
-  }
+  const float inv = over(sum);
   char* const dst = static_cast<char*>(p.out) + 2 * (token * p.out_token + head * p.out_head + 4 * c0);
 #pragma unroll
   for (int c = 0; c < 4; c += 2) {
@@ -989,7 +917,7 @@ __global__ void __launch_bounds__(kTiles * kPpRows) paged_prefill_join_kernel(co
     v.w = pack_16x2<kF16>(o[c + 1].z * inv, o[c + 1].w * inv);
     stg128(dst + 8 * c, v);
   }
-  if (c0 == 0 && p.lse != nullptr) p.lse[token * p.Hq + head] = lse;
+  if (c0 == 0 && p.lse != nullptr) p.lse[token * p.Hq + head] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
 // The same for differential heads: 32 rows of the item (blockIdx.y), a warp per 16 columns, of both maps (the tiles of a part); the sums
@@ -1148,7 +1076,7 @@ inline int paged_prefill_launch_t(const PpMaps& maps, const PpArgs& a, cudaStrea
   if constexpr (kForm == kDiff)
     return launch_dependent(paged_prefill_join_maps_kernel<D, kF16>, "paged_prefill_join_maps_kernel", dim3((unsigned)ctas, kPpRows / 32), 2 * D, 0, stream, a);
   else
-    return launch_dependent(paged_prefill_join_kernel<D, kF16, kTiles, kForm>, "paged_prefill_join_kernel", dim3((unsigned)ctas, D / 16), kTiles * kPpRows, 0, stream, a);
+    return launch_dependent(paged_prefill_join_kernel<D, kF16, kTiles>, "paged_prefill_join_kernel", dim3((unsigned)ctas, D / 16), kTiles * kPpRows, 0, stream, a);
 }
 
 template <int kForm = kPlain>
@@ -1156,10 +1084,8 @@ inline int paged_prefill_launch(const PagedArgs& p, int D, int dtype, void* work
   PpMaps maps;
   PpArgs a = {};
   const bool f16 = dtype == B200_LORA_F16;
-  if (!paged_prefill_plan(p, D, f16, pp_row_tiles(D, kForm), &maps, &a)) {
-    if constexpr (kForm == kSuffix) return fail(B200_LORA_EUNSUPPORTED, "shared_prefix_attention: no tensor map");  // (the prefix launch had one)
-    else return paged_decode_launch<kForm>(p, D, dtype, p.cache.block_size % 8 != 0 ? workspace : nullptr, stream);
-  }
+  if (!paged_prefill_plan(p, D, f16, pp_row_tiles(D, kForm), &maps, &a))
+    return paged_decode_launch<kForm>(p, D, dtype, p.cache.block_size % 8 != 0 ? workspace : nullptr, stream);
   if (pp_splits(p.T, p.n_req, p.Hq, a.h_shift, pp_row_tiles(D, kForm), pp_ctas(D, kForm), (int64_t)p.table_width * p.cache.block_size, p.window)) {
     a.parts = static_cast<float*>(workspace);
     a.joins = static_cast<char*>(workspace) + pp_split_bytes(D, kForm) - pp_ctas(D, kForm) * sizeof(PpJoin);
@@ -1170,52 +1096,64 @@ inline int paged_prefill_launch(const PagedArgs& p, int D, int dtype, void* work
   return f16 ? paged_prefill_launch_t<128, true, false, kForm>(maps, a, stream) : paged_prefill_launch_t<128, false, false, kForm>(maps, a, stream);
 }
 
-// Requests with common prefixes: a launch over the prefixes, the requests of a group side by side, and one over the keys behind them that
-// joins. Host code; what the device makes of the lengths is at px_chunk_tiles.
-struct PxPlan { int most, ctas; size_t own_bytes, ml_bytes, o_bytes; };  // parts of a prefix at most; CTAs that they are to fill
-inline PxPlan px_plan(int T, int n_req, int Hq, int Hk, int D, int block_size, int64_t max_keys, bool packed) {
+// Requests with common prefixes: a launch over the prefixes, the requests of a group side by side, and one over the keys behind them, a row
+// at a time, that joins. Host code; what the device makes of the lengths is at px_chunk_tiles.
+struct PxPlan { int most, ctas; size_t ml_bytes, o_bytes; };  // parts of a prefix at most; CTAs that they are to fill; bytes of workspace
+inline PxPlan px_plan(int T, int Hq, int Hk, int D) {
   PxPlan x;
-  const int h_shift = pp_h_shift(Hq / Hk), span = pp_row_tiles(D, kPrefix) * (kPpRows >> h_shift);
-  x.ctas = 148;
+  const int h_shift = pp_h_shift(Hq / Hk), span = kPpRows >> h_shift;
+  x.ctas = pp_ctas(D, kPrefix);
   const int64_t blocks = (int64_t)ceil_div_i(T, span) * (Hq >> h_shift);
   x.most = (int)std::max<int64_t>(1, std::min<int64_t>(kPpParts, (2 * x.ctas + blocks - 1) / blocks));
-  x.own_bytes = packed ? paged_prefill_workspace_bytes<kSuffix>(T, n_req, Hq, Hk, D, block_size, max_keys, 0) : 0;
-  x.own_bytes = (x.own_bytes + 15) / 16 * 16;
-  x.ml_bytes = ((size_t)x.most * T * Hq * 8 + 15) / 16 * 16;
-  x.o_bytes = (size_t)x.most * T * Hq * D * 4;
+  const size_t sums = (size_t)x.most * T * Hq;
+  x.ml_bytes = (sums * 8 + 15) / 16 * 16;
+  x.o_bytes = sums * D * 4;
   return x;
 }
-// Whether requests are attended by group: where a group has more than one, and copies of the cache's rows take tiles of them.
-inline bool px_shares(int T, int n_req, int n_groups, int block_size, int64_t max_keys) {
-  return n_groups > 0 && n_req > n_groups && block_size % 8 == 0 && max_keys > 0 && max_keys <= kPpMaxKeys && (int64_t)T < (1 << 24);
+// Whether requests are attended by group, as told by what the host knows: where a group has more than one, copies of the cache's rows take
+// tiles of them, and the keys that the tables hold at most are worth a second launch.
+// Decode: 128 MB of keys and values a call, each request's its own. us, request by request / by group, prefixes with 100 keys behind them:
+//   8 / 8 heads of 64: 8 requests of 4096 (70 MB) 15.5 / 19.3, of 16000 38 / 27; 32 of 1024 (74 MB) 14.3 / 16.4, of 4096 40 / 18.5; 128 of
+//   256 (93 MB) 22 / 24, of 1024 47 / 26; in 32 groups of 4 46 / 42; 16 / 2 of 128: 8 of 16000 (132 MB) 28 / 31, 32 of 4096 (138 MB) 26 / 21,
+//   128 of 1024 (147 MB) 25 / 20.5, in 32 groups 25.3 / 25.0
+// Packed: tiles of rows over the whole contexts against those over the prefix and an item for every new token and kv head; what either
+// takes by the formulas below is within a third of what it took over 100 points. us, 32 requests with 2, 6, 12, 24 new tokens behind 4000
+// keys: 16 / 2 heads of 64 25, 25, 26, 39 / 19, 28, 33, 52; 32 / 8 of 128 125, 125, 128, 129 / 32, 53, 87, 166
+inline bool px_shares(int T, int n_req, int n_groups, int Hq, int Hk, int D, int block_size, int64_t max_keys, bool packed) {
+  if (n_groups < 1 || n_req <= n_groups || block_size % 8 != 0 || max_keys < 1 || max_keys > kPpMaxKeys || T >= (1 << 24)) return false;
+  if (!packed) return (double)T * max_keys * Hk * D * 4 >= 128e6;
+  const int h_shift = pp_h_shift(Hq / Hk), per_tile = kPpRows >> h_shift, sets = Hq >> h_shift;
+  const double tiles = (double)max_keys / kPpKeys, each = ceil_div_i(ceil_div_i(T, n_req), per_tile * pp_row_tiles(D, kPlain));
+  const double alone = 8 + n_req * each * sets * tiles * 1.8 / pp_ctas(D, kPlain);
+  const double items = (double)T * Hk * ceil_div_i(Hq / Hk, kItemHeads<kSuffix>), blocks = ceil_div_i(T, per_tile) + n_groups - 1;
+  return 12 + 4.5 * items / kPagedCtas + blocks * sets * tiles * 1.2 / pp_ctas(D, kPrefix) < alone;
 }
 inline size_t shared_prefix_workspace_bytes(int T, int n_req, int n_groups, int Hq, int Hk, int D, int block_size, int64_t max_keys, bool packed) {
   // (a call whose strides a map refuses goes without sharing)
   const size_t plain = packed ? paged_prefill_workspace_bytes(T, n_req, Hq, Hk, D, block_size, max_keys, 0) : paged_workspace_bytes(T, Hq, Hk, D, max_keys, 0, 0);
-  if (!px_shares(T, n_req, n_groups, block_size, max_keys)) return plain;
-  const PxPlan x = px_plan(T, n_req, Hq, Hk, D, block_size, max_keys, packed);
-  return std::max(plain, 16 + x.own_bytes + x.ml_bytes + x.o_bytes);
+  if (!px_shares(T, n_req, n_groups, Hq, Hk, D, block_size, max_keys, packed)) return plain;
+  const PxPlan x = px_plan(T, Hq, Hk, D);
+  return std::max(plain, sizeof(PxHead) + x.ml_bytes + x.o_bytes);
 }
 
 template <int D, bool kF16>
 inline int shared_prefix_launch_t(PagedArgs p, bool packed, void* workspace, cudaStream_t stream) {
-  const int64_t max_keys = (int64_t)p.table_width * p.cache.block_size;
   const int dtype = kF16 ? B200_LORA_F16 : B200_LORA_BF16;
   PpMaps maps;
   PpArgs a = {};
-  if (!px_shares(p.T, p.n_req, p.n_groups, p.cache.block_size, max_keys) || !paged_prefill_plan(p, D, kF16, pp_row_tiles(D, kPrefix), &maps, &a))
+  if (!px_shares(p.T, p.n_req, p.n_groups, p.Hq, p.Hk, D, p.cache.block_size, (int64_t)p.table_width * p.cache.block_size, packed) ||
+      !paged_prefill_plan(p, D, kF16, pp_row_tiles(D, kPrefix), &maps, &a))
     return packed ? paged_prefill_launch(p, D, dtype, workspace, stream) : paged_decode_launch(p, D, dtype, workspace, stream);
-  const PxPlan x = px_plan(p.T, p.n_req, p.Hq, p.Hk, D, p.cache.block_size, max_keys, packed);
-  char* const ws = static_cast<char*>(workspace);
+  const PxPlan x = px_plan(p.T, p.Hq, p.Hk, D);
+  char* const parts = static_cast<char*>(workspace) + sizeof(PxHead);
   p.px_most = x.most;
-  p.px_chunk = reinterpret_cast<int*>(ws);
-  p.px_ml = reinterpret_cast<float2*>(ws + 16 + x.own_bytes);
-  p.px_o = reinterpret_cast<float*>(ws + 16 + x.own_bytes + x.ml_bytes);
+  p.px_head = static_cast<PxHead*>(workspace);
+  p.px_ml = reinterpret_cast<float2*>(parts);
+  p.px_o = reinterpret_cast<float*>(parts + x.ml_bytes);
   a.p = p;
   a.px_ctas = x.ctas;
   const int rc = paged_prefill_launch_t<D, kF16, false, kPrefix>(maps, a, stream);
-  if (rc != B200_LORA_OK) return rc;
-  return packed ? paged_prefill_launch<kSuffix>(p, D, dtype, ws + 16, stream) : paged_decode_launch<kSuffix>(p, D, dtype, nullptr, stream);
+  return rc != B200_LORA_OK ? rc : paged_decode_launch<kSuffix>(p, D, dtype, nullptr, stream);
 }
 inline int shared_prefix_launch(const PagedArgs& p, int D, int dtype, bool packed, void* workspace, cudaStream_t stream) {
   const bool f16 = dtype == B200_LORA_F16;

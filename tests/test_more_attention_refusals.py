@@ -57,8 +57,9 @@ def _shared(**kw):
     (dict(dim=96), N.E_UNSUPPORTED), (dict(out=None), N.E_INVAL), (dict(q=None), N.E_INVAL), (dict(tables=None), N.E_INVAL),
     (dict(ctx=None), N.E_INVAL), (dict(cache=None), N.E_INVAL), (dict(cache=_cache(v=None)), N.E_INVAL), (dict(cache=_cache(num_blocks=0)), N.E_INVAL),
     (dict(cache=_cache(k=AT + 8)), N.E_UNSUPPORTED), (dict(q=AT + 2), N.E_UNSUPPORTED), (dict(oh=68), N.E_UNSUPPORTED), (dict(prefix=None), N.E_INVAL),
-    (dict(cu_groups=None), N.E_INVAL), (dict(n=3), N.E_INVAL), (dict(ws=None), N.E_WORKSPACE), (dict(bytes=16), N.E_WORKSPACE),
-    (dict(ws=AT + 4), N.E_UNSUPPORTED), (dict(cu=AT, ws=None), N.E_WORKSPACE), (dict(T=0), 0), (dict(n=0), 0), (dict(T=0, prefix=None), 0),
+    (dict(cu_groups=None), N.E_INVAL), (dict(n=3), N.E_INVAL), (dict(width=1 << 16, ws=None), N.E_WORKSPACE), (dict(width=1 << 16, bytes=16), N.E_WORKSPACE),
+    (dict(ws=AT + 4), N.E_UNSUPPORTED), (dict(cu=AT, width=1 << 16, ws=None), N.E_WORKSPACE), (dict(T=0), 0), (dict(n=0), 0),
+    (dict(T=0, prefix=None), 0),
 ])
 def test_shared_prefix_statuses(kw, code):
     assert _shared(**kw) == code

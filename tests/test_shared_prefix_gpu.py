@@ -16,8 +16,15 @@ pytestmark = pytest.mark.gpu
 BF16, FP16 = torch.bfloat16, torch.float16
 
 
-def make(heads, kv_heads, dim, page, groups, new=None, *, seed=0, loose=0, **kw):
-    """``groups``: [(prefix, [own tokens of each request])]; own tokens count the new ones. Whole blocks of a prefix are the group's, the
+def way(p):
+    """1: the call is attended by group; 0: request by request."""
+    q, k, _, tables, lens, *cu = p["args"]
+    return N.lib().lora_b200_shared_prefix_way(q.size(0), lens.numel(), p["groups"][0].numel(), q.size(1), k.size(2), q.size(2), tables.size(1),
+                                               k.size(1), bool(cu))
+
+
+def make(heads, kv_heads, dim, page, groups, new=None, *, seed=0, loose=0, wide=True, **kw):
+    """``wide``: tables with as many (missing) blocks behind the contexts as make the call one that is attended by group. ``groups``: [(prefix, [own tokens of each request])]; own tokens count the new ones. Whole blocks of a prefix are the group's, the
     block it ends in is a copy of each request. ``loose``: requests behind the last group, which share nothing."""
     contexts = [p + n for p, own in groups for n in own] + [20 + 7 * i for i in range(loose)]
     p = PP.make(heads, kv_heads, dim, page, contexts, new, seed=seed, **kw)
@@ -43,7 +50,19 @@ def make(heads, kv_heads, dim, page, groups, new=None, *, seed=0, loose=0, **kw)
     args[3] = as_int(tables)
     p["args"] = tuple(args)
     p["groups"] = (as_int([g[0] for g in groups]), as_int(cu))
+    if wide and page % 8 == 0 and len(contexts) > len(groups):
+        widen(p)
     return p
+
+
+def widen(p):
+    args = list(p["args"])
+    for _ in range(40):
+        if way(p):
+            return
+        args[3] = torch.nn.functional.pad(args[3], (0, args[3].size(1)), value=-1)
+        p["args"] = tuple(args)
+    assert way(p)
 
 
 def call(p, **kw):
@@ -137,12 +156,14 @@ def test_stale_rows_do_not_count():
 
 def test_missing_blocks_and_tables_that_end():
     p = make(16, 2, 64, 16, [(160, [5, 40, 9])], seed=7)
+    width = p["args"][3].size(1)
     for r in range(3):
         p["tables"][r][3] = -1
         p["tables"][r][7] = p["k"].size(0)
     p["contexts"] = [165, 2 ** 31 - 1, 169]
     args = list(p["args"])
-    args[3] = torch.tensor(p["tables"], dtype=torch.int32, device="cuda")
+    padded = lambda: torch.tensor([t + [-1] * (width - len(t)) for t in p["tables"]], dtype=torch.int32, device="cuda")  # noqa: E731
+    args[3] = padded()
     args[4] = torch.tensor(p["contexts"], dtype=torch.int32, device="cuda")
     p["args"] = tuple(args)
     p["contexts"] = [165, len(p["tables"][1]) * 16, 169]
@@ -150,8 +171,9 @@ def test_missing_blocks_and_tables_that_end():
     p["groups"] = (torch.tensor([2 ** 31 - 1], dtype=torch.int32, device="cuda"), p["groups"][1])  # a prefix behind the table's end
     for r in (1, 2):
         p["tables"][r] = list(p["tables"][0])
-    args[3] = torch.tensor(p["tables"], dtype=torch.int32, device="cuda")
+    args[3] = padded()
     p["args"] = tuple(args)
+    assert way(p) == 1
     PP.check(p, *call(p, return_lse=True))
 
 
@@ -210,8 +232,7 @@ def test_strided(prefill):
     PP.check(p, wide[:, 4:20])
     assert bool((wide[:, :4] == 3).all()) and bool((wide[:, 20:] == 3).all())
     want = wide[:, 4:20].clone()
-    q1 = q.new_empty(T, 1, 128).expand(T, 16, 128)  # strides of zero: request by request
-    q1 = q[:, :1].expand(T, 16, 128)
+    q1 = q[:, :1].expand(T, 16, 128)  # strides of zero, which a tensor map refuses: request by request
     p["q"] = q1.cpu()
     p["args"] = (q1, *p["args"][1:])
     PP.check(p, call(p))
@@ -275,6 +296,26 @@ def test_queries_and_rows_of_the_launch_ahead():
     q.copy_(qs[3])
     p["q"], p["k"], p["v"] = q.cpu(), k.cpu(), v.cpu()
     PP.check(p, outs[199])
+
+
+@pytest.mark.parametrize("prefill", [False, True])
+def test_narrow_tables_go_request_by_request(prefill):
+    """Where a second launch would not pay: the other calls' result, bit for bit."""
+    p = make(16, 2, 64, 16, [(100, [9, 40, 3])], [9, 4, 3] if prefill else None, wide=False)
+    assert way(p) == 0
+    f = A.paged_prefill_attention if prefill else A.paged_decode_attention
+    assert torch.equal(call(p), f(*p["args"]))
+
+
+def test_ways():
+    """Both launches of a call: items by clusters and by CTAs as they come, in either head size; the rule's line."""
+    for dim, n in ((64, 4), (64, 200), (128, 4), (128, 200)):
+        p = make(16, 2, dim, 64, [(700, [5 + i % 90 for i in range(n)])], seed=n)
+        assert way(p) == 1
+        PP.check(p, *call(p, return_lse=True), f"{n} requests, heads of {dim}")
+    ask = N.lib().lora_b200_shared_prefix_way
+    assert ask(64, 64, 1, 32, 8, 128, 512, 16, 0) == 1 and ask(64, 64, 1, 16, 2, 64, 10, 256, 0) == 0
+    assert ask(64, 64, 64, 32, 8, 128, 512, 16, 0) == 0 and ask(64, 64, 1, 32, 8, 128, 512, 12, 0) == 0 and ask(64, 64, 0, 32, 8, 128, 512, 16, 0) == 0
 
 
 def test_same_as_request_by_request():
