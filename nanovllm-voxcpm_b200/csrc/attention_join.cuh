@@ -52,16 +52,14 @@ struct JoinVec {  // kType: B200_LORA_BF16, _F16, _F32
   }
 };
 
-template <int kType>
-__global__ void __launch_bounds__(kJoinRowThreads) join_attention_kernel(const __grid_constant__ JoinArgs a) {
+template <int kType, typename Index>
+__global__ void __launch_bounds__(kJoinRowThreads, 4) join_attention_kernel(const __grid_constant__ JoinArgs a) {
   constexpr int kSize = kType == B200_LORA_F32 ? 4 : 2;
+  const Index i = (Index)blockIdx.x * kJoinRowThreads + threadIdx.x, row = i / (Index)a.vecs, token = row / (Index)a.H;
+  const int vec = (int)(i - row * (Index)a.vecs), head = (int)(row - token * (Index)a.H);
   glue_enter();
-  const int64_t i = (int64_t)blockIdx.x * kJoinRowThreads + threadIdx.x, row = i / a.vecs;
-  const int vec = (int)(i - row * a.vecs);
-  const int64_t token = row / a.H;
-  const int head = (int)(row - token * a.H);
-  if (token >= a.T) return;
-  const int64_t at = kSize * (token * a.part_token + head * a.part_head) + 16 * vec, lse_at = token * a.lse_token + head * a.lse_head;
+  if (token >= (Index)a.T) return;
+  const int64_t at = kSize * ((int64_t)token * a.part_token + head * a.part_head) + 16 * vec, lse_at = (int64_t)token * a.lse_token + head * a.lse_head;
   float m = -INFINITY, l = 0.f;
   JoinVec<kType> sum, x;
 #pragma unroll
@@ -97,17 +95,24 @@ __global__ void __launch_bounds__(kJoinRowThreads) join_attention_kernel(const _
     }
   }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  *reinterpret_cast<uint4*>(static_cast<char*>(a.out) + kSize * (token * a.out_token + head * a.out_head) + 16 * vec) = sum.packed(inv);
+  *reinterpret_cast<uint4*>(static_cast<char*>(a.out) + kSize * ((int64_t)token * a.out_token + head * a.out_head) + 16 * vec) = sum.packed(inv);
   if (a.lse != nullptr && vec == 0) a.lse[row] = l == 0.f ? -INFINITY : m + logf(l);
 }
 
-inline int join_attention_launch(const JoinArgs& a, int dtype, cudaStream_t stream) {
-  const int64_t items = (int64_t)a.T * a.H * a.vecs, ctas = (items + kJoinRowThreads - 1) / kJoinRowThreads;
-  if (ctas > INT32_MAX) return fail(B200_LORA_EUNSUPPORTED, "join_attention: %d tokens of %d heads are more than a launch takes", a.T, a.H);
+template <int kType>
+inline int join_attention_launch_t(const JoinArgs& a, int64_t ctas, cudaStream_t stream) {
   const dim3 grid((unsigned)ctas);
-  if (dtype == B200_LORA_BF16) return launch_dependent(join_attention_kernel<B200_LORA_BF16>, "join_attention_kernel", grid, kJoinRowThreads, 0, stream, a);
-  if (dtype == B200_LORA_F16) return launch_dependent(join_attention_kernel<B200_LORA_F16>, "join_attention_kernel", grid, kJoinRowThreads, 0, stream, a);
-  return launch_dependent(join_attention_kernel<B200_LORA_F32>, "join_attention_kernel", grid, kJoinRowThreads, 0, stream, a);
+  if (ctas < (1 << 22)) return launch_dependent(join_attention_kernel<kType, uint32_t>, "join_attention_kernel", grid, kJoinRowThreads, 0, stream, a);
+  return launch_dependent(join_attention_kernel<kType, int64_t>, "join_attention_kernel", grid, kJoinRowThreads, 0, stream, a);
+}
+inline int join_attention_launch(const JoinArgs& a, int dtype, cudaStream_t stream) {
+  const int64_t rows = (int64_t)a.T * a.H;
+  if (rows > INT32_MAX || rows * a.vecs > (int64_t)INT32_MAX * kJoinRowThreads)
+    return fail(B200_LORA_EUNSUPPORTED, "join_attention: %d tokens of %d heads are more than a launch takes", a.T, a.H);
+  const int64_t ctas = (rows * a.vecs + kJoinRowThreads - 1) / kJoinRowThreads;
+  if (dtype == B200_LORA_BF16) return join_attention_launch_t<B200_LORA_BF16>(a, ctas, stream);
+  if (dtype == B200_LORA_F16) return join_attention_launch_t<B200_LORA_F16>(a, ctas, stream);
+  return join_attention_launch_t<B200_LORA_F32>(a, ctas, stream);
 }
 
 }  // namespace b200lora
