@@ -10,8 +10,8 @@ table for decode), as in the reference (``layers/attention.py:10-79``). The step
 (residual add + RMSNorm, RoPE + cache store, SiLU * up) run as plain torch ops, or, with
 ``Decoder.fused_glue = True``, as the single-launch kernels of ``glue.py``.
 With ``DecoderConfig.paged_attention`` (which a sliding window implies) attention is ``attention.py``'s over the paged
-cache, for prompts, chunks of them and decode rows alike; with ``qk_norm`` every query and key head is RMS-normed ahead of
-the rotation.
+cache, for prompts, chunks of them and decode rows alike, behind a shared prefix where a step names one; with ``qk_norm`` every
+query and key head is RMS-normed ahead of the rotation; with ``differential`` heads are the difference of two maps.
 
 It exists to time a whole step with the multi-LoRA kernels in their real surroundings (one prefill
 step over all prompts, then decode steps replayed from a CUDA graph) and to compare it with the same
@@ -59,12 +59,26 @@ class DecoderConfig:
     #: keys that a token sees, its own among them (0: all), and first tokens that stay visible besides
     sliding_window: int = 0
     sink_tokens: int = 0
+    #: differential attention: the halves of a head's columns of q and k are two maps (normed and rotated as heads of their own), of which
+    #: the second counts ``lam`` (per head), the difference RMS-normed times ``diff_norm``
+    differential: bool = False
 
     def __post_init__(self) -> None:
         if self.sliding_window < 0 or self.sink_tokens < 0 or (self.sink_tokens and not self.sliding_window):
             raise ValueError("sliding_window and sink_tokens must not be negative, and first tokens stay visible besides a window")
-        if self.sliding_window:
+        if self.differential and self.head_dim not in (64, 128):
+            raise ValueError("differential attention takes heads of 64 or 128 columns")
+        if self.sliding_window or self.differential:
             self.paged_attention = True
+
+    @property
+    def maps(self) -> int:
+        """Heads of q and k, as norm and rotation see them, in a head of v."""
+        return 2 if self.differential else 1
+
+    @property
+    def rotary_dim(self) -> int:
+        return self.head_dim // self.maps
 
 
 @dataclass
@@ -84,6 +98,12 @@ class AttentionStep:
     #: comes in chunks), and their block tables
     prefill_context_lens: torch.Tensor | None = None
     prefill_block_tables: torch.Tensor | None = None
+    #: with ``paged_attention`` over everything: groups of decode requests that begin alike (``attention.shared_prefix_decode_attention``:
+    #: int32 [groups] lengths and [groups + 1] bounds), and of prefill requests; None: nobody shares
+    prefix_lens: torch.Tensor | None = None
+    cu_groups: torch.Tensor | None = None
+    prefill_prefix_lens: torch.Tensor | None = None
+    prefill_cu_groups: torch.Tensor | None = None
 
 
 def _rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
@@ -110,8 +130,12 @@ class DecoderAttention(nn.Module):
         self.o_proj = L.LoRARowParallelLinear(cfg.num_heads * cfg.head_dim, cfg.hidden_size, max_loras=cfg.max_loras,
                                               max_lora_rank=cfg.max_lora_rank, lora_tp_mode=cfg.lora_tp_mode)
         if cfg.qk_norm:
-            self.q_norm = nn.Parameter(torch.ones(cfg.head_dim))
-            self.k_norm = nn.Parameter(torch.ones(cfg.head_dim))
+            self.q_norm = nn.Parameter(torch.ones(cfg.rotary_dim))
+            self.k_norm = nn.Parameter(torch.ones(cfg.rotary_dim))
+        if cfg.differential:
+            # (what a checkpoint makes of its vectors: exp(q1 . k1) - exp(q2 . k2) + lambda_init for every head; 1 - lambda_init is in the weight)
+            self.lam = nn.Parameter(torch.full((self.heads,), 0.5))
+            self.diff_norm = nn.Parameter(torch.ones(cfg.head_dim))
         self.k_cache = self.v_cache = None  # [blocks, block_size, kv_heads, head_dim], set by the harness
 
     def forward(self, positions, hidden, step: AttentionStep, cos_sin) -> torch.Tensor:
@@ -119,11 +143,11 @@ class DecoderAttention(nn.Module):
         qkv = self.qkv_proj(hidden)
         q, k, v = qkv.split([self.q_size, self.kv_size, self.kv_size], dim=-1)
         cos, sin = cos_sin
-        q, k = q.view(-1, self.heads, cfg.head_dim), k.view(-1, self.kv_heads, cfg.head_dim)
+        q, k = q.reshape(-1, self.heads * cfg.maps, cfg.rotary_dim), k.reshape(-1, self.kv_heads * cfg.maps, cfg.rotary_dim)
         if cfg.qk_norm:
             q, k = _rms_norm(q, self.q_norm, cfg.rms_norm_eps), _rms_norm(k, self.k_norm, cfg.rms_norm_eps)
-        q = _rope(q, cos, sin)
-        k = _rope(k, cos, sin)
+        q = _rope(q, cos, sin).view(-1, self.heads, cfg.head_dim)
+        k = _rope(k, cos, sin).view(-1, self.kv_heads, cfg.head_dim)
         v = v.reshape(-1, self.kv_heads, cfg.head_dim)
         flat_k = self.k_cache.view(-1, self.kv_heads, cfg.head_dim)
         flat_v = self.v_cache.view(-1, self.kv_heads, cfg.head_dim)
@@ -141,9 +165,30 @@ class DecoderAttention(nn.Module):
             if getattr(step, name) is None:
                 raise ValueError(f"attention over the paged cache (DecoderConfig.paged_attention, sliding_window) needs AttentionStep.{name}")
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        if nd:
+        shared = (step.prefix_lens, step.cu_groups), (step.prefill_prefix_lens, step.prefill_cu_groups)
+        for lens, groups in shared:
+            if (lens is None) != (groups is None):
+                raise ValueError("prefix_lens and cu_groups of a step come together")
+            if lens is not None and (cfg.sliding_window or cfg.differential):
+                raise ValueError("shared prefixes take attention over everything, by one map")
+        if cfg.differential:
+            how = dict(scale=cfg.rotary_dim ** -0.5, window=cfg.sliding_window, sinks=cfg.sink_tokens, norm_weight=self.diff_norm, eps=cfg.rms_norm_eps)
+            lam = self.lam.float()
+            if nd:
+                A.differential_decode_attention(q[:nd], self.k_cache, self.v_cache, step.block_tables, step.context_lens, lam, out=out[:nd], **how)
+            if step.is_prefill:
+                A.differential_prefill_attention(q[nd:], self.k_cache, self.v_cache, step.prefill_block_tables, step.prefill_context_lens,
+                                                 step.cu_seqlens, lam, out=out[nd:], **how)
+            return out
+        if nd and step.prefix_lens is not None:
+            A.shared_prefix_decode_attention(q[:nd], self.k_cache, self.v_cache, step.block_tables, step.context_lens, *shared[0], scale=how["scale"],
+                                             out=out[:nd])
+        elif nd:
             A.paged_decode_attention(q[:nd], self.k_cache, self.v_cache, step.block_tables, step.context_lens, out=out[:nd], **how)
-        if step.is_prefill:
+        if step.is_prefill and step.prefill_prefix_lens is not None:
+            A.shared_prefix_prefill_attention(q[nd:], self.k_cache, self.v_cache, step.prefill_block_tables, step.prefill_context_lens,
+                                              step.cu_seqlens, *shared[1], scale=how["scale"], out=out[nd:])
+        elif step.is_prefill:
             A.paged_prefill_attention(q[nd:], self.k_cache, self.v_cache, step.prefill_block_tables, step.prefill_context_lens,
                                       step.cu_seqlens, out=out[nd:], **how)
         return out
@@ -168,15 +213,18 @@ class DecoderAttention(nn.Module):
     def forward_fused(self, positions, normed, step: AttentionStep, cos, sin, slot_mapping_i32) -> torch.Tensor:
         """Same as ``forward`` with RoPE and the cache store as one in-place kernel over the packed qkv rows."""
         cfg = self.cfg
-        how = dict(positions=positions, cos=cos, sin=sin, k_cache=self.k_cache, v_cache=self.v_cache, slot_mapping=slot_mapping_i32)
+        heads, kv_heads, dim = self.heads * cfg.maps, self.kv_heads * cfg.maps, cfg.rotary_dim
+        caches = [c.view(*c.shape[:2], kv_heads, dim) if cfg.differential else c for c in (self.k_cache, self.v_cache)]
+        how = dict(positions=positions, cos=cos, sin=sin, k_cache=caches[0], v_cache=caches[1], slot_mapping=slot_mapping_i32)
         qkv = self.qkv_proj(normed)
         if cfg.qk_norm:
             # (attention over the cache reads no k but the cache's: the packed rows need not have it)
-            q_out = torch.empty(qkv.size(0), self.heads, cfg.head_dim, dtype=qkv.dtype, device=qkv.device) if cfg.paged_attention else None
-            q, k, v = G.qk_norm_rope_kv_store(qkv, self.heads, self.kv_heads, cfg.head_dim, self.q_norm, self.k_norm, cfg.rms_norm_eps,
-                                              q_out=q_out, **how)
+            q_out = torch.empty(qkv.size(0), heads, dim, dtype=qkv.dtype, device=qkv.device) if cfg.paged_attention else None
+            q, k, v = G.qk_norm_rope_kv_store(qkv, heads, kv_heads, dim, self.q_norm, self.k_norm, cfg.rms_norm_eps, q_out=q_out, **how)
         else:
-            q, k, v = G.rope_kv_store(qkv, self.heads, self.kv_heads, cfg.head_dim, **how)
+            q, k, v = G.rope_kv_store(qkv, heads, kv_heads, dim, **how)
+        if cfg.differential:
+            q = q.view(q.size(0), self.heads, cfg.head_dim)
         return self.o_proj(self._attend(q, k, v, step).reshape(-1, self.q_size))
 
 
@@ -216,7 +264,7 @@ class Decoder(nn.Module):
         self.cfg = cfg
         self.layers = nn.ModuleList([DecoderLayer(cfg) for _ in range(cfg.num_layers)])
         self.norm = nn.Parameter(torch.ones(cfg.hidden_size))
-        inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, cfg.head_dim, 2, dtype=torch.float32) / cfg.head_dim))
+        inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, cfg.rotary_dim, 2, dtype=torch.float32) / cfg.rotary_dim))
         freqs = torch.outer(torch.arange(cfg.max_position, dtype=torch.float32), inv)
         self.register_buffer("cos", freqs.cos(), persistent=False)
         self.register_buffer("sin", freqs.sin(), persistent=False)

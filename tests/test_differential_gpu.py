@@ -53,11 +53,12 @@ def check(p, out, what=""):
     y = one[0] - lam * two[0]
     err = err + 2.0 ** -22 * (one[1] + lam * two[1])
     if p["weight"] is not None:
-        n = (y.square().mean(-1, keepdim=True) + EPS).sqrt()
+        eps = p.get("eps", EPS)
+        n = (y.square().mean(-1, keepdim=True) + eps).sqrt()
         E = err.square().mean(-1, keepdim=True).sqrt()
         w = p["weight"].double()
-        want = MO.rms_norm(y, w, EPS)
-        bound = w.abs() * (err + y.abs() * E / n) / torch.clamp(n - E, min=EPS ** 0.5) + (dim + 16) * 2.0 ** -24 * want.abs()
+        want = MO.rms_norm(y, w, eps)
+        bound = w.abs() * (err + y.abs() * E / n) / torch.clamp(n - E, min=eps ** 0.5) + (dim + 16) * 2.0 ** -24 * want.abs()
     else:
         want, bound = y, err
     bound = u * want.abs() + (1 + u) * bound + (2.0 ** -25 if q.dtype == FP16 else 0)
