@@ -28,8 +28,10 @@ struct RowKeys {
   __device__ __forceinline__ int key(int i) const { return i < n_sink ? i : i - n_sink + first; }
 };
 
-// What two launches over a prefix and behind it tell each other: tiles of keys in a part; the next item that no CTA has taken
-struct PxHead { int chunk, next_item, pad[2]; };
+// What two launches over a prefix and behind it tell each other: tiles of keys in a part; the next item that no CTA has taken; the rows by
+// how many keys each has behind the prefix, most first (of up to kPxOrder rows; of more, as they are)
+constexpr int kPxOrder = 512;
+struct PxHead { int chunk, next_item, pad[2]; int order[kPxOrder]; };
 
 struct PagedArgs {
   const void* q; int64_t q_token, q_head;      // [T, Hq, D], strides in elements
@@ -93,9 +95,9 @@ __device__ __forceinline__ int px_keys(const PagedArgs& a, const PxGroup& lanes,
   const uint32_t hit = __ballot_sync(0xffffffffu, lanes.r0 <= req && req < lanes.r1);
   return hit == 0 ? 0 : __shfl_sync(0xffffffffu, lanes.keys, __ffs(hit) - 1);
 }
-// (behind the wait for the launch that wrote it)
-__device__ __forceinline__ int px_parts(const PagedArgs& a, int keys) {
-  const int tiles = (int)(((unsigned)keys + kPrefixTile - 1u) / kPrefixTile), chunk = max(1, __ldcg(&a.px_head->chunk));
+// Parts of a prefix of `chunk` tiles each (what the prefix launch left, read behind the wait for it)
+__device__ __forceinline__ int px_parts(const PagedArgs& a, int keys, int chunk) {
+  const int tiles = (int)(((unsigned)keys + kPrefixTile - 1u) / kPrefixTile);
   return min(a.px_most, (tiles + chunk - 1) / chunk);
 }
 
@@ -280,6 +282,7 @@ struct PagedWalk {
       if (step > 0) {
         row = (int)(at / per_row);
         item = (int)(at - (long long)row * per_row);
+        if (kForm == kSuffix && ranks == 1 && a.T <= kPxOrder) row = min(max(__ldcg(a.px_head->order + row), 0), a.T - 1);
         at = kForm == kSuffix && ranks == 1 ? end : at + step;  // (there the caller says what is next)
         w.keys = row_keys<kForm>(a, groups, row);
         w.n_units = units(w.keys);
@@ -332,8 +335,8 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
   __shared__ int s_row;
   __shared__ long long s_at, s_sum[kPagedWarps];
   __shared__ uint32_t s_live[kPagedWarps][kPagedStages];
-  // Behind a prefix a CTA has one item to begin with, and then takes what nobody has: items are of any length, and some CTAs start late,
-  // where CTAs of the prefix launch have been. (Which CTA has an item changes nothing in it.)
+  // Behind a prefix a CTA takes an item that nobody has, the longest first: items are of any length, and some CTAs start late, where CTAs of
+  // the prefix launch have been. (Which CTA has an item changes nothing in it.)
   constexpr bool kQueue = kForm == kSuffix && kWay == kWhole;
   __shared__ int s_next;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -458,25 +461,39 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
     }
   };
 
-  auto take = [&]() { return (int)gridDim.x + atomicAdd(&a.px_head->next_item, 1); };
+  auto take = [&]() { return atomicAdd(&a.px_head->next_item, 1); };
   int taken = 0;
-  if (kQueue && tid == 0) taken = take();
-  PagedPiece w = walk.next(a);
+  PagedPiece w;
   int stage = 0, buf = 0;
   bool first_piece = true;
-  {
+  int chunk = 1;  // behind a prefix: tiles of a part of it
+  auto begin = [&]() {  // an item with none ahead of it
+    if constexpr (kQueue) {
+      if (tid == 0) s_next = take();
+      __syncthreads();
+      walk.at = s_next;
+    }
+    w = walk.next(a);
     const int e0 = entry(w, w.u0 + warp), e1 = entry(w, w.u0 + warp + kPagedWarps);
     load_q(w);
-    load(w, w.u0 + warp, e0, 0);
-    load(w, w.u0 + warp + kPagedWarps, e1, 1);
-    put_q(0);
-    if (kQueue && tid == 0) s_next = taken;
+    load(w, w.u0 + warp, e0, stage);
+    load(w, w.u0 + warp + kPagedWarps, e1, after(stage, 1));
+    put_q(buf);
+  };
+  begin();
+  // A short first item ends with the wait for the prefix launch, while others might have what this CTA took for afterwards: only behind a
+  // long one it takes that ahead. (24 requests with 1 to 12 new tokens behind two prefixes of 4000 to 6000, 16 / 2 heads of 128: ahead 37 us,
+  // not 33.)
+  bool ahead = w.n_units >= 8 * kPagedWarps;
+  if (kQueue && ahead) {
+    __syncthreads();  // (all have read the first)
+    if (tid == 0) s_next = take();
   }
   while (w.row >= 0) {
     int e = entry(w, w.u0 + warp + 2 * kPagedWarps);
     if (kQueue) {
       __syncthreads();  // (q is there, too)
-      walk.at = s_next;
+      walk.at = ahead ? s_next : walk.end;
     }
     const PagedPiece following = walk.next(a);
     const int e0 = entry(following, following.u0 + warp), e1 = entry(following, following.u0 + warp + kPagedWarps);
@@ -604,7 +621,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
         l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 8);
         l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 16);
       }
-    if (kQueue && tid == 0) taken = take();
+    if (kQueue && ahead && tid == 0) taken = take();
     // the warps' results, each in the third stage of its ring, where nothing is under way
     __shared__ int s_third[kPagedWarps];
     float* const mine = reinterpret_cast<float*>(smem + ring_at + after(stage, 2) * kStage);
@@ -630,10 +647,11 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
     constexpr bool kFour = kForm != kPlain;
     constexpr int kSumHeads = 8 * NT / kMaps<kForm>;
     int prefix_parts = 0;
-    if (kForm == kSuffix && kWay != kClusters && whole) {
+    if (kForm == kSuffix && first_piece) {
       glue_enter();
-      prefix_parts = px_parts(a, w.keys.first);
+      chunk = max(1, __ldcg(&a.px_head->chunk));
     }
+    if (kForm == kSuffix) prefix_parts = px_parts(a, w.keys.first, chunk);
     for (int i = tid; kFour && i < kSumHeads * (D / 4); i += kPagedThreads) {
       const int h = i / (D / 4), c = i - h * (D / 4);
       float4 x[kMaps<kForm>];
@@ -697,10 +715,6 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
       // the cluster's parts: every CTA joins some of the columns
       cluster_arrive();
       cluster_wait();
-      if (kForm == kSuffix) {
-        glue_enter();
-        prefix_parts = px_parts(a, w.keys.first);
-      }
       if (kFour) {  // (whole heads, for their norm; whole warps, for its sum)
         const int h0 = (int)(kSumHeads * rank / ranks), h1 = (int)(kSumHeads * (rank + 1) / ranks);
         for (int i = tid; i < ((h1 - h0) * (D / 4) + 31) / 32 * 32; i += kPagedThreads) {
@@ -774,10 +788,19 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
       while (total * last / G >= item_end) --last;
       a.joins[blockIdx.x] = make_int4(w.row, w.head0, slot, last);
     }
-    if (kQueue && tid == 0) s_next = taken;
-    first_piece = false;
     buf ^= 1;
     w = following;
+    if (kQueue) {
+      if (!ahead) {
+        __syncthreads();  // (the stages that held results may be filled again)
+        begin();
+        if (tid == 0) taken = take();
+        __syncthreads();  // (all have read this one)
+        ahead = true;
+      }
+      if (tid == 0) s_next = taken;
+    }
+    first_piece = false;
   }
   cp_async_wait_group<0>();
   if (kForm == kSuffix) glue_enter();  // (this launch ends behind the one ahead whatever its CTAs find)
@@ -840,11 +863,14 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArg
 }
 
 // Dynamic shared memory of a kernel, set once on a device (`known`: the devices that have it; half a microsecond a call otherwise)
-inline int allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>* known) {
+// (`beside`: kernels of two launches that are to share an SM, of which each by itself would settle for a smaller part of the L1 as shared
+// memory)
+inline int allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>* known, bool beside = false) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && dev < 64 && (known->load(std::memory_order_relaxed) >> dev & 1u)) return B200_LORA_OK;
   if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && beside) e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
   if (e != cudaSuccess) return fail(B200_LORA_ECUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   if (dev < 64) known->fetch_or(1ull << dev, std::memory_order_relaxed);
   return B200_LORA_OK;
@@ -882,7 +908,7 @@ template <int D, int NT, bool kF16, int kWay, int kWarps, int kForm>
 inline int paged_decode_launch_t(const PagedArgs& a, int ctas, int cluster, cudaStream_t stream) {
   const auto kernel = paged_decode_kernel<D, NT, kF16, kWay, kWarps, kForm>;
   static std::atomic<uint64_t> known{0};
-  if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), paged_smem<D, NT>(kWarps), &known)) return rc;
+  if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), paged_smem<D, NT>(kWarps), &known, kForm == kSuffix)) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(32 * kWarps);

@@ -161,6 +161,34 @@ __device__ __forceinline__ int px_position(const PagedArgs& p, int row, int r0, 
   return (int)max((int64_t)p.context_lens[r] - (end - row), (int64_t)-1);
 }
 
+// The order of the rows by their keys behind the prefix, most first, by one CTA; `keys`: room for one of each in shared memory
+__device__ __forceinline__ void px_order(const PagedArgs& p, int* keys) {
+  const int n = p.T <= kPxOrder ? p.T : 0;
+  for (int row = threadIdx.x; row < n; row += blockDim.x) {
+    const int r = p.cu_seqlens == nullptr ? row : px_request(p, row, 0, p.n_req);
+    int lo = 0, hi = p.n_groups;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (p.cu_groups[mid] <= r) lo = mid;
+      else hi = mid;
+    }
+    const PxGroup g = px_group(p, lo);
+    const int ctx = p.context_lens[r];
+    keys[row] = max(0, ctx - (g.r0 <= r && r < g.r1 ? g.keys : 0));
+  }
+  __syncthreads();
+  for (int row = threadIdx.x; row < n; row += blockDim.x) {
+    const int mine = keys[row];
+    int rank = 0;
+#pragma unroll 8
+    for (int k = 0; k < n; ++k) rank += keys[k] > mine || (keys[k] == mine && k < row) ? 1 : 0;
+    p.px_head->order[rank] = row;
+  }
+  if (threadIdx.x == 0) p.px_head->next_item = 0;
+  __threadfence();
+  __syncthreads();
+}
+
 // New rows of request i, and its first one; a range that leaves the rows of q counts as none
 __device__ __forceinline__ int pp_rows(const PagedArgs& p, int i, int* begin) {
   *begin = p.cu_seqlens[i];
@@ -263,35 +291,32 @@ __device__ __forceinline__ PxLane px_lane(const PpArgs& a, int span, int g) {
 // A part of `chunk` tiles each: one wave of CTAs where that is possible, since ceil(t / c) <= t / c + 1, so that with R items of one part
 // each and W tiles over them W / c + R <= CTAs; then the least c near it that still fits.
 __device__ __forceinline__ int px_chunk_tiles(const PpArgs& a, int span, const PxLane& lanes0) {
-  long long work = 0, rows = 0;
-  int longest = 0;
+  constexpr unsigned kMost = 1u << 25;  // (of a lane's 32: what more there may be changes nothing in the outcome that matters)
+  unsigned work = 0, rows = 0, longest = 0;
   for (int base = 0; base < a.p.n_groups; base += 32) {
     const PxLane q = base == 0 ? lanes0 : px_lane(a, span, base + (int)(threadIdx.x & 31));
-    work += (long long)q.blocks * q.tiles;
-    rows += q.blocks;
-    longest = max(longest, q.tiles);
+    const unsigned mine = (unsigned)q.blocks * (unsigned)a.head_tiles;  // (fits: the host's items do)
+    rows = min(kMost, rows + min(kMost, mine));
+    work = min(kMost, work + (unsigned)min((unsigned long long)kMost, (unsigned long long)mine * (unsigned)q.tiles));
+    longest = max(longest, (unsigned)q.tiles);
   }
-#pragma unroll
-  for (int d = 16; d > 0; d /= 2) {
-    work += __shfl_xor_sync(0xffffffffu, work, d);
-    rows += __shfl_xor_sync(0xffffffffu, rows, d);
-  }
+  work = __reduce_add_sync(0xffffffffu, work);
+  rows = __reduce_add_sync(0xffffffffu, rows);
   longest = __reduce_max_sync(0xffffffffu, longest);
-  work *= a.head_tiles;
-  rows *= a.head_tiles;
-  const int once = a.px_ctas / 2;  // (a CTA an SM leaves room beside it; two where that is long, too)
-  const long long one = work > 8ll * once ? a.px_ctas : once;
-  const long long ctas = one * max(1ll, (2 * rows + one - 1) / one);  // (as many waves as leave half of the places to cuts)
-  const int least = max(kPxChunk, (longest + a.p.px_most - 1) / a.p.px_most);
-  int chunk = (int)min((work + max(1ll, ctas - rows) - 1) / max(1ll, ctas - rows), (long long)INT32_MAX);
+  const unsigned once = (unsigned)a.px_ctas / 2;  // (a CTA an SM leaves room beside it; two where that is long, too)
+  const unsigned one = work > 8u * once ? (unsigned)a.px_ctas : once;
+  const unsigned ctas = one * max(1u, (2 * rows + one - 1) / one);  // (as many waves as leave half of the places to cuts)
+  const unsigned least = max((unsigned)kPxChunk, (longest + a.p.px_most - 1) / a.p.px_most), room = max(1u, ctas - rows);
+  unsigned chunk = max(1u, (work + room - 1) / room);
   if (a.p.n_groups <= 32) {
-    for (int k = 0; k < 8 && chunk > least; ++k) {
-      const unsigned mine = (unsigned)min((long long)lanes0.blocks * a.head_tiles * ((lanes0.tiles + chunk - 2) / (chunk - 1)), 1ll << 26);
-      if (__reduce_add_sync(0xffffffffu, mine) > ctas) break;
+    const unsigned mine = (unsigned)lanes0.blocks * (unsigned)a.head_tiles;
+    for (int k = 0; k < 4 && chunk > least; ++k) {
+      const unsigned parts = ((unsigned)lanes0.tiles + chunk - 2) / (chunk - 1);
+      if (__reduce_add_sync(0xffffffffu, (unsigned)min((unsigned long long)kMost, (unsigned long long)mine * parts)) > ctas) break;
       --chunk;
     }
   }
-  return max(chunk, least);
+  return (int)max(chunk, least);
 }
 // Items of a group, at most INT32_MAX over all (the host sees to that for groups that do not overlap)
 __device__ __forceinline__ int px_items_of(const PpArgs& a, const PxLane& q, int chunk) {
@@ -378,6 +403,17 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
   const uint32_t raw = smem_u32(smem_raw), v_u32 = (raw + 1023u) & ~1023u, k_u32 = v_u32 + kSt * kTile, q_u32 = k_u32 + kSt * kTile, out_u32 = q_u32 + kRowTiles * kTile;
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
 
+  if (kForm == kPrefix) {
+    // The launch behind this one may start once all CTAs have let it (it has no use for tensor memory). CTA 0 has no part of a
+    // prefix; it leaves the counter that the other's items come from, and their order.
+    griddep_wait();
+    if (blockIdx.x == 0) {
+      px_order(p, reinterpret_cast<int*>(smem_raw));
+      griddep_launch_dependents();
+      return;
+    }
+    griddep_launch_dependents();
+  }
   if (tid == 0) {
     for (int i = 0; i < N_BARS; ++i) mbar_init(bar(i), (i >= P_READY && i < O_DONE) || i == S_TAKEN ? kPpRows : i == SHARED ? 2 * kPpRows : i == TAKEN || i == TAKEN + 1 ? 4 * kTiles + 1 : 1);
     abort_flag = 0;
@@ -387,16 +423,7 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  if (kForm == kPrefix) {
-    // The launch behind this one starts once all CTAs have let it, and takes its items from a counter that is there by then.
-    griddep_wait();
-    if (blockIdx.x == 0 && tid == 0) {
-      p.px_head->next_item = 0;
-      __threadfence();
-    }
-    __syncthreads();
-  }
-  glue_enter();  // (dependents may start: every CTA of this launch holds its tensor memory by then)
+  if (kForm != kPrefix) glue_enter();  // (dependents may start: every CTA of this launch holds its tensor memory by then)
   const uint32_t tmem = s_tmem;
   const int per_tile = kPpRows >> a.h_shift, span = kRowTiles * per_tile;
 
@@ -687,14 +714,14 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
       const uint32_t leader = elect_one();
       const int n_boxes = kPpKeys / a.box;
       uint32_t n = 0, pieces = 0;
-      const int G = gridDim.x;
+      const int G = (int)gridDim.x - (kForm == kPrefix ? 1 : 0);
       PpLane lanes0 = {0, 0, 0, 0, 0};
       PxLane groups0 = {{0, 0, 0, 0, 0}, 0, 0};
       int n_items = 0, chunk = 1;
       if constexpr (kForm == kPrefix) {
         groups0 = px_lane(a, span, lane);
         chunk = px_chunk_tiles(a, span, groups0);
-        if (blockIdx.x == 0 && leader) p.px_head->chunk = chunk;
+        if (blockIdx.x == 1 && leader) p.px_head->chunk = chunk;
       } else {
         lanes0 = pp_lane(a, span, lane);
         n_items = pp_items(a, span, lanes0);
@@ -710,7 +737,7 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
         // (every other wave backwards: contexts get shorter from item to item)
         const int c = k & 1 ? G - 1 - (int)blockIdx.x : (int)blockIdx.x;
         if constexpr (kForm == kPrefix) {
-          px_find(a, span, chunk, k * G + (int)blockIdx.x, groups0, &w);
+          px_find(a, span, chunk, k * G + (int)blockIdx.x - 1, groups0, &w);
         } else if (k < waves) {
           pp_find(a, span, k * G + c, n_items, lanes0, &w);
         } else if (k == waves && most >= 2) {
@@ -1069,8 +1096,8 @@ inline int paged_prefill_launch_t(const PpMaps& maps, const PpArgs& a, cudaStrea
   const auto kernel = paged_prefill_kernel<D, kF16, kSplit, kForm>;
   constexpr int smem = pp_smem<D>(kTiles, pp_row_tiles(D, kForm));
   static std::atomic<uint64_t> known{0};
-  if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), smem, &known)) return rc;
-  const int ctas = kForm == kPrefix ? a.px_ctas : kSplit ? kCtas : (int)std::min<int64_t>(kCtas, (int64_t)a.n_blocks * a.head_tiles);
+  if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), smem, &known, kForm == kPrefix)) return rc;
+  const int ctas = kForm == kPrefix ? a.px_ctas + 1 : kSplit ? kCtas : (int)std::min<int64_t>(kCtas, (int64_t)a.n_blocks * a.head_tiles);
   const int rc = launch_dependent(kernel, "paged_prefill_kernel", dim3((unsigned)ctas), pp_threads(kTiles), (size_t)smem, stream, maps, a);
   if (rc != B200_LORA_OK || !kSplit) return rc;
   if constexpr (kForm == kDiff)
