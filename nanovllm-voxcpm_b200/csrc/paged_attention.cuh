@@ -13,6 +13,14 @@
 // requests 16.9 to 31.5 us, which is 6.0 TB/s behind 5.7 us of launch, first blocks and join); 64 of 128 to 1024, 16 / 2 of 64, 8.2 us
 // (33 %: bound by the longest request, whose eight warps have four blocks each, 1.3 us a block behind 3.9 us of launch, look-ups and
 // join; 38 requests of 1024 each take 9.0 us, 64 9.3; of 512 6.6 and 6.9, of 256 4.9 and 5.3, of 32 3.9 and 4.0).
+//
+// Two more forms of it. Differential heads: out = S1 - lam S2, of the maps that the halves of a head's columns of q and k make over the whole
+// of v, normed. The tiles of eight rows that serve sixteen heads hold the two maps of eight; everything else is as above, and so is what
+// bounds it: 48 requests of 500 to 8192, 32 / 8 heads of 128, 144 us (84 % of the copy bandwidth); 64 with a window of 1024, 16 / 2 of 128,
+// 17 us; one of 333, 16 / 2 of 64, 6.3 us. Behind a prefix that requests share: the keys behind it, a row at a time, and the join with the
+// parts that the launch ahead (paged_prefill.cuh) leaves of the prefix. It runs beside that launch, a CTA of either on an SM; bound by
+// HBM where there is much behind the prefix (96 requests of 50 to 1500 keys behind four prefixes, 32 / 8 of 128: 100 us, 59 at the copy
+// bandwidth, 260 request by request), else by the two chains (64 of 10 to 600 keys behind 4003, 16 / 2 of 64: 17 us; 21 request by request).
 #pragma once
 
 #include <atomic>

@@ -17,6 +17,15 @@
 // behind 6.3 us (2368, 4736 and 7104 tokens are one to three waves: 28.9, 51.5 and 74.1 us), and of 3.4 waves the last costs 17; 12
 // prompts of 100 to 1200, heads of 64, 37 us: 3.3 us, then 1.8 us a tile (the other CTA of the SM at work too; 1.4 alone) and 2.7 us an
 // item, of which the fullest CTA has 13 tiles in 3 items (960 items of 3.4 tiles; 12 equal prompts of 16 to 1200 tokens fit within 2 us).
+//
+// Two more forms of it. Differential heads: the tiles of a CTA are the two maps of the same rows, which share K and V; a map's scores take
+// half of the columns, its O all of those of V, and the warpgroups trade sums, then take the difference and the norm of half of the columns
+// each. 2048 tokens behind 8192, 32 / 8 heads of 128, 570 to 600 us = 0.8 PFLOP/s (1.06 with the second terms of the probabilities): the
+// products, at the clock that the power cap leaves; 12 prompts of 100 to 1200, 16 / 2 of 64, 69 us: twice the exponentials of one map (37 us).
+// Prefixes that requests share: the rows of all requests of a group side by side, cut along the keys so that the parts fill the GPU; a part
+// leaves its sums as they are, for the launch over the keys behind the prefix (paged_attention.cuh). 96 requests behind four prefixes of
+// 3000 to 9000 keys, 32 / 8 of 128: 30 us of 100, a tile of keys in 4000 cycles (two CTAs an SM): S and P V in turn with a softmax of
+// 2000 and the look-ups and loads of the next tile.
 #pragma once
 
 #include "paged_attention.cuh"
@@ -1139,16 +1148,16 @@ inline PxPlan px_plan(int T, int Hq, int Hk, int D) {
 }
 // Whether requests are attended by group, as told by what the host knows: where a group has more than one, copies of the cache's rows take
 // tiles of them, and the keys that the tables hold at most are worth a second launch.
-// Decode: 128 MB of keys and values a call, each request's its own. us, request by request / by group, prefixes with 100 keys behind them:
-//   8 / 8 heads of 64: 8 requests of 4096 (70 MB) 15.5 / 19.3, of 16000 38 / 27; 32 of 1024 (74 MB) 14.3 / 16.4, of 4096 40 / 18.5; 128 of
-//   256 (93 MB) 22 / 24, of 1024 47 / 26; in 32 groups of 4 46 / 42; 16 / 2 of 128: 8 of 16000 (132 MB) 28 / 31, 32 of 4096 (138 MB) 26 / 21,
-//   128 of 1024 (147 MB) 25 / 20.5, in 32 groups 25.3 / 25.0
+// Decode: 100 MB of keys and values a call, each request's its own. us, request by request / by group, prefixes with 100 keys behind them:
+//   16 / 2 heads of 64: 16 requests of 8000 (67 MB) 15.5 / 20.7, 64 of 1500 (55 MB) 11.6 / 14.9, of 3000 (105 MB) 17.7 / 16.4, 192 of 1500
+//   33.6 / 20.9; 8 / 8 of 64: 16 of 3000 (105 MB) 17.8 / 15.8, 64 of 300 (59 MB) 13.1 / 18.6, of 1500 32 / 19.5; 32 / 8 of 128: 4 of 8000
+//   (134 MB) 23.9 / 24.6, 16 of 1500 (109 MB) 17.7 / 16.3, of 3000 29.5 / 17.6; 16 / 2 of 128: 64 of 700 (59 MB) 12.0 / 16.9, of 3000 30 / 19.2
 // Packed: tiles of rows over the whole contexts against those over the prefix and an item for every new token and kv head; what either
 // takes by the formulas below is within a third of what it took over 100 points. us, 32 requests with 2, 6, 12, 24 new tokens behind 4000
-// keys: 16 / 2 heads of 64 25, 25, 26, 39 / 19, 28, 33, 52; 32 / 8 of 128 125, 125, 128, 129 / 32, 53, 87, 166
+// keys: 16 / 2 heads of 64 25, 25, 26, 39 / 17, 27, 33, 53; 32 / 8 of 128 123, 123, 125, 127 / 31, 55, 87, 165
 inline bool px_shares(int T, int n_req, int n_groups, int Hq, int Hk, int D, int block_size, int64_t max_keys, bool packed) {
   if (n_groups < 1 || n_req <= n_groups || block_size % 8 != 0 || max_keys < 1 || max_keys > kPpMaxKeys || T >= (1 << 24)) return false;
-  if (!packed) return (double)T * max_keys * Hk * D * 4 >= 128e6;
+  if (!packed) return (double)T * max_keys * Hk * D * 4 >= 100e6;
   const int h_shift = pp_h_shift(Hq / Hk), per_tile = kPpRows >> h_shift, sets = Hq >> h_shift;
   const double tiles = (double)max_keys / kPpKeys, each = ceil_div_i(ceil_div_i(T, n_req), per_tile * pp_row_tiles(D, kPlain));
   const double alone = 8 + n_req * each * sets * tiles * 1.8 / pp_ctas(D, kPlain);
