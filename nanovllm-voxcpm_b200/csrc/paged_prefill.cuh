@@ -405,6 +405,7 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
   __shared__ uint32_t s_tmem, s_boxes[4];
   __shared__ PpPiece s_piece[2];
   __shared__ volatile int abort_flag;
+  __shared__ __align__(16) float s_weight[kForm == kDiff ? D : 4];   // of the norm
   __shared__ float s_sums[kForm == kDiff ? 2 : 1][kTiles][kPpRows];  // what the maps tell each other: sums, sums of squares
   const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
   const PagedArgs& p = a.p;
@@ -433,6 +434,17 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
   __syncthreads();
   tc_fence_after_sync();
   if (kForm != kPrefix) glue_enter();  // (dependents may start: every CTA of this launch holds its tensor memory by then)
+  if (kForm == kDiff) {
+    for (int i = tid; i < D; i += pp_threads(kTiles)) {
+      float w = 1.f;
+      if (p.norm_weight != nullptr) {
+        const float2 pair = unpack_16x2<kF16>(reinterpret_cast<const uint32_t*>(p.norm_weight)[i >> 1]);
+        w = i & 1 ? pair.y : pair.x;
+      }
+      s_weight[i] = w;
+    }
+    __syncthreads();
+  }
   const uint32_t tmem = s_tmem;
   const int per_tile = kPpRows >> a.h_shift, span = kRowTiles * per_tile;
 
@@ -467,6 +479,9 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
       const int w_lo = p.window > 0 ? max(tile_hi, 0) - (p.window - 1) : 0;
       const int clear0 = (w.sink_boxes + max(0, (int)(((uint32_t)max(w_lo, 0) + a.box - 1u) >> a.box_shift) - w.first_box) + (1 << tile_shift) - 1) >> tile_shift;
       const int clear1 = (((tile_lo + 1) >> a.box_shift) + w.sink_boxes - w.first_box) >> tile_shift;
+      float lam = 0.f;  // (asked for ahead of the tiles)
+      if (kForm == kDiff && tok < w.n_here)
+        lam = p.lam[((int64_t)w.begin + w.q0 + tok) * p.lam_token + (w.head0 + (row & ((1 << a.h_shift) - 1))) * p.lam_head];
       float m = -INFINITY, l = 0.f;  // what the probabilities refer to, in units of log2; their sum
       for (int i = w.i0; i < w.i1; ++i, ++n) {
         pp_wait(bar(S_READY + t), n & 1, &abort_flag);
@@ -588,7 +603,6 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
           return s_sums[which][t ^ 1][row];
         };
         const float other = over(exchange(0, l));
-        const float lam = live ? p.lam[(token0 + tok) * p.lam_token + (w.head0 + (row & ((1 << a.h_shift) - 1))) * p.lam_head] : 0.f;
         const float one = t == 0 ? inv : other, two = lam * (t == 0 ? other : inv);
         float y[D / 2], ss = 0.f;
 #pragma unroll
@@ -614,18 +628,13 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
 #pragma unroll
           for (int j = 0; j < 32; j += 8) {
             float f[8];
-            if (p.norm_weight != nullptr) {
-              const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const char*>(p.norm_weight) + 2 * (col + j));
-              const uint32_t raw[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float2 u = unpack_16x2<kF16>(raw[i]);
-                f[2 * i] = r * u.x;
-                f[2 * i + 1] = r * u.y;
-              }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) f[i] = 1.f;
+            for (int i = 0; i < 8; i += 4) {
+              const float4 w4 = *reinterpret_cast<const float4*>(s_weight + col + j + i);
+              f[i] = r * w4.x;
+              f[i + 1] = r * w4.y;
+              f[i + 2] = r * w4.z;
+              f[i + 3] = r * w4.w;
             }
             const float* const x = y + 32 * c + j;
             uint4 v;
