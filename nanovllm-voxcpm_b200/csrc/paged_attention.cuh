@@ -64,8 +64,7 @@ struct PagedArgs {
 };
 
 // What a kernel makes of a head: one softmax map; or two, of the halves of its columns of q and k over the whole of v, and of them the
-// difference a - lam b, normed.
-// Or, of requests with a common prefix: the keys of the prefix, all requests of a group side by side; the keys behind it, and the join.
+// difference a - lam b, normed. Or, of requests with a common prefix: the keys of the prefix, all requests of a group side by side; the keys behind it, and the join.
 constexpr int kPlain = 0, kDiff = 1, kPrefix = 2, kSuffix = 3;
 template <int kForm> constexpr int kMaps = kForm == kDiff ? 2 : 1;
 template <int kForm> constexpr int kItemHeads = kForm == kDiff ? 8 : 16;  // q heads of an item at most
@@ -285,6 +284,7 @@ struct PagedWalk {
     const int per_row = a.Hk * a.chunks, group = a.Hq / a.Hk;
     PagedPiece w;
     w.row = -1;
+    w.n_units = 0;
     int item = 0;
     while (at < end) {
       if (step > 0) {
@@ -942,8 +942,6 @@ inline int paged_decode_launch_t(const PagedArgs& a, int ctas, int cluster, cuda
 template <int D, int NT, bool kF16, int kForm>
 inline int paged_decode_launch_by(const PagedArgs& a, cudaStream_t stream) {
   const PagedWay w = paged_way(a.T, a.Hq, a.Hk, D, (int64_t)a.table_width * a.cache.block_size, a.window, a.sinks, kItemHeads<kForm>);
-  if constexpr (kForm != kSuffix)
-    if (w.shares && a.part_o != nullptr) return paged_decode_launch_t<D, NT, kF16, kShares, 4, kForm>(a, kPagedCtas, 1, stream);
   const int64_t items = (int64_t)a.T * a.Hk * a.chunks;
   // Behind a prefix, items that CTAs take as they come: four warps, for which an SM has room beside a CTA of the prefix launch (64 requests
   // of 10 to 600 keys behind 2000, 16 / 2 heads of 64, 13.9 us, eight warps 18.5). Shares would be even where the keys behind the prefix
@@ -951,11 +949,13 @@ inline int paged_decode_launch_by(const PagedArgs& a, cudaStream_t stream) {
   if constexpr (kForm == kSuffix) {
     if (w.cluster > 1) return paged_decode_launch_t<D, NT, kF16, kClusters, 8, kForm>(a, (int)std::min<int64_t>(148 / w.cluster, items) * w.cluster, w.cluster, stream);
     return paged_decode_launch_t<D, NT, kF16, kWhole, 4, kForm>(a, (int)std::min<int64_t>(kPagedCtas, items), 1, stream);
+  } else {
+    if (w.shares && a.part_o != nullptr) return paged_decode_launch_t<D, NT, kF16, kShares, 4, kForm>(a, kPagedCtas, 1, stream);
+    const int ctas = (int)std::min<int64_t>((w.warps == 8 ? 148 : kPagedCtas) / w.cluster, items) * w.cluster;
+    if (w.cluster > 1) return paged_decode_launch_t<D, NT, kF16, kClusters, 8, kForm>(a, ctas, w.cluster, stream);
+    if (w.warps == 8) return paged_decode_launch_t<D, NT, kF16, kWhole, 8, kForm>(a, ctas, 1, stream);
+    return paged_decode_launch_t<D, NT, kF16, kWhole, 4, kForm>(a, ctas, 1, stream);
   }
-  const int ctas = (int)std::min<int64_t>((w.warps == 8 ? 148 : kPagedCtas) / w.cluster, items) * w.cluster;
-  if (w.cluster > 1) return paged_decode_launch_t<D, NT, kF16, kClusters, 8, kForm>(a, ctas, w.cluster, stream);
-  if (w.warps == 8) return paged_decode_launch_t<D, NT, kF16, kWhole, 8, kForm>(a, ctas, 1, stream);
-  return paged_decode_launch_t<D, NT, kF16, kWhole, 4, kForm>(a, ctas, 1, stream);
 }
 
 template <int D, int kForm>
