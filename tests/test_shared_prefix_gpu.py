@@ -108,6 +108,16 @@ def test_decode_sizes(n, groups, prefix, own, dim):
     assert N.device_status() == 0
 
 
+@pytest.mark.parametrize("n,groups", [(513, 3), (600, 300), (511, 40)])
+def test_decode_many_requests(n, groups):
+    """More rows than are put in order, more groups than a warp has lanes."""
+    each = [n // groups + (i < n % groups) for i in range(groups)]
+    p = make(4, 2, 64, 8, [(9 + 5 * i % 40, [1 + (i + j) % 7 for j in range(m)]) for i, m in enumerate(each)], seed=n, loose=2)
+    out, lse = call(p, return_lse=True)
+    PP.check(p, out, lse, f"{n} requests")
+    assert torch.equal(out, call(p)) and N.device_status() == 0
+
+
 def test_decode_requests_of_no_group():
     p = make(16, 2, 64, 16, [(64, [1, 5, 9])], loose=4)
     PP.check(p, *call(p, return_lse=True))
@@ -201,6 +211,16 @@ def test_prefill_sizes(n, prefix, own, new, dim):
     PP.check(p, out, lse, f"{n} requests")
     assert torch.equal(out, call(p))
     assert N.device_status() == 0
+
+
+def test_prefill_many_requests():
+    """Packed: 700 tokens of 140 requests in 70 groups, some without new tokens, some rows of no sequence."""
+    new = [(3 * i) % 11 for i in range(140)]
+    p = make(8, 2, 64, 16, [(20 + 3 * i % 90, [new[2 * i] + 1, new[2 * i + 1] + 4]) for i in range(70)], new, seed=1, behind=5)
+    out = torch.full_like(p["args"][0], 7.0)
+    _, lse = call(p, out=out, return_lse=True)
+    PP.check(p, out, lse)
+    assert bool((out[-5:] == 7).all()) and N.device_status() == 0
 
 
 @pytest.mark.parametrize("page", [8, 12, 24, 256])
