@@ -20,7 +20,7 @@
 // 17 us; one of 333, 16 / 2 of 64, 6.3 us. Behind a prefix that requests share: the keys behind it, a row at a time, and the join with the
 // parts that the launch ahead (paged_prefill.cuh) leaves of the prefix. It runs beside that launch, a CTA of either on an SM; bound by
 // HBM where there is much behind the prefix (96 requests of 50 to 1500 keys behind four prefixes, 32 / 8 of 128: 100 us, 59 at the copy
-// bandwidth, 260 request by request), else by the two chains (64 of 10 to 600 keys behind 4003, 16 / 2 of 64: 17 us; 21 request by request).
+// bandwidth, 260 request by request), else by the two chains (64 of 10 to 600 keys behind 4003, 16 / 2 of 64: 17 us; 22 request by request).
 #pragma once
 
 #include <atomic>
@@ -944,8 +944,8 @@ inline int paged_decode_launch_by(const PagedArgs& a, cudaStream_t stream) {
   const PagedWay w = paged_way(a.T, a.Hq, a.Hk, D, (int64_t)a.table_width * a.cache.block_size, a.window, a.sinks, kItemHeads<kForm>);
   const int64_t items = (int64_t)a.T * a.Hk * a.chunks;
   // Behind a prefix, items that CTAs take as they come: four warps, for which an SM has room beside a CTA of the prefix launch (64 requests
-  // of 10 to 600 keys behind 2000, 16 / 2 heads of 64, 13.9 us, eight warps 18.5). Shares would be even where the keys behind the prefix
-  // are many, which the host does not know: 48 requests, 32 / 8 heads of 128, of 500 / 3000 keys behind 8000, items 48 / 168 us, shares 65 / 138.
+  // of 10 to 600 keys behind 2003, 16 / 2 heads of 64, 15 us, eight warps 18.5). Shares would be even where the keys behind the prefix
+  // are many, which the host does not know: 48 requests, 32 / 8 heads of 128, of 500 / 3000 keys behind 8000, items 54 / 150 us, shares 65 / 138.
   if constexpr (kForm == kSuffix) {
     if (w.cluster > 1) return paged_decode_launch_t<D, NT, kF16, kClusters, 8, kForm>(a, (int)std::min<int64_t>(148 / w.cluster, items) * w.cluster, w.cluster, stream);
     return paged_decode_launch_t<D, NT, kF16, kWhole, 4, kForm>(a, (int)std::min<int64_t>(kPagedCtas, items), 1, stream);
