@@ -534,7 +534,7 @@ int lora_b200_differential_attention(void* out, int64_t out_token, int64_t out_h
  * Attention over a paged cache for requests that begin alike: the results of lora_b200_paged_decode_attention (cu_seqlens null, n_seqs
  * = T) or lora_b200_paged_prefill_attention without a window, for which the common keys are read once a group instead of once a
  * request. The sequences [cu_groups[g], cu_groups[g + 1]) have the same keys and values at their first prefix_lens[g] positions; where
- * those lie is read from the block table of the group's first sequence, and what follows from each one's own. prefix_lens int32
+ * those lie is read from the block table of the group's first sequence (which holds them all), and what follows from each one's own. prefix_lens int32
  * [n_groups], cu_groups int32 [n_groups + 1], ascending; a sequence in no group (or in one that leaves the sequences) shares nothing, a
  * prefix of zero (or less) is none. Tokens inside the prefix see it up to themselves. A value that is not finite, of a key of the prefix
  * that some rows of a block see, may reach the block's other rows (as in a prefill call; a block may hold rows of several sequences of

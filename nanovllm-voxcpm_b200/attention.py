@@ -162,9 +162,9 @@ def shared_prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cac
 
     Requests ``cu_groups[g] : cu_groups[g + 1]`` have the same keys and values at their first ``prefix_lens[g]`` positions (any number:
     a prefix may end inside a block, of which every request has a copy of its own). Where those lie is read from the table of the group's
-    first request, what follows from each one's own. ``prefix_lens`` int32 ``[groups]``, ``cu_groups`` int32 ``[groups + 1]``, ascending;
+    first request, which holds them all, what follows from each one's own. ``prefix_lens`` int32 ``[groups]``, ``cu_groups`` int32 ``[groups + 1]``, ascending;
     requests of no group share nothing, a prefix of zero is none. Other arguments, strides, missing blocks, contexts of no key and the
-log sums as ``paged_decode_attention``. Calls whose tables are too narrow for a second launch to pay, block sizes that are no
+    log sums as ``paged_decode_attention``. Calls whose tables are too narrow for a second launch to pay, block sizes that are no
     multiples of 8 and groups of one request are attended request by request. A value that is not finite, of a key of the prefix that
     some requests of a group see, may reach the group's others."""
     return _shared_prefix(q, k_cache, v_cache, block_tables, context_lens, None, prefix_lens, cu_groups, scale, out, return_lse)
