@@ -356,9 +356,17 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
     rank = cluster_ctarank();
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
   }
-  // (Behind the prefix launch, which lets this one start once all of its CTAs have waited for what lies ahead of both: only the join
-  // waits for it.)
-  if (kForm != kSuffix) glue_enter();
+  auto take = [&]() { return atomicAdd(&a.px_head->next_item, 1); };
+  if (kForm != kSuffix) {
+    glue_enter();
+  } else {
+    // The prefix launch lets this one start once all of its CTAs have waited for what lies ahead of both; only the join waits for it.
+    // What is read ahead of that wait (lengths, groups, tables, q, the cache; the order of the items) is ordered by the counter: CTA 0 of the
+    // prefix launch releases it, behind its own wait and the order that it laid down, and only then lets this launch start; here
+    // every CTA acquires it ahead of its first read.
+    if (tid == 0) s_next = kQueue ? atom_add_acquire_gpu(&a.px_head->next_item, 1) : ld_acquire_gpu(&a.px_head->next_item);
+    __syncthreads();
+  }
 
   Walk walk;
   if constexpr (kForm == kSuffix) walk.groups = px_group(a, lane);
@@ -469,18 +477,13 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
     }
   };
 
-  auto take = [&]() { return atomicAdd(&a.px_head->next_item, 1); };
   int taken = 0;
   PagedPiece w;
   int stage = 0, buf = 0;
   bool first_piece = true;
   int chunk = 1;  // behind a prefix: tiles of a part of it
-  auto begin = [&]() {  // an item with none ahead of it
-    if constexpr (kQueue) {
-      if (tid == 0) s_next = take();
-      __syncthreads();
-      walk.at = s_next;
-    }
+  auto begin = [&]() {  // the item s_next, with none ahead of it
+    if constexpr (kQueue) walk.at = s_next;
     w = walk.next(a);
     const int e0 = entry(w, w.u0 + warp), e1 = entry(w, w.u0 + warp + kPagedWarps);
     load_q(w);
@@ -800,7 +803,8 @@ __global__ void __launch_bounds__(32 * kPagedWarps, 8 / kPagedWarps) paged_decod
     w = following;
     if (kQueue) {
       if (!ahead) {
-        __syncthreads();  // (the stages that held results may be filled again)
+        if (tid == 0) s_next = take();
+        __syncthreads();  // (and the stages that held results may be filled again)
         begin();
         if (tid == 0) taken = take();
         __syncthreads();  // (all have read this one)

@@ -193,8 +193,8 @@ __device__ __forceinline__ void px_order(const PagedArgs& p, int* keys) {
     for (int k = 0; k < n; ++k) rank += keys[k] > mine || (keys[k] == mine && k < row) ? 1 : 0;
     p.px_head->order[rank] = row;
   }
-  if (threadIdx.x == 0) p.px_head->next_item = 0;
-  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) st_release_gpu(&p.px_head->next_item, 0);  // (with the order, and with what this CTA has waited for)
   __syncthreads();
 }
 
