@@ -238,12 +238,18 @@ def differential_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cac
     return _differential(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, lam, norm_weight, eps, scale, window, sinks, out)
 
 
+def _steps(t: torch.Tensor) -> tuple:
+    """The strides that matter: a dimension of one entry has none."""
+    return tuple(s if n > 1 else 0 for n, s in zip(t.shape, t.stride()))
+
+
 def join_attention(outs, lses, *, out: torch.Tensor | None = None, return_lse: bool = False):
     """The result over a whole context of results over its parts (each token's keys lie in one part each).
 
     ``outs`` ``[parts, tokens, heads, head_dim]`` or a sequence of ``[tokens, heads, head_dim]`` tensors of one shape and one set of
-    strides, bf16, fp16 or fp32, up to 64 of them; ``lses`` the fp32 ``[tokens, heads]`` logarithms of their sums that came with them
-    (``return_lse``), as ``[parts, ...]`` or a sequence. A part without a key (``-inf``) counts for nothing, whatever its values; a row
+    strides (of dimensions with more than one entry), bf16, fp16 or fp32, up to 64 of them; ``lses`` the fp32 ``[tokens, heads]``
+    logarithms of their sums that came with them (``return_lse``), as ``[parts, ...]`` or a sequence. A part without a key (``-inf``)
+    counts for nothing, whatever its values; a row
     that has none in any part gives zeros. ``out`` may be one of the parts. Returns ``out``, with ``return_lse`` also the logarithm of
     the whole sum."""
     got = N.native().join_attention(outs, lses, out, bool(return_lse))
@@ -257,10 +263,10 @@ def join_attention(outs, lses, *, out: torch.Tensor | None = None, return_lse: b
     first, lse0 = outs[0], lses[0]
     if first.dim() != 3 or first.stride(2) != 1:
         raise ValueError("a part must be [tokens, heads, head_dim] with adjacent elements in a head")
-    if any(o.shape != first.shape or o.dtype != first.dtype or o.stride() != first.stride() for o in outs):
+    if any(o.shape != first.shape or o.dtype != first.dtype or _steps(o) != _steps(first) for o in outs):
         raise ValueError("the parts must have one shape, dtype and set of strides")
     T, heads, dim = first.shape
-    if any(x.dtype != torch.float32 or tuple(x.shape) != (T, heads) or x.stride() != lse0.stride() for x in lses):
+    if any(x.dtype != torch.float32 or tuple(x.shape) != (T, heads) or _steps(x) != _steps(lse0) for x in lses):
         raise ValueError(f"the logarithms must be float32 tensors {(T, heads)} of one set of strides")
     if out is not None and (out.shape != first.shape or out.dtype != first.dtype or out.stride(2) != 1):
         raise ValueError("out must have the shape and dtype of a part, and adjacent elements in a head")
@@ -272,6 +278,6 @@ def join_attention(outs, lses, *, out: torch.Tensor | None = None, return_lse: b
             out = torch.empty(T, heads, dim, dtype=first.dtype, device=first.device)
         lse = torch.empty(T, heads, dtype=torch.float32, device=first.device) if return_lse else None
         N.check(N.lib().lora_b200_join_attention(
-            out.data_ptr(), out.stride(0), out.stride(1), N.ptr(lse), N.ptr_array(outs), N.ptr_array(lses), len(outs), first.stride(0),
-            first.stride(1), lse0.stride(0), lse0.stride(1), T, heads, dim, N.dtype_code(first.dtype), N.current_stream(first.device)))
+            out.data_ptr(), *_steps(out)[:2], N.ptr(lse), N.ptr_array(outs), N.ptr_array(lses), len(outs), *_steps(first)[:2], *_steps(lse0),
+            T, heads, dim, N.dtype_code(first.dtype), N.current_stream(first.device)))
     return (out, lse) if return_lse else out

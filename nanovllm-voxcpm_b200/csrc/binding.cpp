@@ -758,7 +758,9 @@ struct Parts {
   void* at[kMost];
 
   int64_t size(int64_t d) const { return first->size(d + stacked); }
-  int64_t stride(int64_t d) const { return first->stride(d + stacked); }
+  int64_t stride(int64_t d) const { return step(*first, d + stacked); }
+  // (the stride of a dimension of one entry means nothing: any goes with any)
+  static int64_t step(const at::Tensor& t, int64_t d) { return t.size(d) == 1 ? 0 : t.stride(d); }
   bool read(PyObject* o, int64_t dims, int dev) {  // false = not handled
     first = tensor_of(o);
     if (first != nullptr) {
@@ -776,9 +778,9 @@ struct Parts {
     if (first == nullptr || first->dim() != dims || !first->is_cuda() || (dev >= 0 && first->get_device() != dev)) return false;
     for (int64_t i = 0; i < n; ++i) {
       const at::Tensor* t = tensor_of(each[i]);
-      if (t == nullptr || !on(*t, first->get_device()) || t->scalar_type() != first->scalar_type() || t->sizes() != first->sizes() ||
-          t->strides() != first->strides())
-        return false;
+      if (t == nullptr || !on(*t, first->get_device()) || t->scalar_type() != first->scalar_type() || t->sizes() != first->sizes()) return false;
+      for (int64_t d = 0; d < dims; ++d)
+        if (step(*t, d) != step(*first, d)) return false;
       at[i] = t->data_ptr();
     }
     return true;
@@ -808,9 +810,9 @@ PyObject* join_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       return not_handled();
   }
   if (args[3] == Py_True) lse = at::empty({T, heads}, first->options().dtype(at::kFloat));
-  const int rc = p_join(out->data_ptr(), out->stride(0), out->stride(1), lse.defined() ? static_cast<float*>(lse.data_ptr()) : nullptr, outs.at,
-                        reinterpret_cast<const float* const*>(lses.at), (int)outs.n, outs.stride(0), outs.stride(1), lses.stride(0), lses.stride(1), (int)T, (int)heads, (int)d, code,
-                        c10::cuda::getCurrentCUDAStream(dev).stream());
+  const int rc = p_join(out->data_ptr(), Parts::step(*out, 0), Parts::step(*out, 1), lse.defined() ? static_cast<float*>(lse.data_ptr()) : nullptr, outs.at,
+                        reinterpret_cast<const float* const*>(lses.at), (int)outs.n, outs.stride(0), outs.stride(1), lses.stride(0), lses.stride(1),
+                        (int)T, (int)heads, (int)d, code, c10::cuda::getCurrentCUDAStream(dev).stream());
   PyObject* lse_out = Py_None;
   if (lse.defined()) lse_out = THPVariable_Wrap(lse);
   else Py_INCREF(Py_None);
