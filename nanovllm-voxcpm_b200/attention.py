@@ -125,6 +125,8 @@ def paged_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
 
 
 def _shared_prefix(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, prefix_lens, cu_groups, scale, out, return_lse):
+    if prefix_lens is None or cu_groups is None:
+        raise ValueError("prefix_lens and cu_groups say who begins alike: an attention behind shared prefixes needs both")
     if scale is None:
         scale = q.size(-1) ** -0.5
     got = N.native().shared_prefix_attention(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, prefix_lens, cu_groups, scale,
@@ -182,6 +184,8 @@ def shared_prefix_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_ca
 
 
 def _differential(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, lam, norm_weight, eps, scale, window, sinks, out):
+    if lam is None:
+        raise ValueError("lam says what the second map counts: differential attention needs it")
     if scale is None:
         scale = (q.size(-1) // 2) ** -0.5
     got = N.native().differential_attention(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens, lam, norm_weight, eps, scale,
