@@ -515,7 +515,8 @@ int lora_b200_paged_prefill_attention(void* out, int64_t out_token, int64_t out_
  * Differential attention over a paged cache: the halves of a head's columns of q and k (head_dim / 2 each) make two softmax maps over
  * the same keys, and with S1, S2 their results over the whole columns of v
  *   out[t, h] = S1 - lam[t, h] * S2,  with norm_weight: y / sqrt(mean(y^2) + eps) * norm_weight, y that difference
- * (fp32 throughout, rounded once). lam float, [T, num_heads] by strides in elements (0: one for all); norm_weight [head_dim] of the
+ * (fp32, rounded once; a probability enters the product with v as the sum of two numbers of its type, 2^-15 of it off at most in bf16,
+ * 2^-23 in fp16, whether decode or prefill, wherever the key lies). lam float, [T, num_heads] by strides in elements (0: one for all); norm_weight [head_dim] of the
  * type of q, 16-byte aligned, or null. A token without a visible key gives zeros. cu_seqlens null: decode (n_seqs = T), else packed
  * as lora_b200_paged_prefill_attention; everything else as there. packed (of the workspace's size): with cu_seqlens.
  * No counterpart in the reference (Ye et al., "Differential Transformer", 2024).

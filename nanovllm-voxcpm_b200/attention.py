@@ -223,7 +223,8 @@ def differential_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cach
     """Differential attention (Ye et al., "Differential Transformer", 2024) of one new token of every request. The halves of a head's
     columns of q and k make two softmax maps over the keys that ``paged_decode_attention`` would show the token; with ``S1`` and ``S2``
     their results over the whole columns of v, a head gives ``S1 - lam * S2``. With ``norm_weight [head_dim]`` that difference is
-    RMS-normed over the head and scaled by it (a constant factor, ``1 - lambda_init``, belongs into it). All of it fp32, rounded once.
+    RMS-normed over the head and scaled by it (a constant factor, ``1 - lambda_init``, belongs into it). All of it fp32, rounded once; a
+    probability enters the product with v as the sum of two numbers of its type (off by 2^-15 of it at most in bf16, by 2^-23 in fp16).
 
     ``lam`` float32 ``[heads]`` or, of every token its own, ``[requests, heads]``; ``scale`` defaults to that of half a head. The halves
     are rotated as heads of their own: ``rope_kv_store`` fills such a cache as one of twice the heads of half the size. Other

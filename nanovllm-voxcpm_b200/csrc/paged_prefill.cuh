@@ -20,7 +20,7 @@
 //
 // Two more forms of it. Differential heads: the tiles of a CTA are the two maps of the same rows, which share K and V; a map's scores take
 // half of the columns, its O all of those of V, and the warpgroups trade sums, then take the difference and the norm of half of the columns
-// each. 2048 tokens behind 8192, 32 / 8 heads of 128, 570 to 600 us = 0.8 PFLOP/s (1.06 with the second terms of the probabilities): the
+// each. 2048 tokens behind 8192, 32 / 8 heads of 128, 675 us = 0.69 PFLOP/s (1.14 with the second terms of the probabilities): the
 // products, at the clock that the power cap leaves; 12 prompts of 100 to 1200, 16 / 2 of 64, 69 us: twice the exponentials of one map (37 us).
 // Prefixes that requests share: the rows of all requests of a group side by side, cut along the keys so that the parts fill the GPU; a part
 // leaves its sums as they are, for the launch over the keys behind the prefix (paged_attention.cuh). 96 requests behind four prefixes of
@@ -393,11 +393,13 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
   // there is to wait for, and an eighth of the exponentials on the FMA units pays. (8192 tokens, 16 / 2 heads of 64: 208 us with P in
   // S, 198 with columns of its own, 190 with an eighth, 197 with a quarter, 233 with half; heads of 128 gain from neither.)
   constexpr bool kOwnP = kTiles == 1 && D == 64;
-  // Columns of 32 of a tile whose probabilities are two 16-bit numbers in the product with V, since what the maps have in common leaves with
-  // the difference and what rounding did to it stays. Scores of spread 1, lam of 0.5, against 64 bits where the rounding of the result alone
-  // has 1: none 1.55, half of them 1.31, all 1. 2048 tokens behind 8192, 32 / 8 heads of 128, 474, 580, 662 us (P V is what bounds it); 12
-  // prompts of 101 to 1200, 16 / 2 heads of 64, 66, 67, 69.
-  constexpr int kFine = kForm != kDiff ? 0 : D == 64 ? 4 : 2;
+  // Differential: probabilities are two 16-bit numbers each in the product with V (bf16: both truncated, 2^-15 of a probability at most),
+  // since what the maps have in common leaves with the difference and what rounding did to it stays. Scores of spread 1, lam of 0.5,
+  // against 64 bits where the rounding of the result alone has 1: one number 1.55, second terms for half of the keys 1.31, for all 1.
+  // 2048 tokens behind 8192, 32 / 8 heads of 128, 474, 580, 662 us (P V is what bounds it); 12 prompts of 101 to 1200, 16 / 2 heads of
+  // 64, 66, 67, 69. (For half of them a key would count with the more bits the earlier it lies in its tile, and with other ones than a decode
+  // step gives it.)
+  constexpr bool kFine = kForm == kDiff;
   constexpr int kLoader = 4 * kTiles, kIssuer = kLoader + 1, kTmem = 256 * kTiles, kO = kTiles * kPpKeys;  // warps; columns: all, the first of O
   enum { Q_FULL, Q_FREE, S_READY, P_READY = S_READY + 2, O_DONE = P_READY + 4, K_FULL = O_DONE + 2, K_FREE = K_FULL + kSt, V_FULL = K_FREE + kSt,
          V_FREE = V_FULL + kSt, PIECE = V_FREE + kSt, TAKEN = PIECE + 2, S_TAKEN = TAKEN + 2, PV_DONE, SHARED, N_BARS };
@@ -556,17 +558,17 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
             const float2 x = fma2(make_float2(__uint_as_float(s[c][j]), __uint_as_float(s[c][j + 1])), scale2, base2);
             const float2 y = kOwnP && j % 16 == 14 ? exp2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
             sum[j / 2 % 2] = add2(sum[j / 2 % 2], y);
-            if (c < kFine && !kF16) {  // (the upper halves as they are, and what they leave)
+            if (kFine && !kF16) {  // (the upper halves as they are, and what they leave)
               packed[j / 2] = __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x7632);
               const float2 low = fma2(make_float2(__uint_as_float(__float_as_uint(y.x) & 0xffff0000u), __uint_as_float(__float_as_uint(y.y) & 0xffff0000u)), make_float2(-1.f, -1.f), y);
               rest[j / 2] = __byte_perm(__float_as_uint(low.x), __float_as_uint(low.y), 0x7632);
             } else {
               packed[j / 2] = pack_16x2<kF16>(y.x, y.y);  // (rounded to the type of V; the sum is that of the unrounded ones)
-              if (c < kFine) rest[j / 2] = rest_16x2<kF16>(y, packed[j / 2]);
+              if (kFine) rest[j / 2] = rest_16x2<kF16>(y, packed[j / 2]);
             }
           }
           tmem_st_32x16(p_at + 16 * c, packed);
-          if (c < kFine) tmem_st_32x16(p_at + kPpKeys / 2 + 16 * c, rest);
+          if (kFine) tmem_st_32x16(p_at + kPpKeys / 2 + 16 * c, rest);
           if (c & 1) {  // half of P: its products may begin
             tmem_st_wait();
             tc_fence_before_sync();
@@ -886,7 +888,7 @@ __global__ void __launch_bounds__(pp_threads(pp_tiles(D, kForm)), 3 - pp_tiles(D
               }
               umma_ts_elected(tmem + kO + t * D, tmem + (kOwnP ? kO + D : t * kPpKeys) + 8 * k, lo_v(v_u32 + st * kTile + k * 2048), hi_k, idesc_o,
                               i > w.i0 || k > 0, leader);
-              if (k / 2 < kFine)
+              if (kFine)
                 umma_ts_elected(tmem + kO + t * D, tmem + t * kPpKeys + kPpKeys / 2 + 8 * k, lo_v(v_u32 + st * kTile + k * 2048), hi_k, idesc_o, 1, leader);
             }
             if (kOwnP) {
