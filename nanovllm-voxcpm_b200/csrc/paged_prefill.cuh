@@ -164,7 +164,7 @@ __device__ __forceinline__ int px_request(const PagedArgs& p, int row, int r0, i
 }
 // Position of a row of the group that begins with request r0; -1 if its request's rows leave those of q
 __device__ __forceinline__ int px_position(const PagedArgs& p, int row, int r0, int r1) {
-  if (p.cu_seqlens == nullptr) return p.context_lens[row] - 1;
+  if (p.cu_seqlens == nullptr) return max(p.context_lens[row], 0) - 1;  // (less than none is none, the least int too)
   const int r = px_request(p, row, r0, r1), end = p.cu_seqlens[r + 1];
   if (p.cu_seqlens[r] < 0 || end > p.T || row >= end) return -1;
   return (int)max((int64_t)p.context_lens[r] - (end - row), (int64_t)-1);
@@ -183,7 +183,7 @@ __device__ __forceinline__ void px_order(const PagedArgs& p, int* keys) {
     }
     const PxGroup g = px_group(p, lo);
     const int ctx = p.context_lens[r];
-    keys[row] = max(0, ctx - (g.r0 <= r && r < g.r1 ? g.keys : 0));
+    keys[row] = max(0, max(ctx, 0) - (g.r0 <= r && r < g.r1 ? g.keys : 0));
   }
   __syncthreads();
   for (int row = threadIdx.x; row < n; row += blockDim.x) {
