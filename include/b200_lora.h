@@ -523,6 +523,9 @@ int lora_b200_paged_prefill_attention(void* out, int64_t out_token, int64_t out_
  */
 size_t lora_b200_differential_workspace_bytes(int32_t T, int32_t n_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                                               int32_t table_width, int32_t block_size, int32_t window, int32_t sinks, int32_t packed);
+/* How a decode call of it meets the GPU, as lora_b200_paged_decode_way says it (an item has up to 8 heads). */
+int32_t lora_b200_differential_way(int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t table_width,
+                                   int32_t block_size, int32_t window, int32_t sinks);
 int lora_b200_differential_attention(void* out, int64_t out_token, int64_t out_head, const void* q, int64_t q_token, int64_t q_head,
                                      int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                                      const lora_b200_paged_cache* cache, const int32_t* block_tables, int64_t table_ld,

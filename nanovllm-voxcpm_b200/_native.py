@@ -152,6 +152,7 @@ _SIGNATURES = {
     "lora_b200_differential_workspace_bytes": (
         c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32],
     ),
+    "lora_b200_differential_way": (c_int32, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
     "lora_b200_differential_attention": (
         c_int32,
         [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, POINTER(PagedCache), c_void_p, c_int64,

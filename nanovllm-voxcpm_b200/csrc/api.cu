@@ -464,6 +464,13 @@ size_t lora_b200_differential_workspace_bytes(int32_t T, int32_t n_seqs, int32_t
   return paged_workspace_bytes<kDiff>(T, num_heads, num_kv_heads, head_dim, keys, window, sinks);
 }
 
+int32_t lora_b200_differential_way(int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t table_width, int32_t block_size,
+                                   int32_t window, int32_t sinks) {
+  if (num_kv_heads < 1 || num_heads < num_kv_heads) return fail(B200_LORA_EINVAL, "differential_way: %d heads over %d kv heads", num_heads, num_kv_heads);
+  const PagedWay w = paged_way(T, num_heads, num_kv_heads, head_dim, (int64_t)table_width * block_size, window, sinks, kItemHeads<kDiff>);
+  return w.shares ? 0 : 16 * w.cluster + w.warps;
+}
+
 int lora_b200_differential_attention(void* out, int64_t out_token, int64_t out_head, const void* q, int64_t q_token, int64_t q_head,
                                      int32_t T, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                                      const lora_b200_paged_cache* cache, const int32_t* block_tables, int64_t table_ld,
