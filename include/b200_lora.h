@@ -542,8 +542,9 @@ int lora_b200_differential_attention(void* out, int64_t out_token, int64_t out_h
  * [n_groups], cu_groups int32 [n_groups + 1], ascending; a sequence in no group (or in one that leaves the sequences) shares nothing, a
  * prefix of zero (or less) is none. Tokens inside the prefix see it up to themselves. A value that is not finite, of a key of the prefix
  * that some rows of a block see, may reach the block's other rows (as in a prefill call; a block may hold rows of several sequences of
- * the group). Sharing takes block sizes that are multiples of 8, two sequences in a group, and tables wide enough for the second launch
- * to pay (lora_b200_shared_prefix_way: 1); other calls run as those two do. No counterpart in the reference.
+ * the group). Sharing takes block sizes that are multiples of 8, more sequences than groups, and tables wide enough for the second launch
+ * to pay (lora_b200_shared_prefix_way: 1; a group of one sequence then goes with the others); other calls run as those two do. The host
+ * knows the tables' width, not the lengths: where little is shared, those two are the faster calls. No counterpart in the reference.
  */
 int32_t lora_b200_shared_prefix_way(int32_t T, int32_t n_seqs, int32_t n_groups, int32_t num_heads, int32_t num_kv_heads,
                                     int32_t head_dim, int32_t table_width, int32_t block_size, int32_t packed);

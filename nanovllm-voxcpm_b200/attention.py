@@ -166,9 +166,11 @@ def shared_prefix_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cac
     a prefix may end inside a block, of which every request has a copy of its own). Where those lie is read from the table of the group's
     first request, which holds them all, what follows from each one's own. ``prefix_lens`` int32 ``[groups]``, ``cu_groups`` int32 ``[groups + 1]``, ascending;
     requests of no group share nothing, a prefix of zero is none. Other arguments, strides, missing blocks, contexts of no key and the
-    log sums as ``paged_decode_attention``. Calls whose tables are too narrow for a second launch to pay, block sizes that are no
-    multiples of 8 and groups of one request are attended request by request. A value that is not finite, of a key of the prefix that
-    some requests of a group see, may reach the group's others."""
+    log sums as ``paged_decode_attention``. Calls whose tables are too narrow for a second launch to pay, whose block size is no multiple
+    of 8 or that have no more requests than groups are attended request by request; in the others a group of one goes with the rest. The
+    lengths are on the device, so that the tables' width decides: where most keys lie behind the prefixes, or groups have one to three
+    requests, ``paged_decode_attention`` is the faster call. A value that is not finite, of a key of the prefix that some requests of a group see,
+    may reach the group's others."""
     return _shared_prefix(q, k_cache, v_cache, block_tables, context_lens, None, prefix_lens, cu_groups, scale, out, return_lse)
 
 

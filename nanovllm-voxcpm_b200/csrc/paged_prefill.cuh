@@ -1163,9 +1163,12 @@ inline PxPlan px_plan(int T, int Hq, int Hk, int D) {
 //   16 / 2 heads of 64: 16 requests of 8000 (67 MB) 15.5 / 20.7, 64 of 1500 (55 MB) 11.6 / 14.9, of 3000 (105 MB) 17.7 / 16.4, 192 of 1500
 //   33.6 / 20.9; 8 / 8 of 64: 16 of 3000 (105 MB) 17.8 / 15.8, 64 of 300 (59 MB) 13.1 / 18.6, of 1500 32 / 19.5; 32 / 8 of 128: 4 of 8000
 //   (134 MB) 23.9 / 24.6, 16 of 1500 (109 MB) 17.7 / 16.3, of 3000 29.5 / 17.6; 16 / 2 of 128: 64 of 700 (59 MB) 12.0 / 16.9, of 3000 30 / 19.2
-// Packed: tiles of rows over the whole contexts against those over the prefix and an item for every new token and kv head; what either
-// takes by the formulas below is within a third of what it took over 100 points. us, 32 requests with 2, 6, 12, 24 new tokens behind 4000
-// keys: 16 / 2 heads of 64 25, 25, 26, 39 / 17, 27, 33, 53; 32 / 8 of 128 123, 123, 125, 127 / 31, 55, 87, 165
+//   On the wrong side of that line: many keys behind the prefixes (the host knows their sum alone: 16 requests, 32 / 8 of 128, of 3000 behind 1000
+//   45 / 83, 48 of them 112 / 139), and groups of one to three requests (96 of 2100, 16 / 2 of 64, in 95, 48, 32, 24 and 8 groups 22 / 43,
+//   28, 26, 23, 19; 32 / 8 of 128 144 to 99 / 173, 113, 80, 68, 50).
+// Packed: tiles of rows over the whole contexts against those over the prefix and an item for every new token and kv head, by formulas
+// that tell which is less rather than how much (at 4 of 120 points the slower way, by more than 15 %). us, 32 requests with 2, 6, 12, 24 new
+// tokens behind 4000 keys: 16 / 2 heads of 64 25, 25, 26, 39 / 17, 27, 33, 53; 32 / 8 of 128 123, 123, 125, 127 / 32, 55, 88, 165
 inline bool px_shares(int T, int n_req, int n_groups, int Hq, int Hk, int D, int block_size, int64_t max_keys, bool packed) {
   if (n_groups < 1 || n_req <= n_groups || block_size % 8 != 0 || max_keys < 1 || max_keys > kPpMaxKeys || T >= (1 << 24)) return false;
   if (!packed) return (double)T * max_keys * Hk * D * 4 >= 100e6;
