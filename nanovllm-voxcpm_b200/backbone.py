@@ -138,14 +138,6 @@ class DecoderAttention(nn.Module):
             self.diff_norm = nn.Parameter(torch.ones(cfg.head_dim))
         self.k_cache = self.v_cache = None  # [blocks, block_size, kv_heads, head_dim], set by the harness
 
-    def _apply(self, fn, recurse=True):
-        """``lam`` stays the fp32 that the attention takes when the module's type changes: as it was, not by way of fewer bits."""
-        lam = self.lam.data if self.cfg.differential else None
-        super()._apply(fn, recurse)
-        if lam is not None and self.lam.dtype != torch.float32:
-            self.lam.data = lam.to(self.lam.device, torch.float32)
-        return self
-
     def forward(self, positions, hidden, step: AttentionStep, cos_sin) -> torch.Tensor:
         cfg = self.cfg
         qkv = self.qkv_proj(hidden)
@@ -181,11 +173,12 @@ class DecoderAttention(nn.Module):
                 raise ValueError("shared prefixes take attention over everything, by one map")
         if cfg.differential:
             how = dict(scale=cfg.rotary_dim ** -0.5, window=cfg.sliding_window, sinks=cfg.sink_tokens, norm_weight=self.diff_norm, eps=cfg.rms_norm_eps)
+            lam = self.lam.float()
             if nd:
-                A.differential_decode_attention(q[:nd], self.k_cache, self.v_cache, step.block_tables, step.context_lens, self.lam, out=out[:nd], **how)
+                A.differential_decode_attention(q[:nd], self.k_cache, self.v_cache, step.block_tables, step.context_lens, lam, out=out[:nd], **how)
             if step.is_prefill:
                 A.differential_prefill_attention(q[nd:], self.k_cache, self.v_cache, step.prefill_block_tables, step.prefill_context_lens,
-                                                 step.cu_seqlens, self.lam, out=out[nd:], **how)
+                                                 step.cu_seqlens, lam, out=out[nd:], **how)
             return out
         if nd and step.prefix_lens is not None:
             A.shared_prefix_decode_attention(q[:nd], self.k_cache, self.v_cache, step.block_tables, step.context_lens, *shared[0], scale=how["scale"],
